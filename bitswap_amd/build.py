@@ -9,9 +9,11 @@ SRC = os.path.join(HERE, "csrc", "bitswap_hip.hip")
 # one translation unit per kernel family (round 4: the 1,850-line bitswap_hip.hip with ~100 template instantiations took
 # 20 s on one core; the units compile in parallel) around the shared device helpers of csrc/bitswap_dev.h
 SRCS = [os.path.join(HERE, "csrc", f) for f in ("bitswap_hip.hip", "tables.hip", "pop.hip", "push.hip", "layer64.hip",
-                                                 "net_epilogue.hip", "wino_gemm.hip", "wino_gemm_bf16x3.hip")]
+                                                 "net_epilogue.hip", "wino_gemm.hip", "wino_gemm_bf16x3.hip",
+                                                 "linear.hip", "norm_act.hip", "pack8.hip")]
 HDR = os.path.join(HERE, "..", "include", "bitswap_hip.h")
 DEV_HDR = os.path.join(HERE, "csrc", "bitswap_dev.h")
+ROWS_HDR = os.path.join(HERE, "csrc", "rows_dev.h")      # shared by the channels-last layer kernels
 OBJ_DIR = os.path.join(HERE, "csrc", "_obj")
 PRODUCT_LIB = os.path.join(HERE, "csrc", "libbitswap_hip.so")
 
@@ -27,7 +29,10 @@ EXTRA_FLAGS = [f for f in os.environ.get("BITSWAP_HIPCC_EXTRA", "").split() if f
 # The -D is the source-level half of the guard: net_epilogue.hip refuses to compile (#error) unless the build says it turned the
 # vectorizer off, so another build system cannot silently produce the packed code; tests/test_host_cpu.py
 # disassembles the shipped library for packed float32 arithmetic on top of that.
-FILE_FLAGS = {"net_epilogue.hip": ["-fno-slp-vectorize", "-DBS_BUILT_WITHOUT_SLP_VECTORIZER"]}
+# The channels-last layer kernels take packed float32 arithmetic out at the source: the target feature itself is switched off.
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+FILE_FLAGS = {"net_epilogue.hip": ["-fno-slp-vectorize", "-DBS_BUILT_WITHOUT_SLP_VECTORIZER"],
+              "linear.hip": NO_PACKED_F32, "norm_act.hip": NO_PACKED_F32, "pack8.hip": NO_PACKED_F32}
 
 
 def _flag_hash():
@@ -63,7 +68,7 @@ def is_stale():
     if not os.path.exists(LIB):
         return True
     t = os.path.getmtime(LIB)
-    if any(os.path.getmtime(p) > t for p in SRCS + [HDR, DEV_HDR] if os.path.exists(p)):
+    if any(os.path.getmtime(p) > t for p in SRCS + [HDR, DEV_HDR, ROWS_HDR] if os.path.exists(p)):
         return True
     if os.environ.get("BITSWAP_HIP_LIB"):       # a library named by hand (diagnostics) is taken as it is -- and says so once
         global _warned_by_hand
@@ -108,7 +113,7 @@ def build_hip(force=False, verbose=False):
     # objects of another flag set (tools/gemm_probe.py --lab appends -DBS_GEMM_LAB) never mix with the product's
     objdir = OBJ_DIR + "_" + _flag_hash()
     os.makedirs(objdir, exist_ok=True)
-    deps = max(os.path.getmtime(p) for p in (HDR, DEV_HDR, os.path.abspath(__file__)))
+    deps = max(os.path.getmtime(p) for p in (HDR, DEV_HDR, ROWS_HDR, os.path.abspath(__file__)))
 
     def compile_one(src):
         obj = os.path.join(objdir, os.path.basename(src) + ".o")

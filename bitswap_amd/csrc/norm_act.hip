@@ -1,0 +1,568 @@
+// norm_act.hip -- group norm with an activation on channels-last activations, and its gradient.
+//
+//   m = mean, v = variance of a group (all pixels, channels / groups neighbouring channels);  r = 1 / sqrt(v + eps)
+//   h = (x - m) r,  u = h gamma + beta,  y = act(u)
+//   du = g act'(u), t = du gamma:   dx = r (t - mean(t) - h mean(t h)),  dgamma = sum du h,  dbeta = sum du
+//
+// Bound by memory: x (and g) in, y (dx) out.  Where the pixels of a few whole groups fit a workgroup's registers (k_norm,
+// k_norm_grad) everything is read once: a thread keeps 32 elements (V neighbouring channels of 32 / V pixels), sums go over its
+// pixels, then over the workgroup's pixel lanes and a group's channels through shared memory, the variance as the mean squared
+// distance from the mean already known.  Larger images (k_part_* / k_stats / k_apply*) are cut into runs of pixels whose
+// per-channel sums are joined in a second launch and applied in a third.  Which way is taken, and every order of addition, follows
+// from (pixels, channels, groups, type) alone: an image's bits do not depend on how many there are.
+#include "rows_dev.h"
+
+namespace {
+
+struct NormArgs {
+    const char *x, *g;
+    const int8_t* exps;                 // x in 8 bits
+    int64_t ldn, ldp, ldgn, ldgp;
+    const char *gamma, *beta;
+    int aff_f32, act;
+    float eps;
+    int64_t n, pixels;
+    int C, G, per;
+    int pl_log2;                        // pixel lanes of a workgroup
+    int cl;                             // lanes along the channels
+    int gs;                             // groups of a workgroup
+    int slabs;
+    int nb;                             // 8-bit blocks of a row
+    char* y;
+    float* stats;                       // in or out
+    float* parts;                       // grad: [n][2][C] sums of du h, du; split: per run of pixels
+    int runs;
+    int64_t run;
+};
+
+template <int DT>
+__device__ __forceinline__ void affine(const char* p, int f32, int c, int left, float fill, float* v) {
+    constexpr int V = vlen(DT);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        v[i] = (p && i < left) ? (f32 ? reinterpret_cast<const float*>(p)[c + i] : load1<DT>(p + (int64_t)(c + i) * esize(DT))) : fill;
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) v += __shfl_xor(v, o);
+    return v;
+}
+
+// Sums per thread and channel -> sums per group, known to every thread of the workgroup.
+//   a: this thread's sums of its channels, added up over its pixels; slot [pixel lane][channel of the slab] in `red`
+//   out[g] for the gs groups of the slab.  weight (null: 1) multiplies a channel's sum.  chan_out (nullable): the channel sums.
+struct SlabSum {
+    float *red, *part, *out;
+    int ch, PL, Q, gs, per, nthr, tid;           // ch: channels of the slab (chunks x V); Q: parts the pixel lanes are added in
+    template <int NV>
+    __device__ __forceinline__ void run(const float* a, int pl, int c, bool live, const char* weight, int w_f32, int c0, int C, int dt,
+                                        float* chan_out) const {
+        if (live)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) red[pl * ch + c + i] = a[i];
+        __syncthreads();
+        for (int i = tid; i < ch * Q; i += nthr) {
+            const int q = i / ch, k = i - q * ch;
+            float s = 0.0f;
+            for (int p = q; p < PL; p += Q) s += red[p * ch + k];
+            part[i] = s;
+        }
+        __syncthreads();
+        if (chan_out)
+            for (int k = tid; k < ch; k += nthr)
+                if (k < gs * per && c0 + k < C) {
+                    float s = 0.0f;
+                    for (int q = 0; q < Q; ++q) s += part[q * ch + k];
+                    chan_out[k] = s;
+                }
+        for (int g = tid >> 6; g < gs; g += nthr >> 6) {
+            float s = 0.0f;
+            for (int k = tid & 63; k < per; k += 64) {
+                float t = 0.0f;
+                for (int q = 0; q < Q; ++q) t += part[q * ch + g * per + k];
+                const int c_ = c0 + g * per + k;
+                if (weight && c_ < C)
+                    t *= w_f32 ? reinterpret_cast<const float*>(weight)[c_]
+                               : dt == BS_DT_BF16 ? load1<BS_DT_BF16>(weight + 2 * (int64_t)c_) : load1<BS_DT_F16>(weight + 2 * (int64_t)c_);
+                s += t;
+            }
+            s = wave_sum(s);
+            if ((tid & 63) == 0) out[g] = s;
+        }
+        __syncthreads();
+    }
+};
+
+// ---- images that fit -------------------------------------------------------------------------------------------------------
+template <int DT>
+__global__ __launch_bounds__(1024) void k_norm(const NormArgs a) {
+    constexpr int V = vlen(DT), R = 32 / V, ES = esize(DT);
+    extern __shared__ __align__(16) float sh[];
+    const int PL = 1 << a.pl_log2, CL = a.cl, tid = threadIdx.x;
+    const int64_t img = blockIdx.x / a.slabs;
+    const int slab = blockIdx.x % a.slabs, c0 = slab * a.gs * a.per;
+    const int width = min(a.gs * a.per, a.C - c0);               // channels of this slab
+    const int pl = tid / CL, cl = tid - pl * CL, k = cl * V, left = width - k;
+    const bool live = pl < PL && left > 0;
+    SlabSum ss;
+    ss.ch = CL * V; ss.PL = PL; ss.Q = max(1, PL / V); ss.gs = min(a.gs, a.G - slab * a.gs); ss.per = a.per;
+    ss.nthr = blockDim.x; ss.tid = tid;
+    ss.red = sh; ss.part = sh + PL * ss.ch; ss.out = ss.part + ss.Q * ss.ch;
+
+    float f[R][V];
+    const char* const xp = a.x + (img * a.ldn + c0 + k) * ES;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[r][i] = 0.0f;
+        const int64_t p = pl + (int64_t)r * PL;
+        if (live && p < a.pixels) load_vec<DT>(xp + p * a.ldp * ES, left, f[r]);
+    }
+    const float inv = 1.0f / ((float)a.pixels * (float)a.per);
+    float s[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        s[i] = 0.0f;
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[i] += f[r][i];
+    }
+    ss.run<V>(s, pl, k, live, nullptr, 0, c0, a.C, DT, nullptr);
+    float m[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) m[i] = i < left ? ss.out[(k + i) / a.per] * inv : 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        s[i] = 0.0f;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (pl + r * PL < a.pixels) {
+                const float d = f[r][i] - m[i];
+                s[i] = fmaf(d, d, s[i]);
+            }
+    }
+    float* const mean_sh = ss.out;                               // the means move on: out is written again
+    ss.out += ss.gs;
+    ss.run<V>(s, pl, k, live, nullptr, 0, c0, a.C, DT, nullptr);
+    float rs[V], ga[V], be[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) rs[i] = i < left ? 1.0f / sqrtf(ss.out[(k + i) / a.per] * inv + a.eps) : 0.0f;
+    if (a.stats && tid < ss.gs) {
+        float* const o = a.stats + (img * a.G + slab * a.gs + tid) * 2;
+        o[0] = mean_sh[tid] * inv;
+        o[1] = 1.0f / sqrtf(ss.out[tid] * inv + a.eps);
+    }
+    if (!live) return;
+    affine<DT>(a.gamma, a.aff_f32, c0 + k, left, 1.0f, ga);
+    affine<DT>(a.beta, a.aff_f32, c0 + k, left, 0.0f, be);
+    char* const yp = a.y + (img * a.pixels * a.C + c0 + k) * ES;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int64_t p = pl + (int64_t)r * PL;
+        if (p >= a.pixels) break;
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[r][i] = act_value(a.act, fmaf((f[r][i] - m[i]) * rs[i], ga[i], be[i]));
+        store_vec<DT>(yp + p * a.C * ES, left, f[r]);
+    }
+}
+
+template <int DT, bool SAVED8>
+__device__ __forceinline__ void load_x(const NormArgs& a, int64_t img, int64_t p, int c, int left, float* f) {
+    constexpr int V = vlen(DT);
+    if (SAVED8) {
+        const int64_t row = img * a.pixels + p;
+        load_codes<V>((const int8_t*)a.x + row * a.C, a.exps + row * a.nb, c, left, f);
+    } else {
+        load_vec<DT>(a.x + (img * a.ldn + p * a.ldp + c) * esize(DT), left, f);
+    }
+}
+
+template <int DT, bool SAVED8>
+__global__ __launch_bounds__(1024) void k_norm_grad(const NormArgs a) {
+    constexpr int V = vlen(DT), R = 32 / V, ES = esize(DT);
+    extern __shared__ __align__(16) float sh[];
+    const int PL = 1 << a.pl_log2, CL = a.cl, tid = threadIdx.x;
+    const int64_t img = blockIdx.x / a.slabs;
+    const int slab = blockIdx.x % a.slabs, c0 = slab * a.gs * a.per;
+    const int width = min(a.gs * a.per, a.C - c0);
+    const int pl = tid / CL, cl = tid - pl * CL, k = cl * V, left = width - k;
+    const bool live = pl < PL && left > 0;
+    SlabSum ss;
+    ss.ch = CL * V; ss.PL = PL; ss.Q = max(1, PL / V); ss.gs = min(a.gs, a.G - slab * a.gs); ss.per = a.per;
+    ss.nthr = blockDim.x; ss.tid = tid;
+    ss.red = sh; ss.part = sh + PL * ss.ch; ss.out = ss.part + ss.Q * ss.ch;
+
+    float h[R][V], d[R][V], m[V], rs[V], ga[V], be[V];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) h[r][i] = d[r][i] = 0.0f;
+        const int64_t p = pl + (int64_t)r * PL;
+        if (live && p < a.pixels) {
+            load_x<DT, SAVED8>(a, img, p, c0 + k, left, h[r]);
+            load_vec<DT>(a.g + (img * a.ldgn + p * a.ldgp + c0 + k) * ES, left, d[r]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const float* const st = a.stats + (img * a.G + (c0 + min(k + i, width - 1)) / a.per) * 2;
+        m[i] = st[0];
+        rs[i] = st[1];
+    }
+    affine<DT>(a.gamma, a.aff_f32, c0 + k, left, 1.0f, ga);
+    affine<DT>(a.beta, a.aff_f32, c0 + k, left, 0.0f, be);
+    float s1[V], s2[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        if (pl + r * PL < a.pixels) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                h[r][i] = (h[r][i] - m[i]) * rs[i];
+                d[r][i] *= act_slope(a.act, fmaf(h[r][i], ga[i], be[i]));
+                s1[i] += d[r][i];
+                s2[i] = fmaf(d[r][i], h[r][i], s2[i]);
+            }
+        }
+    float* const po = a.parts ? a.parts + img * 2 * a.C + c0 : nullptr;
+    ss.run<V>(s2, pl, k, live, a.gamma, a.aff_f32, c0, a.C, DT, po);
+    const float* const two = ss.out;
+    ss.out += ss.gs;
+    ss.run<V>(s1, pl, k, live, a.gamma, a.aff_f32, c0, a.C, DT, po ? po + a.C : nullptr);
+    if (!live) return;
+    const float inv = 1.0f / ((float)a.pixels * (float)a.per);
+    float m1[V], m2[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int g = min(k + i, width - 1) / a.per;
+        m1[i] = ss.out[g] * inv;
+        m2[i] = two[g] * inv;
+    }
+    char* const yp = a.y + (img * a.pixels * a.C + c0 + k) * ES;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int64_t p = pl + (int64_t)r * PL;
+        if (p >= a.pixels) break;
+#pragma unroll
+        for (int i = 0; i < V; ++i) d[r][i] = rs[i] * (fmaf(d[r][i], ga[i], -m1[i]) - h[r][i] * m2[i]);
+        store_vec<DT>(yp + p * a.C * ES, left, d[r]);
+    }
+}
+
+// ---- images that do not: runs of pixels ------------------------------------------------------------------------------------
+// workgroup: CL lanes along the channels x PL pixel lanes over one run of pixels of one image.
+//   forward: parts [n][runs][2][C] = mean and summed squared distance from it, per channel of the run
+//   grad:    parts [n][runs][2][C] = sums of du h and of du
+template <int DT, bool SAVED8, bool GRAD>
+__global__ __launch_bounds__(256) void k_part(const NormArgs a) {
+    constexpr int V = vlen(DT), ES = esize(DT);
+    __shared__ float red[256 * V];
+    __shared__ float tot[64 * V];
+    const int CL = a.cl, PL = 256 / CL, tid = threadIdx.x, pl = tid / CL, cl = tid - pl * CL;
+    const int64_t img = blockIdx.x / a.runs;
+    const int run = (int)(blockIdx.x % a.runs);
+    const int c = (blockIdx.y * CL + cl) * V, left = a.C - c;
+    const bool live = pl < PL && left > 0;
+    const int64_t p0 = run * a.run, p1 = min(p0 + a.run, a.pixels);
+    float* const out = a.parts + (img * a.runs + run) * 2 * a.C;
+    float s1[V], s2[V], m[V], rs[V], ga[V], be[V];
+    if (GRAD && live) {
+        affine<DT>(a.gamma, a.aff_f32, c, left, 1.0f, ga);
+        affine<DT>(a.beta, a.aff_f32, c, left, 0.0f, be);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float* const st = a.stats + (img * a.G + min(c + i, a.C - 1) / a.per) * 2;
+            m[i] = st[0];
+            rs[i] = st[1];
+        }
+    }
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {              // forward: sums, then squared distances; grad: one pass, two joins
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if (!GRAD || pass == 0) s1[i] = 0.0f;
+            if (pass == 0) s2[i] = 0.0f;
+        }
+        if (live && (!GRAD || pass == 0))
+            for (int64_t p = p0 + pl; p < p1; p += PL) {
+                float f[V];
+                load_x<DT, SAVED8>(a, img, p, c, left, f);
+                if (GRAD) {
+                    float g[V];
+                    load_vec<DT>(a.g + (img * a.ldgn + p * a.ldgp + c) * ES, left, g);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float h = (f[i] - m[i]) * rs[i];
+                        const float d = g[i] * act_slope(a.act, fmaf(h, ga[i], be[i]));
+                        s1[i] = fmaf(d, h, s1[i]);
+                        s2[i] += d;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float d = pass == 0 ? f[i] : f[i] - m[i];
+                        s1[i] = pass == 0 ? s1[i] + d : fmaf(d, d, s1[i]);
+                    }
+                }
+            }
+        if (pl < PL)
+#pragma unroll
+            for (int i = 0; i < V; ++i) red[(pl * CL + cl) * V + i] = (GRAD && pass == 1) ? s2[i] : s1[i];
+        __syncthreads();
+        for (int i = tid; i < CL * V; i += 256) {
+            float s = 0.0f;
+            for (int p = 0; p < PL; ++p) s += red[p * CL * V + i];
+            if (!GRAD && pass == 0) s = s / (float)(p1 - p0);
+            tot[i] = s;
+            const int col = blockIdx.y * CL * V + i;
+            if (col < a.C) out[pass * a.C + col] = s;
+        }
+        __syncthreads();
+        if (!GRAD && pass == 0 && pl < PL)
+#pragma unroll
+            for (int i = 0; i < V; ++i) m[i] = tot[cl * V + i];
+    }
+}
+
+// one workgroup per (image, group): joins the runs.  forward: stats; grad: sums [n][G][2] of gamma du h and gamma du
+template <bool GRAD>
+__global__ __launch_bounds__(256) void k_join(const NormArgs a, int dt, float* __restrict__ out) {
+    __shared__ float red[2][4];
+    const int64_t img = blockIdx.x / a.G;
+    const int g = (int)(blockIdx.x % a.G), tid = threadIdx.x;
+    const int64_t items = (int64_t)a.runs * a.per;
+    const float* const parts = a.parts + img * a.runs * 2 * a.C + g * a.per;
+    auto join = [&](int slot, float v) {
+        v = wave_sum(v);
+        if ((tid & 63) == 0) red[slot][tid >> 6] = v;
+        __syncthreads();
+        return (red[slot][0] + red[slot][1]) + (red[slot][2] + red[slot][3]);
+    };
+    const float count = (float)a.pixels * (float)a.per;
+    float s = 0.0f, q = 0.0f;
+    if (GRAD) {
+        for (int64_t i = tid; i < items; i += 256) {
+            const int64_t r = i / a.per;
+            const int c = (int)(i - r * a.per), ch = g * a.per + c;
+            const float w = !a.gamma ? 1.0f : a.aff_f32 ? reinterpret_cast<const float*>(a.gamma)[ch]
+                                      : dt == BS_DT_BF16 ? load1<BS_DT_BF16>(a.gamma + 2 * (int64_t)ch) : load1<BS_DT_F16>(a.gamma + 2 * (int64_t)ch);
+            s = fmaf(parts[r * 2 * a.C + c], w, s);
+            q = fmaf(parts[(r * 2 + 1) * a.C + c], w, q);
+        }
+        s = join(0, s);
+        q = join(1, q);
+        if (tid == 0) {
+            out[blockIdx.x * 2] = s / count;
+            out[blockIdx.x * 2 + 1] = q / count;
+        }
+        return;
+    }
+    for (int64_t i = tid; i < items; i += 256) {
+        const int64_t r = i / a.per;
+        const float cnt = (float)(min((r + 1) * a.run, a.pixels) - r * a.run);
+        s = fmaf(parts[r * 2 * a.C + (i - r * a.per)], cnt, s);
+    }
+    const float mean = join(0, s) / count;
+    for (int64_t i = tid; i < items; i += 256) {
+        const int64_t r = i / a.per, c = i - r * a.per;
+        const float cnt = (float)(min((r + 1) * a.run, a.pixels) - r * a.run);
+        const float d = parts[r * 2 * a.C + c] - mean;
+        q += fmaf(d * d, cnt, parts[(r * 2 + 1) * a.C + c]);
+    }
+    q = join(1, q) / count;
+    if (tid == 0) {
+        out[blockIdx.x * 2] = mean;
+        out[blockIdx.x * 2 + 1] = 1.0f / sqrtf(q + a.eps);
+    }
+}
+
+// stats known (and, for the gradient, the group means): one pass
+template <int DT, bool SAVED8, bool GRAD>
+__global__ __launch_bounds__(256) void k_apply(const NormArgs a, const float* __restrict__ stats, const float* __restrict__ means) {
+    constexpr int V = vlen(DT), ES = esize(DT);
+    const int CL = a.cl, PL = 256 / CL, tid = threadIdx.x, pl = tid / CL, cl = tid - pl * CL;
+    const int64_t img = blockIdx.x / a.runs;
+    const int run = (int)(blockIdx.x % a.runs);
+    const int c = (blockIdx.y * CL + cl) * V, left = a.C - c;
+    if (pl >= PL || left <= 0) return;
+    const int64_t p0 = run * a.run, p1 = min(p0 + a.run, a.pixels);
+    float m[V], rs[V], ga[V], be[V], m1[V], m2[V];
+    affine<DT>(a.gamma, a.aff_f32, c, left, 1.0f, ga);
+    affine<DT>(a.beta, a.aff_f32, c, left, 0.0f, be);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int64_t at = (img * a.G + min(c + i, a.C - 1) / a.per) * 2;
+        m[i] = stats[at];
+        rs[i] = stats[at + 1];
+        m2[i] = GRAD ? means[at] : 0.0f;
+        m1[i] = GRAD ? means[at + 1] : 0.0f;
+    }
+    for (int64_t p = p0 + pl; p < p1; p += PL) {
+        float f[V], g[V];
+        load_x<DT, SAVED8>(a, img, p, c, left, f);
+        if (GRAD) load_vec<DT>(a.g + (img * a.ldgn + p * a.ldgp + c) * ES, left, g);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float h = (f[i] - m[i]) * rs[i], u = fmaf(h, ga[i], be[i]);
+            f[i] = GRAD ? rs[i] * (fmaf(g[i] * act_slope(a.act, u), ga[i], -m1[i]) - h * m2[i]) : act_value(a.act, u);
+        }
+        store_vec<DT>(a.y + ((img * a.pixels + p) * a.C + c) * ES, left, f);
+    }
+}
+
+// ---- which way, and how it is cut --------------------------------------------------------------------------------------------
+struct Plan {
+    bool fits;
+    int pl_log2, cl, gs, slabs, threads, lds;
+    int runs;
+    int64_t run;
+    int cly;              // split: workgroups along the channels
+};
+
+Plan plan(int dtype, int64_t n, int64_t pixels, int C, int G, int outs) {
+    Plan p = {};
+    const int V = dtype == BS_DT_F32 ? 4 : 8, R = 32 / V, per = C / G;
+    int64_t need = (pixels + R - 1) / R;
+    while ((1 << p.pl_log2) < need && p.pl_log2 < 10) ++p.pl_log2;
+    const int PL = 1 << p.pl_log2, cap = 1024 / PL;
+    const int one = (per + V - 1) / V;                  // lanes that one group takes
+    p.fits = need <= 256 && one <= cap;
+    if (p.fits) {
+        // as many groups as give rows of 256 bytes, or 512 threads; fewer when there are few images (neither changes a bit)
+        int gs = 1;
+        while (gs < G) {
+            const int lanes = (2 * gs * per + V - 1) / V;
+            if (lanes > cap || lanes * PL > 512 || gs * per * 16 / V >= 256) break;
+            if (n * ((G + 2 * gs - 1) / (2 * gs)) < 512) break;
+            gs *= 2;
+        }
+        p.gs = gs;
+        p.cl = (gs * per + V - 1) / V;
+        p.slabs = (G + gs - 1) / gs;
+        p.threads = (PL * p.cl + 63) / 64 * 64;
+        const int ch = p.cl * V, Q = PL / V > 1 ? PL / V : 1;
+        p.lds = (PL * ch + Q * ch + 2 * gs) * 4;
+        return p;
+    }
+    const int chunks = (C + V - 1) / V;
+    p.cl = chunks < 32 ? chunks : 32;
+    p.cly = (chunks + p.cl - 1) / p.cl;
+    p.run = 256;                                        // pixels of a run, more when there would be over 1024 runs
+    while ((pixels + p.run - 1) / p.run > 1024) p.run *= 2;
+    p.runs = (int)((pixels + p.run - 1) / p.run);
+    return p;
+}
+
+int bad_norm(int dtype, int64_t n, int64_t pixels, int channels, int groups, int act) {
+    return bad_type(dtype) || n < 0 || n > MAX_ROWS || pixels < 0 || pixels > MAX_ROWS || channels < 1 || channels > (1 << 24) || groups < 1 ||
+           channels % groups || act < BS_ACT_NONE || act > BS_ACT_GELU;
+}
+
+void fill(NormArgs* a, const Plan& p) {
+    a->pl_log2 = p.pl_log2; a->cl = p.cl; a->gs = p.gs; a->slabs = p.slabs; a->runs = p.runs; a->run = p.run;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t bs_group_norm_workspace(int dtype, int64_t n, int64_t pixels, int channels, int groups, int grad) {
+    if (bad_norm(dtype, n, pixels, channels, groups, 0)) return BS_EINVAL;
+    const Plan p = plan(dtype, n, pixels, channels, groups, grad);
+    if (p.fits) return grad ? n * 2 * channels * 4 : 0;
+    return (n * p.runs * 2 * channels + n * groups * 2) * 4;
+}
+
+int bs_group_norm_act(const void* x, int64_t ldn, int64_t ldp, const void* gamma, const void* beta, int affine_dtype, float eps,
+                      int act, int dtype, int64_t n, int64_t pixels, int channels, int groups, void* y, float* stats,
+                      void* workspace, int64_t workspace_bytes, void* stream) {
+    if (bad_norm(dtype, n, pixels, channels, groups, act) || !(eps >= 0.0f)) return BS_EINVAL;
+    if (n == 0 || pixels == 0) return BS_OK;
+    if (!x || !y || ldp < channels || ldn < 0) return BS_EINVAL;
+    if ((gamma || beta) && affine_dtype != BS_DT_F32 && affine_dtype != dtype) return BS_EINVAL;
+    const Plan p = plan(dtype, n, pixels, channels, groups, 0);
+    const int64_t need = bs_group_norm_workspace(dtype, n, pixels, channels, groups, 0);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return BS_EINVAL;
+    NormArgs a = {};
+    a.x = (const char*)x; a.ldn = ldn; a.ldp = ldp; a.gamma = (const char*)gamma; a.beta = (const char*)beta;
+    a.aff_f32 = affine_dtype == BS_DT_F32; a.act = act; a.eps = eps; a.n = n; a.pixels = pixels;
+    a.C = channels; a.G = groups; a.per = channels / groups; a.y = (char*)y; a.stats = stats;
+    fill(&a, p);
+    hipStream_t st = rows_stream(stream);
+    const int64_t blocks = p.fits ? n * p.slabs : n * p.runs;
+    if (blocks > 0x7fffffff || n * groups > 0x7fffffff) return BS_EINVAL;
+    if (p.fits) {
+#define GO(DT) hipLaunchKernelGGL(k_norm<DT>, dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a)
+        if (dtype == BS_DT_F32) GO(BS_DT_F32);
+        else if (dtype == BS_DT_BF16) GO(BS_DT_BF16);
+        else GO(BS_DT_F16);
+#undef GO
+        return rows_rc();
+    }
+    a.parts = (float*)workspace;
+    float* const own = a.parts + n * p.runs * 2 * channels;
+    float* const st_out = stats ? stats : own;
+    const dim3 grid((unsigned)blocks, (unsigned)p.cly);
+#define GO(DT) do { hipLaunchKernelGGL((k_part<DT, false, false>), grid, dim3(256), 0, st, a); \
+                    hipLaunchKernelGGL(k_join<false>, dim3((unsigned)(n * groups)), dim3(256), 0, st, a, dtype, st_out); \
+                    hipLaunchKernelGGL((k_apply<DT, false, false>), grid, dim3(256), 0, st, a, (const float*)st_out, (const float*)nullptr); } while (0)
+    if (dtype == BS_DT_F32) GO(BS_DT_F32);
+    else if (dtype == BS_DT_BF16) GO(BS_DT_BF16);
+    else GO(BS_DT_F16);
+#undef GO
+    return rows_rc();
+}
+
+int bs_group_norm_act_grad(const void* g, int64_t ldgn, int64_t ldgp, const void* x, const int8_t* x_exps, int64_t ldn, int64_t ldp,
+                           const float* stats, const void* gamma, const void* beta, int affine_dtype, int act, int dtype, int64_t n,
+                           int64_t pixels, int channels, int groups, void* dx, float* dgamma, float* dbeta, void* workspace,
+                           int64_t workspace_bytes, void* stream) {
+    if (bad_norm(dtype, n, pixels, channels, groups, act)) return BS_EINVAL;
+    hipStream_t st = rows_stream(stream);
+    const dim3 cols((unsigned)((2 * (int64_t)channels + 63) / 64));
+    if (n == 0 || pixels == 0) {
+        if (dgamma || dbeta) hipLaunchKernelGGL(k_sum_columns, cols, dim3(256), 0, st, (const float*)nullptr, (int64_t)0, 2 * channels, channels, dgamma, dbeta);
+        return rows_rc();
+    }
+    if (!g || !x || !stats || !dx || ldgp < channels || ldgn < 0 || (!x_exps && (ldp < channels || ldn < 0))) return BS_EINVAL;
+    if ((gamma || beta) && affine_dtype != BS_DT_F32 && affine_dtype != dtype) return BS_EINVAL;
+    const Plan p = plan(dtype, n, pixels, channels, groups, 1);
+    const int64_t need = bs_group_norm_workspace(dtype, n, pixels, channels, groups, 1);
+    if (!workspace || workspace_bytes < need) return BS_EINVAL;
+    NormArgs a = {};
+    a.g = (const char*)g; a.ldgn = ldgn; a.ldgp = ldgp;
+    a.x = (const char*)x; a.exps = x_exps; a.ldn = ldn; a.ldp = ldp; a.nb = (channels + P8_BLOCK - 1) / P8_BLOCK;
+    a.gamma = (const char*)gamma; a.beta = (const char*)beta; a.aff_f32 = affine_dtype == BS_DT_F32; a.act = act;
+    a.n = n; a.pixels = pixels; a.C = channels; a.G = groups; a.per = channels / groups;
+    a.y = (char*)dx; a.stats = (float*)stats; a.parts = (float*)workspace;
+    fill(&a, p);
+    const int64_t blocks = p.fits ? n * p.slabs : n * p.runs;
+    if (blocks > 0x7fffffff || n * groups > 0x7fffffff) return BS_EINVAL;
+    if (p.fits) {
+        if (!dgamma && !dbeta) a.parts = nullptr;
+#define GO(DT) do { if (x_exps) hipLaunchKernelGGL((k_norm_grad<DT, true>), dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a); \
+                    else hipLaunchKernelGGL((k_norm_grad<DT, false>), dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a); } while (0)
+        if (dtype == BS_DT_F32) GO(BS_DT_F32);
+        else if (dtype == BS_DT_BF16) GO(BS_DT_BF16);
+        else GO(BS_DT_F16);
+#undef GO
+    } else {
+        float* const means = a.parts + n * p.runs * 2 * channels;
+        const dim3 grid((unsigned)blocks, (unsigned)p.cly);
+#define STEPS(DT, P8) do { hipLaunchKernelGGL((k_part<DT, P8, true>), grid, dim3(256), 0, st, a); \
+                           hipLaunchKernelGGL(k_join<true>, dim3((unsigned)(n * groups)), dim3(256), 0, st, a, dtype, means); \
+                           hipLaunchKernelGGL((k_apply<DT, P8, true>), grid, dim3(256), 0, st, a, stats, (const float*)means); } while (0)
+#define GO(DT) do { if (x_exps) STEPS(DT, true); else STEPS(DT, false); } while (0)
+        if (dtype == BS_DT_F32) GO(BS_DT_F32);
+        else if (dtype == BS_DT_BF16) GO(BS_DT_BF16);
+        else GO(BS_DT_F16);
+#undef GO
+#undef STEPS
+    }
+    if (dgamma || dbeta)
+        hipLaunchKernelGGL(k_sum_columns, cols, dim3(256), 0, st, (const float*)workspace, p.fits ? n : n * p.runs, 2 * channels, channels, dgamma, dbeta);
+    return rows_rc();
+}
+
+}  // extern "C"

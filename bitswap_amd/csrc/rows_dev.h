@@ -1,0 +1,194 @@
+// rows_dev.h -- device helpers of the channels-last layer kernels (linear.hip, norm_act.hip, pack8.hip): element types, 16-byte
+// accesses at any alignment, activations and their slopes, the 8-bit form of a saved activation.
+#ifndef BITSWAP_ROWS_DEV_H
+#define BITSWAP_ROWS_DEV_H
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/bitswap_hip.h"
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int esize(int dt) { return dt == BS_DT_F32 ? 4 : 2; }
+constexpr int vlen(int dt) { return 16 / esize(dt); }        // elements of a 16-byte access
+
+__device__ __forceinline__ float bits_f32(uint32_t u) { return __builtin_bit_cast(float, u); }
+__device__ __forceinline__ uint32_t f32_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
+// two floats -> two bfloat16 / float16 in one word, round to nearest even (one v_cvt_pk on gfx950)
+__device__ __forceinline__ uint32_t pk_bf16(float a, float b) {
+    const f32x2 v = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+}
+__device__ __forceinline__ uint32_t pk_f16(float a, float b) {
+    const f32x2 v = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+}
+
+// one element
+template <int DT>
+__device__ __forceinline__ float load1(const char* p) {
+    if (DT == BS_DT_F32) return *reinterpret_cast<const float*>(p);
+    const uint16_t u = *reinterpret_cast<const uint16_t*>(p);
+    if (DT == BS_DT_BF16) return bits_f32((uint32_t)u << 16);
+    return (float)__builtin_bit_cast(_Float16, u);
+}
+template <int DT>
+__device__ __forceinline__ void store1(char* p, float v) {
+    if (DT == BS_DT_F32) *reinterpret_cast<float*>(p) = v;
+    else if (DT == BS_DT_BF16) *reinterpret_cast<uint16_t*>(p) = (uint16_t)pk_bf16(v, 0.0f);
+    else *reinterpret_cast<_Float16*>(p) = (_Float16)v;
+}
+
+// 4 / 8 / 16 bytes at an address that need not be aligned to more than an element: gfx950 takes such vector accesses as they are,
+// so rows of an odd number of channels cost no more instructions than others
+__device__ __forceinline__ u32x4 load16(const char* p) { u32x4 r; __builtin_memcpy(&r, p, 16); return r; }
+__device__ __forceinline__ u32x2 load8(const char* p) { u32x2 r; __builtin_memcpy(&r, p, 8); return r; }
+__device__ __forceinline__ uint32_t load4(const char* p) { uint32_t r; __builtin_memcpy(&r, p, 4); return r; }
+__device__ __forceinline__ void store16(char* p, u32x4 v) { __builtin_memcpy(p, &v, 16); }
+__device__ __forceinline__ void store8(char* p, u32x2 v) { __builtin_memcpy(p, &v, 8); }
+
+// 16 bytes <-> the floats they hold (4 or 8)
+template <int DT>
+__device__ __forceinline__ void unpack16(u32x4 r, float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (DT == BS_DT_F32) {
+            f[i] = bits_f32(r[i]);
+        } else if (DT == BS_DT_BF16) {
+            f[2 * i] = bits_f32(r[i] << 16);
+            f[2 * i + 1] = bits_f32(r[i] & 0xffff0000u);
+        } else {
+            const f16x2 h = __builtin_bit_cast(f16x2, (uint32_t)r[i]);
+            f[2 * i] = (float)h[0];
+            f[2 * i + 1] = (float)h[1];
+        }
+    }
+}
+template <int DT>
+__device__ __forceinline__ u32x4 pack16(const float* f) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (DT == BS_DT_F32) r[i] = f32_bits(f[i]);
+        else if (DT == BS_DT_BF16) r[i] = pk_bf16(f[2 * i], f[2 * i + 1]);
+        else r[i] = pk_f16(f[2 * i], f[2 * i + 1]);
+    }
+    return r;
+}
+// the first n elements of such a vector (0 < n; all of them when n >= vlen), the others zero
+template <int DT>
+__device__ __forceinline__ void load_vec(const char* p, int n, float* f) {
+    constexpr int V = vlen(DT);
+    if (n >= V) {
+        unpack16<DT>(load16(p), f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = i < n ? load1<DT>(p + i * esize(DT)) : 0.0f;
+    }
+}
+template <int DT>
+__device__ __forceinline__ void store_vec(char* p, int n, const float* f) {
+    constexpr int V = vlen(DT);
+    if (n >= V) {
+        store16(p, pack16<DT>(f));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < n) store1<DT>(p + i * esize(DT), f[i]);
+    }
+}
+
+// ---- activations ----------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float act_value(int act, float s) {
+    if (act == BS_ACT_ELU) return s > 0.0f ? s : expm1f(s);
+    if (act == BS_ACT_SILU) return s / (1.0f + expf(-s));
+    if (act == BS_ACT_GELU) return 0.5f * s * (1.0f + erff(s * 0.70710678118654752f));
+    return s;
+}
+__device__ __forceinline__ float act_slope(int act, float s) {
+    if (act == BS_ACT_ELU) return s > 0.0f ? 1.0f : expf(s);
+    if (act == BS_ACT_SILU) {
+        const float p = 1.0f / (1.0f + expf(-s));
+        return p * (1.0f + s * (1.0f - p));
+    }
+    if (act == BS_ACT_GELU)
+        return 0.5f * (1.0f + erff(s * 0.70710678118654752f)) + s * expf(-0.5f * s * s) * 0.39894228040143268f;
+    return 1.0f;
+}
+
+// ---- the 8-bit form of a saved activation ---------------------------------------------------------------------------------
+// 32 consecutive channels of a row share 2^e, e the smallest exponent >= -126 with amax <= 127 2^e, but no larger than 127 2^e is
+// a value of the type (121; float16: 9); code = rint(v 2^-e), at most 127 either way, -128 stands for a value that is not finite
+// (and is kept out of amax).  A power of two keeps every step exact: v 2^-e, code 2^e, and
+// code 2^e as bfloat16 (7 significant bits), so the gradients' matrix products take the codes as bfloat16 operands unrounded.
+constexpr int P8_BLOCK = 32;
+
+template <int DT>
+__device__ __forceinline__ int p8_exponent(float amax) {      // amax finite, >= 0
+    const uint32_t u = f32_bits(amax);
+    const int p = (int)(u >> 23) - 127;                         // amax in [2^p, 2^(p+1)); subnormal: p = -127
+    const int e = p - 6 + ((u & 0x7fffffu) > 0x7e0000u ? 1 : 0);        // 1.984375 = 127 / 64
+    constexpr int top = DT == BS_DT_F16 ? 9 : 121;
+    return e < -126 ? -126 : e > top ? top : e;
+}
+__device__ __forceinline__ float p8_pow2(int e) { return bits_f32((uint32_t)(e + 127) << 23); }      // e >= -126
+__device__ __forceinline__ float p8_value(int code, float step) { return code == -128 ? __builtin_nanf("") : (float)code * step; }
+
+// V codes of a row from channel c on (n of them exist) -> floats
+template <int V>
+__device__ __forceinline__ void load_codes(const int8_t* __restrict__ codes, const int8_t* __restrict__ exps, int c, int n, float* f) {
+    // at most two blocks of 32 channels meet in V <= 8 consecutive channels
+    const int b0 = c / P8_BLOCK, b1 = (c + (n < V ? n : V) - 1) / P8_BLOCK;
+    const float s0 = p8_pow2(exps[b0]), s1 = p8_pow2(exps[b1]);
+    uint32_t w[2] = {0, 0};
+    if (n >= V) {
+        if (V == 4) w[0] = load4((const char*)codes + c);
+        else {
+            const u32x2 t = load8((const char*)codes + c);
+            w[0] = t[0]; w[1] = t[1];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < n) w[i / 4] |= (uint32_t)(uint8_t)codes[c + i] << (8 * (i % 4));
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = p8_value((int)(int8_t)(w[i / 4] >> (8 * (i % 4))), (c + i) / P8_BLOCK == b0 ? s0 : s1);
+}
+
+// parts [nparts][n] -> their sums, columns below n0 to out0 and the others to out1 (either may be null); 64 columns x 4 lanes over the
+// parts a workgroup, always the same order
+static __global__ __launch_bounds__(256) void k_sum_columns(const float* __restrict__ parts, int64_t nparts, int n, int n0,
+                                                     float* __restrict__ out0, float* __restrict__ out1) {
+    __shared__ float red[256];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63), l = threadIdx.x >> 6;
+    float s = 0.0f;
+    if (c < n)
+        for (int64_t k = l; k < nparts; k += 4) s += parts[k * n + c];
+    red[threadIdx.x] = s;
+    __syncthreads();
+    if (l == 0 && c < n) {
+        const float v = (red[threadIdx.x] + red[threadIdx.x + 64]) + (red[threadIdx.x + 128] + red[threadIdx.x + 192]);
+        if (c < n0) { if (out0) out0[c] = v; }
+        else if (out1) out1[c - n0] = v;
+    }
+}
+
+inline bool bad_type(int dt) { return dt != BS_DT_F32 && dt != BS_DT_BF16 && dt != BS_DT_F16; }
+constexpr int64_t MAX_ROWS = (int64_t)1 << 40;
+inline hipStream_t rows_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
+inline int rows_rc() { return hipGetLastError() == hipSuccess ? BS_OK : BS_ELAUNCH; }
+
+}  // namespace
+#endif

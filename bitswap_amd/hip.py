@@ -24,6 +24,8 @@ SYMBOLS = [
     "bs_layer_push64", "bs_stream_create_cu_mask", "bs_stream_destroy", "bs_debug_where",
     "bs_selftest", "bs_sigmoid_f64", "bs_bias_residual_elu_f32", "bs_head_params_f32", "bs_expand_rows5_f32", "bs_wino_in_f32", "bs_wino_out_f32", "bs_wino_fused_f32",
     "bs_small_k_gemm_f32", "bs_conv3_wino_f32", "bs_wino_gemm_f32", "bs_wino_gemm_bf16x3",
+    "bs_linear_act", "bs_act_grad_workspace", "bs_act_grad", "bs_linear_grad_x", "bs_linear_grad_w_workspace", "bs_linear_grad_w",
+    "bs_group_norm_workspace", "bs_group_norm_act", "bs_group_norm_act_grad", "bs_pack8", "bs_unpack8",
 ]
 HEAD_SIGMOID, HEAD_SOFTPLUS = 0, 1
 
@@ -81,9 +83,20 @@ def load():
     L.bs_wino_gemm_bf16x3.argtypes = [p, p, p, i32, i32, i32, i64, i32, p]
     L.bs_conv3_wino_f32.argtypes = [p, p, p, i32, p, p, i32, i64, i32, i32, i32, i32, p]
     L.bs_wino_out_f32.argtypes = [p, p, p, p, p, i64, i32, i32, i32, i32, i32, p]
+    L.bs_linear_act.argtypes = [p, i64, p, i64, p, i32, p, i64, p, p, i32, i32, i64, i32, i32, p]
+    L.bs_act_grad_workspace.argtypes = [i64, i32]
+    L.bs_act_grad.argtypes = [p, i64, p, i64, p, p, i64, i32, i32, i64, i32, p, p, p, i64, p]
+    L.bs_linear_grad_x.argtypes = [p, i64, p, i64, p, i32, i64, i32, i32, p]
+    L.bs_linear_grad_w_workspace.argtypes = [i32, i64, i32, i32]
+    L.bs_linear_grad_w.argtypes = [p, i64, p, p, i64, p, i32, i64, i32, i32, p, i64, p]
+    L.bs_group_norm_workspace.argtypes = [i32, i64, i64, i32, i32, i32]
+    L.bs_group_norm_act.argtypes = [p, i64, i64, p, p, i32, C.c_float, i32, i32, i64, i64, i32, i32, p, p, p, i64, p]
+    L.bs_group_norm_act_grad.argtypes = [p, i64, i64, p, p, i64, i64, p, p, p, i32, i32, i32, i64, i64, i32, i32, p, p, p, p, i64, p]
+    L.bs_pack8.argtypes = [p, i64, p, p, i32, i64, i32, p]
+    L.bs_unpack8.argtypes = [p, p, p, i32, i64, i32, p]
     for n in SYMBOLS:
         if n != "bs_strerror":
-            getattr(L, n).restype = i32
+            getattr(L, n).restype = i64 if n.endswith("_workspace") else i32
     if L.bs_abi_version() != ABI_VERSION:
         raise BitswapHipError(f"{path} has ABI version {L.bs_abi_version()}, this binding needs {ABI_VERSION}: "
                               "rebuild with `python -m bitswap_amd.build`")
@@ -808,6 +821,293 @@ def wino_fused(src, shape, ts_in=0, bias=None, res=None, act=True, want_sum=Fals
     _check(load().bs_wino_fused_f32(_ptr(src), ts_in, _ptr(bias), _ptr(res), int(act), _ptr(s_out), _ptr(a_out),
                                     _ptr(V), ts_out, N, Cc, H, W, _stream()), "bs_wino_fused_f32")
     return s_out, a_out, V
+
+
+# ---- channels-last layers: products, group norm, 8-bit saves (linear.hip, norm_act.hip, pack8.hip) ------------------------------
+ACT_NONE, ACT_ELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # BS_DT_*
+PACK8_BLOCK = 32
+
+
+def _dtype_code(t, what):
+    if t.dtype not in _DTYPES:
+        raise BitswapHipError(f"{what}: float32, bfloat16 or float16, got {t.dtype}")
+    return _DTYPES[t.dtype]
+
+
+def _act_code(act):
+    if act not in (ACT_NONE, ACT_ELU, ACT_SILU, ACT_GELU):
+        raise BitswapHipError(f"unknown activation {act!r}")
+    return int(act)
+
+
+def _as_rows(t, width, what):
+    """[..., width] as rows of channels -> (tensor that owns the memory, row stride in elements, rows).  Leading axes that do not
+    collapse to one stride, rows that overlap (an expanded gradient) or strided channels are copied."""
+    if t.dim() < 1 or t.shape[-1] != width:
+        raise BitswapHipError(f"{what}: expected [..., {width}], got {tuple(t.shape)}")
+    rows = 1
+    for n in t.shape[:-1]:
+        rows *= n
+    axes = [(n, st) for n, st in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
+    ld = axes[-1][1] if axes else width
+    ok = (width == 1 or t.stride(-1) == 1) and ld >= width
+    for (_, outer), (n, inner) in zip(axes[:-1], axes[1:]):
+        ok = ok and outer == inner * n
+    if not ok:
+        t, ld = t.contiguous(), width
+    return t, ld, rows
+
+
+def _affine(name, v, n, like):
+    if v is None:
+        return None, 0
+    if tuple(v.shape) != (n,) or v.dtype not in (torch.float32, like.dtype):
+        raise BitswapHipError(f"{name}: expected [{n}] of float32 or {like.dtype}, got {tuple(v.shape)} {v.dtype}")
+    return v.contiguous(), _DTYPES[v.dtype]
+
+
+def _workspace(nbytes, device):
+    if nbytes < 0:
+        raise BitswapHipError("sizes the kernels do not take")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+class Packed8:
+    """An activation [..., C] in 8 bits: codes int8 [rows, C] and, per 32 channels of a row, exps int8 [rows, ceil(C / 32)];
+    value = code 2^exp, code -128 a value that was not finite (include/bitswap_hip.h, bs_pack8).  `dtype` is the type it was
+    packed from and unpacks to.  1.03 bytes per value instead of 4 or 2."""
+
+    __slots__ = ("codes", "exps", "shape", "dtype")
+
+    def __init__(self, codes, exps, shape, dtype):
+        shape = tuple(int(n) for n in shape)
+        rows = 1
+        for n in shape[:-1]:
+            rows *= n
+        if dtype not in _DTYPES or not shape or shape[-1] < 1:
+            raise BitswapHipError(f"Packed8: an activation [..., C] of float32, bfloat16 or float16, got {shape} {dtype}")
+        for name, t, n in (("codes", codes, shape[-1]), ("exps", exps, -(-shape[-1] // PACK8_BLOCK))):
+            if t.dtype != torch.int8 or tuple(t.shape) != (rows, n) or not t.is_contiguous():
+                raise BitswapHipError(f"Packed8: {name} must be a contiguous int8 tensor [{rows}, {n}], got {t.dtype} {tuple(t.shape)}")
+        if codes.device != exps.device:
+            raise BitswapHipError("Packed8: codes and exps on one device")
+        self.codes, self.exps, self.shape, self.dtype = codes, exps, shape, dtype
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def pack8(x):
+    """x [..., C] float32 / bfloat16 / float16 -> Packed8."""
+    _need_cuda(x)
+    code = _dtype_code(x, "pack8")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise BitswapHipError(f"pack8: expected [..., C], got {tuple(x.shape)}")
+    width = x.shape[-1]
+    t, ld, rows = _as_rows(x, width, "pack8")
+    codes = torch.empty((rows, width), dtype=torch.int8, device=x.device)
+    exps = torch.empty((rows, -(-width // PACK8_BLOCK)), dtype=torch.int8, device=x.device)
+    _check(load().bs_pack8(_ptr(t), ld, _ptr(codes), _ptr(exps), code, rows, width, _stream()), "bs_pack8")
+    return Packed8(codes, exps, x.shape, x.dtype)
+
+
+def unpack8(p):
+    """Packed8 -> the values it holds, contiguous, in the type it was packed from."""
+    if not isinstance(p, Packed8):
+        raise BitswapHipError("unpack8 takes the Packed8 that pack8() returns")
+    _need_cuda(p.codes, p.exps)
+    x = torch.empty(p.shape, dtype=p.dtype, device=p.device)
+    _check(load().bs_unpack8(_ptr(p.codes), _ptr(p.exps), _ptr(x), _DTYPES[p.dtype], p.codes.shape[0], p.codes.shape[1], _stream()),
+           "bs_unpack8")
+    return x
+
+
+def _saved_rows(v, width, dtype, rows, what):
+    """A saved activation (tensor or Packed8) -> (tensor that owns the memory, exponents | None, row stride)."""
+    if isinstance(v, Packed8):
+        if v.dtype != dtype or v.codes.shape != (rows, width):
+            raise BitswapHipError(f"{what}: expected {rows} rows of {width} {dtype}, got {v.shape} {v.dtype}")
+        _need_cuda(v.codes, v.exps)
+        return v.codes, v.exps, width
+    _need_cuda(v)
+    if v.dtype != dtype:
+        raise BitswapHipError(f"{what}: expected {dtype}, got {v.dtype}")
+    t, ld, n = _as_rows(v, width, what)
+    if n != rows:
+        raise BitswapHipError(f"{what}: {n} rows beside {rows}")
+    return t, None, ld
+
+
+def linear_act(x, w, bias=None, res=None, act=ACT_ELU, want_sum=False, want_act=True):
+    """s = x w^T + bias (+ res) over rows of channels -> (s | None, act(s) | None), in x's type: a pointwise convolution on
+    channels-last activations with its epilogue in one launch.  x [..., K] (any row stride), w [N, K], bias [N], res [..., N];
+    float32 (limb products, as wino_gemm_bf16x3), bfloat16 or float16, float32 sums.  A row's bits do not depend on how many rows
+    there are (include/bitswap_hip.h, bs_linear_act)."""
+    _need_cuda(x, w, bias, res)
+    code, act = _dtype_code(x, "linear_act"), _act_code(act)
+    if w.dim() != 2 or w.dtype != x.dtype or w.shape[0] < 1 or w.shape[1] < 1:
+        raise BitswapHipError(f"linear_act: w must be [N, K] of {x.dtype}, got {tuple(w.shape)} {w.dtype}")
+    if not (want_sum or want_act):
+        raise BitswapHipError("linear_act: nothing is asked for")
+    N, K = w.shape
+    xt, ldx, rows = _as_rows(x, K, "linear_act x")
+    wt, ldw, _ = _as_rows(w, K, "linear_act w")
+    bias, bcode = _affine("linear_act bias", bias, N, x)
+    shape = tuple(x.shape[:-1]) + (N,)
+    rt, ldr = None, 0
+    if res is not None:
+        if tuple(res.shape) != shape or res.dtype != x.dtype:
+            raise BitswapHipError(f"linear_act: res must be {shape} of {x.dtype}, got {tuple(res.shape)} {res.dtype}")
+        rt, ldr, _ = _as_rows(res, N, "linear_act res")
+    s = torch.empty(shape, dtype=x.dtype, device=x.device) if want_sum else None
+    y = torch.empty(shape, dtype=x.dtype, device=x.device) if want_act else None
+    _check(load().bs_linear_act(_ptr(xt), ldx, _ptr(wt), ldw, _ptr(bias), bcode, _ptr(rt), ldr, _ptr(s), _ptr(y), act, code, rows,
+                                K, N, _stream()), "bs_linear_act")
+    return s, y
+
+
+def linear_act_grad(x, w, s=None, act=ACT_NONE, g_sum=None, g_act=None, want_x=True, want_w=True, want_bias=True, want_res=False):
+    """Gradients of linear_act -> (dx | None, dw | None, db float32 [N] | None, dres | None) for the gradients g_sum of its sum and
+    g_act of its activation (either may be None, not both): ds = g_sum + g_act act'(s), dx = ds w, dw = ds^T x, db = sum of ds over
+    the rows, dres = ds (the incoming gradient itself where nothing changes it).  x and s are the saved input and sum -- whole, or
+    as Packed8, whose codes the kernels read as they are; s is only needed for g_act with an activation, x only for dw."""
+    if g_sum is None and g_act is None:
+        raise BitswapHipError("linear_act_grad: no gradient")
+    g0 = g_sum if g_sum is not None else g_act
+    _need_cuda(w, g_sum, g_act)
+    act = _act_code(act)
+    if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1:
+        raise BitswapHipError(f"linear_act_grad: w must be [N, K], got {tuple(w.shape)}")
+    code = _dtype_code(w, "linear_act_grad")
+    N, K = w.shape
+    gs = []
+    for g in (g_sum, g_act):
+        if g is None:
+            gs.append((None, 0))
+            continue
+        if g.dtype != w.dtype or g.shape != g0.shape:
+            raise BitswapHipError(f"linear_act_grad: gradients must be of {w.dtype} and one shape, got {g.dtype} {tuple(g.shape)}")
+        t, ld, rows = _as_rows(g, N, "linear_act_grad gradient")
+        gs.append((t, ld))
+    st, se, lds = None, None, 0
+    sloped = g_act is not None and act != ACT_NONE
+    if sloped:
+        if s is None:
+            raise BitswapHipError("linear_act_grad: the gradient of an activation needs the saved sum s")
+        st, se, lds = _saved_rows(s, N, w.dtype, rows, "linear_act_grad s")
+    if want_w:
+        if x is None:
+            raise BitswapHipError("linear_act_grad: the gradient of w needs the saved input x")
+        xt, xe, ldx = _saved_rows(x, K, w.dtype, rows, "linear_act_grad x")
+    dev, L = w.device, load()
+    # one gradient and no slope: it is ds already
+    made = sloped or (g_sum is not None and g_act is not None)
+    need_ds = want_x or want_w or want_res
+    ds = torch.empty(g0.shape, dtype=w.dtype, device=dev) if made and need_ds else None
+    db = torch.empty(N, dtype=torch.float32, device=dev) if want_bias else None
+    if ds is not None or db is not None:
+        nb = L.bs_act_grad_workspace(rows, N) if want_bias else 0
+        ws = _workspace(nb, dev)
+        _check(L.bs_act_grad(_ptr(gs[0][0]), gs[0][1], _ptr(gs[1][0]), gs[1][1], _ptr(st), _ptr(se), lds, act, code, rows, N, _ptr(ds),
+                             _ptr(db), _ptr(ws), nb, _stream()), "bs_act_grad")
+    if ds is not None:
+        dt, ldd = ds, N
+    else:
+        dt, ldd = gs[0] if g_sum is not None else gs[1]
+    dx = dw = None
+    if want_x:
+        wt, ldw, _ = _as_rows(w, K, "linear_act_grad w")
+        dx = torch.empty(tuple(g0.shape[:-1]) + (K,), dtype=w.dtype, device=dev)
+        _check(L.bs_linear_grad_x(_ptr(dt), ldd, _ptr(wt), ldw, _ptr(dx), code, rows, K, N, _stream()), "bs_linear_grad_x")
+    if want_w:
+        dw = torch.empty((N, K), dtype=w.dtype, device=dev)
+        nb = L.bs_linear_grad_w_workspace(code, rows, K, N)
+        ws = _workspace(nb, dev)
+        _check(L.bs_linear_grad_w(_ptr(dt), ldd, _ptr(xt), _ptr(xe), ldx, _ptr(dw), code, rows, K, N, _ptr(ws), nb, _stream()),
+               "bs_linear_grad_w")
+    return dx, dw, db, ((ds if ds is not None else g0) if want_res else None)
+
+
+def _as_images(t, what):
+    """[n, ..., C] channels last -> (tensor that owns the memory, image stride, pixel stride, n, pixels, C)."""
+    if t.dim() < 2 or t.shape[-1] < 1:
+        raise BitswapHipError(f"{what}: expected [n, ..., C], got {tuple(t.shape)}")
+    n, C = t.shape[0], t.shape[-1]
+    pixels = 1
+    for k in t.shape[1:-1]:
+        pixels *= k
+    axes = [(k, st) for k, st in zip(t.shape[1:-1], t.stride()[1:-1]) if k != 1]
+    ldp = axes[-1][1] if axes else C
+    ok = (C == 1 or t.stride(-1) == 1) and ldp >= C
+    for (_, outer), (k, inner) in zip(axes[:-1], axes[1:]):
+        ok = ok and outer == inner * k
+    if not ok:
+        t, ldp = t.contiguous(), C
+    return t, t.stride(0) if n > 1 else pixels * C, ldp, n, pixels, C
+
+
+def group_norm_act(x, groups, gamma=None, beta=None, eps=1e-5, act=ACT_ELU, want_stats=False, want_pack=False):
+    """Group norm with an activation on channels-last x [n, ..., C] (a batch axis first, channels last, pixels between) ->
+    (y, stats | None, Packed8 of x | None): u = (x - mean) / sqrt(var + eps) gamma + beta over the pixels and C / groups channels
+    of a group, y = act(u), contiguous.  stats float32 [n, groups, 2] = (mean, 1 / sqrt(var + eps)): what the gradient needs
+    besides x.  gamma, beta [C] float32 or x's type.  An image's bits do not depend on n."""
+    _need_cuda(x, gamma, beta)
+    code, act = _dtype_code(x, "group_norm_act"), _act_code(act)
+    t, ldn, ldp, n, pixels, C = _as_images(x, "group_norm_act")
+    groups = int(groups)
+    if groups < 1 or C % groups:
+        raise BitswapHipError(f"group_norm_act: {groups} groups do not divide {C} channels")
+    if not eps >= 0:
+        raise BitswapHipError(f"group_norm_act: eps {eps}")
+    gamma, gcode = _affine("group_norm_act gamma", gamma, C, x)
+    beta, bcode = _affine("group_norm_act beta", beta, C, x)
+    if gamma is not None and beta is not None and gcode != bcode:
+        raise BitswapHipError("group_norm_act: gamma and beta of one type")
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = (torch.empty if x.numel() else torch.zeros)((n, groups, 2), dtype=torch.float32, device=x.device) if want_stats else None
+    L = load()
+    nb = L.bs_group_norm_workspace(code, n, pixels, C, groups, 0)
+    ws = _workspace(nb, x.device)
+    _check(L.bs_group_norm_act(_ptr(t), ldn, ldp, _ptr(gamma), _ptr(beta), gcode if gamma is not None else bcode, float(eps), act, code,
+                               n, pixels, C, groups, _ptr(y), _ptr(stats), _ptr(ws), nb, _stream()), "bs_group_norm_act")
+    return y, stats, pack8(x) if want_pack else None
+
+
+def group_norm_act_grad(x, stats, groups, g, gamma=None, beta=None, act=ACT_ELU, want_affine=True):
+    """Gradients of group_norm_act -> (dx, dgamma float32 [C] | None, dbeta float32 [C] | None) from the saved input x (whole or as
+    Packed8), the stats of the forward call and the gradient g of its y."""
+    _need_cuda(stats, g, gamma, beta)
+    code, act = _dtype_code(g, "group_norm_act_grad"), _act_code(act)
+    gt, ldgn, ldgp, n, pixels, C = _as_images(g, "group_norm_act_grad")
+    groups = int(groups)
+    if groups < 1 or C % groups:
+        raise BitswapHipError(f"group_norm_act_grad: {groups} groups do not divide {C} channels")
+    if tuple(x.shape) != tuple(g.shape) or x.dtype != g.dtype:
+        raise BitswapHipError(f"group_norm_act_grad: x must be {tuple(g.shape)} of {g.dtype}, got {tuple(x.shape)} {x.dtype}")
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (n, groups, 2):
+        raise BitswapHipError(f"group_norm_act_grad: stats must be float32 [{n}, {groups}, 2]")
+    stats = stats.contiguous()
+    if isinstance(x, Packed8):
+        _need_cuda(x.codes, x.exps)
+        xt, xe, ldn, ldp = x.codes, x.exps, pixels * C, C
+    else:
+        _need_cuda(x)
+        (xt, ldn, ldp), xe = _as_images(x, "group_norm_act_grad")[:3], None
+    gamma, gcode = _affine("group_norm_act_grad gamma", gamma, C, g)
+    beta, bcode = _affine("group_norm_act_grad beta", beta, C, g)
+    if gamma is not None and beta is not None and gcode != bcode:
+        raise BitswapHipError("group_norm_act_grad: gamma and beta of one type")
+    dx = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+    dgamma, dbeta = (torch.empty(C, dtype=torch.float32, device=g.device) if want_affine else None for _ in range(2))
+    L = load()
+    nb = L.bs_group_norm_workspace(code, n, pixels, C, groups, 1)
+    ws = _workspace(nb, g.device)
+    _check(L.bs_group_norm_act_grad(_ptr(gt), ldgn, ldgp, _ptr(xt), _ptr(xe), ldn, ldp, _ptr(stats), _ptr(gamma), _ptr(beta),
+                                    gcode if gamma is not None else bcode, act, code, n, pixels, C, groups, _ptr(dx), _ptr(dgamma),
+                                    _ptr(dbeta), _ptr(ws), nb, _stream()), "bs_group_norm_act_grad")
+    return dx, dgamma, dbeta
 
 
 # ---- diagnostics: run a kernel wrapper twice and record on the device whether (and for which image) the two results differ ---

@@ -345,6 +345,72 @@ int bs_wino_in_f32(const float* in, const float* bias, float* V, int64_t N, int 
 int bs_wino_out_f32(const float* M, const float* bias, const float* res, float* sum_out, float* act_out,
                     int64_t N, int C, int H, int W, int ts, int ms, void* stream);
 
+/*
+ * Channels-last layer operators (bitswap_amd/csrc/linear.hip, norm_act.hip, pack8.hip): a layer over rows of channels -- the
+ * pixels of channels-last latents, or any [rows, channels] -- and its gradients.  dtype: BS_DT_F32 / BF16 / F16, the type of x, w,
+ * res, s, gradients and outputs; bias, gamma and beta may be float32 beside a 16-bit dtype (their own dtype argument).  Row
+ * strides (ld*) are in elements, channels of a row are contiguous, addresses need the alignment of an element only.  Sums and
+ * statistics are float32; every output is rounded once, to nearest even.
+ *
+ * bs_linear_act -- s = x w^T + bias (+ res), a = act(s); x [rows, K], w [N, K], bias [N] (nullable), res [rows, N] (nullable);
+ *   sum_out = s, act_out = a, contiguous [rows, N] (each nullable, at least one).  act sees s before its rounding.  float32
+ *   operands are split into three bfloat16 limbs and multiplied as six limb products (as bs_wino_gemm_bf16x3); a sum that does
+ *   not come out finite is added up again in float32, so infinities and NaN arrive as they do in float32 arithmetic.  A row's
+ *   bits do not depend on `rows`.
+ *
+ * bs_act_grad -- ds = g_sum + g_act act'(s) (either gradient nullable, not both), rows [rows, N]: ds_out contiguous (nullable),
+ *   db_out [N] float32 = sum over the rows of ds before its rounding (nullable; workspace of bs_act_grad_workspace bytes then).
+ *   s: [rows, N] of dtype (row stride lds), or, if s_exps is given, int8 codes [rows, N] with their exponents (bs_pack8).
+ *   act BS_ACT_NONE: s is not read and may be null.
+ * bs_linear_grad_x -- dx [rows, K] = ds w;  ds [rows, N] (row stride ldds), w [N, K].
+ * bs_linear_grad_w -- dw [N, K] = ds^T x;  x [rows, K] of dtype (row stride ldx) or, if x_exps is given, codes of bs_pack8.  The
+ *   rows are split over the chip into parts of a size fixed by (rows, N, K) and the parts added in order: the same call gives the
+ *   same bits.  workspace: bs_linear_grad_w_workspace bytes (may be 0).
+ *
+ * bs_group_norm_act -- x [n, pixels, channels] (strides ldn, ldp), groups dividing channels: mean and biased variance over the
+ *   pixels and channels of a group, u = (x - mean) / sqrt(var + eps) * gamma + beta, y = act(u), y contiguous; stats
+ *   [n, groups, 2] float32 = (mean, 1 / sqrt(var + eps)) (nullable).  An image's bits do not depend on n.
+ *   workspace: bs_group_norm_workspace bytes (0 for images that fit a workgroup's registers).
+ * bs_group_norm_act_grad -- with h = (x - mean) rstd, du = g act'(h gamma + beta), t = du gamma:
+ *   dx = rstd (t - mean_g(t) - h mean_g(t h)), dgamma = sum du h, dbeta = sum du (float32 [channels], each nullable).
+ *   x [n, pixels, channels] of dtype, or codes of bs_pack8 over [n * pixels, channels] if x_exps is given.
+ *
+ * bs_pack8 -- x [rows, channels] -> codes int8 [rows, channels] and exps int8 [rows, ceil(channels / 32)]: 32 channels of a row
+ *   share 2^e, e the smallest integer >= -126 with max|x| <= 127 2^e, at most 121 (float16: 9: 127 2^e stays a value of the type);
+ *   code = rint(x 2^-e) (ties to even) within +-127; -128 marks a value that is not finite (left out of the maximum).  bs_unpack8 -- x = code 2^e, exact in every dtype that held x; -128 gives NaN.
+ *
+ * All of them: BS_EINVAL for null operands, negative sizes, strides below the row length, unknown types or activations, a
+ * workspace that is too small; rows == 0 or n == 0 is a call without rows (gradients of parameters are then zero).
+ */
+#define BS_DT_F32 0
+#define BS_DT_BF16 1
+#define BS_DT_F16 2
+#define BS_ACT_NONE 0
+#define BS_ACT_ELU 1
+#define BS_ACT_SILU 2
+#define BS_ACT_GELU 3
+int bs_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype, const void* res,
+                  int64_t ldr, void* sum_out, void* act_out, int act, int dtype, int64_t rows, int K, int N, void* stream);
+int64_t bs_act_grad_workspace(int64_t rows, int N);
+int bs_act_grad(const void* g_sum, int64_t ldgs, const void* g_act, int64_t ldga, const void* s, const int8_t* s_exps, int64_t lds,
+                int act, int dtype, int64_t rows, int N, void* ds_out, float* db_out, void* workspace, int64_t workspace_bytes,
+                void* stream);
+int bs_linear_grad_x(const void* ds, int64_t ldds, const void* w, int64_t ldw, void* dx, int dtype, int64_t rows, int K, int N,
+                     void* stream);
+int64_t bs_linear_grad_w_workspace(int dtype, int64_t rows, int K, int N);
+int bs_linear_grad_w(const void* ds, int64_t ldds, const void* x, const int8_t* x_exps, int64_t ldx, void* dw, int dtype,
+                     int64_t rows, int K, int N, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t bs_group_norm_workspace(int dtype, int64_t n, int64_t pixels, int channels, int groups, int grad);
+int bs_group_norm_act(const void* x, int64_t ldn, int64_t ldp, const void* gamma, const void* beta, int affine_dtype, float eps,
+                      int act, int dtype, int64_t n, int64_t pixels, int channels, int groups, void* y, float* stats,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+int bs_group_norm_act_grad(const void* g, int64_t ldgn, int64_t ldgp, const void* x, const int8_t* x_exps, int64_t ldn, int64_t ldp,
+                           const float* stats, const void* gamma, const void* beta, int affine_dtype, int act, int dtype, int64_t n,
+                           int64_t pixels, int channels, int groups, void* dx, float* dgamma, float* dbeta, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+int bs_pack8(const void* x, int64_t ldx, int8_t* codes, int8_t* exps, int dtype, int64_t rows, int channels, void* stream);
+int bs_unpack8(const int8_t* codes, const int8_t* exps, void* x, int dtype, int64_t rows, int channels, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,104 @@
+"""CPU: what the channels-last layer operators refuse before any launch, and what their workspaces come to."""
+import ctypes
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def L():
+    from bitswap_amd import hip
+    return hip.load()
+
+
+def buf():
+    b = (ctypes.c_char * 64)()
+    return b, ctypes.c_void_p(ctypes.addressof(b))
+
+
+def test_null_operands_sizes_types_and_strides_are_refused(L):
+    from bitswap_amd import hip
+    keep, p = buf()
+    E = hip.EINVAL
+    #                          x ldx  w ldw bias bt res ldr sum act  a  dt rows K  N  stream
+    ok = lambda **k: L.bs_linear_act(*[k.get(n, d) for n, d in (("x", p), ("ldx", 8), ("w", p), ("ldw", 8), ("bias", None), ("bt", 0), ("res", None),      # noqa: E731
+                                     ("ldr", 0), ("s", p), ("y", None), ("act", 1), ("dt", 0), ("rows", 4), ("K", 8), ("N", 8), ("stream", None))])
+    for bad in (dict(x=None), dict(w=None), dict(s=None), dict(ldx=7), dict(ldw=7), dict(res=p, ldr=7), dict(act=4), dict(act=-1), dict(dt=3),
+                dict(dt=-1), dict(rows=-1), dict(rows=1 << 41), dict(K=0), dict(N=0), dict(bias=p, bt=1)):
+        assert ok(**bad) == E, bad
+    assert ok(rows=0, x=None) == hip.OK                                     # no rows: nothing to do
+    assert L.bs_linear_grad_x(None, 8, p, 8, p, 0, 4, 8, 8, None) == E
+    assert L.bs_linear_grad_x(p, 7, p, 8, p, 0, 4, 8, 8, None) == E
+    assert L.bs_linear_grad_w(p, 8, None, None, 8, p, 0, 4, 8, 8, None, 0, None) == E
+    assert L.bs_linear_grad_w(p, 8, p, None, 8, None, 0, 4, 8, 8, None, 0, None) == E
+    n = L.bs_linear_grad_w_workspace(0, 100000, 8, 8)
+    assert n > 0 and L.bs_linear_grad_w(p, 8, p, None, 8, p, 0, 100000, 8, 8, p, n - 1, None) == E
+    assert L.bs_linear_grad_w(p, 8, p, None, 8, p, 0, 100000, 8, 8, None, n, None) == E
+    assert L.bs_act_grad(None, 8, None, 8, None, None, 8, 1, 0, 4, 8, p, None, None, 0, None) == E           # no gradient
+    assert L.bs_act_grad(None, 8, p, 8, None, None, 8, 1, 0, 4, 8, p, None, None, 0, None) == E              # no sum
+    assert L.bs_act_grad(p, 8, None, 8, None, None, 8, 1, 0, 4, 8, None, None, None, 0, None) == E           # nothing asked
+    n = L.bs_act_grad_workspace(100000, 8)
+    assert n > 0 and L.bs_act_grad(p, 8, None, 8, None, None, 8, 0, 0, 100000, 8, None, p, p, n - 1, None) == E
+    assert L.bs_group_norm_act(p, 64, 8, None, None, 0, 1e-5, 0, 0, 2, 8, 8, 3, p, None, None, 0, None) == E  # 3 groups of 8 channels
+    assert L.bs_group_norm_act(p, 64, 7, None, None, 0, 1e-5, 0, 0, 2, 8, 8, 2, p, None, None, 0, None) == E
+    assert L.bs_group_norm_act(p, 64, 8, p, None, 2, 1e-5, 0, 0, 2, 8, 8, 2, p, None, None, 0, None) == E     # gamma of a third type
+    assert L.bs_group_norm_act(p, 64, 8, None, None, 0, -1.0, 0, 0, 2, 8, 8, 2, p, None, None, 0, None) == E
+    assert L.bs_group_norm_act(p, 64, 8, None, None, 0, 1e-5, 0, 0, 2, 8000, 8, 2, p, None, None, 0, None) == E      # needs a workspace
+    assert L.bs_group_norm_act_grad(p, 64, 8, p, None, 64, 8, None, None, None, 0, 0, 0, 2, 8, 8, 2, p, None, None, p, 1 << 20, None) == E
+    assert L.bs_pack8(None, 8, p, p, 0, 4, 8, None) == E and L.bs_pack8(p, 7, p, p, 0, 4, 8, None) == E
+    assert L.bs_pack8(p, 8, p, p, 5, 4, 8, None) == E and L.bs_unpack8(p, None, p, 0, 4, 8, None) == E
+    assert L.bs_pack8(None, 8, p, p, 0, 0, 8, None) == hip.OK
+    del keep
+
+
+def test_workspaces(L):
+    for rows in (0, 1, 63, 64, 65, 1000, 102400, 1 << 33):
+        for k, n in ((1, 1), (61, 130), (2048, 2048)):
+            assert 0 <= L.bs_linear_grad_w_workspace(1, rows, k, n) < 1 << 28
+            assert 0 <= L.bs_act_grad_workspace(rows, n) < 1 << 26
+    assert L.bs_linear_grad_w_workspace(1, 1, 8, 8) == 0
+    for bad in ((3, 8, 8, 8), (1, -1, 8, 8), (1, 8, 0, 8), (1, 8, 8, 0)):
+        assert L.bs_linear_grad_w_workspace(*bad) < 0
+    assert L.bs_group_norm_workspace(0, 3, 256, 256, 32, 0) == 0
+    assert L.bs_group_norm_workspace(0, 3, 1 << 20, 64, 32, 1) > 0
+    assert L.bs_group_norm_workspace(0, 3, 256, 256, 33, 0) < 0
+
+
+def test_tensors_off_the_gpu_are_refused():
+    from bitswap_amd import hip
+    x, w = torch.zeros(4, 6), torch.zeros(5, 6)
+    for call in (lambda: hip.linear_act(x, w), lambda: hip.linear_act_grad(x, w, g_act=torch.zeros(4, 5)), lambda: hip.group_norm_act(x, 2),
+                 lambda: hip.group_norm_act_grad(x, torch.zeros(4, 2, 2), 2, x), lambda: hip.pack8(x),
+                 lambda: hip.unpack8(hip.Packed8(torch.zeros(4, 6, dtype=torch.int8), torch.zeros(4, 1, dtype=torch.int8), (4, 6), torch.float32))):
+        with pytest.raises(hip.BitswapHipError):
+            call()
+
+
+def test_packed8_checks_its_parts():
+    from bitswap_amd import hip
+    codes, exps = torch.zeros(6, 40, dtype=torch.int8), torch.zeros(6, 2, dtype=torch.int8)
+    p = hip.Packed8(codes, exps, (2, 3, 40), torch.bfloat16)
+    assert p.shape == (2, 3, 40) and p.dtype == torch.bfloat16
+    for bad in ((codes[:5], exps, (2, 3, 40)), (codes, exps[:, :1], (2, 3, 40)), (codes.int(), exps, (2, 3, 40)), (codes, exps, (2, 3, 41)),
+                (codes, exps, ()), (torch.zeros(6, 80, dtype=torch.int8)[:, ::2], exps, (2, 3, 40))):
+        with pytest.raises(hip.BitswapHipError):
+            hip.Packed8(bad[0], bad[1], bad[2], torch.float32)
+    with pytest.raises(hip.BitswapHipError):
+        hip.Packed8(codes, exps, (2, 3, 40), torch.float64)
+
+
+def test_rows_and_images_are_read_in_place_where_their_strides_allow():
+    from bitswap_amd import hip
+    x = torch.arange(2 * 3 * 4 * 10.).view(2, 3, 4, 10)
+    for v, ld, rows, inplace in ((x, 10, 24, True), (x[..., 2:9], 10, 24, True), (x[:, :, ::2], 20, 12, True), (x[:, ::2], 10, 16, False),
+                                 (x[0, 0, 0], 10, 1, True), (x[:, 0, 0], 120, 2, True), (x[..., ::2], 5, 24, False),
+                                 (x[:1, :1, :1].expand(2, 3, 4, 10), 10, 24, False)):
+        t, got, n = hip._as_rows(v, v.shape[-1], "x")
+        assert (got, n) == (ld, rows) and (t.data_ptr() == v.data_ptr()) == inplace
+        flat = torch.as_strided(t, (n, v.shape[-1]), (got, 1))
+        assert torch.equal(flat, v.reshape(-1, v.shape[-1]))
+    for v, inplace in ((x, True), (x[:, :, :, 1:7], True), (x[::2], True), (x[:, :, ::2], True), (x[:, ::2], False), (x[:, 0], True), (x[:, 0, 0], True),
+                       (x.permute(0, 3, 1, 2), False), (x[:1].expand(5, 3, 4, 10), True)):
+        t, ldn, ldp, n, pixels, c = hip._as_images(v, "x")
+        assert (t.data_ptr() == v.data_ptr()) == inplace
+        assert torch.equal(torch.as_strided(t, (n, pixels, c), (ldn, ldp, 1)), v.reshape(n, pixels, c))
