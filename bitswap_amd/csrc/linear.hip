@@ -1,35 +1,26 @@
 // linear.hip -- products over rows of channels (channels-last activations): s = x w^T + bias (+ res) with its activation, and the
-// two products of its backward pass.  One kernel template; what differs is which axis of an operand is contiguous in memory.
+// two products of its backward pass, on the bf16 / f16 matrix cores (v_mfma_f32_32x32x16), float32 sums.
 //
-//   out[q][p] = sum_k P(p, k) Q(q, k)                    p the contiguous axis of the output
-//   forward   P = w  [N, K]      (k contiguous)      Q = x  [rows, K]  (k contiguous)
-//   dx        P = w^T            (p contiguous)      Q = ds [rows, N]  (k contiguous)
-//   dw        P = x^T or codes   (p contiguous)      Q = ds^T          (q contiguous), k = rows, split over workgroups
+//   forward  out[q][p] = sum_k w[p][k] x[q][k]          k = K, the contiguous axis of both: k_rows / k_relay
+//   dx       out[q][p] = sum_k w[k][p] ds[q][k]         k = N; w is small and is turned round first (k_lay_w), then as the forward
+//   dw       out[q][p] = sum_k x[k][p] ds[k][q]         k = rows, the strided axis of both: k_over_rows, cut into parts of the rows
+//
+// float32 operands are split into three bfloat16 limbs (their sum is the float exactly) and multiplied as the six limb products of
+// total order <= 2; what is left out is of relative size 2^-24.  Limb products of an infinity or of a value that rounds to one are
+// NaN, so a sum that does not come out finite is added up again in float32.
+//
+// The output channel is the row index of the matrix instruction: a lane then holds, for one row q = lane % 32 of activations, the
+// channels 8 g + 4 (lane / 32) + 0..3, g = 0..3, of a 32x32 tile.
 #include "rows_dev.h"
 
 namespace {
 
-enum { L_KC = 0, L_IC = 1, L_P8 = 2 };                    // k contiguous | index contiguous | index contiguous 8-bit codes
-enum { E_LAYER = 0, E_PLAIN = 1, E_PART = 2 };            // bias + residual + activation | one rounding | float32 partial sums
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
-struct GemmArgs {
-    const char* P;
-    const char* Q;
-    const int8_t* Pexp;       // L_P8: exponents [nk, lpe]
-    int64_t ldp, ldq;         // row strides in elements
-    int lpe;
-    int np;
-    int64_t nq, nk;
-    int64_t kpart;            // k per part (split products), else nk
-    int tp;                   // tiles along p
-    int64_t tiles;
-    const char* bias;
-    const char* res;
-    int64_t ldr;
-    char* out0;               // sum / plain output / partials
-    char* out1;               // activation
-    int act, bias_f32;
-};
+enum { E_LAYER = 0, E_PLAIN = 1 };                        // bias + residual + activation | one rounding
+constexpr int limbs_of(int dt) { return dt == BS_DT_F32 ? 3 : 1; }
 
 template <int DT>
 __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
@@ -38,202 +29,225 @@ __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// 8 floats -> their three bfloat16 limbs (round to nearest; the three add up to the float exactly)
-__device__ __forceinline__ void limbs3(const float* f, u32x4* l) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float a = f[2 * i], b = f[2 * i + 1];
-        const uint32_t h0 = pk_bf16(a, b);
-        a -= bits_f32(h0 << 16);
-        b -= bits_f32(h0 & 0xffff0000u);
-        const uint32_t h1 = pk_bf16(a, b);
-        a -= bits_f32(h1 << 16);
-        b -= bits_f32(h1 & 0xffff0000u);
-        l[0][i] = h0;
-        l[1][i] = h1;
-        l[2][i] = pk_bf16(a, b);
-    }
+// two floats -> their three bfloat16 limbs, round to nearest
+__device__ __forceinline__ void limbs2(float a, float b, uint32_t* l) {
+    l[0] = pk_bf16(a, b);
+    a -= bits_f32(l[0] << 16);
+    b -= bits_f32(l[0] & 0xffff0000u);
+    l[1] = pk_bf16(a, b);
+    a -= bits_f32(l[1] << 16);
+    b -= bits_f32(l[1] & 0xffff0000u);
+    l[2] = pk_bf16(a, b);
 }
 
-// One operand's tile [BI indexes][BK k]: global -> registers -> shared memory, as 16-byte chunks of 8 consecutive k.  Chunk c of
-// index i lies in slot c ^ f(i) of its row, f chosen so that the 8 lanes a 16-byte LDS access serves together touch all banks.
-template <int DT, int LAY, int BI, int BK, int NT>
-struct Tile {
-    static constexpr int LIMBS = (DT == BS_DT_F32 && LAY != L_P8) ? 3 : 1;
-    static constexpr int SL = BK / 8, RL = 8 / SL;
-    static constexpr int BYTES = LIMBS * BI * BK * 2;
-    static constexpr int UNITS = LAY == L_KC ? BI * SL : BI / 4 * SL;
-    static constexpr int PER = (UNITS + NT - 1) / NT;
-    static constexpr int ES = esize(DT);
-    static constexpr int RAWN = LAY == L_KC ? (DT == BS_DT_F32 ? 8 : 4) : LAY == L_IC ? (DT == BS_DT_F32 ? 32 : 16) : 16;
-    uint32_t raw[PER][RAWN];
-
-    static __device__ __forceinline__ int slot(int i, int c) { return c ^ (((i / RL) ^ (LAY == L_KC ? 0 : i >> 3)) & (SL - 1)); }
-    static __device__ __forceinline__ int lds_at(int limb, int i, int c) { return ((limb * BI + i) * SL + slot(i, c)) * 16; }
-
-    __device__ __forceinline__ void load(const GemmArgs& a, const char* base, int64_t ld, int64_t ni, int64_t i0, int64_t k0, int64_t k1,
-                                         int tid) {
+// all limb products of a 16-deep block, small ones first: ONE order for every kernel here, so that which kernel takes a product
+// does not show in its bits
+template <int DT, int LP, int LQ, int NP, int NQ>
+__device__ __forceinline__ void multiply(const u32x4 (&fp)[NP][LP], const u32x4 (&fq)[NQ][LQ], f32x16 (&acc)[NP][NQ]) {
 #pragma unroll
-        for (int n = 0; n < PER; ++n) {
-            const int u = tid + n * NT;
-            if (UNITS % NT != 0 && u >= UNITS) break;
-            if (LAY == L_KC) {
-                int64_t i = i0 + u / SL;
-                i = i < ni ? i : ni - 1;                       // rows behind the last: any row, their sums are not stored
-                const int64_t k = k0 + (u % SL) * 8;
-                const char* p = base + (i * ld + k) * ES;
-                const int64_t left = k1 - k;
-                if (left >= 8) {
-                    const u32x4 v = load16(p);
-                    raw[n][0] = v[0]; raw[n][1] = v[1]; raw[n][2] = v[2]; raw[n][3] = v[3];
-                    if (DT == BS_DT_F32) {
-                        const u32x4 w = load16(p + 16);
-                        raw[n][4 % RAWN] = w[0]; raw[n][5 % RAWN] = w[1]; raw[n][6 % RAWN] = w[2]; raw[n][7 % RAWN] = w[3];
-                    }
-                } else {
+    for (int o = LP + LQ > 2 ? 2 : 0; o >= 0; --o)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        uint32_t v = 0;
-                        if (e < left) v = DT == BS_DT_F32 ? *reinterpret_cast<const uint32_t*>(p + e * 4) : *reinterpret_cast<const uint16_t*>(p + e * 2);
-                        if (DT == BS_DT_F32) raw[n][e % RAWN] = v;
-                        else raw[n][e / 2] = e % 2 ? (raw[n][e / 2] | (v << 16)) : v;
-                    }
-                }
-            } else {
-                const int64_t i = i0 + (u % (BI / 4)) * 4;
-                const int64_t kb = k0 + (u / (BI / 4)) * 8;
-                const bool whole = i + 4 <= ni;
+        for (int l = 0; l < LP; ++l) {
+            if (o - l < 0 || o - l >= LQ) continue;
 #pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    const int64_t k = kb + r < k1 ? kb + r : k1 - 1;           // rows behind the last: zeroed below
-                    const bool live = kb + r < k1;
-                    if (LAY == L_P8) {
-                        const char* p = base + k * ld + i;
-                        uint32_t v = 0, e = 0;
-                        if (whole) {
-                            v = load4(p);
-                        } else {
+            for (int i = 0; i < NP; ++i)
 #pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                if (i + j < ni) v |= (uint32_t)(uint8_t)p[j] << (8 * j);
-                        }
-                        if (i < ni) e = (uint32_t)(int)a.Pexp[k * a.lpe + i / P8_BLOCK];
-                        raw[n][r] = live ? v : 0;
-                        raw[n][(8 + r) % RAWN] = e;
-                    } else {
-                        const char* p = base + (k * ld + i) * ES;
-                        uint32_t v[4] = {0, 0, 0, 0};
-                        if (whole) {
-                            if (DT == BS_DT_F32) {
-                                const u32x4 t = load16(p);
-                                v[0] = t[0]; v[1] = t[1]; v[2] = t[2]; v[3] = t[3];
-                            } else {
-                                const u32x2 t = load8(p);
-                                v[0] = t[0]; v[1] = t[1];
-                            }
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                if (i + j < ni) {
-                                    if (DT == BS_DT_F32) v[j] = *reinterpret_cast<const uint32_t*>(p + j * 4);
-                                    else v[j / 2] |= (uint32_t) * reinterpret_cast<const uint16_t*>(p + j * 2) << (16 * (j % 2));
-                                }
-                        }
-                        constexpr int W = DT == BS_DT_F32 ? 4 : 2;
-#pragma unroll
-                        for (int j = 0; j < W; ++j) raw[n][(r * W + j) % RAWN] = live ? v[j] : 0;
-                    }
-                }
-            }
+                for (int j = 0; j < NQ; ++j) acc[i][j] = mfma<DT>(fp[i][l], fq[j][(o - l >= 0 && o - l < LQ) ? o - l : 0], acc[i][j]);
         }
-    }
+}
 
-    __device__ __forceinline__ void put(char* lds, int i, int c, const float* f) const {      // 8 floats of consecutive k
-        if (LIMBS == 3) {
-            u32x4 l[3];
-            limbs3(f, l);
-#pragma unroll
-            for (int b = 0; b < 3; ++b) *reinterpret_cast<u32x4*>(lds + lds_at(b, i, c)) = l[b];
-        } else {
-            u32x4 v;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = DT == BS_DT_F16 ? pk_f16(f[2 * j], f[2 * j + 1]) : pk_bf16(f[2 * j], f[2 * j + 1]);
-            *reinterpret_cast<u32x4*>(lds + lds_at(0, i, c)) = v;
-        }
-    }
-
-    __device__ __forceinline__ void store(char* lds, int tid) const {
-#pragma unroll
-        for (int n = 0; n < PER; ++n) {
-            const int u = tid + n * NT;
-            if (UNITS % NT != 0 && u >= UNITS) break;
-            if (LAY == L_KC) {
-                const int i = u / SL, c = u % SL;
-                if (DT == BS_DT_F32) {
-                    float f[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] = bits_f32(raw[n][e % RAWN]);
-                    put(lds, i, c, f);
-                } else {
-                    const u32x4 v = {raw[n][0], raw[n][1], raw[n][2], raw[n][3]};
-                    *reinterpret_cast<u32x4*>(lds + lds_at(0, i, c)) = v;
-                }
-            } else {
-                const int i = (u % (BI / 4)) * 4, c = u / (BI / 4);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (LAY == L_P8) {
-                        float f[8];
-#pragma unroll
-                        for (int r = 0; r < 8; ++r)
-                            f[r] = p8_value((int)(int8_t)(raw[n][r] >> (8 * j)), p8_pow2((int)raw[n][(8 + r) % RAWN]));
-                        put(lds, i + j, c, f);
-                    } else if (DT == BS_DT_F32) {
-                        float f[8];
-#pragma unroll
-                        for (int r = 0; r < 8; ++r) f[r] = bits_f32(raw[n][(r * 4 + j) % RAWN]);
-                        put(lds, i + j, c, f);
-                    } else {
-                        u32x4 v;
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const uint32_t lo = raw[n][(4 * r + j / 2) % RAWN], hi = raw[n][(4 * r + 2 + j / 2) % RAWN];
-                            v[r] = j % 2 ? ((lo >> 16) | (hi & 0xffff0000u)) : ((lo & 0xffffu) | (hi << 16));
-                        }
-                        *reinterpret_cast<u32x4*>(lds + lds_at(0, i + j, c)) = v;
-                    }
-                }
-            }
-        }
-    }
+struct RowsArgs {
+    const char *x, *w;                 // operands as the caller holds them
+    int64_t ldx, ldw;
+    const char* wl;                    // w as the kernel reads it: [limb][N][kp] 16-bit, zero behind K; or w itself
+    int64_t ldl, limb_stride;          // in elements
+    int64_t rows;
+    int K, N;
+    int wt;                            // w is [K, N] (the gradient of x)
+    int tp;
+    int64_t tiles;
+    const char *bias, *res;
+    int64_t ldr;
+    char *sum, *act_out;               // E_PLAIN: sum
+    int act, bias_f32;
 };
 
-// operand element as float, for the sums that are added up again (float32 only)
-template <int DT, int LAY>
-__device__ __forceinline__ float element(const GemmArgs& a, const char* base, int64_t ld, int64_t i, int64_t k) {
-    if (LAY == L_KC) return load1<DT>(base + (i * ld + k) * esize(DT));
-    if (LAY == L_IC) return load1<DT>(base + (k * ld + i) * esize(DT));
-    return p8_value((int)(int8_t)base[k * ld + i], p8_pow2((int)a.Pexp[k * a.lpe + i / P8_BLOCK]));
+// the sum once more, in float32 arithmetic
+template <int DT>
+__device__ __forceinline__ float again(const RowsArgs& a, int64_t q, int64_t p) {
+    float s = 0.0f;
+    for (int k = 0; k < a.K; ++k)
+        s = fmaf(load1<DT>(a.w + (a.wt ? (int64_t)k * a.ldw + p : p * a.ldw + k) * esize(DT)), load1<DT>(a.x + (q * a.ldx + k) * esize(DT)), s);
+    return s;
 }
 
-template <int DT, int PLAY, int QLAY, int EPI, int BP, int BQ, int WP, int WQ, int BK>
-__global__ __launch_bounds__((BP / WP) * (BQ / WQ) * 64) void k_rows_gemm(const GemmArgs a) {
-    constexpr int NT = (BP / WP) * (BQ / WQ) * 64;
-    typedef Tile<DT, PLAY, BP, BK, NT> TP;
-    typedef Tile<DT, QLAY, BQ, BK, NT> TQ;
-    constexpr int STAGE = TP::BYTES + TQ::BYTES;
+// what becomes of V neighbouring channels of a row (n of them exist)
+template <int DT, int EPI>
+__device__ __forceinline__ void finish(const RowsArgs& a, int64_t q, int64_t p, int n, float* v) {
+    constexpr int V = vlen(DT), ES = esize(DT);
+    if (DT == BS_DT_F32) {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if ((f32_bits(v[e]) & 0x7f800000u) == 0x7f800000u && e < n) v[e] = again<DT>(a, q, p + e);
+    }
+    const int64_t at = (q * a.N + p) * ES;
+    if (EPI == E_LAYER) {
+        float t[V];
+        if (a.bias) {
+            if (DT != BS_DT_F32 && a.bias_f32) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) t[e] = e < n ? reinterpret_cast<const float*>(a.bias)[p + e] : 0.0f;
+            } else {
+                load_vec<DT>(a.bias + p * ES, n, t);
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] += t[e];
+        }
+        if (a.res) {
+            load_vec<DT>(a.res + (q * a.ldr + p) * ES, n, t);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] += t[e];
+        }
+        if (a.sum) store_vec<DT>(a.sum + at, n, v);
+        if (a.act_out) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) t[e] = act_value(a.act, v[e]);
+            store_vec<DT>(a.act_out + at, n, t);
+        }
+    } else {
+        store_vec<DT>(a.sum + at, n, v);
+    }
+}
+
+// A wavefront's 32 rows x 64 channels from the registers of the matrix instruction to rows of memory, by way of its own piece of
+// shared memory (row stride 68 floats: 16 lanes of a 16-byte access touch all banks): whole 16-byte accesses, 128 or 256 bytes of a
+// row side by side.
+constexpr int TURN = 32 * 68 * 4;
+template <int DT, int EPI>
+__device__ __forceinline__ void turn_and_finish(const RowsArgs& a, const f32x16& a0, const f32x16& a1, float* mine, int lane, int64_t q0,
+                                                int64_t p0, bool two) {
+    constexpr int V = vlen(DT), LPR = 64 / V;                // lanes per row of 64 channels
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const f32x4 v0 = {a0[4 * g], a0[4 * g + 1], a0[4 * g + 2], a0[4 * g + 3]};
+        const f32x4 v1 = {a1[4 * g], a1[4 * g + 1], a1[4 * g + 2], a1[4 * g + 3]};
+        float* const at = mine + (lane & 31) * 68 + 8 * g + 4 * (lane >> 5);
+        *reinterpret_cast<f32x4*>(at) = v0;
+        if (two) *reinterpret_cast<f32x4*>(at + 32) = v1;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int c = (lane % LPR) * V;
+    const int64_t p = p0 + c;
+    const int64_t left = (two ? a.N : (a.N < p0 + 32 ? a.N : p0 + 32)) - p;
+    if (left > 0) {
+#pragma unroll 2
+        for (int r = lane / LPR; r < 32; r += 64 / LPR) {
+            if (q0 + r >= a.rows) break;
+            float v[V];
+#pragma unroll
+            for (int e = 0; e < V; e += 4) {
+                const f32x4 t = *reinterpret_cast<const f32x4*>(mine + r * 68 + c + e);
+                v[e] = t[0]; v[e + 1] = t[1]; v[e + 2] = t[2]; v[e + 3] = t[3];
+            }
+            finish<DT, EPI>(a, q0 + r, p, left < V ? (int)left : V, v);
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// ---- forward and dx, many rows ------------------------------------------------------------------------------------------------
+// Tile of BQ rows x BP channels, BK deep steps through two buffers of shared memory.  Rows of BK k lie there as 16-byte chunks of 8,
+// chunk c in slot c ^ f(row), f such that the 8 lanes a 16-byte access serves together touch all banks.  w comes by DMA (laid out
+// for it: whole steps, zero behind K); x by DMA too where its rows allow (XD: 16-bit, rows of whole aligned chunks), else through
+// registers, where float32 is split.
+template <int DT, int EPI, bool XD, int BQ, int BP, int WQ, int WP, int BK>
+__global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_rows(const RowsArgs a) {
+    constexpr int NW = (BQ / WQ) * (BP / WP), NT = NW * 64, L = limbs_of(DT), ES = esize(DT);
+    constexpr int SL = BK / 8, RB = BK * 2;                    // chunks and bytes of a row
+    constexpr int XB = L * BQ * RB, WB = L * BP * RB, STAGE = XB + WB;
     constexpr int NP = WP / 32, NQ = WQ / 32;
+    static_assert(2 * STAGE <= 160 * 1024 && NW * TURN <= 2 * STAGE && (NP == 2 || NP == 4), "shared memory");
     __shared__ __align__(16) char lds[2 * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wp = wave % (BP / WP), wq = wave / (BP / WP);
+    auto swz = [](int row, int c) { return SL == 8 ? (c ^ (row & 7)) : (c ^ ((row >> 1) & 3)); };
 
-    // workgroups of one XCD (blockIdx % 8) take a run of tiles, p fastest: the rows of Q that several p tiles read are in its L2
+    // workgroups of one XCD (blockIdx % 8) take a run of tiles, channels fastest: rows that several tiles read are in its L2
     const int64_t per = (a.tiles + 7) / 8;
     const int64_t t = (blockIdx.x % 8) * per + blockIdx.x / 8;
-    if (blockIdx.x / 8 >= per || t >= a.tiles) return;
-    const int64_t p0 = (t % a.tp) * BP, q0 = (t / a.tp) * BQ;
-    const int64_t kb = blockIdx.y * a.kpart;
-    const int64_t ke = kb + a.kpart < a.nk ? kb + a.kpart : a.nk;
+    if (t >= a.tiles) return;
+    const int64_t q0 = t / a.tp * BQ;
+    const int p0 = (int)(t % a.tp) * BP;
+    const int steps = (a.K + BK - 1) / BK;
+
+    // DMA: a wavefront's instruction fills 1 KB, 64 / SL rows
+    constexpr int WI = WB / 1024, XI = XB / 1024;
+    auto dma_w = [&](int s, char* st) {
+#pragma unroll
+        for (int n = 0; n < (WI + NW - 1) / NW; ++n) {
+            const int i = wave + n * NW;
+            if (WI % NW != 0 && i >= WI) break;
+            const int r = i * (64 / SL) + lane / SL, limb = r / BP, row = r % BP;
+            const int p = p0 + row < a.N ? p0 + row : a.N - 1;         // channels behind the last: not stored
+            const char* const src = a.wl + ((int64_t)limb * a.limb_stride + (int64_t)p * a.ldl + (int64_t)s * BK + swz(row, lane % SL) * 8) * 2;
+            __builtin_amdgcn_global_load_lds(src, (lds_ptr)(st + XB + i * 1024), 16, 0, 0);
+        }
+    };
+    auto dma_x = [&](int s, char* st) {
+#pragma unroll
+        for (int n = 0; n < (XI + NW - 1) / NW; ++n) {
+            const int i = wave + n * NW;
+            if (XI % NW != 0 && i >= XI) break;
+            const int row = i * (64 / SL) + lane / SL, c = swz(row, lane % SL);
+            const int64_t q = q0 + row < a.rows ? q0 + row : a.rows - 1;
+            const int k = s * BK + c * 8;
+            if (k < a.K) __builtin_amdgcn_global_load_lds(a.x + (q * a.ldx + k) * 2, (lds_ptr)(st + i * 1024), 16, 0, 0);
+            else *reinterpret_cast<u32x4*>(st + i * 1024 + lane * 16) = u32x4{0, 0, 0, 0};      // behind K: zero
+        }
+    };
+    // registers: float32 four values a unit (8 units a row: 128 bytes side by side), 16-bit eight
+    constexpr int UPR = DT == BS_DT_F32 ? BK / 4 : SL, UNITS = BQ * UPR, XN = XD ? 1 : UNITS / NT;
+    u32x4 xr[XN];
+    auto load_x = [&](int s) {
+#pragma unroll
+        for (int n = 0; n < XN; ++n) {
+            const int u = tid + n * NT, row = u / UPR;
+            const int64_t q = q0 + row < a.rows ? q0 + row : a.rows - 1;
+            constexpr int V = vlen(DT);
+            const int k = s * BK + (u % UPR) * V, left = a.K - k;
+            const char* const src = a.x + (q * a.ldx + k) * ES;
+            if (left >= V) {
+                xr[n] = load16(src);
+            } else {
+                u32x4 v = {0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (e < left) {
+                        if (DT == BS_DT_F32) v[e % 4] = *reinterpret_cast<const uint32_t*>(src + e * 4);
+                        else v[e / 2] |= (uint32_t) * reinterpret_cast<const uint16_t*>(src + e * 2) << (16 * (e % 2));
+                    }
+                xr[n] = v;
+            }
+        }
+    };
+    auto store_x = [&](char* st) {
+#pragma unroll
+        for (int n = 0; n < XN; ++n) {
+            const int u = tid + n * NT, row = u / UPR, c = u % UPR;
+            if (DT == BS_DT_F32) {
+                uint32_t lo[3], hi[3];
+                limbs2(bits_f32(xr[n][0]), bits_f32(xr[n][1]), lo);
+                limbs2(bits_f32(xr[n][2]), bits_f32(xr[n][3]), hi);
+#pragma unroll
+                for (int l = 0; l < L; ++l)
+                    *reinterpret_cast<u32x2*>(st + (l * BQ + row) * RB + swz(row, c / 2) * 16 + (c & 1) * 8) = u32x2{lo[l % 3], hi[l % 3]};
+            } else {
+                *reinterpret_cast<u32x4*>(st + row * RB + swz(row, c) * 16) = xr[n];
+            }
+        }
+    };
 
     f32x16 acc[NP][NQ];
 #pragma unroll
@@ -243,119 +257,458 @@ __global__ __launch_bounds__((BP / WP) * (BQ / WQ) * 64) void k_rows_gemm(const 
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
 
-    TP tp;
-    TQ tq;
-    tp.load(a, a.P, a.ldp, a.np, p0, kb, ke, tid);
-    tq.load(a, a.Q, a.ldq, a.nq, q0, kb, ke, tid);
-    int buf = 0;
-    for (int64_t k = kb; k < ke; k += BK) {
-        char* const lp = lds + buf * STAGE;
-        char* const lq = lp + TP::BYTES;
-        tp.store(lp, tid);
-        tq.store(lq, tid);
-        __syncthreads();          // one barrier a step: the buffer written next was read before the previous barrier
-        if (k + BK < ke) {
-            tp.load(a, a.P, a.ldp, a.np, p0, k + BK, ke, tid);
-            tq.load(a, a.Q, a.ldq, a.nq, q0, k + BK, ke, tid);
+    if (!XD) load_x(0);
+    dma_w(0, lds);
+    if (XD) dma_x(0, lds);
+    else store_x(lds);
+    for (int s = 0; s < steps; ++s) {
+        char* const cur = lds + (s & 1) * STAGE;
+        char* const nxt = lds + ((s & 1) ^ 1) * STAGE;
+        __syncthreads();                        // this step has landed; the other buffer's readers are done
+        const bool more = s + 1 < steps;
+        if (more) {
+            if (!XD) load_x(s + 1);
+            dma_w(s + 1, nxt);
+            if (XD) dma_x(s + 1, nxt);
         }
 #pragma unroll
-        for (int s = 0; s < BK / 16; ++s) {
-            u32x4 fp[NP][TP::LIMBS], fq[NQ][TQ::LIMBS];
-            const int c = 2 * s + (lane >> 5);
+        for (int b = 0; b < BK / 16; ++b) {
+            u32x4 fp[NP][L], fq[NQ][L];
+            const int c = 2 * b + (lane >> 5);
 #pragma unroll
-            for (int i = 0; i < NP; ++i)
+            for (int i = 0; i < NP; ++i) {
+                const int row = wp * WP + i * 32 + (lane & 31);
 #pragma unroll
-                for (int l = 0; l < TP::LIMBS; ++l)
-                    fp[i][l] = *reinterpret_cast<const u32x4*>(lp + TP::lds_at(l, wp * WP + i * 32 + (lane & 31), c));
+                for (int l = 0; l < L; ++l) fp[i][l] = *reinterpret_cast<const u32x4*>(cur + XB + (l * BP + row) * RB + swz(row, c) * 16);
+            }
 #pragma unroll
-            for (int j = 0; j < NQ; ++j)
+            for (int j = 0; j < NQ; ++j) {
+                const int row = wq * WQ + j * 32 + (lane & 31);
 #pragma unroll
-                for (int l = 0; l < TQ::LIMBS; ++l)
-                    fq[j][l] = *reinterpret_cast<const u32x4*>(lq + TQ::lds_at(l, wq * WQ + j * 32 + (lane & 31), c));
-            // limb products of total order <= 2, small ones first: what is left out is of relative size 2^-24
-#pragma unroll
-            for (int o = TP::LIMBS + TQ::LIMBS > 2 ? 2 : 0; o >= 0; --o)
-#pragma unroll
-                for (int lp_ = 0; lp_ < TP::LIMBS; ++lp_)
-#pragma unroll
-                    for (int i = 0; i < NP; ++i)
-#pragma unroll
-                        for (int j = 0; j < NQ; ++j)
-                            if (o - lp_ >= 0 && o - lp_ < TQ::LIMBS)
-                                acc[i][j] = mfma<DT>(fp[i][lp_], fq[j][(o - lp_ >= 0 && o - lp_ < TQ::LIMBS) ? o - lp_ : 0], acc[i][j]);
+                for (int l = 0; l < L; ++l) fq[j][l] = *reinterpret_cast<const u32x4*>(cur + (l * BQ + row) * RB + swz(row, c) * 16);
+            }
+            multiply<DT, L, L, NP, NQ>(fp, fq, acc);
         }
-        buf ^= 1;
+        if (more && !XD) store_x(nxt);
     }
+    __syncthreads();
+    float* const mine = reinterpret_cast<float*>(lds + wave * TURN);
+#pragma unroll
+    for (int j = 0; j < NQ; ++j)
+#pragma unroll
+        for (int i = 0; i < NP; i += 2)
+            turn_and_finish<DT, EPI>(a, acc[i][j], acc[i + 1][j], mine, lane, q0 + wq * WQ + j * 32, p0 + wp * WP + i * 32, true);
+}
 
-    // lane l holds, for q = l % 32 of a 32x32 tile, the p of rows 8 g + 4 (l / 32) + 0..3, g = 0..3: four channels side by side
+// ---- forward and dx, few rows -------------------------------------------------------------------------------------------------
+// One 32x32 tile a workgroup.  Its four wavefronts hold four runs of k in registers, loaded at once straight from memory, and pass
+// the sums on from run to run (a relay): the order of k_rows, at the latency of about one load.
+template <int DT, int EPI, bool WL>
+__global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {
+    constexpr int L = limbs_of(DT), NS = DT == BS_DT_F32 ? 4 : 8, ES = esize(DT), RUN = NS * 16;
+    __shared__ __align__(16) char lds[TURN];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t q0 = blockIdx.x / a.tp * 32;
+    const int p0 = (int)(blockIdx.x % a.tp) * 32;
+    const int64_t q = q0 + (lane & 31) < a.rows ? q0 + (lane & 31) : a.rows - 1;
+    const int p = p0 + (lane & 31) < a.N ? p0 + (lane & 31) : a.N - 1;
+    const char* const xp = a.x + q * a.ldx * ES;
+    const char* const wp = WL ? a.wl + (int64_t)p * a.ldl * 2 : a.w + (int64_t)p * a.ldw * ES;
+    f32x16 acc;
 #pragma unroll
-    for (int j = 0; j < NQ; ++j) {
-        const int64_t q = q0 + wq * WQ + j * 32 + (lane & 31);
-        if (q >= a.nq) continue;
+    for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
+    constexpr int RAW = DT == BS_DT_F32 ? 2 : 1;
+    auto fetch = [&](const char* base, int k, u32x4* r) {          // 8 values from k on, zero behind K
+        const int left = a.K - k;
+        if (left >= 8) {
+            r[0] = load16(base + (int64_t)k * ES);
+            if (RAW == 2) r[RAW - 1] = load16(base + (int64_t)k * ES + 16);
+        } else {
 #pragma unroll
-        for (int i = 0; i < NP; ++i)
+            for (int n = 0; n < RAW; ++n) r[n] = u32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int64_t p = p0 + wp * WP + i * 32 + 8 * g + 4 * (lane >> 5);
-                if (p >= a.np) continue;
-                const int n = a.np - p < 4 ? (int)(a.np - p) : 4;
-                float v[4];
+            for (int e = 0; e < 8; ++e)
+                if (e < left) {
+                    if (DT == BS_DT_F32) r[(e / 4) % RAW][e % 4] = *reinterpret_cast<const uint32_t*>(base + (int64_t)(k + e) * ES);
+                    else r[0][e / 2] |= (uint32_t) * reinterpret_cast<const uint16_t*>(base + (int64_t)(k + e) * ES) << (16 * (e % 2));
+                }
+        }
+    };
+    auto split = [&](const u32x4* r, u32x4* l) {
+        if (DT == BS_DT_F32) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v[e] = acc[i][j][4 * g + e];
-                    if (DT == BS_DT_F32 && e < n && (f32_bits(v[e]) & 0x7f800000u) == 0x7f800000u) {
-                        // an infinity or a NaN among the operands (or a limb that overflowed): the sum again, in float32
-                        float s = 0.0f;
-                        for (int64_t k = kb; k < ke; ++k)
-                            s = fmaf(element<DT, PLAY>(a, a.P, a.ldp, p + e, k), element<DT, QLAY>(a, a.Q, a.ldq, q, k), s);
-                        v[e] = s;
+            for (int n = 0; n < 4; ++n) {
+                uint32_t t[3];
+                limbs2(bits_f32(r[(n / 2) % RAW][2 * (n & 1)]), bits_f32(r[(n / 2) % RAW][2 * (n & 1) + 1]), t);
+#pragma unroll
+                for (int b = 0; b < L; ++b) l[b][n] = t[b];
+            }
+        } else {
+            l[0] = r[0];
+        }
+    };
+    for (int k0 = 0; k0 < a.K; k0 += 4 * RUN) {
+        u32x4 xr[NS][RAW], wr[NS][WL ? L : RAW];
+        const int kb = k0 + wave * RUN + 8 * (lane >> 5);
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            const int k = kb + n * 16;
+            fetch(xp, k, xr[n]);
+            if (WL) {
+#pragma unroll
+                for (int l = 0; l < L; ++l)
+                    wr[n][l] = k < a.ldl ? load16(wp + ((int64_t)l * a.limb_stride + k) * 2) : u32x4{0, 0, 0, 0};
+            } else {
+                fetch(wp, k, wr[n]);
+            }
+        }
+        for (int turn = 0; turn < 4; ++turn) {
+            if (turn == wave && k0 + wave * RUN < a.K) {
+                if (k0 + turn > 0) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const f32x4 t = *reinterpret_cast<const f32x4*>(lds + (e * 64 + lane * 4) * 4);
+                        acc[e] = t[0]; acc[e + 1] = t[1]; acc[e + 2] = t[2]; acc[e + 3] = t[3];
                     }
                 }
-                if (EPI == E_PART) {
-                    float* o = reinterpret_cast<float*>(a.out0) + ((int64_t)blockIdx.y * a.nq + q) * a.np + p;
+#pragma unroll
+                for (int n = 0; n < NS; ++n) {
+                    u32x4 fp[1][L], fq[1][L];
+                    if (WL) {
+#pragma unroll
+                        for (int l = 0; l < L; ++l) fp[0][l] = wr[n][l % (WL ? L : RAW)];
+                    } else {
+                        split(wr[n], fp[0]);
+                    }
+                    split(xr[n], fq[0]);
+                    f32x16 one[1][1] = {{acc}};
+                    multiply<DT, L, L, 1, 1>(fp, fq, one);
+                    acc = one[0][0];
+                }
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<f32x4*>(lds + (e * 64 + lane * 4) * 4) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+            }
+            __syncthreads();
+        }
+    }
+    // the sums lie in shared memory as the last wavefront left them; every wavefront finishes 8 of the 32 rows
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+        const f32x4 t = *reinterpret_cast<const f32x4*>(lds + (e * 64 + lane * 4) * 4);
+        acc[e] = t[0]; acc[e + 1] = t[1]; acc[e + 2] = t[2]; acc[e + 3] = t[3];
+    }
+    __syncthreads();
+    float* const turn = reinterpret_cast<float*>(lds);
+    if (wave == 0) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f32x4*>(turn + (lane & 31) * 68 + 8 * g + 4 * (lane >> 5)) = f32x4{acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+    }
+    __syncthreads();
+    constexpr int V = vlen(DT), LPR = 32 / V;
+    for (int r = threadIdx.x / LPR; r < 32; r += 256 / LPR) {
+        const int c = (threadIdx.x % LPR) * V, left = a.N - p0 - c;
+        if (q0 + r >= a.rows || left <= 0) break;
+        float v[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = turn[r * 68 + c + e];
+        finish<DT, EPI>(a, q0 + r, p0 + c, left < V ? left : V, v);
+    }
+}
+
+// ---- w laid out for the kernels above -------------------------------------------------------------------------------------------
+// out [limb][P][kp] 16-bit: w [P, K], or with TURNED w [K, P] turned round; zero from K to kp
+template <int DT, bool TURNED>
+__global__ __launch_bounds__(256) void k_lay_w(const char* __restrict__ w, int64_t ldw, int P, int K, int kp, char* __restrict__ out) {
+    constexpr int ES = esize(DT), L = limbs_of(DT);
+    __shared__ uint32_t tile[32][33];
+    const int p0 = blockIdx.y * 32, k0 = blockIdx.x * 64;
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {                       // 32 p x 32 k at a time
+        const int kb = k0 + half * 32;
+        __syncthreads();
+        for (int r = ty; r < 32; r += 8) {
+            const int p = TURNED ? p0 + tx : p0 + r, k = TURNED ? kb + r : kb + tx;
+            uint32_t v = 0;
+            if (p < P && k < K) {
+                const char* const src = w + (TURNED ? (int64_t)k * ldw + p : (int64_t)p * ldw + k) * ES;
+                v = DT == BS_DT_F32 ? *reinterpret_cast<const uint32_t*>(src) : *reinterpret_cast<const uint16_t*>(src);
+            }
+            tile[TURNED ? tx : r][TURNED ? r : tx] = v;
+        }
+        __syncthreads();
+        // two k a thread: words of a row side by side
+        for (int u = threadIdx.x; u < 32 * 16; u += 256) {
+            const int r = u >> 4, k2 = (u & 15) * 2, p = p0 + r;
+            if (p >= P || kb + k2 >= kp) continue;
+            uint32_t l[3];
+            if (DT == BS_DT_F32) limbs2(bits_f32(tile[r][k2]), bits_f32(tile[r][k2 + 1]), l);
+            else l[0] = tile[r][k2] | (tile[r][k2 + 1] << 16);
+#pragma unroll
+            for (int b = 0; b < L; ++b) *reinterpret_cast<uint32_t*>(out + (((int64_t)b * P + p) * kp + kb + k2) * 2) = l[b];
+        }
+    }
+}
+
+// ---- dw -------------------------------------------------------------------------------------------------------------------------
+struct OverArgs {
+    const char *x, *ds;
+    const int8_t* exps;
+    int64_t ldx, ldds, rows, part;
+    int K, N, nb, parts;
+    int tp;
+    int64_t tiles;                     // tiles x parts
+    char* out;
+};
+enum { S_DMA = 0, S_REG = 1, S_P8 = 2 };
+
+// One operand's tile of BK rows x 128 channels as it lies in memory; 16-byte chunk c of row r in slot c ^ 2 (r & 3), so that the
+// four rows a transposing read takes 32 bytes of lie in different banks.
+template <int DT, int SRC, int BK>
+struct Strip {
+    static constexpr int L = (DT == BS_DT_F32 && SRC != S_P8) ? 3 : 1;
+    static constexpr int BYTES = L * BK * 256;
+    static constexpr int ES = SRC == S_P8 ? 1 : esize(DT);
+    static constexpr int V = SRC == S_P8 ? 8 : vlen(DT);                         // channels of a unit
+    static constexpr int UPR = 128 / V, UNITS = BK * UPR, N = SRC == S_DMA ? 1 : UNITS / 256;
+    u32x4 raw[N];
+    float step[SRC == S_P8 ? N : 1];
+
+    static __device__ __forceinline__ int at(int limb, int row, int c) { return (limb * BK + row) * 256 + ((c ^ (2 * (row & 3))) * 16); }
+
+    __device__ __forceinline__ void dma(const char* base, int64_t ld, int ni, int i0, int64_t k, int64_t ke, char* st, int wave, int lane) const {
+#pragma unroll
+        for (int n = 0; n < BYTES / 4096; ++n) {
+            const int i = wave + n * 4, row = i * 4 + lane / 16, c = (lane % 16) ^ (2 * (row & 3));
+            int ch = i0 + c * 8;
+            ch = ch < ni ? ch : i0;                                              // channels behind the last: not stored
+            if (k + row < ke) __builtin_amdgcn_global_load_lds(base + ((k + row) * ld + ch) * 2, (lds_ptr)(st + i * 1024), 16, 0, 0);
+            else *reinterpret_cast<u32x4*>(st + i * 1024 + lane * 16) = u32x4{0, 0, 0, 0};       // rows behind the last
+        }
+    }
+    __device__ __forceinline__ void load(const OverArgs& a, const char* base, int64_t ld, int ni, int i0, int64_t k, int64_t ke, int tid) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int u = tid + n * 256, row = u / UPR, ch = i0 + (u % UPR) * V, left = ni - ch;
+            u32x4 v = {0, 0, 0, 0};
+            if (SRC == S_P8) step[n % (SRC == S_P8 ? N : 1)] = 0.0f;
+            if (k + row < ke && left > 0) {
+                const char* const src = base + ((k + row) * ld + ch) * ES;
+                if (SRC == S_P8) step[n % (SRC == S_P8 ? N : 1)] = p8_pow2(a.exps[(k + row) * a.nb + ch / P8_BLOCK]);
+                if (left >= V) {
+                    if (SRC == S_P8) {
+                        const u32x2 t = load8(src);
+                        v[0] = t[0]; v[1] = t[1];
+                    } else {
+                        v = load16(src);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (e < left) {
+                            if (SRC == S_P8) v[e / 4] |= (uint32_t) * reinterpret_cast<const uint8_t*>(src + e) << (8 * (e % 4));
+                            else if (DT == BS_DT_F32) v[e % 4] = *reinterpret_cast<const uint32_t*>(src + e * 4);
+                            else v[e / 2] |= (uint32_t) * reinterpret_cast<const uint16_t*>(src + e * 2) << (16 * (e % 2));
+                        }
+                }
+            }
+            raw[n] = v;
+        }
+    }
+    __device__ __forceinline__ void store(char* st, int tid) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int u = tid + n * 256, row = u / UPR, g = u % UPR;
+            if (SRC == S_P8) {
+                const float s = step[n % (SRC == S_P8 ? N : 1)];
+                u32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t w = raw[n][e / 2] >> (16 * (e & 1));
+                    const float f0 = p8_value((int)(int8_t)w, s), f1 = p8_value((int)(int8_t)(w >> 8), s);
+                    v[e] = DT == BS_DT_F16 ? pk_f16(f0, f1) : pk_bf16(f0, f1);
+                }
+                *reinterpret_cast<u32x4*>(st + at(0, row, g)) = v;
+            } else if (DT == BS_DT_F32) {
+                uint32_t lo[3], hi[3];
+                limbs2(bits_f32(raw[n][0]), bits_f32(raw[n][1]), lo);
+                limbs2(bits_f32(raw[n][2]), bits_f32(raw[n][3]), hi);
+#pragma unroll
+                for (int l = 0; l < L; ++l) *reinterpret_cast<u32x2*>(st + at(l, row, g / 2) + (g & 1) * 8) = u32x2{lo[l % 3], hi[l % 3]};
+            } else {
+                *reinterpret_cast<u32x4*>(st + at(0, row, g)) = raw[n];
+            }
+        }
+    }
+    // the fragment of 32 channels from c0 on and 16 rows from r0 on: lane's channel c0 + lane % 32, rows r0 + 8 (lane / 32) + 0..7.
+    // A transposing read hands each 16 lanes 16 channels of 4 rows; lane i of them points at row i / 4, channels 4 (i % 4).
+    static __device__ __forceinline__ u32x4 fragment(const char* st, int limb, int r0, int c0, int lane) {
+        u32x4 v;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int row = r0 + 8 * (lane >> 5) + 4 * h + ((lane & 15) >> 2), ch = c0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+            const s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(st + at(limb, row, ch >> 3) + (ch & 4) * 2));
+            const u32x2 w = __builtin_bit_cast(u32x2, t);
+            v[2 * h] = w[0];
+            v[2 * h + 1] = w[1];
+        }
+        return v;
+    }
+};
+
+template <int DT, int XS, int DS, int BK>
+__global__ __launch_bounds__(256) void k_over_rows(const OverArgs a) {
+    typedef Strip<DT, XS, BK> TX;
+    typedef Strip<DT, DS, BK> TD;
+    constexpr int STAGE = TX::BYTES + TD::BYTES;
+    __shared__ __align__(16) char lds[2 * STAGE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wp = wave & 1, wq = wave >> 1;
+    const int64_t per = (a.tiles + 7) / 8;
+    const int64_t t = (blockIdx.x % 8) * per + blockIdx.x / 8;        // an XCD takes whole runs of tiles of the same rows
+    if (t >= a.tiles) return;
+    const int64_t tiles = a.tiles / a.parts;
+    const int part = (int)(t / tiles), tile = (int)(t % tiles);
+    const int p0 = tile % a.tp * 128, q0 = tile / a.tp * 128;
+    const int64_t kb = part * a.part, ke = kb + a.part < a.rows ? kb + a.part : a.rows;
+    TX tx;
+    TD td;
+    f32x16 acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+    auto begin = [&](int64_t k, char* st) {
+        if (XS != S_DMA) tx.load(a, a.x, a.ldx, a.K, p0, k, ke, tid);
+        if (DS != S_DMA) td.load(a, a.ds, a.ldds, a.N, q0, k, ke, tid);
+        if (XS == S_DMA) tx.dma(a.x, a.ldx, a.K, p0, k, ke, st, wave, lane);
+        if (DS == S_DMA) td.dma(a.ds, a.ldds, a.N, q0, k, ke, st + TX::BYTES, wave, lane);
+    };
+    auto end = [&](char* st) {
+        if (XS != S_DMA) tx.store(st, tid);
+        if (DS != S_DMA) td.store(st + TX::BYTES, tid);
+    };
+    begin(kb, lds);
+    end(lds);
+    int buf = 0;
+    for (int64_t k = kb; k < ke; k += BK) {
+        char* const cur = lds + buf * STAGE;
+        char* const nxt = lds + (buf ^ 1) * STAGE;
+        __syncthreads();
+        const bool more = k + BK < ke;
+        if (more) begin(k + BK, nxt);
+#pragma unroll
+        for (int b = 0; b < BK / 16; ++b) {
+            u32x4 fp[2][TX::L], fq[2][TD::L];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int l = 0; l < TX::L; ++l) fp[i][l] = TX::fragment(cur, l, b * 16, wp * 64 + i * 32, lane);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int l = 0; l < TD::L; ++l) fq[j][l] = TD::fragment(cur + TX::BYTES, l, b * 16, wq * 64 + j * 32, lane);
+            multiply<DT, TX::L, TD::L, 2, 2>(fp, fq, acc);
+        }
+        if (more) end(nxt);
+        buf ^= 1;
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int q = q0 + wq * 64 + j * 32 + (lane & 31);
+        if (q >= a.N) continue;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int p = p0 + wp * 64 + i * 32 + 8 * g + 4 * (lane >> 5), n = a.K - p;
+                if (n <= 0) continue;
+                f32x4 v = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+                if (DT == BS_DT_F32) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if ((f32_bits(v[e]) & 0x7f800000u) == 0x7f800000u && e < n) {          // the sum again, in float32
+                            float s = 0.0f;
+                            for (int64_t k = kb; k < ke; ++k) {
+                                const float xv = XS == S_P8 ? p8_value((int)(int8_t)a.x[k * a.ldx + p + e], p8_pow2(a.exps[k * a.nb + (p + e) / P8_BLOCK]))
+                                                            : load1<DT>(a.x + (k * a.ldx + p + e) * esize(DT));
+                                s = fmaf(xv, load1<DT>(a.ds + (k * a.ldds + q) * esize(DT)), s);
+                            }
+                            v[e] = s;
+                        }
+                }
+                float* const o = reinterpret_cast<float*>(a.out) + ((int64_t)part * a.N + q) * a.K + p;
+                if (n >= 4) store16((char*)o, __builtin_bit_cast(u32x4, v));
+                else
                     for (int e = 0; e < n; ++e) o[e] = v[e];
-                    continue;
-                }
-                const int64_t at = (q * a.np + p) * esize(DT);
-                if (EPI == E_PLAIN) {
-                    for (int e = 0; e < n; ++e) store1<DT>(a.out0 + at + e * esize(DT), v[e]);
-                    continue;
-                }
-                for (int e = 0; e < n; ++e) {
-                    float s = v[e];
-                    if (a.bias) s += a.bias_f32 ? reinterpret_cast<const float*>(a.bias)[p + e] : load1<DT>(a.bias + (p + e) * esize(DT));
-                    if (a.res) s += load1<DT>(a.res + (q * a.ldr + p + e) * esize(DT));
-                    if (a.out0) store1<DT>(a.out0 + at + e * esize(DT), s);
-                    if (a.out1) store1<DT>(a.out1 + at + e * esize(DT), act_value(a.act, s));
-                }
             }
     }
 }
 
-// parts [nparts][n] float32 -> their sum, part 0 first, in dtype
+// parts [nparts][n] float32 -> their sum in dtype; 64 threads of four neighbours x 4 lanes over the parts
 template <int DT>
 __global__ __launch_bounds__(256) void k_add_parts(const float* __restrict__ parts, int nparts, int64_t n, char* __restrict__ out) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    float s = 0.0f;
-    for (int k = 0; k < nparts; ++k) s += parts[k * n + i];
-    store1<DT>(out + i * esize(DT), s);
+    __shared__ __align__(16) f32x4 red[256];
+    const int64_t i = ((int64_t)blockIdx.x * 64 + (threadIdx.x & 63)) * 4;
+    const int l = threadIdx.x >> 6;
+    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (i + 4 <= n) {
+        for (int k = l; k < nparts; k += 4) {
+            const f32x4 v = __builtin_bit_cast(f32x4, load16((const char*)(parts + k * n + i)));
+            s[0] += v[0]; s[1] += v[1]; s[2] += v[2]; s[3] += v[3];
+        }
+    } else if (i < n) {
+        for (int k = l; k < nparts; k += 4)
+            for (int e = 0; e < n - i; ++e) s[e] += parts[k * n + i + e];
+    }
+    red[threadIdx.x] = s;
+    __syncthreads();
+    if (l || i >= n) return;
+    const f32x4 *r = red + threadIdx.x;
+    for (int e = 0; e < 4 && i + e < n; ++e) store1<DT>(out + (i + e) * esize(DT), (r[0][e] + r[64][e]) + (r[128][e] + r[192][e]));
 }
 
-template <int DT>
-__global__ __launch_bounds__(256) void k_zero(int64_t n, char* __restrict__ out) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < n) store1<DT>(out + i * esize(DT), 0.0f);
-}
+// ---- which way --------------------------------------------------------------------------------------------------------------------
+bool few(int64_t rows, int N) { return (rows + 31) / 32 * ((N + 31) / 32) <= 1024; }
 
-template <int DT, int PLAY, int QLAY, int EPI>
-int launch_gemm(GemmArgs a, int parts, hipStream_t st) {
-    constexpr int BP = 128, BQ = 128, BK = DT == BS_DT_F32 ? 16 : 64;
-    a.tp = (a.np + BP - 1) / BP;
-    a.tiles = (int64_t)a.tp * ((a.nq + BQ - 1) / BQ);
+int64_t lay_bytes(int dtype, int K, int P) { return (int64_t)limbs_of(dtype) * P * ((K + 63) / 64 * 64) * 2; }
+
+// out [rows, N] over K: w [N, K], or [K, N] when turned
+template <int DT, int EPI>
+int launch_rows(RowsArgs a, void* workspace, int64_t bytes, hipStream_t st) {
+    const int kp = (a.K + 63) / 64 * 64;
+    const bool small = few(a.rows, a.N);
+    const bool as_is = DT != BS_DT_F32 && !a.wt && a.K % 64 == 0 && a.ldw % 8 == 0 && ((uintptr_t)a.w & 15) == 0;
+    const bool lay = a.wt || (!small && !as_is);
+    if (lay) {
+        if (!workspace || bytes < lay_bytes(DT, a.K, a.N)) return BS_EINVAL;
+        const dim3 grid((unsigned)(kp / 64), (unsigned)((a.N + 31) / 32));
+        if (a.wt) hipLaunchKernelGGL((k_lay_w<DT, true>), grid, dim3(256), 0, st, a.w, a.ldw, a.N, a.K, kp, (char*)workspace);
+        else hipLaunchKernelGGL((k_lay_w<DT, false>), grid, dim3(256), 0, st, a.w, a.ldw, a.N, a.K, kp, (char*)workspace);
+        a.wl = (const char*)workspace; a.ldl = kp; a.limb_stride = (int64_t)a.N * kp;
+    } else {
+        a.wl = a.w; a.ldl = a.ldw; a.limb_stride = 0;
+    }
+    if (small) {
+        a.tp = (a.N + 31) / 32;
+        const unsigned blocks = (unsigned)((a.rows + 31) / 32 * a.tp);
+        if (lay) hipLaunchKernelGGL((k_relay<DT, EPI, true>), dim3(blocks), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((k_relay<DT, EPI, false>), dim3(blocks), dim3(256), 0, st, a);
+        return rows_rc();
+    }
+    constexpr int BQ = 128, BP = DT == BS_DT_F32 ? 256 : 128, BK = DT == BS_DT_F32 ? 32 : 64;
+    a.tp = (a.N + BP - 1) / BP;
+    a.tiles = (a.rows + BQ - 1) / BQ * a.tp;
     const int64_t blocks = (a.tiles + 7) / 8 * 8;
     if (blocks > 0x7fffffff) return BS_EINVAL;
-    hipLaunchKernelGGL((k_rows_gemm<DT, PLAY, QLAY, EPI, BP, BQ, 64, 64, BK>), dim3((unsigned)blocks, (unsigned)parts), dim3(256), 0, st, a);
+    const dim3 grid((unsigned)blocks);
+    const bool xd = DT != BS_DT_F32 && a.K % 8 == 0 && a.ldx % 8 == 0 && ((uintptr_t)a.x & 15) == 0;
+    constexpr int NT = (BQ / 64) * (BP / 64) * 64;
+    if (DT != BS_DT_F32 && xd) hipLaunchKernelGGL((k_rows<DT, EPI, DT != BS_DT_F32, BQ, BP, 64, 64, BK>), grid, dim3(NT), 0, st, a);
+    else hipLaunchKernelGGL((k_rows<DT, EPI, false, BQ, BP, 64, 64, BK>), grid, dim3(NT), 0, st, a);
     return rows_rc();
 }
 
@@ -371,84 +724,103 @@ void split_rows(int64_t rows, int K, int N, int64_t* part, int64_t* parts) {
     *parts = rows ? (rows + *part - 1) / *part : 1;
 }
 
+template <int DT>
+int launch_over(OverArgs a, hipStream_t st) {
+    constexpr int BK = DT == BS_DT_F32 ? 16 : 64;
+    const int64_t blocks = (a.tiles + 7) / 8 * 8;
+    if (blocks > 0x7fffffff) return BS_EINVAL;
+    const dim3 grid((unsigned)blocks);
+    auto whole = [](const char* p, int64_t ld, int n) { return DT != BS_DT_F32 && n % 8 == 0 && ld % 8 == 0 && ((uintptr_t)p & 15) == 0; };
+    const bool xd = !a.exps && whole(a.x, a.ldx, a.K), dd = whole(a.ds, a.ldds, a.N);
+    constexpr int DMA = DT != BS_DT_F32 ? S_DMA : S_REG;
+    if (a.exps && dd) hipLaunchKernelGGL((k_over_rows<DT, S_P8, DMA, BK>), grid, dim3(256), 0, st, a);
+    else if (a.exps) hipLaunchKernelGGL((k_over_rows<DT, S_P8, S_REG, BK>), grid, dim3(256), 0, st, a);
+    else if (xd && dd) hipLaunchKernelGGL((k_over_rows<DT, DMA, DMA, BK>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_over_rows<DT, S_REG, S_REG, BK>), grid, dim3(256), 0, st, a);
+    return rows_rc();
+}
+
 }  // namespace
 
 extern "C" {
 
+int64_t bs_linear_workspace(int dtype, int64_t rows, int K, int N) {
+    if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1) return BS_EINVAL;
+    return few(rows, N) ? 0 : lay_bytes(dtype, K, N);
+}
+
 int bs_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype, const void* res,
-                  int64_t ldr, void* sum_out, void* act_out, int act, int dtype, int64_t rows, int K, int N, void* stream) {
+                  int64_t ldr, void* sum_out, void* act_out, int act, int dtype, int64_t rows, int K, int N, void* workspace,
+                  int64_t workspace_bytes, void* stream) {
     if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1 || act < BS_ACT_NONE || act > BS_ACT_GELU) return BS_EINVAL;
     if (rows == 0) return BS_OK;
     if (!x || !w || ldx < K || ldw < K || (res && ldr < N) || (!sum_out && !act_out)) return BS_EINVAL;
     if (bias && bias_dtype != BS_DT_F32 && bias_dtype != dtype) return BS_EINVAL;
-    GemmArgs a = {};
-    a.P = (const char*)w; a.ldp = ldw; a.np = N;
-    a.Q = (const char*)x; a.ldq = ldx; a.nq = rows;
-    a.nk = a.kpart = K;
+    RowsArgs a = {};
+    a.x = (const char*)x; a.ldx = ldx; a.w = (const char*)w; a.ldw = ldw; a.rows = rows; a.K = K; a.N = N;
     a.bias = (const char*)bias; a.bias_f32 = bias_dtype == BS_DT_F32;
     a.res = (const char*)res; a.ldr = ldr;
-    a.out0 = (char*)sum_out; a.out1 = (char*)act_out; a.act = act;
+    a.sum = (char*)sum_out; a.act_out = (char*)act_out; a.act = act;
     hipStream_t st = rows_stream(stream);
-    if (dtype == BS_DT_F32) return launch_gemm<BS_DT_F32, L_KC, L_KC, E_LAYER>(a, 1, st);
-    if (dtype == BS_DT_BF16) return launch_gemm<BS_DT_BF16, L_KC, L_KC, E_LAYER>(a, 1, st);
-    return launch_gemm<BS_DT_F16, L_KC, L_KC, E_LAYER>(a, 1, st);
+    if (dtype == BS_DT_F32) return launch_rows<BS_DT_F32, E_LAYER>(a, workspace, workspace_bytes, st);
+    if (dtype == BS_DT_BF16) return launch_rows<BS_DT_BF16, E_LAYER>(a, workspace, workspace_bytes, st);
+    return launch_rows<BS_DT_F16, E_LAYER>(a, workspace, workspace_bytes, st);
+}
+
+int64_t bs_linear_grad_x_workspace(int dtype, int64_t rows, int K, int N) {
+    if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1) return BS_EINVAL;
+    return lay_bytes(dtype, N, K);
 }
 
 int bs_linear_grad_x(const void* ds, int64_t ldds, const void* w, int64_t ldw, void* dx, int dtype, int64_t rows, int K, int N,
-                     void* stream) {
+                     void* workspace, int64_t workspace_bytes, void* stream) {
     if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1) return BS_EINVAL;
     if (rows == 0) return BS_OK;
     if (!ds || !w || !dx || ldds < N || ldw < K) return BS_EINVAL;
-    GemmArgs a = {};
-    a.P = (const char*)w; a.ldp = ldw; a.np = K;
-    a.Q = (const char*)ds; a.ldq = ldds; a.nq = rows;
-    a.nk = a.kpart = N;
-    a.out0 = (char*)dx;
+    RowsArgs a = {};
+    a.x = (const char*)ds; a.ldx = ldds; a.w = (const char*)w; a.ldw = ldw; a.rows = rows; a.K = N; a.N = K; a.wt = 1;
+    a.sum = (char*)dx;
     hipStream_t st = rows_stream(stream);
-    if (dtype == BS_DT_F32) return launch_gemm<BS_DT_F32, L_IC, L_KC, E_PLAIN>(a, 1, st);
-    if (dtype == BS_DT_BF16) return launch_gemm<BS_DT_BF16, L_IC, L_KC, E_PLAIN>(a, 1, st);
-    return launch_gemm<BS_DT_F16, L_IC, L_KC, E_PLAIN>(a, 1, st);
+    if (dtype == BS_DT_F32) return launch_rows<BS_DT_F32, E_PLAIN>(a, workspace, workspace_bytes, st);
+    if (dtype == BS_DT_BF16) return launch_rows<BS_DT_BF16, E_PLAIN>(a, workspace, workspace_bytes, st);
+    return launch_rows<BS_DT_F16, E_PLAIN>(a, workspace, workspace_bytes, st);
 }
 
 int64_t bs_linear_grad_w_workspace(int dtype, int64_t rows, int K, int N) {
     if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1) return BS_EINVAL;
     int64_t part, parts;
     split_rows(rows, K, N, &part, &parts);
-    return parts > 1 ? parts * K * N * 4 : 0;
+    return parts > 1 || dtype != BS_DT_F32 ? parts * K * N * 4 : 0;
 }
 
 int bs_linear_grad_w(const void* ds, int64_t ldds, const void* x, const int8_t* x_exps, int64_t ldx, void* dw, int dtype,
                      int64_t rows, int K, int N, void* workspace, int64_t workspace_bytes, void* stream) {
     if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1 || !dw) return BS_EINVAL;
+    if (rows > 0 && (!ds || !x || ldds < N || ldx < K)) return BS_EINVAL;
     hipStream_t st = rows_stream(stream);
     const int64_t n = (int64_t)K * N;
-    const unsigned blocks = (unsigned)((n + 255) / 256);
-    if (rows == 0) {
-        if (dtype == BS_DT_F32) hipLaunchKernelGGL(k_zero<BS_DT_F32>, dim3(blocks), dim3(256), 0, st, n, (char*)dw);
-        else hipLaunchKernelGGL(k_zero<BS_DT_F16>, dim3(blocks), dim3(256), 0, st, n, (char*)dw);
-        return rows_rc();
-    }
-    if (!ds || !x || ldds < N || ldx < K) return BS_EINVAL;
     int64_t part, parts;
     split_rows(rows, K, N, &part, &parts);
-    if (parts > 1 && (!workspace || workspace_bytes < parts * n * 4)) return BS_EINVAL;
-    GemmArgs a = {};
-    a.P = (const char*)x; a.Pexp = x_exps; a.lpe = (K + P8_BLOCK - 1) / P8_BLOCK; a.ldp = ldx; a.np = K;
-    a.Q = (const char*)ds; a.ldq = ldds; a.nq = N;
-    a.nk = rows; a.kpart = part;
-    a.out0 = (char*)(parts > 1 ? workspace : dw);
-    int rc;
-#define GRAD_W(DT) (parts > 1 ? (x_exps ? launch_gemm<DT, L_P8, L_IC, E_PART>(a, (int)parts, st) : launch_gemm<DT, L_IC, L_IC, E_PART>(a, (int)parts, st)) \
-                              : (x_exps ? launch_gemm<DT, L_P8, L_IC, E_PLAIN>(a, 1, st) : launch_gemm<DT, L_IC, L_IC, E_PLAIN>(a, 1, st)))
-    if (dtype == BS_DT_F32) rc = GRAD_W(BS_DT_F32);
-    else if (dtype == BS_DT_BF16) rc = GRAD_W(BS_DT_BF16);
-    else rc = GRAD_W(BS_DT_F16);
-#undef GRAD_W
-    if (rc != BS_OK || parts == 1) return rc;
+    const bool joined = parts > 1 || dtype != BS_DT_F32;
+    if (joined && rows > 0 && (!workspace || workspace_bytes < parts * n * 4)) return BS_EINVAL;
+    int rc = BS_OK;
+    if (rows > 0) {
+        OverArgs a = {};
+        a.x = (const char*)x; a.exps = x_exps; a.ldx = ldx; a.ds = (const char*)ds; a.ldds = ldds; a.rows = rows; a.part = part;
+        a.K = K; a.N = N; a.nb = (K + P8_BLOCK - 1) / P8_BLOCK; a.parts = (int)parts;
+        a.tp = (K + 127) / 128;
+        a.tiles = (int64_t)a.tp * ((N + 127) / 128) * parts;
+        a.out = (char*)(joined ? workspace : dw);
+        rc = dtype == BS_DT_F32 ? launch_over<BS_DT_F32>(a, st) : dtype == BS_DT_BF16 ? launch_over<BS_DT_BF16>(a, st) : launch_over<BS_DT_F16>(a, st);
+        if (rc != BS_OK || !joined) return rc;
+    } else {
+        parts = 0;                                            // the sum of no parts
+    }
     const float* ws = (const float*)workspace;
-    if (dtype == BS_DT_F32) hipLaunchKernelGGL(k_add_parts<BS_DT_F32>, dim3(blocks), dim3(256), 0, st, ws, (int)parts, n, (char*)dw);
-    else if (dtype == BS_DT_BF16) hipLaunchKernelGGL(k_add_parts<BS_DT_BF16>, dim3(blocks), dim3(256), 0, st, ws, (int)parts, n, (char*)dw);
-    else hipLaunchKernelGGL(k_add_parts<BS_DT_F16>, dim3(blocks), dim3(256), 0, st, ws, (int)parts, n, (char*)dw);
+    const dim3 blocks((unsigned)((n + 255) / 256));
+    if (dtype == BS_DT_F32) hipLaunchKernelGGL(k_add_parts<BS_DT_F32>, blocks, dim3(256), 0, st, ws, (int)parts, n, (char*)dw);
+    else if (dtype == BS_DT_BF16) hipLaunchKernelGGL(k_add_parts<BS_DT_BF16>, blocks, dim3(256), 0, st, ws, (int)parts, n, (char*)dw);
+    else hipLaunchKernelGGL(k_add_parts<BS_DT_F16>, blocks, dim3(256), 0, st, ws, (int)parts, n, (char*)dw);
     return rows_rc();
 }
 

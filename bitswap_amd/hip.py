@@ -24,7 +24,8 @@ SYMBOLS = [
     "bs_layer_push64", "bs_stream_create_cu_mask", "bs_stream_destroy", "bs_debug_where",
     "bs_selftest", "bs_sigmoid_f64", "bs_bias_residual_elu_f32", "bs_head_params_f32", "bs_expand_rows5_f32", "bs_wino_in_f32", "bs_wino_out_f32", "bs_wino_fused_f32",
     "bs_small_k_gemm_f32", "bs_conv3_wino_f32", "bs_wino_gemm_f32", "bs_wino_gemm_bf16x3",
-    "bs_linear_act", "bs_act_grad_workspace", "bs_act_grad", "bs_linear_grad_x", "bs_linear_grad_w_workspace", "bs_linear_grad_w",
+    "bs_linear_workspace", "bs_linear_act", "bs_act_grad_workspace", "bs_act_grad", "bs_linear_grad_x_workspace", "bs_linear_grad_x",
+    "bs_linear_grad_w_workspace", "bs_linear_grad_w",
     "bs_group_norm_workspace", "bs_group_norm_act", "bs_group_norm_act_grad", "bs_pack8", "bs_unpack8",
 ]
 HEAD_SIGMOID, HEAD_SOFTPLUS = 0, 1
@@ -83,10 +84,11 @@ def load():
     L.bs_wino_gemm_bf16x3.argtypes = [p, p, p, i32, i32, i32, i64, i32, p]
     L.bs_conv3_wino_f32.argtypes = [p, p, p, i32, p, p, i32, i64, i32, i32, i32, i32, p]
     L.bs_wino_out_f32.argtypes = [p, p, p, p, p, i64, i32, i32, i32, i32, i32, p]
-    L.bs_linear_act.argtypes = [p, i64, p, i64, p, i32, p, i64, p, p, i32, i32, i64, i32, i32, p]
+    L.bs_linear_workspace.argtypes = L.bs_linear_grad_x_workspace.argtypes = [i32, i64, i32, i32]
+    L.bs_linear_act.argtypes = [p, i64, p, i64, p, i32, p, i64, p, p, i32, i32, i64, i32, i32, p, i64, p]
     L.bs_act_grad_workspace.argtypes = [i64, i32]
     L.bs_act_grad.argtypes = [p, i64, p, i64, p, p, i64, i32, i32, i64, i32, p, p, p, i64, p]
-    L.bs_linear_grad_x.argtypes = [p, i64, p, i64, p, i32, i64, i32, i32, p]
+    L.bs_linear_grad_x.argtypes = [p, i64, p, i64, p, i32, i64, i32, i32, p, i64, p]
     L.bs_linear_grad_w_workspace.argtypes = [i32, i64, i32, i32]
     L.bs_linear_grad_w.argtypes = [p, i64, p, p, i64, p, i32, i64, i32, i32, p, i64, p]
     L.bs_group_norm_workspace.argtypes = [i32, i64, i64, i32, i32, i32]
@@ -963,8 +965,11 @@ def linear_act(x, w, bias=None, res=None, act=ACT_ELU, want_sum=False, want_act=
         rt, ldr, _ = _as_rows(res, N, "linear_act res")
     s = torch.empty(shape, dtype=x.dtype, device=x.device) if want_sum else None
     y = torch.empty(shape, dtype=x.dtype, device=x.device) if want_act else None
-    _check(load().bs_linear_act(_ptr(xt), ldx, _ptr(wt), ldw, _ptr(bias), bcode, _ptr(rt), ldr, _ptr(s), _ptr(y), act, code, rows,
-                                K, N, _stream()), "bs_linear_act")
+    L = load()
+    nb = L.bs_linear_workspace(code, rows, K, N)
+    ws = _workspace(nb, x.device)
+    _check(L.bs_linear_act(_ptr(xt), ldx, _ptr(wt), ldw, _ptr(bias), bcode, _ptr(rt), ldr, _ptr(s), _ptr(y), act, code, rows, K, N,
+                           _ptr(ws), nb, _stream()), "bs_linear_act")
     return s, y
 
 
@@ -1020,7 +1025,9 @@ def linear_act_grad(x, w, s=None, act=ACT_NONE, g_sum=None, g_act=None, want_x=T
     if want_x:
         wt, ldw, _ = _as_rows(w, K, "linear_act_grad w")
         dx = torch.empty(tuple(g0.shape[:-1]) + (K,), dtype=w.dtype, device=dev)
-        _check(L.bs_linear_grad_x(_ptr(dt), ldd, _ptr(wt), ldw, _ptr(dx), code, rows, K, N, _stream()), "bs_linear_grad_x")
+        nb = L.bs_linear_grad_x_workspace(code, rows, K, N)
+        ws = _workspace(nb, dev)
+        _check(L.bs_linear_grad_x(_ptr(dt), ldd, _ptr(wt), ldw, _ptr(dx), code, rows, K, N, _ptr(ws), nb, _stream()), "bs_linear_grad_x")
     if want_w:
         dw = torch.empty((N, K), dtype=w.dtype, device=dev)
         nb = L.bs_linear_grad_w_workspace(code, rows, K, N)

@@ -22,13 +22,15 @@ def test_null_operands_sizes_types_and_strides_are_refused(L):
     E = hip.EINVAL
     #                          x ldx  w ldw bias bt res ldr sum act  a  dt rows K  N  stream
     ok = lambda **k: L.bs_linear_act(*[k.get(n, d) for n, d in (("x", p), ("ldx", 8), ("w", p), ("ldw", 8), ("bias", None), ("bt", 0), ("res", None),      # noqa: E731
-                                     ("ldr", 0), ("s", p), ("y", None), ("act", 1), ("dt", 0), ("rows", 4), ("K", 8), ("N", 8), ("stream", None))])
+                                     ("ldr", 0), ("s", p), ("y", None), ("act", 1), ("dt", 0), ("rows", 4), ("K", 8), ("N", 8), ("ws", None), ("nb", 0), ("stream", None))])
     for bad in (dict(x=None), dict(w=None), dict(s=None), dict(ldx=7), dict(ldw=7), dict(res=p, ldr=7), dict(act=4), dict(act=-1), dict(dt=3),
-                dict(dt=-1), dict(rows=-1), dict(rows=1 << 41), dict(K=0), dict(N=0), dict(bias=p, bt=1)):
+                dict(dt=-1), dict(rows=-1), dict(rows=1 << 41), dict(K=0), dict(N=0), dict(bias=p, bt=1), dict(rows=100000)):
         assert ok(**bad) == E, bad
     assert ok(rows=0, x=None) == hip.OK                                     # no rows: nothing to do
-    assert L.bs_linear_grad_x(None, 8, p, 8, p, 0, 4, 8, 8, None) == E
-    assert L.bs_linear_grad_x(p, 7, p, 8, p, 0, 4, 8, 8, None) == E
+    n = L.bs_linear_grad_x_workspace(0, 4, 8, 8)
+    assert L.bs_linear_grad_x(None, 8, p, 8, p, 0, 4, 8, 8, p, n, None) == E
+    assert L.bs_linear_grad_x(p, 7, p, 8, p, 0, 4, 8, 8, p, n, None) == E
+    assert L.bs_linear_grad_x(p, 8, p, 8, p, 0, 4, 8, 8, p, n - 1, None) == E
     assert L.bs_linear_grad_w(p, 8, None, None, 8, p, 0, 4, 8, 8, None, 0, None) == E
     assert L.bs_linear_grad_w(p, 8, p, None, 8, None, 0, 4, 8, 8, None, 0, None) == E
     n = L.bs_linear_grad_w_workspace(0, 100000, 8, 8)
@@ -56,7 +58,7 @@ def test_workspaces(L):
         for k, n in ((1, 1), (61, 130), (2048, 2048)):
             assert 0 <= L.bs_linear_grad_w_workspace(1, rows, k, n) < 1 << 28
             assert 0 <= L.bs_act_grad_workspace(rows, n) < 1 << 26
-    assert L.bs_linear_grad_w_workspace(1, 1, 8, 8) == 0
+    assert L.bs_linear_grad_w_workspace(0, 1, 8, 8) == 0 and L.bs_linear_workspace(0, 256, 256, 256) == 0
     for bad in ((3, 8, 8, 8), (1, -1, 8, 8), (1, 8, 0, 8), (1, 8, 8, 0)):
         assert L.bs_linear_grad_w_workspace(*bad) < 0
     assert L.bs_group_norm_workspace(0, 3, 256, 256, 32, 0) == 0
