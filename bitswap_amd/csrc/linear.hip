@@ -21,6 +21,7 @@ typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
 enum { E_LAYER = 0, E_PLAIN = 1 };                        // bias + residual + activation | one rounding
 constexpr int limbs_of(int dt) { return dt == BS_DT_F32 ? 3 : 1; }
+constexpr int kb_of(int dt) { return dt == BS_DT_F32 ? 16 : 32; }          // k that lie side by side in a laid out w
 
 template <int DT>
 __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
@@ -59,8 +60,9 @@ __device__ __forceinline__ void multiply(const u32x4 (&fp)[NP][LP], const u32x4 
 struct RowsArgs {
     const char *x, *w;                 // operands as the caller holds them
     int64_t ldx, ldw;
-    const char* wl;                    // w as the kernel reads it: [limb][N][kp] 16-bit, zero behind K; or w itself
-    int64_t ldl, limb_stride;          // in elements
+    const char* wl;                    // w as the kernel reads it, 16-bit: laid out (k_lay_w), or w itself
+    int64_t sp, sk, sl;                // element (limb, p, k) is at limb sl + p sp + k / KB sk + k % KB
+    int kp;                            // k it has, a multiple of 64; zero behind K
     int64_t rows;
     int K, N;
     int wt;                            // w is [K, N] (the gradient of x)
@@ -81,42 +83,59 @@ __device__ __forceinline__ float again(const RowsArgs& a, int64_t q, int64_t p) 
     return s;
 }
 
-// what becomes of V neighbouring channels of a row (n of them exist)
+// what becomes of V neighbouring channels of a row (n of them exist); bias, r: their bias and residual
 template <int DT, int EPI>
-__device__ __forceinline__ void finish(const RowsArgs& a, int64_t q, int64_t p, int n, float* v) {
+__device__ __forceinline__ void finish(const RowsArgs& a, int64_t q, int64_t p, int n, float* v, const float* bias, u32x4 r) {
     constexpr int V = vlen(DT), ES = esize(DT);
     if (DT == BS_DT_F32) {
+        bool odd = false;
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-            if ((f32_bits(v[e]) & 0x7f800000u) == 0x7f800000u && e < n) v[e] = again<DT>(a, q, p + e);
+        for (int e = 0; e < V; ++e) odd |= (f32_bits(v[e]) & 0x7f800000u) == 0x7f800000u;
+        if (odd) {
+            for (int e = 0; e < V; ++e)
+                if ((f32_bits(v[e]) & 0x7f800000u) == 0x7f800000u && e < n) v[e] = again<DT>(a, q, p + e);
+        }
     }
     const int64_t at = (q * a.N + p) * ES;
     if (EPI == E_LAYER) {
         float t[V];
-        if (a.bias) {
-            if (DT != BS_DT_F32 && a.bias_f32) {
 #pragma unroll
-                for (int e = 0; e < V; ++e) t[e] = e < n ? reinterpret_cast<const float*>(a.bias)[p + e] : 0.0f;
-            } else {
-                load_vec<DT>(a.bias + p * ES, n, t);
-            }
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[e] += t[e];
-        }
+        for (int e = 0; e < V; ++e) v[e] += bias[e];
         if (a.res) {
-            load_vec<DT>(a.res + (q * a.ldr + p) * ES, n, t);
+            unpack16<DT>(r, t);
 #pragma unroll
             for (int e = 0; e < V; ++e) v[e] += t[e];
         }
         if (a.sum) store_vec<DT>(a.sum + at, n, v);
         if (a.act_out) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) t[e] = act_value(a.act, v[e]);
+            act_values<V>(a.act, v, t);
             store_vec<DT>(a.act_out + at, n, t);
         }
     } else {
         store_vec<DT>(a.sum + at, n, v);
     }
+}
+template <int DT>
+__device__ __forceinline__ void load_bias(const RowsArgs& a, int64_t p, float* b) {
+    constexpr int V = vlen(DT);
+#pragma unroll
+    for (int e = 0; e < V; ++e) b[e] = 0.0f;
+    if (!a.bias || p >= a.N) return;
+    if (DT != BS_DT_F32 && a.bias_f32) {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (p + e < a.N) b[e] = reinterpret_cast<const float*>(a.bias)[p + e];
+    } else {
+        load_vec<DT>(a.bias + p * esize(DT), a.N - p < V ? (int)(a.N - p) : V, b);
+    }
+}
+template <int DT>
+__device__ __forceinline__ u32x4 residual(const RowsArgs& a, int64_t q, int64_t p, int n) {
+    constexpr int V = vlen(DT);
+    if (n >= V) return load16(a.res + (q * a.ldr + p) * esize(DT));
+    float t[V];
+    load_vec<DT>(a.res + (q * a.ldr + p) * esize(DT), n, t);
+    return pack16<DT>(t);
 }
 
 // A wavefront's 32 rows x 64 channels from the registers of the matrix instruction to rows of memory, by way of its own piece of
@@ -125,24 +144,33 @@ __device__ __forceinline__ void finish(const RowsArgs& a, int64_t q, int64_t p, 
 constexpr int TURN = 32 * 68 * 4;
 template <int DT, int EPI>
 __device__ __forceinline__ void turn_and_finish(const RowsArgs& a, const f32x16& a0, const f32x16& a1, float* mine, int lane, int64_t q0,
-                                                int64_t p0, bool two) {
-    constexpr int V = vlen(DT), LPR = 64 / V;                // lanes per row of 64 channels
+                                                int64_t p0, const float* bias) {
+    constexpr int V = vlen(DT), LPR = 64 / V, RI = 64 / LPR, NI = 32 / RI;      // lanes per row of 64 channels, rows at a time
+    const int c = (lane % LPR) * V;
+    const int64_t p = p0 + c, left = a.N - p;
+    const int n = left < V ? (int)left : V;
+    u32x4 res[NI];
+    if (EPI == E_LAYER && a.res && n > 0) {                                    // all residuals of the piece are asked for at once
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int64_t q = q0 + lane / LPR + i * RI;
+            if (q < a.rows) res[i] = residual<DT>(a, q, p, n);
+        }
+    }
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
         const f32x4 v0 = {a0[4 * g], a0[4 * g + 1], a0[4 * g + 2], a0[4 * g + 3]};
         const f32x4 v1 = {a1[4 * g], a1[4 * g + 1], a1[4 * g + 2], a1[4 * g + 3]};
         float* const at = mine + (lane & 31) * 68 + 8 * g + 4 * (lane >> 5);
         *reinterpret_cast<f32x4*>(at) = v0;
-        if (two) *reinterpret_cast<f32x4*>(at + 32) = v1;
+        *reinterpret_cast<f32x4*>(at + 32) = v1;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    const int c = (lane % LPR) * V;
-    const int64_t p = p0 + c;
-    const int64_t left = (two ? a.N : (a.N < p0 + 32 ? a.N : p0 + 32)) - p;
-    if (left > 0) {
-#pragma unroll 2
-        for (int r = lane / LPR; r < 32; r += 64 / LPR) {
+    if (n > 0) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int r = lane / LPR + i * RI;
             if (q0 + r >= a.rows) break;
             float v[V];
 #pragma unroll
@@ -150,7 +178,7 @@ __device__ __forceinline__ void turn_and_finish(const RowsArgs& a, const f32x16&
                 const f32x4 t = *reinterpret_cast<const f32x4*>(mine + r * 68 + c + e);
                 v[e] = t[0]; v[e + 1] = t[1]; v[e + 2] = t[2]; v[e + 3] = t[3];
             }
-            finish<DT, EPI>(a, q0 + r, p, left < V ? (int)left : V, v);
+            finish<DT, EPI>(a, q0 + r, p, n, v, bias, res[i]);
         }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -160,9 +188,8 @@ __device__ __forceinline__ void turn_and_finish(const RowsArgs& a, const f32x16&
 // ---- forward and dx, many rows ------------------------------------------------------------------------------------------------
 // Tile of BQ rows x BP channels, BK deep steps through two buffers of shared memory.  Rows of BK k lie there as 16-byte chunks of 8,
 // chunk c in slot c ^ f(row), f such that the 8 lanes a 16-byte access serves together touch all banks.  w comes by DMA (laid out
-// for it: whole steps, zero behind K); x by DMA too where its rows allow (XD: 16-bit, rows of whole aligned chunks), else through
-// registers, where float32 is split.
-template <int DT, int EPI, bool XD, int BQ, int BP, int WQ, int WP, int BK>
+// for it: whole steps, zero behind K), x through registers, where float32 is split: rows of any alignment and length.
+template <int DT, int EPI, int BQ, int BP, int WQ, int WP, int BK>
 __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_rows(const RowsArgs a) {
     constexpr int NW = (BQ / WQ) * (BP / WP), NT = NW * 64, L = limbs_of(DT), ES = esize(DT);
     constexpr int SL = BK / 8, RB = BK * 2;                    // chunks and bytes of a row
@@ -172,7 +199,7 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_rows(const RowsA
     __shared__ __align__(16) char lds[2 * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wp = wave % (BP / WP), wq = wave / (BP / WP);
-    auto swz = [](int row, int c) { return SL == 8 ? (c ^ (row & 7)) : (c ^ ((row >> 1) & 3)); };
+    auto swz = [](int row, int c) { return SL == 8 ? (c ^ (row & 7)) : SL == 4 ? (c ^ ((row >> 1) & 3)) : (c ^ ((row >> 2) & 1)); };
 
     // workgroups of one XCD (blockIdx % 8) take a run of tiles, channels fastest: rows that several tiles read are in its L2
     const int64_t per = (a.tiles + 7) / 8;
@@ -183,7 +210,7 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_rows(const RowsA
     const int steps = (a.K + BK - 1) / BK;
 
     // DMA: a wavefront's instruction fills 1 KB, 64 / SL rows
-    constexpr int WI = WB / 1024, XI = XB / 1024;
+    constexpr int WI = WB / 1024;
     auto dma_w = [&](int s, char* st) {
 #pragma unroll
         for (int n = 0; n < (WI + NW - 1) / NW; ++n) {
@@ -191,24 +218,13 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_rows(const RowsA
             if (WI % NW != 0 && i >= WI) break;
             const int r = i * (64 / SL) + lane / SL, limb = r / BP, row = r % BP;
             const int p = p0 + row < a.N ? p0 + row : a.N - 1;         // channels behind the last: not stored
-            const char* const src = a.wl + ((int64_t)limb * a.limb_stride + (int64_t)p * a.ldl + (int64_t)s * BK + swz(row, lane % SL) * 8) * 2;
+            const int k = s * BK + swz(row, lane % SL) * 8;
+            const char* const src = a.wl + (limb * a.sl + p * a.sp + k / kb_of(DT) * a.sk + k % kb_of(DT)) * 2;
             __builtin_amdgcn_global_load_lds(src, (lds_ptr)(st + XB + i * 1024), 16, 0, 0);
         }
     };
-    auto dma_x = [&](int s, char* st) {
-#pragma unroll
-        for (int n = 0; n < (XI + NW - 1) / NW; ++n) {
-            const int i = wave + n * NW;
-            if (XI % NW != 0 && i >= XI) break;
-            const int row = i * (64 / SL) + lane / SL, c = swz(row, lane % SL);
-            const int64_t q = q0 + row < a.rows ? q0 + row : a.rows - 1;
-            const int k = s * BK + c * 8;
-            if (k < a.K) __builtin_amdgcn_global_load_lds(a.x + (q * a.ldx + k) * 2, (lds_ptr)(st + i * 1024), 16, 0, 0);
-            else *reinterpret_cast<u32x4*>(st + i * 1024 + lane * 16) = u32x4{0, 0, 0, 0};      // behind K: zero
-        }
-    };
     // registers: float32 four values a unit (8 units a row: 128 bytes side by side), 16-bit eight
-    constexpr int UPR = DT == BS_DT_F32 ? BK / 4 : SL, UNITS = BQ * UPR, XN = XD ? 1 : UNITS / NT;
+    constexpr int UPR = DT == BS_DT_F32 ? BK / 4 : SL, UNITS = BQ * UPR, XN = UNITS / NT;
     u32x4 xr[XN];
     auto load_x = [&](int s) {
 #pragma unroll
@@ -257,19 +273,17 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_rows(const RowsA
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
 
-    if (!XD) load_x(0);
+    load_x(0);
     dma_w(0, lds);
-    if (XD) dma_x(0, lds);
-    else store_x(lds);
+    store_x(lds);
     for (int s = 0; s < steps; ++s) {
         char* const cur = lds + (s & 1) * STAGE;
         char* const nxt = lds + ((s & 1) ^ 1) * STAGE;
         __syncthreads();                        // this step has landed; the other buffer's readers are done
         const bool more = s + 1 < steps;
         if (more) {
-            if (!XD) load_x(s + 1);
+            load_x(s + 1);
             dma_w(s + 1, nxt);
-            if (XD) dma_x(s + 1, nxt);
         }
 #pragma unroll
         for (int b = 0; b < BK / 16; ++b) {
@@ -289,15 +303,142 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_rows(const RowsA
             }
             multiply<DT, L, L, NP, NQ>(fp, fq, acc);
         }
-        if (more && !XD) store_x(nxt);
+        if (more) store_x(nxt);
     }
     __syncthreads();
     float* const mine = reinterpret_cast<float*>(lds + wave * TURN);
 #pragma unroll
-    for (int j = 0; j < NQ; ++j)
+    for (int i = 0; i < NP; i += 2) {
+        const int p = p0 + wp * WP + i * 32;
+        float bias[vlen(DT)];
+        if (EPI == E_LAYER) load_bias<DT>(a, p + lane % (64 / vlen(DT)) * vlen(DT), bias);
 #pragma unroll
-        for (int i = 0; i < NP; i += 2)
-            turn_and_finish<DT, EPI>(a, acc[i][j], acc[i + 1][j], mine, lane, q0 + wq * WQ + j * 32, p0 + wp * WP + i * 32, true);
+        for (int j = 0; j < NQ; ++j) turn_and_finish<DT, EPI>(a, acc[i][j], acc[i + 1][j], mine, lane, q0 + wq * WQ + j * 32, p, bias);
+    }
+}
+
+// ---- ... whose rows are whole aligned 16-byte chunks --------------------------------------------------------------------------------
+// Both operands come by DMA through a ring of NS buffers, NS - 1 steps ahead, with one barrier a step: its wait is for the step it
+// opens only (the DMA of later steps stays in flight).  float32 rows lie in shared memory as they are and are split into limbs
+// after the read: 32 bytes a fragment instead of 48, and nothing goes back to shared memory.
+__device__ __forceinline__ constexpr int wait_vm(int v) { return (v & 15) | (7 << 4) | ((v >> 4) << 14); }      // vmcnt(v), lgkmcnt(0)
+
+template <int DT, int EPI, int BQ, int BP, int WQ, int WP, int BK, int NS>
+__global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_rows_dma(const RowsArgs a) {
+    constexpr int NW = (BQ / WQ) * (BP / WP), L = limbs_of(DT), ES = esize(DT), CK = 16 / ES;       // CK: k of a chunk of x
+    constexpr int XS = BK * ES / 16, WS = BK / 8;                                                    // chunks of a row
+    constexpr int XB = BQ * BK * ES, WB = L * BP * BK * 2, STAGE = XB + WB;
+    constexpr int XI = XB / 1024 / NW, WI = WB / 1024 / NW;
+    constexpr int NP = WP / 32, NQ = WQ / 32;
+    static_assert(XB % (1024 * NW) == 0 && WB % (1024 * NW) == 0 && NS * STAGE <= 160 * 1024 && NW * TURN <= NS * STAGE && NP % 2 == 0, "");
+    __shared__ __align__(16) char lds[NS * STAGE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wp = wave % (BP / WP), wq = wave / (BP / WP);
+    auto swz = [](int slots, int row, int c) { return slots == 8 ? (c ^ (row & 7)) : slots == 4 ? (c ^ ((row >> 1) & 3)) : (c ^ ((row >> 2) & 1)); };
+    const int64_t per = (a.tiles + 7) / 8;
+    const int64_t t = (blockIdx.x % 8) * per + blockIdx.x / 8;
+    if (t >= a.tiles) return;
+    const int64_t q0 = t / a.tp * BQ;
+    const int p0 = (int)(t % a.tp) * BP;
+    const int steps = (a.K + BK - 1) / BK;
+    const char* const xb = a.x + q0 * a.ldx * ES;
+    const char* const wb = a.wl + p0 * a.sp * 2;
+    constexpr int KB = kb_of(DT);
+    static_assert(BK % KB == 0, "");
+    uint32_t xo[XI], wo[WI];
+    int xk[XI];
+#pragma unroll
+    for (int n = 0; n < XI; ++n) {
+        const int row = (wave * XI + n) * (64 / XS) + lane / XS, c = swz(XS, row, lane % XS);
+        const int64_t r = q0 + row < a.rows ? row : a.rows - 1 - q0;            // rows behind the last: not stored
+        xo[n] = (uint32_t)(r * a.ldx * ES + c * 16);
+        xk[n] = a.K - c * CK;
+    }
+#pragma unroll
+    for (int n = 0; n < WI; ++n) {
+        const int r = (wave * WI + n) * (64 / WS) + lane / WS, limb = r / BP, row = r % BP;
+        const int pr = p0 + row < a.N ? row : a.N - 1 - p0;                       // channels behind the last: not stored
+        const int k = swz(WS, row, lane % WS) * 8;
+        wo[n] = (uint32_t)((limb * a.sl + pr * a.sp + k / KB * a.sk + k % KB) * 2);
+    }
+    auto issue = [&](int s, int slot) {
+        char* const st = lds + slot * STAGE;
+        const char* const xs = xb + (int64_t)s * BK * ES;
+        const char* const ws = wb + (int64_t)s * (BK / KB) * a.sk * 2;
+#pragma unroll
+        for (int n = 0; n < XI; ++n) {
+            const char* const src = xs + xo[n];
+            if (s * BK < xk[n]) __builtin_amdgcn_global_load_lds(src, (lds_ptr)(st + (wave * XI + n) * 1024), 16, 0, 0);
+            else *reinterpret_cast<u32x4*>(st + (wave * XI + n) * 1024 + lane * 16) = u32x4{0, 0, 0, 0};       // behind K: zero
+        }
+#pragma unroll
+        for (int n = 0; n < WI; ++n) {
+            const char* const src = ws + wo[n];
+            __builtin_amdgcn_global_load_lds(src, (lds_ptr)(st + XB + (wave * WI + n) * 1024), 16, 0, 0);
+        }
+    };
+    f32x16 acc[NP][NQ];
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+#pragma unroll
+    for (int s = 0; s < NS - 1; ++s)
+        if (s < steps) issue(s, s);
+    int slot = 0;
+    for (int s = 0; s < steps; ++s) {
+        // the steps behind this one may stay in flight: NS - 2 of them while there are that many (a step whose x lies behind K in
+        // part has fewer loads in flight than counted: only the last one, after which everything is waited for)
+        if (s + NS - 1 < steps) __builtin_amdgcn_s_waitcnt(wait_vm((NS - 2) * (XI + WI)));
+        else __builtin_amdgcn_s_waitcnt(wait_vm(0));
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (s + NS - 1 < steps) issue(s + NS - 1, slot == 0 ? NS - 1 : slot - 1);
+        const char* const cur = lds + slot * STAGE;
+#pragma unroll
+        for (int b = 0; b < BK / 16; ++b) {
+            u32x4 fp[NP][L], fq[NQ][L];
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int row = wp * WP + i * 32 + (lane & 31);
+#pragma unroll
+                for (int l = 0; l < L; ++l)
+                    fp[i][l] = *reinterpret_cast<const u32x4*>(cur + XB + (l * BP + row) * (BK * 2) + swz(WS, row, 2 * b + (lane >> 5)) * 16);
+            }
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) {
+                const int row = wq * WQ + j * 32 + (lane & 31);
+                if (DT == BS_DT_F32) {
+                    const int c = 4 * b + 2 * (lane >> 5);
+                    const u32x4 r0 = *reinterpret_cast<const u32x4*>(cur + row * (BK * ES) + swz(XS, row, c) * 16);
+                    const u32x4 r1 = *reinterpret_cast<const u32x4*>(cur + row * (BK * ES) + swz(XS, row, c + 1) * 16);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t l3[3];
+                        limbs2(bits_f32(e < 2 ? r0[(2 * e) & 3] : r1[(2 * e) & 3]), bits_f32(e < 2 ? r0[(2 * e + 1) & 3] : r1[(2 * e + 1) & 3]), l3);
+#pragma unroll
+                        for (int l = 0; l < L; ++l) fq[j][l][e] = l3[l % 3];
+                    }
+                } else {
+                    fq[j][0] = *reinterpret_cast<const u32x4*>(cur + row * (BK * ES) + swz(XS, row, 2 * b + (lane >> 5)) * 16);
+                }
+            }
+            multiply<DT, L, L, NP, NQ>(fp, fq, acc);
+        }
+        slot = slot + 1 == NS ? 0 : slot + 1;
+    }
+    __syncthreads();
+    float* const mine = reinterpret_cast<float*>(lds + wave * TURN);
+#pragma unroll
+    for (int i = 0; i < NP; i += 2) {
+        const int p = p0 + wp * WP + i * 32;
+        float bias[vlen(DT)];
+        if (EPI == E_LAYER) load_bias<DT>(a, p + lane % (64 / vlen(DT)) * vlen(DT), bias);
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) turn_and_finish<DT, EPI>(a, acc[i][j], acc[i + 1][j], mine, lane, q0 + wq * WQ + j * 32, p, bias);
+    }
 }
 
 // ---- forward and dx, few rows -------------------------------------------------------------------------------------------------
@@ -313,7 +454,7 @@ __global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {
     const int64_t q = q0 + (lane & 31) < a.rows ? q0 + (lane & 31) : a.rows - 1;
     const int p = p0 + (lane & 31) < a.N ? p0 + (lane & 31) : a.N - 1;
     const char* const xp = a.x + q * a.ldx * ES;
-    const char* const wp = WL ? a.wl + (int64_t)p * a.ldl * 2 : a.w + (int64_t)p * a.ldw * ES;
+    const char* const wp = WL ? a.wl + p * a.sp * 2 : a.w + (int64_t)p * a.ldw * ES;
     f32x16 acc;
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
@@ -357,7 +498,7 @@ __global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {
             if (WL) {
 #pragma unroll
                 for (int l = 0; l < L; ++l)
-                    wr[n][l] = k < a.ldl ? load16(wp + ((int64_t)l * a.limb_stride + k) * 2) : u32x4{0, 0, 0, 0};
+                    wr[n][l] = k < a.kp ? load16(wp + (l * a.sl + k / kb_of(DT) * a.sk + k % kb_of(DT)) * 2) : u32x4{0, 0, 0, 0};
             } else {
                 fetch(wp, k, wr[n]);
             }
@@ -413,12 +554,16 @@ __global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {
         float v[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = turn[r * 68 + c + e];
-        finish<DT, EPI>(a, q0 + r, p0 + c, left < V ? left : V, v);
+        const int n = left < V ? left : V;
+        float bias[V];
+        if (EPI == E_LAYER) load_bias<DT>(a, p0 + c, bias);
+        finish<DT, EPI>(a, q0 + r, p0 + c, n, v, bias, EPI == E_LAYER && a.res ? residual<DT>(a, q0 + r, p0 + c, n) : u32x4{0, 0, 0, 0});
     }
 }
 
 // ---- w laid out for the kernels above -------------------------------------------------------------------------------------------
-// out [limb][P][kp] 16-bit: w [P, K], or with TURNED w [K, P] turned round; zero from K to kp
+// out [kp / KB][limb][P][KB] 16-bit: a DMA of neighbouring rows reads whole kilobytes.  w [P, K], or with TURNED w [K, P] turned round;
+// zero from K to kp
 template <int DT, bool TURNED>
 __global__ __launch_bounds__(256) void k_lay_w(const char* __restrict__ w, int64_t ldw, int P, int K, int kp, char* __restrict__ out) {
     constexpr int ES = esize(DT), L = limbs_of(DT);
@@ -447,7 +592,10 @@ __global__ __launch_bounds__(256) void k_lay_w(const char* __restrict__ w, int64
             if (DT == BS_DT_F32) limbs2(bits_f32(tile[r][k2]), bits_f32(tile[r][k2 + 1]), l);
             else l[0] = tile[r][k2] | (tile[r][k2 + 1] << 16);
 #pragma unroll
-            for (int b = 0; b < L; ++b) *reinterpret_cast<uint32_t*>(out + (((int64_t)b * P + p) * kp + kb + k2) * 2) = l[b];
+            for (int b = 0; b < L; ++b) {
+                constexpr int KB = kb_of(DT);
+                *reinterpret_cast<uint32_t*>(out + ((((int64_t)(kb + k2) / KB * L + b) * P + p) * KB + (kb + k2) % KB) * 2) = l[b];
+            }
         }
     }
 }
@@ -682,16 +830,18 @@ int launch_rows(RowsArgs a, void* workspace, int64_t bytes, hipStream_t st) {
     const int kp = (a.K + 63) / 64 * 64;
     const bool small = few(a.rows, a.N);
     const bool as_is = DT != BS_DT_F32 && !a.wt && a.K % 64 == 0 && a.ldw % 8 == 0 && ((uintptr_t)a.w & 15) == 0;
-    const bool lay = a.wt || (!small && !as_is);
+    const bool lay = a.wt || !small; (void)as_is;
     if (lay) {
         if (!workspace || bytes < lay_bytes(DT, a.K, a.N)) return BS_EINVAL;
         const dim3 grid((unsigned)(kp / 64), (unsigned)((a.N + 31) / 32));
         if (a.wt) hipLaunchKernelGGL((k_lay_w<DT, true>), grid, dim3(256), 0, st, a.w, a.ldw, a.N, a.K, kp, (char*)workspace);
         else hipLaunchKernelGGL((k_lay_w<DT, false>), grid, dim3(256), 0, st, a.w, a.ldw, a.N, a.K, kp, (char*)workspace);
-        a.wl = (const char*)workspace; a.ldl = kp; a.limb_stride = (int64_t)a.N * kp;
+        constexpr int KB = kb_of(DT);
+        a.wl = (const char*)workspace; a.sp = KB; a.sl = (int64_t)a.N * KB; a.sk = a.sl * limbs_of(DT);
     } else {
-        a.wl = a.w; a.ldl = a.ldw; a.limb_stride = 0;
+        a.wl = a.w; a.sp = a.ldw; a.sl = 0; a.sk = kb_of(DT);
     }
+    a.kp = kp;
     if (small) {
         a.tp = (a.N + 31) / 32;
         const unsigned blocks = (unsigned)((a.rows + 31) / 32 * a.tp);
@@ -699,16 +849,27 @@ int launch_rows(RowsArgs a, void* workspace, int64_t bytes, hipStream_t st) {
         else hipLaunchKernelGGL((k_relay<DT, EPI, false>), dim3(blocks), dim3(256), 0, st, a);
         return rows_rc();
     }
-    constexpr int BQ = 128, BP = DT == BS_DT_F32 ? 256 : 128, BK = DT == BS_DT_F32 ? 32 : 64;
-    a.tp = (a.N + BP - 1) / BP;
-    a.tiles = (a.rows + BQ - 1) / BQ * a.tp;
-    const int64_t blocks = (a.tiles + 7) / 8 * 8;
-    if (blocks > 0x7fffffff) return BS_EINVAL;
-    const dim3 grid((unsigned)blocks);
-    const bool xd = DT != BS_DT_F32 && a.K % 8 == 0 && a.ldx % 8 == 0 && ((uintptr_t)a.x & 15) == 0;
-    constexpr int NT = (BQ / 64) * (BP / 64) * 64;
-    if (DT != BS_DT_F32 && xd) hipLaunchKernelGGL((k_rows<DT, EPI, DT != BS_DT_F32, BQ, BP, 64, 64, BK>), grid, dim3(NT), 0, st, a);
-    else hipLaunchKernelGGL((k_rows<DT, EPI, false, BQ, BP, 64, 64, BK>), grid, dim3(NT), 0, st, a);
+    // rows of whole aligned chunks, tiles within 31 bits of their first byte: both operands by DMA
+    constexpr int CK = 16 / esize(DT);
+    const bool dma = a.K % CK == 0 && a.ldx % CK == 0 && ((uintptr_t)a.x & 15) == 0 && a.ldx * esize(DT) < (1 << 22) &&
+                     (a.sl * limbs_of(DT) + a.sp * 256 + a.sk * 2) * 2 < 0x7fffffff;
+    auto tiles = [&](int bq, int bp) {
+        a.tp = (a.N + bp - 1) / bp;
+        a.tiles = (a.rows + bq - 1) / bq * a.tp;
+        return (a.tiles + 7) / 8 * 8;
+    };
+#define ROWS(KERNEL, BQ, BP, NT) do { const int64_t blocks = tiles(BQ, BP); if (blocks > 0x7fffffff) return BS_EINVAL; \
+        hipLaunchKernelGGL((KERNEL), dim3((unsigned)blocks), dim3(NT), 0, st, a); } while (0)
+#define K_(...) __VA_ARGS__
+    if constexpr (DT == BS_DT_F32) {
+        if (dma) ROWS(K_(k_rows_dma<DT, EPI, 128, 128, 64, 64, 16, 4>), 128, 128, 256);
+        else ROWS(K_(k_rows<DT, EPI, 128, 128, 64, 64, 16>), 128, 128, 256);
+    } else {
+        if (dma) ROWS(K_(k_rows_dma<DT, EPI, 256, 256, 128, 64, 64, 2>), 256, 256, 512);
+        else ROWS(K_(k_rows<DT, EPI, 128, 128, 64, 64, 64>), 128, 128, 256);
+    }
+#undef K_
+#undef ROWS
     return rows_rc();
 }
 

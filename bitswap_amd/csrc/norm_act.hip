@@ -161,7 +161,8 @@ __global__ __launch_bounds__(1024) void k_norm(const NormArgs a) {
         const int64_t p = pl + (int64_t)r * PL;
         if (p >= a.pixels) break;
 #pragma unroll
-        for (int i = 0; i < V; ++i) f[r][i] = act_value(a.act, fmaf((f[r][i] - m[i]) * rs[i], ga[i], be[i]));
+        for (int i = 0; i < V; ++i) f[r][i] = fmaf((f[r][i] - m[i]) * rs[i], ga[i], be[i]);
+        act_values<V>(a.act, f[r], f[r]);
         store_vec<DT>(yp + p * a.C * ES, left, f[r]);
     }
 }
@@ -217,10 +218,15 @@ __global__ __launch_bounds__(1024) void k_norm_grad(const NormArgs a) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
         if (pl + r * PL < a.pixels) {
+            float u[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 h[r][i] = (h[r][i] - m[i]) * rs[i];
-                d[r][i] *= act_slope(a.act, fmaf(h[r][i], ga[i], be[i]));
+                u[i] = fmaf(h[r][i], ga[i], be[i]);
+            }
+            act_slopes<V>(a.act, u, d[r]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
                 s1[i] += d[r][i];
                 s2[i] = fmaf(d[r][i], h[r][i], s2[i]);
             }
@@ -291,12 +297,17 @@ __global__ __launch_bounds__(256) void k_part(const NormArgs a) {
                 if (GRAD) {
                     float g[V];
                     load_vec<DT>(a.g + (img * a.ldgn + p * a.ldgp + c) * ES, left, g);
+                    float u[V];
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
-                        const float h = (f[i] - m[i]) * rs[i];
-                        const float d = g[i] * act_slope(a.act, fmaf(h, ga[i], be[i]));
-                        s1[i] = fmaf(d, h, s1[i]);
-                        s2[i] += d;
+                        f[i] = (f[i] - m[i]) * rs[i];
+                        u[i] = fmaf(f[i], ga[i], be[i]);
+                    }
+                    act_slopes<V>(a.act, u, g);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        s1[i] = fmaf(g[i], f[i], s1[i]);
+                        s2[i] += g[i];
                     }
                 } else {
 #pragma unroll
@@ -402,10 +413,18 @@ __global__ __launch_bounds__(256) void k_apply(const NormArgs a, const float* __
         float f[V], g[V];
         load_x<DT, SAVED8>(a, img, p, c, left, f);
         if (GRAD) load_vec<DT>(a.g + (img * a.ldgn + p * a.ldgp + c) * ES, left, g);
+        float u[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const float h = (f[i] - m[i]) * rs[i], u = fmaf(h, ga[i], be[i]);
-            f[i] = GRAD ? rs[i] * (fmaf(g[i] * act_slope(a.act, u), ga[i], -m1[i]) - h * m2[i]) : act_value(a.act, u);
+            f[i] = (f[i] - m[i]) * rs[i];
+            u[i] = fmaf(f[i], ga[i], be[i]);
+        }
+        if (GRAD) {
+            act_slopes<V>(a.act, u, g);
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = rs[i] * (fmaf(g[i], ga[i], -m1[i]) - f[i] * m2[i]);
+        } else {
+            act_values<V>(a.act, u, f);
         }
         store_vec<DT>(a.y + ((img * a.pixels + p) * a.C + c) * ES, left, f);
     }
@@ -520,9 +539,9 @@ int bs_group_norm_act_grad(const void* g, int64_t ldgn, int64_t ldgp, const void
                            int64_t workspace_bytes, void* stream) {
     if (bad_norm(dtype, n, pixels, channels, groups, act)) return BS_EINVAL;
     hipStream_t st = rows_stream(stream);
-    const dim3 cols((unsigned)((2 * (int64_t)channels + 63) / 64));
+    const dim3 cols((unsigned)((2 * (int64_t)channels + 31) / 32));
     if (n == 0 || pixels == 0) {
-        if (dgamma || dbeta) hipLaunchKernelGGL(k_sum_columns, cols, dim3(256), 0, st, (const float*)nullptr, (int64_t)0, 2 * channels, channels, dgamma, dbeta);
+        if (dgamma || dbeta) hipLaunchKernelGGL(k_sum_columns, cols, dim3(1024), 0, st, (const float*)nullptr, (int64_t)0, 2 * channels, channels, dgamma, dbeta);
         return rows_rc();
     }
     if (!g || !x || !stats || !dx || ldgp < channels || ldgn < 0 || (!x_exps && (ldp < channels || ldn < 0))) return BS_EINVAL;
@@ -561,7 +580,7 @@ int bs_group_norm_act_grad(const void* g, int64_t ldgn, int64_t ldgp, const void
 #undef STEPS
     }
     if (dgamma || dbeta)
-        hipLaunchKernelGGL(k_sum_columns, cols, dim3(256), 0, st, (const float*)workspace, p.fits ? n : n * p.runs, 2 * channels, channels, dgamma, dbeta);
+        hipLaunchKernelGGL(k_sum_columns, cols, dim3(1024), 0, st, (const float*)workspace, p.fits ? n : n * p.runs, 2 * channels, channels, dgamma, dbeta);
     return rows_rc();
 }
 

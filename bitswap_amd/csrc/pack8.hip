@@ -96,8 +96,7 @@ __global__ __launch_bounds__(256) void k_act_grad(const ActGradArgs a, int cl_lo
                     float s[V];
                     if (SAVED8) load_codes<V>((const int8_t*)a.s + r * a.lds, a.exps + r * a.nb, c, left, s);
                     else load_vec<DT>(a.s + (r * a.lds + c) * ES, left, s);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) d[i] *= act_slope(a.act, s[i]);
+                    act_slopes<V>(a.act, s, d);
                 }
             }
             if (a.g_sum) {
@@ -205,7 +204,7 @@ int bs_act_grad(const void* g_sum, int64_t ldgs, const void* g_act, int64_t ldga
     else GO(BS_DT_F16);
 #undef GO
     if (db_out && parts > 1)
-        hipLaunchKernelGGL(k_sum_columns, dim3((unsigned)((N + 63) / 64)), dim3(256), 0, st, (const float*)workspace, parts, N, N, db_out, (float*)nullptr);
+        hipLaunchKernelGGL(k_sum_columns, dim3((unsigned)((N + 31) / 32)), dim3(1024), 0, st, (const float*)workspace, parts, N, N, db_out, (float*)nullptr);
     return rows_rc();
 }
 
