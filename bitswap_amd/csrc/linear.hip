@@ -18,6 +18,8 @@ namespace {
 typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i32x2* lds_i32x2;
 
 enum { E_LAYER = 0, E_PLAIN = 1 };                        // bias + residual + activation | one rounding
 constexpr int limbs_of(int dt) { return dt == BS_DT_F32 ? 3 : 1; }
@@ -610,7 +612,7 @@ struct OverArgs {
     int64_t tiles;                     // tiles x parts
     char* out;
 };
-enum { S_DMA = 0, S_REG = 1, S_P8 = 2 };
+enum { S_REG = 1, S_P8 = 2 };
 
 // One operand's tile of BK rows x 128 channels as it lies in memory; 16-byte chunk c of row r in slot c ^ 2 (r & 3), so that the
 // four rows a transposing read takes 32 bytes of lie in different banks.
@@ -620,22 +622,12 @@ struct Strip {
     static constexpr int BYTES = L * BK * 256;
     static constexpr int ES = SRC == S_P8 ? 1 : esize(DT);
     static constexpr int V = SRC == S_P8 ? 8 : vlen(DT);                         // channels of a unit
-    static constexpr int UPR = 128 / V, UNITS = BK * UPR, N = SRC == S_DMA ? 1 : UNITS / 256;
+    static constexpr int UPR = 128 / V, UNITS = BK * UPR, N = UNITS / 256;
     u32x4 raw[N];
     float step[SRC == S_P8 ? N : 1];
 
     static __device__ __forceinline__ int at(int limb, int row, int c) { return (limb * BK + row) * 256 + ((c ^ (2 * (row & 3))) * 16); }
 
-    __device__ __forceinline__ void dma(const char* base, int64_t ld, int ni, int i0, int64_t k, int64_t ke, char* st, int wave, int lane) const {
-#pragma unroll
-        for (int n = 0; n < BYTES / 4096; ++n) {
-            const int i = wave + n * 4, row = i * 4 + lane / 16, c = (lane % 16) ^ (2 * (row & 3));
-            int ch = i0 + c * 8;
-            ch = ch < ni ? ch : i0;                                              // channels behind the last: not stored
-            if (k + row < ke) __builtin_amdgcn_global_load_lds(base + ((k + row) * ld + ch) * 2, (lds_ptr)(st + i * 1024), 16, 0, 0);
-            else *reinterpret_cast<u32x4*>(st + i * 1024 + lane * 16) = u32x4{0, 0, 0, 0};       // rows behind the last
-        }
-    }
     __device__ __forceinline__ void load(const OverArgs& a, const char* base, int64_t ld, int ni, int i0, int64_t k, int64_t ke, int tid) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
@@ -706,6 +698,26 @@ struct Strip {
     }
 };
 
+// sums over rows kb..ke that did not come out finite once more, in float32 arithmetic
+template <int DT, bool P8>
+__device__ __forceinline__ void again_over(const OverArgs& a, int64_t kb, int64_t ke, int p, int q, int n, f32x4& v) {
+    bool odd = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) odd |= (f32_bits(v[e]) & 0x7f800000u) == 0x7f800000u;
+    if (!odd) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if ((f32_bits(v[e]) & 0x7f800000u) == 0x7f800000u && e < n) {
+            float s = 0.0f;
+            for (int64_t k = kb; k < ke; ++k) {
+                const float xv = P8 ? p8_value((int)(int8_t)a.x[k * a.ldx + p + e], p8_pow2(a.exps[k * a.nb + (p + e) / P8_BLOCK]))
+                                    : load1<DT>(a.x + (k * a.ldx + p + e) * esize(DT));
+                s = fmaf(xv, load1<DT>(a.ds + (k * a.ldds + q) * esize(DT)), s);
+            }
+            v[e] = s;
+        }
+}
+
 template <int DT, int XS, int DS, int BK>
 __global__ __launch_bounds__(256) void k_over_rows(const OverArgs a) {
     typedef Strip<DT, XS, BK> TX;
@@ -729,17 +741,15 @@ __global__ __launch_bounds__(256) void k_over_rows(const OverArgs a) {
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-    auto begin = [&](int64_t k, char* st) {
-        if (XS != S_DMA) tx.load(a, a.x, a.ldx, a.K, p0, k, ke, tid);
-        if (DS != S_DMA) td.load(a, a.ds, a.ldds, a.N, q0, k, ke, tid);
-        if (XS == S_DMA) tx.dma(a.x, a.ldx, a.K, p0, k, ke, st, wave, lane);
-        if (DS == S_DMA) td.dma(a.ds, a.ldds, a.N, q0, k, ke, st + TX::BYTES, wave, lane);
+    auto begin = [&](int64_t k) {
+        tx.load(a, a.x, a.ldx, a.K, p0, k, ke, tid);
+        td.load(a, a.ds, a.ldds, a.N, q0, k, ke, tid);
     };
     auto end = [&](char* st) {
-        if (XS != S_DMA) tx.store(st, tid);
-        if (DS != S_DMA) td.store(st + TX::BYTES, tid);
+        tx.store(st, tid);
+        td.store(st + TX::BYTES, tid);
     };
-    begin(kb, lds);
+    begin(kb);
     end(lds);
     int buf = 0;
     for (int64_t k = kb; k < ke; k += BK) {
@@ -747,7 +757,7 @@ __global__ __launch_bounds__(256) void k_over_rows(const OverArgs a) {
         char* const nxt = lds + (buf ^ 1) * STAGE;
         __syncthreads();
         const bool more = k + BK < ke;
-        if (more) begin(k + BK, nxt);
+        if (more) begin(k + BK);
 #pragma unroll
         for (int b = 0; b < BK / 16; ++b) {
             u32x4 fp[2][TX::L], fq[2][TD::L];
@@ -775,25 +785,216 @@ __global__ __launch_bounds__(256) void k_over_rows(const OverArgs a) {
                 const int p = p0 + wp * 64 + i * 32 + 8 * g + 4 * (lane >> 5), n = a.K - p;
                 if (n <= 0) continue;
                 f32x4 v = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-                if (DT == BS_DT_F32) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if ((f32_bits(v[e]) & 0x7f800000u) == 0x7f800000u && e < n) {          // the sum again, in float32
-                            float s = 0.0f;
-                            for (int64_t k = kb; k < ke; ++k) {
-                                const float xv = XS == S_P8 ? p8_value((int)(int8_t)a.x[k * a.ldx + p + e], p8_pow2(a.exps[k * a.nb + (p + e) / P8_BLOCK]))
-                                                            : load1<DT>(a.x + (k * a.ldx + p + e) * esize(DT));
-                                s = fmaf(xv, load1<DT>(a.ds + (k * a.ldds + q) * esize(DT)), s);
-                            }
-                            v[e] = s;
-                        }
-                }
+                if (DT == BS_DT_F32) again_over<DT, XS == S_P8>(a, kb, ke, p, q, n, v);
                 float* const o = reinterpret_cast<float*>(a.out) + ((int64_t)part * a.N + q) * a.K + p;
                 if (n >= 4) store16((char*)o, __builtin_bit_cast(u32x4, v));
                 else
                     for (int e = 0; e < n; ++e) o[e] = v[e];
             }
     }
+}
+
+// ---- ... whose rows are whole aligned 16-byte chunks ---------------------------------------------------------------------------------
+// x and ds by DMA through a ring, as in k_rows_dma, every tile as it lies in memory: [BK rows][channels].  The transposition that the
+// matrix instruction wants (8 rows of one channel side by side) happens in the read from shared memory: transposing reads for 16-bit
+// values (4 rows) and for codes (8 rows, turned into bfloat16 / float16 in registers: exact), dword reads along the channels and a
+// split into limbs for float32.  steps: 2^e of the codes, laid out [blocks of 32 channels][rows] beforehand (k_lay_steps).
+template <int DT, bool P8, int BQ, int BP, int WQ, int WP, int BK, int NS>
+__global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const OverArgs a, const float* __restrict__ steps, int64_t ldsteps) {
+    constexpr int NW = (BQ / WQ) * (BP / WP), ES = esize(DT), XE = P8 ? 1 : ES;
+    constexpr int LX = (DT == BS_DT_F32 && !P8) ? 3 : 1, LD = limbs_of(DT);
+    constexpr int XR = BP * XE, DR = BQ * ES;                            // bytes of a row
+    constexpr int XB = BK * XR, DB = BK * DR, SB = P8 ? BP / 32 * BK * 4 : 0, STAGE = XB + DB + SB;
+    constexpr int XI = XB / 1024 / NW, DI = DB / 1024 / NW, SI = P8 ? 1 : 0;
+    constexpr int NP = WP / 32, NQ = WQ / 32;
+    static_assert(XB % (1024 * NW) == 0 && DB % (1024 * NW) == 0 && NS * STAGE <= 160 * 1024 && NW * TURN <= NS * STAGE, "shared memory");
+    static_assert(!P8 || (SB % NW == 0 && SB / NW <= 256), "steps: one dword a lane and wavefront");
+    __shared__ __align__(16) char lds[NS * STAGE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wp = wave % (BP / WP), wq = wave / (BP / WP);
+    // chunk c of row r lies in slot c ^ sx(r): rows that one transposing read gathers then lie in different banks
+    auto sx = [](int r) { return P8 ? (r & 7) : ES == 2 ? 2 * (r & 3) : 0; };
+    auto sd = [](int r) { return ES == 2 ? 2 * (r & 3) : 0; };
+    const int64_t per = (a.tiles + 7) / 8;
+    const int64_t t = (blockIdx.x % 8) * per + blockIdx.x / 8;        // an XCD takes runs of tiles over the same rows
+    if (t >= a.tiles) return;
+    const int64_t tiles = a.tiles / a.parts;
+    const int part = (int)(t / tiles), tile = (int)(t % tiles);
+    const int p0 = tile % a.tp * BP, q0 = tile / a.tp * BQ;
+    const int64_t kb = part * a.part, ke = kb + a.part < a.rows ? kb + a.part : a.rows;
+    const int nk = (int)(ke - kb), count = (nk + BK - 1) / BK;
+    const char* const xb = a.x + (kb * a.ldx + p0) * XE;
+    const char* const db = a.ds + (kb * a.ldds + q0) * ES;
+    uint32_t xo[XI], dof[DI];
+    int xr[XI], dr[DI];
+#pragma unroll
+    for (int n = 0; n < XI; ++n) {
+        constexpr int CH = XR / 16;
+        const int u = (wave * XI + n) * 64 + lane, row = u / CH, c = (u % CH) ^ sx(row);
+        xr[n] = row;
+        xo[n] = (uint32_t)((int64_t)row * a.ldx * XE + (p0 + c * (16 / XE) < a.K ? c * 16 : 0));        // channels behind the last: not stored
+    }
+#pragma unroll
+    for (int n = 0; n < DI; ++n) {
+        constexpr int CH = DR / 16;
+        const int u = (wave * DI + n) * 64 + lane, row = u / CH, c = (u % CH) ^ sd(row);
+        dr[n] = row;
+        dof[n] = (uint32_t)((int64_t)row * a.ldds * ES + (q0 + c * (16 / ES) < a.N ? c * 16 : 0));
+    }
+    const float* sp = nullptr;
+    if (P8) {
+        const int i = wave * (SB / 4 / NW) + (lane < SB / 4 / NW ? lane : 0), blk = i / BK, nb = (a.K + 31) / 32;
+        sp = steps + (int64_t)(p0 / 32 + blk < nb ? p0 / 32 + blk : nb - 1) * ldsteps + kb + i % BK;
+    }
+    auto issue = [&](int s, int slot) {
+        char* const st = lds + slot * STAGE;
+        const char* const xs = xb + (int64_t)s * BK * a.ldx * XE;
+        const char* const ds = db + (int64_t)s * BK * a.ldds * ES;
+        const int left = nk - s * BK;
+#pragma unroll
+        for (int n = 0; n < XI; ++n) {
+            const char* const src = xs + xo[n];
+            char* const dst = st + (wave * XI + n) * 1024;
+            if (xr[n] < left) __builtin_amdgcn_global_load_lds(src, (lds_ptr)dst, 16, 0, 0);
+            else *reinterpret_cast<u32x4*>(dst + lane * 16) = u32x4{0, 0, 0, 0};                 // rows behind the last: zero
+        }
+#pragma unroll
+        for (int n = 0; n < DI; ++n) {
+            const char* const src = ds + dof[n];
+            char* const dst = st + XB + (wave * DI + n) * 1024;
+            if (dr[n] < left) __builtin_amdgcn_global_load_lds(src, (lds_ptr)dst, 16, 0, 0);
+            else *reinterpret_cast<u32x4*>(dst + lane * 16) = u32x4{0, 0, 0, 0};
+        }
+        if (P8) {
+            const char* const src = (const char*)(sp + s * BK);
+            char* const dst = st + XB + DB + wave * (SB / NW);
+            if (lane < SB / 4 / NW) __builtin_amdgcn_global_load_lds(src, (lds_ptr)dst, 4, 0, 0);
+        }
+    };
+    // channel c0 + lane % 32, rows r0 + 8 (lane / 32) + 0..7 of a 16-bit tile with rows of RB bytes
+    auto frag16 = [&](const char* base, int RB, int r0, int c0) {
+        u32x4 v;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int row = r0 + 8 * (lane >> 5) + 4 * h + ((lane & 15) >> 2), ch = c0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+            const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(base + row * RB + (((ch >> 3) ^ (2 * (row & 3))) * 16) + (ch & 4) * 2));
+            const u32x2 w2 = __builtin_bit_cast(u32x2, w);
+            v[2 * h] = w2[0];
+            v[2 * h + 1] = w2[1];
+        }
+        return v;
+    };
+    auto frag32 = [&](const char* base, int RB, int r0, int c0, u32x4* l) {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = *reinterpret_cast<const float*>(base + (r0 + 8 * (lane >> 5) + e) * RB + (c0 + (lane & 31)) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            uint32_t t3[3];
+            limbs2(f[2 * e], f[2 * e + 1], t3);
+            l[0][e] = t3[0];
+            l[1][e] = t3[1];
+            l[2][e] = t3[2];
+        }
+    };
+    auto frag8 = [&](const char* base, const char* sbase, int r0, int c0) {
+        const int row = r0 + 8 * (lane >> 5) + ((lane & 15) >> 1), ch = c0 + 16 * ((lane >> 4) & 1) + 8 * (lane & 1);
+        const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2)(base + row * XR + (((ch >> 4) ^ (row & 7)) * 16) + (ch & 8)));
+        float s[8], f[8];
+        *reinterpret_cast<f32x4*>(s) = *reinterpret_cast<const f32x4*>(sbase + (c0 / 32 * BK + r0 + 8 * (lane >> 5)) * 4);
+        *reinterpret_cast<f32x4*>(s + 4) = *reinterpret_cast<const f32x4*>(sbase + (c0 / 32 * BK + r0 + 8 * (lane >> 5) + 4) * 4);
+        uint32_t odd = 0;                                              // a byte 0x80 anywhere
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)((uint32_t)w[e / 4] >> (8 * (e % 4))) * s[e];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint32_t y = (uint32_t)w[e] ^ 0x80808080u;
+            odd |= (y - 0x01010101u) & ~y & 0x80808080u;
+        }
+        if (odd) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if ((((uint32_t)w[e / 4] >> (8 * (e % 4))) & 255u) == 0x80u) f[e] = __builtin_nanf("");
+        }
+        u32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = DT == BS_DT_F16 ? pk_f16(f[2 * e], f[2 * e + 1]) : pk_bf16(f[2 * e], f[2 * e + 1]);
+        return v;
+    };
+    f32x16 acc[NP][NQ];
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+#pragma unroll
+    for (int s = 0; s < NS - 1; ++s)
+        if (s < count) issue(s, s);
+    int slot = 0;
+    for (int s = 0; s < count; ++s) {
+        if (s + NS - 1 < count) __builtin_amdgcn_s_waitcnt(wait_vm((NS - 2) * (XI + DI + SI)));      // as in k_rows_dma
+        else __builtin_amdgcn_s_waitcnt(wait_vm(0));
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (s + NS - 1 < count) issue(s + NS - 1, slot == 0 ? NS - 1 : slot - 1);
+        const char* const cur = lds + slot * STAGE;
+#pragma unroll
+        for (int b = 0; b < BK / 16; ++b) {
+            u32x4 fp[NP][LX], fq[NQ][LD];
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int c0 = wp * WP + i * 32;
+                if constexpr (P8) fp[i][0] = frag8(cur, cur + XB + DB, b * 16, c0);
+                else if constexpr (DT == BS_DT_F32) frag32(cur, XR, b * 16, c0, fp[i]);
+                else fp[i][0] = frag16(cur, XR, b * 16, c0);
+            }
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) {
+                const int c0 = wq * WQ + j * 32;
+                if constexpr (DT == BS_DT_F32) frag32(cur + XB, DR, b * 16, c0, fq[j]);
+                else fq[j][0] = frag16(cur + XB, DR, b * 16, c0);
+            }
+            multiply<DT, LX, LD, NP, NQ>(fp, fq, acc);
+        }
+        slot = slot + 1 == NS ? 0 : slot + 1;
+    }
+    __syncthreads();
+    float* const mine = reinterpret_cast<float*>(lds + wave * TURN);
+#pragma unroll
+    for (int j = 0; j < NQ; ++j)
+#pragma unroll
+        for (int i = 0; i < NP; i += 2) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                float* const at = mine + (lane & 31) * 68 + 8 * g + 4 * (lane >> 5);
+                *reinterpret_cast<f32x4*>(at) = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+                *reinterpret_cast<f32x4*>(at + 32) = f32x4{acc[i + 1][j][4 * g], acc[i + 1][j][4 * g + 1], acc[i + 1][j][4 * g + 2], acc[i + 1][j][4 * g + 3]};
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const int p = p0 + wp * WP + i * 32 + lane % 16 * 4, n = a.K - p;
+            if (n > 0)
+                for (int r = lane / 16; r < 32; r += 4) {
+                    const int q = q0 + wq * WQ + j * 32 + r;
+                    if (q >= a.N) break;
+                    f32x4 v = *reinterpret_cast<const f32x4*>(mine + r * 68 + lane % 16 * 4);
+                    if (DT == BS_DT_F32) again_over<DT, P8>(a, kb, ke, p, q, n, v);
+                    float* const o = reinterpret_cast<float*>(a.out) + ((int64_t)part * a.N + q) * a.K + p;
+                    if (n >= 4) store16((char*)o, __builtin_bit_cast(u32x4, v));
+                    else
+                        for (int e = 0; e < n; ++e) o[e] = v[e];
+                }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+}
+
+// exponents [rows, nb] -> 2^e as floats [nb][ld], zero from rows to ld
+__global__ __launch_bounds__(256) void k_lay_steps(const int8_t* __restrict__ exps, int64_t rows, int nb, float* __restrict__ out, int64_t ld) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= ld) return;
+    for (int b = 0; b < nb; ++b) out[b * ld + i] = i < rows ? p8_pow2(exps[i * nb + b]) : 0.0f;
 }
 
 // parts [nparts][n] float32 -> their sum in dtype; 64 threads of four neighbours x 4 lanes over the parts
@@ -873,9 +1074,12 @@ int launch_rows(RowsArgs a, void* workspace, int64_t bytes, hipStream_t st) {
     return rows_rc();
 }
 
-// how the rows of a weight gradient are cut into parts: enough workgroups to fill the chip twice over, none under 256 rows
-void split_rows(int64_t rows, int K, int N, int64_t* part, int64_t* parts) {
-    const int64_t tiles = (int64_t)((K + 127) / 128) * ((N + 127) / 128);
+// How a weight gradient is cut: tiles of BQ x 128 outputs (256 channels of ds where there are that many), and the rows into as many
+// parts as give the chip two workgroups a compute unit, none under 256 rows.
+int over_bq(int dtype, int N) { return dtype != BS_DT_F32 && N > 128 ? 256 : 128; }
+void split_rows(int dtype, int64_t rows, int K, int N, int64_t* part, int64_t* parts) {
+    const int bq = over_bq(dtype, N);
+    const int64_t tiles = (int64_t)((K + 127) / 128) * ((N + bq - 1) / bq);
     int64_t want = (512 + tiles - 1) / tiles;
     const int64_t most = (rows + 255) / 256;
     if (want > most) want = most;
@@ -884,19 +1088,43 @@ void split_rows(int64_t rows, int K, int N, int64_t* part, int64_t* parts) {
     if (*part < 64) *part = 64;                               // no rows
     *parts = rows ? (rows + *part - 1) / *part : 1;
 }
+int64_t steps_bytes(int64_t rows, int K) { return (int64_t)((K + 31) / 32) * ((rows + 63) / 64 * 64) * 4; }
 
 template <int DT>
-int launch_over(OverArgs a, hipStream_t st) {
-    constexpr int BK = DT == BS_DT_F32 ? 16 : 64;
-    const int64_t blocks = (a.tiles + 7) / 8 * 8;
+int launch_over(OverArgs a, char* steps, hipStream_t st) {
+    constexpr int BK = DT == BS_DT_F32 ? 16 : 64, CK = 16 / esize(DT);
+    auto go = [&](int bq) {
+        a.tp = (a.K + 127) / 128;
+        a.tiles = (int64_t)a.tp * ((a.N + bq - 1) / bq) * a.parts;
+        return (a.tiles + 7) / 8 * 8;
+    };
+    auto whole = [](const void* p, int64_t ld, int n, int ck, int es) {
+        return n % ck == 0 && ld % ck == 0 && ((uintptr_t)p & 15) == 0 && ld * es < (1 << 22);
+    };
+    const bool dd = whole(a.ds, a.ldds, a.N, CK, esize(DT));
+    const bool xd = a.exps ? whole(a.x, a.ldx, a.K, 16, 1) : whole(a.x, a.ldx, a.K, CK, esize(DT));
+    const int64_t ld = (a.rows + 63) / 64 * 64;
+#define OVER(P8, BQ, WQ, BK_, NS) do { const int64_t blocks = go(BQ); if (blocks > 0x7fffffff) return BS_EINVAL; \
+        hipLaunchKernelGGL((k_over_dma<DT, P8, BQ, 128, WQ, 64, BK_, NS>), dim3((unsigned)blocks), dim3(256), 0, st, a, (const float*)steps, ld); } while (0)
+    if (xd && dd && a.rows < (1 << 30)) {
+        if (a.exps) {
+            const int nb = (a.K + 31) / 32;
+            hipLaunchKernelGGL(k_lay_steps, dim3((unsigned)((ld + 255) / 256)), dim3(256), 0, st, a.exps, a.rows, nb, (float*)steps, ld);
+            if constexpr (DT == BS_DT_F32) OVER(true, 128, 64, 32, 3);
+            else if (over_bq(DT, a.N) == 256) OVER(true, 256, 128, 32, 3);
+            else OVER(true, 128, 64, 32, 4);
+        } else {
+            if constexpr (DT == BS_DT_F32) OVER(false, 128, 64, 16, 4);
+            else if (over_bq(DT, a.N) == 256) OVER(false, 256, 128, 32, 3);
+            else OVER(false, 128, 64, 32, 4);
+        }
+        return rows_rc();
+    }
+#undef OVER
+    const int64_t blocks = go(128);
     if (blocks > 0x7fffffff) return BS_EINVAL;
     const dim3 grid((unsigned)blocks);
-    auto whole = [](const char* p, int64_t ld, int n) { return DT != BS_DT_F32 && n % 8 == 0 && ld % 8 == 0 && ((uintptr_t)p & 15) == 0; };
-    const bool xd = !a.exps && whole(a.x, a.ldx, a.K), dd = whole(a.ds, a.ldds, a.N);
-    constexpr int DMA = DT != BS_DT_F32 ? S_DMA : S_REG;
-    if (a.exps && dd) hipLaunchKernelGGL((k_over_rows<DT, S_P8, DMA, BK>), grid, dim3(256), 0, st, a);
-    else if (a.exps) hipLaunchKernelGGL((k_over_rows<DT, S_P8, S_REG, BK>), grid, dim3(256), 0, st, a);
-    else if (xd && dd) hipLaunchKernelGGL((k_over_rows<DT, DMA, DMA, BK>), grid, dim3(256), 0, st, a);
+    if (a.exps) hipLaunchKernelGGL((k_over_rows<DT, S_P8, S_REG, BK>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((k_over_rows<DT, S_REG, S_REG, BK>), grid, dim3(256), 0, st, a);
     return rows_rc();
 }
@@ -947,11 +1175,11 @@ int bs_linear_grad_x(const void* ds, int64_t ldds, const void* w, int64_t ldw, v
     return launch_rows<BS_DT_F16, E_PLAIN>(a, workspace, workspace_bytes, st);
 }
 
-int64_t bs_linear_grad_w_workspace(int dtype, int64_t rows, int K, int N) {
+int64_t bs_linear_grad_w_workspace(int dtype, int64_t rows, int K, int N, int codes) {
     if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1) return BS_EINVAL;
     int64_t part, parts;
-    split_rows(rows, K, N, &part, &parts);
-    return parts > 1 || dtype != BS_DT_F32 ? parts * K * N * 4 : 0;
+    split_rows(dtype, rows, K, N, &part, &parts);
+    return (codes ? steps_bytes(rows, K) : 0) + (parts > 1 || dtype != BS_DT_F32 ? parts * K * N * 4 : 0);
 }
 
 int bs_linear_grad_w(const void* ds, int64_t ldds, const void* x, const int8_t* x_exps, int64_t ldx, void* dw, int dtype,
@@ -961,23 +1189,24 @@ int bs_linear_grad_w(const void* ds, int64_t ldds, const void* x, const int8_t* 
     hipStream_t st = rows_stream(stream);
     const int64_t n = (int64_t)K * N;
     int64_t part, parts;
-    split_rows(rows, K, N, &part, &parts);
+    split_rows(dtype, rows, K, N, &part, &parts);
     const bool joined = parts > 1 || dtype != BS_DT_F32;
-    if (joined && rows > 0 && (!workspace || workspace_bytes < parts * n * 4)) return BS_EINVAL;
+    const int64_t before = x_exps ? steps_bytes(rows, K) : 0;           // workspace: steps of the codes, then the parts
+    const int64_t need = before + (joined ? parts * n * 4 : 0);
+    if (need > 0 && rows > 0 && (!workspace || workspace_bytes < need)) return BS_EINVAL;
     int rc = BS_OK;
     if (rows > 0) {
         OverArgs a = {};
         a.x = (const char*)x; a.exps = x_exps; a.ldx = ldx; a.ds = (const char*)ds; a.ldds = ldds; a.rows = rows; a.part = part;
         a.K = K; a.N = N; a.nb = (K + P8_BLOCK - 1) / P8_BLOCK; a.parts = (int)parts;
-        a.tp = (K + 127) / 128;
-        a.tiles = (int64_t)a.tp * ((N + 127) / 128) * parts;
-        a.out = (char*)(joined ? workspace : dw);
-        rc = dtype == BS_DT_F32 ? launch_over<BS_DT_F32>(a, st) : dtype == BS_DT_BF16 ? launch_over<BS_DT_BF16>(a, st) : launch_over<BS_DT_F16>(a, st);
+        char* const ws = (char*)workspace;
+        a.out = joined ? ws + before : (char*)dw;
+        rc = dtype == BS_DT_F32 ? launch_over<BS_DT_F32>(a, ws, st) : dtype == BS_DT_BF16 ? launch_over<BS_DT_BF16>(a, ws, st) : launch_over<BS_DT_F16>(a, ws, st);
         if (rc != BS_OK || !joined) return rc;
     } else {
         parts = 0;                                            // the sum of no parts
     }
-    const float* ws = (const float*)workspace;
+    const float* ws = (const float*)((const char*)workspace + before);
     const dim3 blocks((unsigned)((n + 255) / 256));
     if (dtype == BS_DT_F32) hipLaunchKernelGGL(k_add_parts<BS_DT_F32>, blocks, dim3(256), 0, st, ws, (int)parts, n, (char*)dw);
     else if (dtype == BS_DT_BF16) hipLaunchKernelGGL(k_add_parts<BS_DT_BF16>, blocks, dim3(256), 0, st, ws, (int)parts, n, (char*)dw);

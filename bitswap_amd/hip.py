@@ -89,7 +89,7 @@ def load():
     L.bs_act_grad_workspace.argtypes = [i64, i32]
     L.bs_act_grad.argtypes = [p, i64, p, i64, p, p, i64, i32, i32, i64, i32, p, p, p, i64, p]
     L.bs_linear_grad_x.argtypes = [p, i64, p, i64, p, i32, i64, i32, i32, p, i64, p]
-    L.bs_linear_grad_w_workspace.argtypes = [i32, i64, i32, i32]
+    L.bs_linear_grad_w_workspace.argtypes = [i32, i64, i32, i32, i32]
     L.bs_linear_grad_w.argtypes = [p, i64, p, p, i64, p, i32, i64, i32, i32, p, i64, p]
     L.bs_group_norm_workspace.argtypes = [i32, i64, i64, i32, i32, i32]
     L.bs_group_norm_act.argtypes = [p, i64, i64, p, p, i32, C.c_float, i32, i32, i64, i64, i32, i32, p, p, p, i64, p]
@@ -1030,7 +1030,7 @@ def linear_act_grad(x, w, s=None, act=ACT_NONE, g_sum=None, g_act=None, want_x=T
         _check(L.bs_linear_grad_x(_ptr(dt), ldd, _ptr(wt), ldw, _ptr(dx), code, rows, K, N, _ptr(ws), nb, _stream()), "bs_linear_grad_x")
     if want_w:
         dw = torch.empty((N, K), dtype=w.dtype, device=dev)
-        nb = L.bs_linear_grad_w_workspace(code, rows, K, N)
+        nb = L.bs_linear_grad_w_workspace(code, rows, K, N, int(xe is not None))
         ws = _workspace(nb, dev)
         _check(L.bs_linear_grad_w(_ptr(dt), ldd, _ptr(xt), _ptr(xe), ldx, _ptr(dw), code, rows, K, N, _ptr(ws), nb, _stream()),
                "bs_linear_grad_w")

@@ -365,7 +365,7 @@ int bs_wino_out_f32(const float* M, const float* bias, const float* res, float* 
  * bs_linear_grad_x -- dx [rows, K] = ds w;  ds [rows, N] (row stride ldds), w [N, K].  workspace: bs_linear_grad_x_workspace bytes.
  * bs_linear_grad_w -- dw [N, K] = ds^T x;  x [rows, K] of dtype (row stride ldx) or, if x_exps is given, codes of bs_pack8.  The
  *   rows are split over the chip into parts of a size fixed by (rows, N, K) and the parts added in order: the same call gives the
- *   same bits.  workspace: bs_linear_grad_w_workspace bytes (may be 0).
+ *   same bits.  workspace: bs_linear_grad_w_workspace bytes (may be 0; codes: whether x is in 8 bits).
  *
  * bs_group_norm_act -- x [n, pixels, channels] (strides ldn, ldp), groups dividing channels: mean and biased variance over the
  *   pixels and channels of a group, u = (x - mean) / sqrt(var + eps) * gamma + beta, y = act(u), y contiguous; stats
@@ -400,7 +400,7 @@ int bs_act_grad(const void* g_sum, int64_t ldgs, const void* g_act, int64_t ldga
 int64_t bs_linear_grad_x_workspace(int dtype, int64_t rows, int K, int N);
 int bs_linear_grad_x(const void* ds, int64_t ldds, const void* w, int64_t ldw, void* dx, int dtype, int64_t rows, int K, int N,
                      void* workspace, int64_t workspace_bytes, void* stream);
-int64_t bs_linear_grad_w_workspace(int dtype, int64_t rows, int K, int N);
+int64_t bs_linear_grad_w_workspace(int dtype, int64_t rows, int K, int N, int codes);
 int bs_linear_grad_w(const void* ds, int64_t ldds, const void* x, const int8_t* x_exps, int64_t ldx, void* dw, int dtype,
                      int64_t rows, int K, int N, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t bs_group_norm_workspace(int dtype, int64_t n, int64_t pixels, int channels, int groups, int grad);
