@@ -11,6 +11,8 @@
 //
 // The output channel is the row index of the matrix instruction: a lane then holds, for one row q = lane % 32 of activations, the
 // channels 8 g + 4 (lane / 32) + 0..3, g = 0..3, of a 32x32 tile.
+#include <type_traits>
+
 #include "rows_dev.h"
 
 namespace {
@@ -320,9 +322,9 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_rows(const RowsA
 }
 
 // ---- ... whose rows are whole aligned 16-byte chunks --------------------------------------------------------------------------------
-// Both operands come by DMA through a ring of NS buffers, NS - 1 steps ahead, with one barrier a step: its wait is for the step it
-// opens only (the DMA of later steps stays in flight).  float32 rows lie in shared memory as they are and are split into limbs
-// after the read: 32 bytes a fragment instead of 48, and nothing goes back to shared memory.
+// Both operands come by DMA through a ring of NS buffers with one barrier a step; fragments are read one 16-deep block ahead of
+// the matrix instructions.  float32 rows lie in shared memory as they are and are split into limbs after the read, between the
+// matrix instructions of the block before: 32 bytes a fragment instead of 48, and nothing goes back to shared memory.
 __device__ __forceinline__ constexpr int wait_vm(int v) { return (v & 15) | (7 << 4) | ((v >> 4) << 14); }      // vmcnt(v), lgkmcnt(0)
 
 template <int DT, int EPI, int BQ, int BP, int WQ, int WP, int BK, int NS>
@@ -363,7 +365,24 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_rows_dma(const R
         const int k = swz(WS, row, lane % WS) * 8;
         wo[n] = (uint32_t)((limb * a.sl + pr * a.sp + k / KB * a.sk + k % KB) * 2);
     }
+    // a step whose k all exist: no branch among the loads
+    auto issue_whole = [&](int s, int slot) {
+        char* const st = lds + slot * STAGE;
+        const char* const xs = xb + (int64_t)s * BK * ES;
+        const char* const ws = wb + (int64_t)s * (BK / KB) * a.sk * 2;
+#pragma unroll
+        for (int n = 0; n < XI; ++n) {
+            const char* const src = xs + xo[n];
+            __builtin_amdgcn_global_load_lds(src, (lds_ptr)(st + (wave * XI + n) * 1024), 16, 0, 0);
+        }
+#pragma unroll
+        for (int n = 0; n < WI; ++n) {
+            const char* const src = ws + wo[n];
+            __builtin_amdgcn_global_load_lds(src, (lds_ptr)(st + XB + (wave * WI + n) * 1024), 16, 0, 0);
+        }
+    };
     auto issue = [&](int s, int slot) {
+        if ((s + 1) * BK <= a.K) return issue_whole(s, slot);
         char* const st = lds + slot * STAGE;
         const char* const xs = xb + (int64_t)s * BK * ES;
         const char* const ws = wb + (int64_t)s * (BK / KB) * a.sk * 2;
@@ -379,6 +398,45 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_rows_dma(const R
             __builtin_amdgcn_global_load_lds(src, (lds_ptr)(st + XB + (wave * WI + n) * 1024), 16, 0, 0);
         }
     };
+    // fragments of 16 k: w's limbs, x as it lies in shared memory
+    struct Frag {
+        u32x4 p[NP][L], q[NQ][DT == BS_DT_F32 ? 2 : 1];
+    };
+    auto read = [&](const char* st, int b, Frag& f) {
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+            const int row = wq * WQ + j * 32 + (lane & 31);
+#pragma unroll
+            for (int h = 0; h < (DT == BS_DT_F32 ? 2 : 1); ++h) {
+                const int c = DT == BS_DT_F32 ? 4 * b + 2 * (lane >> 5) + h : 2 * b + (lane >> 5);
+                f.q[j][h] = *reinterpret_cast<const u32x4*>(st + row * (BK * ES) + swz(XS, row, c) * 16);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int row = wp * WP + i * 32 + (lane & 31);
+#pragma unroll
+            for (int l = 0; l < L; ++l)
+                f.p[i][l] = *reinterpret_cast<const u32x4*>(st + XB + (l * BP + row) * (BK * 2) + swz(WS, row, 2 * b + (lane >> 5)) * 16);
+        }
+    };
+    auto split = [&](const Frag& f, u32x4 (&q)[NQ][L]) {
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+            if constexpr (DT == BS_DT_F32) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t l3[3];
+                    limbs2(bits_f32(f.q[j][e / 2][(2 * e) & 3]), bits_f32(f.q[j][e / 2][(2 * e + 1) & 3]), l3);
+                    q[j][0][e] = l3[0];
+                    q[j][1][e] = l3[1];
+                    q[j][2][e] = l3[2];
+                }
+            } else {
+                q[j][0] = f.q[j][0];
+            }
+        }
+    };
     f32x16 acc[NP][NQ];
 #pragma unroll
     for (int i = 0; i < NP; ++i)
@@ -387,50 +445,66 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_rows_dma(const R
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
 #pragma unroll
-    for (int s = 0; s < NS - 1; ++s)
+    for (int s = 0; s < NS; ++s)
         if (s < steps) issue(s, s);
+    if (NS <= a.K / BK) __builtin_amdgcn_s_waitcnt(wait_vm((NS - 1) * (XI + WI)));      // NS whole steps are on their way
+    else __builtin_amdgcn_s_waitcnt(wait_vm(0));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    constexpr int SB = BK / 16;
+    Frag f;
+    u32x4 q[NQ][L];
+    read(lds, 0, f);
+    split(f, q);
     int slot = 0;
-    for (int s = 0; s < steps; ++s) {
-        // the steps behind this one may stay in flight: NS - 2 of them while there are that many (a step whose x lies behind K in
-        // part has fewer loads in flight than counted: only the last one, after which everything is waited for)
-        if (s + NS - 1 < steps) __builtin_amdgcn_s_waitcnt(wait_vm((NS - 2) * (XI + WI)));
-        else __builtin_amdgcn_s_waitcnt(wait_vm(0));
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (s + NS - 1 < steps) issue(s + NS - 1, slot == 0 ? NS - 1 : slot - 1);
-        const char* const cur = lds + slot * STAGE;
+    // One step.  RUN: the step NS ahead exists whole.  The next step has landed for this wavefront once only the DMA of the NS - 2 steps
+    // behind it is in flight (near the end everything is waited for), and for all of them after the barrier; what was read of this
+    // step is in registers (lgkmcnt), its buffer takes the step NS ahead.  Reads, DMA and the split go between the matrix
+    // instructions, which work on what was read a block before.
+    auto step = [&](int s, auto run) {
+        constexpr bool RUN = decltype(run)::value;
+        constexpr int M = (L == 3 ? 6 : 1) * NP * NQ, R = NQ * (DT == BS_DT_F32 ? 2 : 1) + NP * L, D = XI + WI;
+        const int next = slot + 1 == NS ? 0 : slot + 1;
 #pragma unroll
-        for (int b = 0; b < BK / 16; ++b) {
-            u32x4 fp[NP][L], fq[NQ][L];
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const int row = wp * WP + i * 32 + (lane & 31);
-#pragma unroll
-                for (int l = 0; l < L; ++l)
-                    fp[i][l] = *reinterpret_cast<const u32x4*>(cur + XB + (l * BP + row) * (BK * 2) + swz(WS, row, 2 * b + (lane >> 5)) * 16);
+        for (int b = 0; b < SB; ++b) {
+            Frag g;
+            if (b == SB - 1) {
+                if (RUN) __builtin_amdgcn_s_waitcnt(wait_vm((NS - 2) * D));
+                else __builtin_amdgcn_s_waitcnt(wait_vm(0));
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                if (!RUN && s + NS < steps) issue(s + NS, slot);
+                __builtin_amdgcn_sched_barrier(0);
+                read(lds + next * STAGE, 0, g);               // (behind the last step: not used)
+                if (RUN) issue_whole(s + NS, slot);
+            } else {
+                __builtin_amdgcn_sched_barrier(0);
+                read(lds + slot * STAGE, b + 1, g);
             }
+            u32x4 qn[NQ][L];
+            multiply<DT, L, L, NP, NQ>(f.p, q, acc);
+            split(g, qn);
 #pragma unroll
-            for (int j = 0; j < NQ; ++j) {
-                const int row = wq * WQ + j * 32 + (lane & 31);
-                if (DT == BS_DT_F32) {
-                    const int c = 4 * b + 2 * (lane >> 5);
-                    const u32x4 r0 = *reinterpret_cast<const u32x4*>(cur + row * (BK * ES) + swz(XS, row, c) * 16);
-                    const u32x4 r1 = *reinterpret_cast<const u32x4*>(cur + row * (BK * ES) + swz(XS, row, c + 1) * 16);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        uint32_t l3[3];
-                        limbs2(bits_f32(e < 2 ? r0[(2 * e) & 3] : r1[(2 * e) & 3]), bits_f32(e < 2 ? r0[(2 * e + 1) & 3] : r1[(2 * e + 1) & 3]), l3);
-#pragma unroll
-                        for (int l = 0; l < L; ++l) fq[j][l][e] = l3[l % 3];
-                    }
-                } else {
-                    fq[j][0] = *reinterpret_cast<const u32x4*>(cur + row * (BK * ES) + swz(XS, row, 2 * b + (lane >> 5)) * 16);
-                }
+            for (int m = 0; m < M; ++m) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                                       // one matrix instruction
+                if (m < (R + 1) / 2) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);                  // two LDS reads
+                else if (RUN && b == SB - 1 && m < (R + 1) / 2 + D) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+                if (L == 3 && m >= M / 2) __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
             }
-            multiply<DT, L, L, NP, NQ>(fp, fq, acc);
+            __builtin_amdgcn_sched_barrier(0);
+            f = g;
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                for (int l = 0; l < L; ++l) q[j][l] = qn[j][l];
         }
-        slot = slot + 1 == NS ? 0 : slot + 1;
-    }
+        slot = next;
+    };
+    const int whole = a.K / BK;                               // steps s with s + NS < whole have a whole step NS ahead
+    int s = 0;
+#pragma unroll SB == 1 ? 2 : 1
+    for (; s + NS < whole; ++s) step(s, std::true_type{});
+    for (; s < steps; ++s) step(s, std::false_type{});
     __syncthreads();
     float* const mine = reinterpret_cast<float*>(lds + wave * TURN);
 #pragma unroll
@@ -1066,10 +1140,10 @@ int launch_rows(RowsArgs a, void* workspace, int64_t bytes, hipStream_t st) {
         hipLaunchKernelGGL((KERNEL), dim3((unsigned)blocks), dim3(NT), 0, st, a); } while (0)
 #define K_(...) __VA_ARGS__
     if constexpr (DT == BS_DT_F32) {
-        if (dma) ROWS(K_(k_rows_dma<DT, EPI, 128, 128, 64, 64, 16, 2>), 128, 128, 256);
+        if (dma) ROWS(K_(k_rows_dma<DT, EPI, 128, 128, 64, 64, 16, 4>), 128, 128, 256);
         else ROWS(K_(k_rows<DT, EPI, 128, 128, 64, 64, 16>), 128, 128, 256);
     } else {
-        if (dma) ROWS(K_(k_rows_dma<DT, EPI, 256, 256, 128, 64, 64, 2>), 256, 256, 512);
+        if (dma) ROWS(K_(k_rows_dma<DT, EPI, 256, 256, 128, 64, 32, 4>), 256, 256, 512);
         else ROWS(K_(k_rows<DT, EPI, 128, 128, 64, 64, 64>), 128, 128, 256);
     }
 #undef K_
