@@ -327,15 +327,15 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_rows(const RowsA
 // matrix instructions of the block before: 32 bytes a fragment instead of 48, and nothing goes back to shared memory.
 __device__ __forceinline__ constexpr int wait_vm(int v) { return (v & 15) | (7 << 4) | ((v >> 4) << 14); }      // vmcnt(v), lgkmcnt(0)
 
-template <int DT, int EPI, int BQ, int BP, int WQ, int WP, int BK, int NS>
-__global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_rows_dma(const RowsArgs a) {
+template <int DT, int EPI, int BQ, int BP, int WQ, int WP, int BK, int NS, int PER_SIMD>
+__global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64, PER_SIMD) void k_rows_dma(const RowsArgs a) {
     constexpr int NW = (BQ / WQ) * (BP / WP), L = limbs_of(DT), ES = esize(DT), CK = 16 / ES;       // CK: k of a chunk of x
     constexpr int XS = BK * ES / 16, WS = BK / 8;                                                    // chunks of a row
     constexpr int XB = BQ * BK * ES, WB = L * BP * BK * 2, STAGE = XB + WB;
     constexpr int XI = XB / 1024 / NW, WI = WB / 1024 / NW;
     constexpr int NP = WP / 32, NQ = WQ / 32;
-    static_assert(XB % (1024 * NW) == 0 && WB % (1024 * NW) == 0 && NS * STAGE <= 160 * 1024 && NW * TURN <= NS * STAGE && NP % 2 == 0, "");
-    __shared__ __align__(16) char lds[NS * STAGE];
+    static_assert(XB % (1024 * NW) == 0 && WB % (1024 * NW) == 0 && NS * STAGE <= 160 * 1024 && NP % 2 == 0, "");
+    __shared__ __align__(16) char lds[NS * STAGE > NW * TURN ? NS * STAGE : NW * TURN];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wp = wave % (BP / WP), wq = wave / (BP / WP);
     auto swz = [](int slots, int row, int c) { return slots == 8 ? (c ^ ((row >> 1) & 7)) : slots == 4 ? (c ^ ((row >> 2) & 3)) : (c ^ ((row >> 3) & 1)); };
@@ -882,7 +882,7 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
     constexpr int XI = XB / 1024 / NW, DI = DB / 1024 / NW, SI = P8 ? 1 : 0;
     constexpr int NP = WP / 32, NQ = WQ / 32;
     static_assert(XB % (1024 * NW) == 0 && DB % (1024 * NW) == 0 && NS * STAGE <= 160 * 1024 && NW * TURN <= NS * STAGE, "shared memory");
-    static_assert(!P8 || (SB % NW == 0 && SB / NW <= 256), "steps: one dword a lane and wavefront");
+    static_assert(!P8 || (SB % 256 == 0 && SB / 256 <= NW), "steps: one dword a lane");
     __shared__ __align__(16) char lds[NS * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wp = wave % (BP / WP), wq = wave / (BP / WP);
@@ -916,11 +916,31 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
         dof[n] = (uint32_t)((int64_t)row * a.ldds * ES + (q0 + c * (16 / ES) < a.N ? c * 16 : 0));
     }
     const float* sp = nullptr;
-    if (P8) {
-        const int i = wave * (SB / 4 / NW) + (lane < SB / 4 / NW ? lane : 0), blk = i / BK, nb = (a.K + 31) / 32;
+    if constexpr (P8) {
+        const int i = wave % (SB / 256) * 64 + lane, blk = i / BK, nb = (a.K + 31) / 32;
         sp = steps + (int64_t)(p0 / 32 + blk < nb ? p0 / 32 + blk : nb - 1) * ldsteps + kb + i % BK;
     }
+    auto issue_whole = [&](int s, int slot) {                             // all its rows exist: no branch among the loads
+        char* const st = lds + slot * STAGE;
+        const char* const xs = xb + (int64_t)s * BK * a.ldx * XE;
+        const char* const ds = db + (int64_t)s * BK * a.ldds * ES;
+#pragma unroll
+        for (int n = 0; n < XI; ++n) {
+            const char* const src = xs + xo[n];
+            __builtin_amdgcn_global_load_lds(src, (lds_ptr)(st + (wave * XI + n) * 1024), 16, 0, 0);
+        }
+#pragma unroll
+        for (int n = 0; n < DI; ++n) {
+            const char* const src = ds + dof[n];
+            __builtin_amdgcn_global_load_lds(src, (lds_ptr)(st + XB + (wave * DI + n) * 1024), 16, 0, 0);
+        }
+        if constexpr (P8) {              // (wavefronts beyond the first SB / 256 write the same steps once more: every one counts alike)
+            const char* const src = (const char*)(sp + s * BK);
+            __builtin_amdgcn_global_load_lds(src, (lds_ptr)(st + XB + DB + wave % (SB / 256) * 256), 4, 0, 0);
+        }
+    };
     auto issue = [&](int s, int slot) {
+        if ((s + 1) * BK <= nk) return issue_whole(s, slot);
         char* const st = lds + slot * STAGE;
         const char* const xs = xb + (int64_t)s * BK * a.ldx * XE;
         const char* const ds = db + (int64_t)s * BK * a.ldds * ES;
@@ -939,64 +959,104 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
             if (dr[n] < left) __builtin_amdgcn_global_load_lds(src, (lds_ptr)dst, 16, 0, 0);
             else *reinterpret_cast<u32x4*>(dst + lane * 16) = u32x4{0, 0, 0, 0};
         }
-        if (P8) {
+        if constexpr (P8) {
             const char* const src = (const char*)(sp + s * BK);
-            char* const dst = st + XB + DB + wave * (SB / NW);
-            if (lane < SB / 4 / NW) __builtin_amdgcn_global_load_lds(src, (lds_ptr)dst, 4, 0, 0);
+            __builtin_amdgcn_global_load_lds(src, (lds_ptr)(st + XB + DB + wave % (SB / 256) * 256), 4, 0, 0);
         }
     };
-    // channel c0 + lane % 32, rows r0 + 8 (lane / 32) + 0..7 of a 16-bit tile with rows of RB bytes
-    auto frag16 = [&](const char* base, int RB, int r0, int c0) {
-        u32x4 v;
+    uint32_t bad = 0;
+    // Fragments as they are read: channel c0 + lane % 32, rows r0 + 8 (lane / 32) + 0..7.  16-bit: two transposing reads of 4 rows,
+    // codes: one of 8 rows and the rows' steps, float32: 8 dwords.
+    struct Raw16 { u32x4 v; };
+    struct Raw32 { float f[8]; };
+    struct Raw8 { i32x2 w; f32x4 s[2]; };
+    typedef typename std::conditional<P8, Raw8, typename std::conditional<DT == BS_DT_F32, Raw32, Raw16>::type>::type RawX;
+    typedef typename std::conditional<DT == BS_DT_F32, Raw32, Raw16>::type RawD;
+    constexpr int RX = P8 ? 3 : DT == BS_DT_F32 ? 8 : 2, RD = DT == BS_DT_F32 ? 8 : 2;              // reads of a fragment
+    auto read_plain = [&](const char* base, int RB, int r0, int c0, auto& r) {
+        if constexpr (DT == BS_DT_F32) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int row = r0 + 8 * (lane >> 5) + 4 * h + ((lane & 15) >> 2), ch = c0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-            const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(base + row * RB + (((ch >> 3) ^ sd(row)) * 16) + (ch & 4) * 2));
-            const u32x2 w2 = __builtin_bit_cast(u32x2, w);
-            v[2 * h] = w2[0];
-            v[2 * h + 1] = w2[1];
-        }
-        return v;
-    };
-    auto frag32 = [&](const char* base, int RB, int r0, int c0, u32x4* l) {
-        float f[8];
+            for (int e = 0; e < 8; ++e) {
+                const int row = r0 + 8 * (lane >> 5) + e, ch = c0 + (lane & 31);
+                r.f[e] = *reinterpret_cast<const float*>(base + row * RB + ((ch >> 2) ^ sd(row)) * 16 + (ch & 3) * 4);
+            }
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int row = r0 + 8 * (lane >> 5) + e, ch = c0 + (lane & 31);
-            f[e] = *reinterpret_cast<const float*>(base + row * RB + ((ch >> 2) ^ sd(row)) * 16 + (ch & 3) * 4);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            uint32_t t3[3];
-            limbs2(f[2 * e], f[2 * e + 1], t3);
-            l[0][e] = t3[0];
-            l[1][e] = t3[1];
-            l[2][e] = t3[2];
+            for (int h = 0; h < 2; ++h) {
+                const int row = r0 + 8 * (lane >> 5) + 4 * h + ((lane & 15) >> 2), ch = c0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(base + row * RB + (((ch >> 3) ^ sd(row)) * 16) + (ch & 4) * 2));
+                const u32x2 w2 = __builtin_bit_cast(u32x2, w);
+                r.v[2 * h] = w2[0];
+                r.v[2 * h + 1] = w2[1];
+            }
         }
     };
-    auto frag8 = [&](const char* base, const char* sbase, int r0, int c0) {
-        const int row = r0 + 8 * (lane >> 5) + ((lane & 15) >> 1), ch = c0 + 16 * ((lane >> 4) & 1) + 8 * (lane & 1);
-        const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2)(base + row * XR + (((ch >> 4) ^ sx(row)) * 16) + (ch & 8)));
-        float s[8], f[8];
-        *reinterpret_cast<f32x4*>(s) = *reinterpret_cast<const f32x4*>(sbase + (c0 / 32 * BK + r0 + 8 * (lane >> 5)) * 4);
-        *reinterpret_cast<f32x4*>(s + 4) = *reinterpret_cast<const f32x4*>(sbase + (c0 / 32 * BK + r0 + 8 * (lane >> 5) + 4) * 4);
-        uint32_t odd = 0;                                              // a byte 0x80 anywhere
+    auto turn_plain = [&](const auto& r, auto& l) {
+        if constexpr (DT == BS_DT_F32) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)((uint32_t)w[e / 4] >> (8 * (e % 4))) * s[e];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const uint32_t y = (uint32_t)w[e] ^ 0x80808080u;
-            odd |= (y - 0x01010101u) & ~y & 0x80808080u;
+            for (int e = 0; e < 4; ++e) {
+                uint32_t t3[3];
+                limbs2(r.f[2 * e], r.f[2 * e + 1], t3);
+                l[0][e] = t3[0];
+                l[1][e] = t3[1];
+                l[2][e] = t3[2];
+            }
+        } else {
+            l[0] = r.v;
         }
-        if (odd) {
+    };
+    auto read = [&](const char* st, int b, RawX (&x)[NP], RawD (&d)[NQ]) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if ((((uint32_t)w[e / 4] >> (8 * (e % 4))) & 255u) == 0x80u) f[e] = __builtin_nanf("");
+        for (int i = 0; i < NP; ++i) {
+            const int c0 = wp * WP + i * 32;
+            if constexpr (P8) {
+                const int row = b * 16 + 8 * (lane >> 5) + ((lane & 15) >> 1), ch = c0 + 16 * ((lane >> 4) & 1) + 8 * (lane & 1);
+                x[i].w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2)(st + row * XR + (((ch >> 4) ^ sx(row)) * 16) + (ch & 8)));
+                const char* const sb = st + XB + DB + (c0 / 32 * BK + b * 16 + 8 * (lane >> 5)) * 4;
+                x[i].s[0] = *reinterpret_cast<const f32x4*>(sb);
+                x[i].s[1] = *reinterpret_cast<const f32x4*>(sb + 16);
+            } else {
+                read_plain(st, XR, b * 16, c0, x[i]);
+            }
         }
-        u32x4 v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = DT == BS_DT_F16 ? pk_f16(f[2 * e], f[2 * e + 1]) : pk_bf16(f[2 * e], f[2 * e + 1]);
-        return v;
+        for (int j = 0; j < NQ; ++j) read_plain(st + XB, DR, b * 16, wq * WQ + j * 32, d[j]);
+    };
+    auto turn = [&](const RawX (&x)[NP], const RawD (&d)[NQ], u32x4 (&fp)[NP][LX], u32x4 (&fq)[NQ][LD]) {
+        if constexpr (P8) {
+            uint32_t odd = 0;                                            // a byte 0x80 anywhere: a value that was not finite
+            float f[NP][8];
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[i][e] = (float)(int8_t)((uint32_t)x[i].w[e / 4] >> (8 * (e % 4))) * x[i].s[e / 4][e % 4];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t y = (uint32_t)x[i].w[e] ^ 0x80808080u;
+                    odd |= (y - 0x01010101u) & ~y & 0x80808080u;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) fp[i][0][e] = DT == BS_DT_F16 ? pk_f16(f[i][2 * e], f[i][2 * e + 1]) : pk_bf16(f[i][2 * e], f[i][2 * e + 1]);
+            }
+            bad = odd;
+        } else {
+#pragma unroll
+            for (int i = 0; i < NP; ++i) turn_plain(x[i], fp[i]);
+        }
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) turn_plain(d[j], fq[j]);
+    };
+    // (rare) the codes 0x80 of what was just turned, as NaN
+    auto mend = [&](const RawX (&x)[NP], u32x4 (&fp)[NP][LX]) {
+        if constexpr (P8) {
+            if (__builtin_expect(__any(bad != 0), 0)) {
+#pragma unroll
+                for (int i = 0; i < NP; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if ((((uint32_t)x[i].w[e / 4] >> (8 * (e % 4))) & 255u) == 0x80u) fp[i][0][e / 2] |= e & 1 ? 0x7fff0000u : 0x00007fffu;
+            }
+        }
     };
     f32x16 acc[NP][NQ];
 #pragma unroll
@@ -1005,37 +1065,71 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
         for (int j = 0; j < NQ; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+    const int whole = nk / BK;
 #pragma unroll
-    for (int s = 0; s < NS - 1; ++s)
+    for (int s = 0; s < NS; ++s)
         if (s < count) issue(s, s);
+    constexpr int D = XI + DI + SI, SBK = BK / 16;
+    if (NS <= whole) __builtin_amdgcn_s_waitcnt(wait_vm((NS - 1) * D));
+    else __builtin_amdgcn_s_waitcnt(wait_vm(0));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    RawX x0[NP];
+    RawD d0[NQ];
+    u32x4 fp[NP][LX], fq[NQ][LD];
+    read(lds, 0, x0, d0);
+    turn(x0, d0, fp, fq);
+    mend(x0, fp);
     int slot = 0;
-    for (int s = 0; s < count; ++s) {
-        if (s + NS - 1 < count) __builtin_amdgcn_s_waitcnt(wait_vm((NS - 2) * (XI + DI + SI)));      // as in k_rows_dma
-        else __builtin_amdgcn_s_waitcnt(wait_vm(0));
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (s + NS - 1 < count) issue(s + NS - 1, slot == 0 ? NS - 1 : slot - 1);
-        const char* const cur = lds + slot * STAGE;
+    // one step, as in k_rows_dma
+    auto step = [&](int s, auto run) {
+        constexpr bool RUN = decltype(run)::value;
+        constexpr int M = (LX == 3 ? 6 : LD == 3 ? 3 : 1) * NP * NQ, R = NP * RX + NQ * RD, RM = (R + M - 1) / M > 2 ? (R + M - 1) / M : 2;
+        const int next = slot + 1 == NS ? 0 : slot + 1;
 #pragma unroll
-        for (int b = 0; b < BK / 16; ++b) {
-            u32x4 fp[NP][LX], fq[NQ][LD];
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const int c0 = wp * WP + i * 32;
-                if constexpr (P8) fp[i][0] = frag8(cur, cur + XB + DB, b * 16, c0);
-                else if constexpr (DT == BS_DT_F32) frag32(cur, XR, b * 16, c0, fp[i]);
-                else fp[i][0] = frag16(cur, XR, b * 16, c0);
+        for (int b = 0; b < SBK; ++b) {
+            RawX xn[NP];
+            RawD dn[NQ];
+            if (b == SBK - 1) {
+                if (RUN) __builtin_amdgcn_s_waitcnt(wait_vm((NS - 2) * D));
+                else __builtin_amdgcn_s_waitcnt(wait_vm(0));
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                if (!RUN && s + NS < count) issue(s + NS, slot);
+                __builtin_amdgcn_sched_barrier(0);
+                read(lds + next * STAGE, 0, xn, dn);               // (behind the last step: not used)
+                if (RUN) issue_whole(s + NS, slot);
+            } else {
+                __builtin_amdgcn_sched_barrier(0);
+                read(lds + slot * STAGE, b + 1, xn, dn);
             }
-#pragma unroll
-            for (int j = 0; j < NQ; ++j) {
-                const int c0 = wq * WQ + j * 32;
-                if constexpr (DT == BS_DT_F32) frag32(cur + XB, DR, b * 16, c0, fq[j]);
-                else fq[j][0] = frag16(cur + XB, DR, b * 16, c0);
-            }
+            u32x4 pn[NP][LX], qn[NQ][LD];
             multiply<DT, LX, LD, NP, NQ>(fp, fq, acc);
+            turn(xn, dn, pn, qn);
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                if (m * RM < R) __builtin_amdgcn_sched_group_barrier(0x100, RM, 0);
+                if (RUN && b == SBK - 1 && m >= M - D) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+                if ((P8 || DT == BS_DT_F32) && m >= M / 2) __builtin_amdgcn_sched_group_barrier(0x002, P8 && LD == 1 ? 16 : 8, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            mend(xn, pn);
+#pragma unroll
+            for (int i = 0; i < NP; ++i)
+#pragma unroll
+                for (int l = 0; l < LX; ++l) fp[i][l] = pn[i][l];
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                for (int l = 0; l < LD; ++l) fq[j][l] = qn[j][l];
         }
-        slot = slot + 1 == NS ? 0 : slot + 1;
-    }
+        slot = next;
+    };
+    int s = 0;
+#pragma unroll SBK == 1 ? 2 : 1
+    for (; s + NS < whole; ++s) step(s, std::true_type{});
+    for (; s < count; ++s) step(s, std::false_type{});
     __syncthreads();
     float* const mine = reinterpret_cast<float*>(lds + wave * TURN);
 #pragma unroll
@@ -1140,10 +1234,10 @@ int launch_rows(RowsArgs a, void* workspace, int64_t bytes, hipStream_t st) {
         hipLaunchKernelGGL((KERNEL), dim3((unsigned)blocks), dim3(NT), 0, st, a); } while (0)
 #define K_(...) __VA_ARGS__
     if constexpr (DT == BS_DT_F32) {
-        if (dma) ROWS(K_(k_rows_dma<DT, EPI, 128, 128, 64, 64, 16, 4>), 128, 128, 256);
+        if (dma) ROWS(K_(k_rows_dma<DT, EPI, 64, 128, 32, 64, 16, 3, 3>), 64, 128, 256);
         else ROWS(K_(k_rows<DT, EPI, 128, 128, 64, 64, 16>), 128, 128, 256);
     } else {
-        if (dma) ROWS(K_(k_rows_dma<DT, EPI, 256, 256, 128, 64, 32, 4>), 256, 256, 512);
+        if (dma) ROWS(K_(k_rows_dma<DT, EPI, 256, 256, 128, 64, 32, 4, 1>), 256, 256, 512);
         else ROWS(K_(k_rows<DT, EPI, 128, 128, 64, 64, 64>), 128, 128, 256);
     }
 #undef K_

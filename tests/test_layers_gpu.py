@@ -88,6 +88,20 @@ def test_linear_act(hip, rows, k, n, dtype):
         check_linear(hip, x, w, b, r, act, want_sum=act != 3)
 
 
+MANY = [(8300, 96, 130), (33000, 16, 31), (33000, 61, 5), (4200, 256, 272), (4100, 1000, 512), (33100, 8, 24), (9000, 45, 130), (5001, 48, 304)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,n", MANY)
+def test_linear_act_many_rows(hip, rows, k, n, dtype):
+    x, w, b, r = randn((rows, k), dtype, 1), randn((n, k), dtype, 2, k ** -0.5), randn((n,), dtype, 3), randn((rows, n), dtype, 4)
+    check_linear(hip, x, w, b, r, 1)
+    check_linear(hip, x, w, None, None, 3, want_sum=False)
+    wide = randn((rows, k + 16), dtype, 5)
+    check_linear(hip, wide[:, 8:8 + k], w, b, None, 2)                    # aligned as well as its rows are
+    check_linear(hip, wide[:, 3:3 + k], w, None, r, 0)                    # not aligned
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_linear_act_strides_and_leading_axes(hip, dtype):
     wide = randn((3, 50, 80), dtype, 1)
@@ -105,11 +119,12 @@ def test_linear_act_strides_and_leading_axes(hip, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("k,n", [(256, 256), (61, 122), (1000, 72)])
+@pytest.mark.parametrize("k,n", [(256, 256), (61, 122), (1000, 72), (40, 520)])
 def test_linear_act_row_bits_do_not_depend_on_the_number_of_rows(hip, k, n, dtype):
-    x, w, b, r = randn((3000, k), dtype, 1), randn((n, k), dtype, 2, k ** -0.5), randn((n,), dtype, 3), randn((3000, n), dtype, 4)
+    rows = 17000
+    x, w, b, r = randn((rows, k), dtype, 1), randn((n, k), dtype, 2, k ** -0.5), randn((n,), dtype, 3), randn((rows, n), dtype, 4)
     s, y = hip.linear_act(x, w, b, r, act=1, want_sum=True)
-    for lo, hi in ((0, 1), (0, 17), (5, 133), (100, 612), (1, 2000), (2999, 3000)):
+    for lo, hi in ((0, 1), (0, 17), (5, 133), (100, 612), (1, 2000), (16999, 17000), (3, 16500)):
         s2, y2 = hip.linear_act(x[lo:hi], w, b, r[lo:hi], act=1, want_sum=True)
         assert torch.equal(s2, s[lo:hi]) and torch.equal(y2, y[lo:hi]), (lo, hi)
 
@@ -260,6 +275,35 @@ def test_linear_act_grad(hip, rows, k, n, dtype, saved8):
         gs = randn((rows, n), dtype, 5, 0.1) if act % 2 else None
         check_linear_grad(hip, x, w, s, act, gs, ga, saved8)
     check_linear_grad(hip, x, w, s, 1, gs, None, saved8)                  # the sum's gradient alone
+
+
+@pytest.mark.parametrize("saved8", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,n", MANY)
+def test_linear_act_grad_many_rows(hip, rows, k, n, dtype, saved8):
+    x, w, s = randn((rows, k), dtype, 1), randn((n, k), dtype, 2, k ** -0.5), randn((rows, n), dtype, 3)
+    check_linear_grad(hip, x, w, s, 2, randn((rows, n), dtype, 5, 0.1), randn((rows, n), dtype, 4, 0.1), saved8)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,n", [(70, 40, 24), (5000, 64, 144)])
+def test_linear_act_grad_not_finite(hip, rows, k, n, dtype):
+    """A value that was not finite when it was saved makes its column of dw NaN, and no other."""
+    x, w, g = randn((rows, k), dtype, 1), randn((n, k), dtype, 2), randn((rows, n), dtype, 3)
+    clean = hip.linear_act_grad(hip.pack8(x), w, g_act=g)[1]
+    x = x.clone()
+    x[rows // 2, 5] = float("nan")
+    x[rows - 1, 33] = float("inf")
+    p = hip.pack8(x)
+    dw = hip.linear_act_grad(p, w, g_act=g)[1]
+    hit = torch.zeros(k, dtype=torch.bool, device="cuda")
+    hit[[5, 33]] = True
+    assert torch.isnan(dw[:, hit]).all() and torch.isfinite(dw[:, ~hit]).all()
+    other = (torch.arange(k, device="cuda") // 32 != 0) & (torch.arange(k, device="cuda") // 32 != 1)
+    assert torch.equal(dw[:, other], clean[:, other])
+    whole = hip.linear_act_grad(x, w, g_act=g)[1]
+    want = g[:, :].double().t() @ x.double()
+    assert torch.equal(torch.isnan(whole), torch.isnan(want)) and torch.equal(torch.isinf(whole), torch.isinf(want))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
