@@ -4,6 +4,7 @@ There is NO fallback: if the library is missing or there is no GPU, every functi
 raises.  torch is used only for device memory and the current HIP stream.
 """
 import ctypes as C
+import functools
 import os
 
 import numpy as np
@@ -831,6 +832,41 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # BS_DT_*
 PACK8_BLOCK = 32
 
 
+# A call on one latent takes the GPU a few microseconds: the bookkeeping around it is kept to about as much.
+def _gpu(*ts):
+    """_need_cuda, and the current device's index."""
+    cur = None
+    for t in ts:
+        if t is not None:
+            d = t.get_device()
+            if cur is None:
+                cur = torch._C._cuda_getDevice() if d >= 0 else -1
+            if d < 0 or d != cur:
+                _need_cuda(t)
+    return cur
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(name, *sizes):
+    n = getattr(load(), name)(*sizes)
+    if n < 0:
+        raise BitswapHipError(f"{name}: sizes the kernels do not take {sizes}")
+    return n
+
+
+def _raw_stream(dev):
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _scratch(like, nbytes):
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+
+
+
 def _dtype_code(t, what):
     if t.dtype not in _DTYPES:
         raise BitswapHipError(f"{what}: float32, bfloat16 or float16, got {t.dtype}")
@@ -848,6 +884,8 @@ def _as_rows(t, width, what):
     collapse to one stride, rows that overlap (an expanded gradient) or strided channels are copied."""
     if t.dim() < 1 or t.shape[-1] != width:
         raise BitswapHipError(f"{what}: expected [..., {width}], got {tuple(t.shape)}")
+    if t.is_contiguous():
+        return t, width, t.numel() // width
     rows = 1
     for n in t.shape[:-1]:
         rows *= n
@@ -867,12 +905,6 @@ def _affine(name, v, n, like):
     if tuple(v.shape) != (n,) or v.dtype not in (torch.float32, like.dtype):
         raise BitswapHipError(f"{name}: expected [{n}] of float32 or {like.dtype}, got {tuple(v.shape)} {v.dtype}")
     return v.contiguous(), _DTYPES[v.dtype]
-
-
-def _workspace(nbytes, device):
-    if nbytes < 0:
-        raise BitswapHipError("sizes the kernels do not take")
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 class Packed8:
@@ -903,15 +935,15 @@ class Packed8:
 
 def pack8(x):
     """x [..., C] float32 / bfloat16 / float16 -> Packed8."""
-    _need_cuda(x)
+    dev = _gpu(x)
     code = _dtype_code(x, "pack8")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise BitswapHipError(f"pack8: expected [..., C], got {tuple(x.shape)}")
     width = x.shape[-1]
     t, ld, rows = _as_rows(x, width, "pack8")
-    codes = torch.empty((rows, width), dtype=torch.int8, device=x.device)
-    exps = torch.empty((rows, -(-width // PACK8_BLOCK)), dtype=torch.int8, device=x.device)
-    _check(load().bs_pack8(_ptr(t), ld, _ptr(codes), _ptr(exps), code, rows, width, _stream()), "bs_pack8")
+    codes = x.new_empty((rows, width), dtype=torch.int8)
+    exps = x.new_empty((rows, -(-width // PACK8_BLOCK)), dtype=torch.int8)
+    _check(load().bs_pack8(_at(t), ld, _at(codes), _at(exps), code, rows, width, _raw_stream(dev)), "bs_pack8")
     return Packed8(codes, exps, x.shape, x.dtype)
 
 
@@ -919,9 +951,9 @@ def unpack8(p):
     """Packed8 -> the values it holds, contiguous, in the type it was packed from."""
     if not isinstance(p, Packed8):
         raise BitswapHipError("unpack8 takes the Packed8 that pack8() returns")
-    _need_cuda(p.codes, p.exps)
-    x = torch.empty(p.shape, dtype=p.dtype, device=p.device)
-    _check(load().bs_unpack8(_ptr(p.codes), _ptr(p.exps), _ptr(x), _DTYPES[p.dtype], p.codes.shape[0], p.codes.shape[1], _stream()),
+    dev = _gpu(p.codes, p.exps)
+    x = p.codes.new_empty(p.shape, dtype=p.dtype)
+    _check(load().bs_unpack8(_at(p.codes), _at(p.exps), _at(x), _DTYPES[p.dtype], p.codes.shape[0], p.codes.shape[1], _raw_stream(dev)),
            "bs_unpack8")
     return x
 
@@ -931,9 +963,9 @@ def _saved_rows(v, width, dtype, rows, what):
     if isinstance(v, Packed8):
         if v.dtype != dtype or v.codes.shape != (rows, width):
             raise BitswapHipError(f"{what}: expected {rows} rows of {width} {dtype}, got {v.shape} {v.dtype}")
-        _need_cuda(v.codes, v.exps)
+        _gpu(v.codes, v.exps)
         return v.codes, v.exps, width
-    _need_cuda(v)
+    _gpu(v)
     if v.dtype != dtype:
         raise BitswapHipError(f"{what}: expected {dtype}, got {v.dtype}")
     t, ld, n = _as_rows(v, width, what)
@@ -947,7 +979,7 @@ def linear_act(x, w, bias=None, res=None, act=ACT_ELU, want_sum=False, want_act=
     channels-last activations with its epilogue in one launch.  x [..., K] (any row stride), w [N, K], bias [N], res [..., N];
     float32 (limb products, as wino_gemm_bf16x3), bfloat16 or float16, float32 sums.  A row's bits do not depend on how many rows
     there are (include/bitswap_hip.h, bs_linear_act)."""
-    _need_cuda(x, w, bias, res)
+    dev = _gpu(x, w, bias, res)
     code, act = _dtype_code(x, "linear_act"), _act_code(act)
     if w.dim() != 2 or w.dtype != x.dtype or w.shape[0] < 1 or w.shape[1] < 1:
         raise BitswapHipError(f"linear_act: w must be [N, K] of {x.dtype}, got {tuple(w.shape)} {w.dtype}")
@@ -963,13 +995,12 @@ def linear_act(x, w, bias=None, res=None, act=ACT_ELU, want_sum=False, want_act=
         if tuple(res.shape) != shape or res.dtype != x.dtype:
             raise BitswapHipError(f"linear_act: res must be {shape} of {x.dtype}, got {tuple(res.shape)} {res.dtype}")
         rt, ldr, _ = _as_rows(res, N, "linear_act res")
-    s = torch.empty(shape, dtype=x.dtype, device=x.device) if want_sum else None
-    y = torch.empty(shape, dtype=x.dtype, device=x.device) if want_act else None
-    L = load()
-    nb = L.bs_linear_workspace(code, rows, K, N)
-    ws = _workspace(nb, x.device)
-    _check(L.bs_linear_act(_ptr(xt), ldx, _ptr(wt), ldw, _ptr(bias), bcode, _ptr(rt), ldr, _ptr(s), _ptr(y), act, code, rows, K, N,
-                           _ptr(ws), nb, _stream()), "bs_linear_act")
+    s = x.new_empty(shape) if want_sum else None
+    y = x.new_empty(shape) if want_act else None
+    nb = _workspace_bytes("bs_linear_workspace", code, rows, K, N)
+    ws = _scratch(x, nb)
+    _check(load().bs_linear_act(_at(xt), ldx, _at(wt), ldw, _at(bias), bcode, _at(rt), ldr, _at(s), _at(y), act, code, rows, K, N,
+                           _at(ws), nb, _raw_stream(dev)), "bs_linear_act")
     return s, y
 
 
@@ -981,7 +1012,7 @@ def linear_act_grad(x, w, s=None, act=ACT_NONE, g_sum=None, g_act=None, want_x=T
     if g_sum is None and g_act is None:
         raise BitswapHipError("linear_act_grad: no gradient")
     g0 = g_sum if g_sum is not None else g_act
-    _need_cuda(w, g_sum, g_act)
+    dev = _gpu(w, g_sum, g_act)
     act = _act_code(act)
     if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1:
         raise BitswapHipError(f"linear_act_grad: w must be [N, K], got {tuple(w.shape)}")
@@ -1006,17 +1037,17 @@ def linear_act_grad(x, w, s=None, act=ACT_NONE, g_sum=None, g_act=None, want_x=T
         if x is None:
             raise BitswapHipError("linear_act_grad: the gradient of w needs the saved input x")
         xt, xe, ldx = _saved_rows(x, K, w.dtype, rows, "linear_act_grad x")
-    dev, L = w.device, load()
+    L = load()
     # one gradient and no slope: it is ds already
     made = sloped or (g_sum is not None and g_act is not None)
     need_ds = want_x or want_w or want_res
-    ds = torch.empty(g0.shape, dtype=w.dtype, device=dev) if made and need_ds else None
-    db = torch.empty(N, dtype=torch.float32, device=dev) if want_bias else None
+    ds = w.new_empty(g0.shape) if made and need_ds else None
+    db = w.new_empty(N, dtype=torch.float32) if want_bias else None
     if ds is not None or db is not None:
-        nb = L.bs_act_grad_workspace(rows, N) if want_bias else 0
-        ws = _workspace(nb, dev)
-        _check(L.bs_act_grad(_ptr(gs[0][0]), gs[0][1], _ptr(gs[1][0]), gs[1][1], _ptr(st), _ptr(se), lds, act, code, rows, N, _ptr(ds),
-                             _ptr(db), _ptr(ws), nb, _stream()), "bs_act_grad")
+        nb = _workspace_bytes("bs_act_grad_workspace", rows, N) if want_bias else 0
+        ws = _scratch(w, nb)
+        _check(L.bs_act_grad(_at(gs[0][0]), gs[0][1], _at(gs[1][0]), gs[1][1], _at(st), _at(se), lds, act, code, rows, N, _at(ds),
+                             _at(db), _at(ws), nb, _raw_stream(dev)), "bs_act_grad")
     if ds is not None:
         dt, ldd = ds, N
     else:
@@ -1024,15 +1055,15 @@ def linear_act_grad(x, w, s=None, act=ACT_NONE, g_sum=None, g_act=None, want_x=T
     dx = dw = None
     if want_x:
         wt, ldw, _ = _as_rows(w, K, "linear_act_grad w")
-        dx = torch.empty(tuple(g0.shape[:-1]) + (K,), dtype=w.dtype, device=dev)
-        nb = L.bs_linear_grad_x_workspace(code, rows, K, N)
-        ws = _workspace(nb, dev)
-        _check(L.bs_linear_grad_x(_ptr(dt), ldd, _ptr(wt), ldw, _ptr(dx), code, rows, K, N, _ptr(ws), nb, _stream()), "bs_linear_grad_x")
+        dx = w.new_empty(tuple(g0.shape[:-1]) + (K,))
+        nb = _workspace_bytes("bs_linear_grad_x_workspace", code, rows, K, N)
+        ws = _scratch(w, nb)
+        _check(L.bs_linear_grad_x(_at(dt), ldd, _at(wt), ldw, _at(dx), code, rows, K, N, _at(ws), nb, _raw_stream(dev)), "bs_linear_grad_x")
     if want_w:
-        dw = torch.empty((N, K), dtype=w.dtype, device=dev)
-        nb = L.bs_linear_grad_w_workspace(code, rows, K, N, int(xe is not None))
-        ws = _workspace(nb, dev)
-        _check(L.bs_linear_grad_w(_ptr(dt), ldd, _ptr(xt), _ptr(xe), ldx, _ptr(dw), code, rows, K, N, _ptr(ws), nb, _stream()),
+        dw = w.new_empty((N, K))
+        nb = _workspace_bytes("bs_linear_grad_w_workspace", code, rows, K, N, int(xe is not None))
+        ws = _scratch(w, nb)
+        _check(L.bs_linear_grad_w(_at(dt), ldd, _at(xt), _at(xe), ldx, _at(dw), code, rows, K, N, _at(ws), nb, _raw_stream(dev)),
                "bs_linear_grad_w")
     return dx, dw, db, ((ds if ds is not None else g0) if want_res else None)
 
@@ -1042,6 +1073,9 @@ def _as_images(t, what):
     if t.dim() < 2 or t.shape[-1] < 1:
         raise BitswapHipError(f"{what}: expected [n, ..., C], got {tuple(t.shape)}")
     n, C = t.shape[0], t.shape[-1]
+    if t.is_contiguous() and n:
+        pixels = t.numel() // (n * C)
+        return t, pixels * C, C, n, pixels, C
     pixels = 1
     for k in t.shape[1:-1]:
         pixels *= k
@@ -1060,7 +1094,7 @@ def group_norm_act(x, groups, gamma=None, beta=None, eps=1e-5, act=ACT_ELU, want
     (y, stats | None, Packed8 of x | None): u = (x - mean) / sqrt(var + eps) gamma + beta over the pixels and C / groups channels
     of a group, y = act(u), contiguous.  stats float32 [n, groups, 2] = (mean, 1 / sqrt(var + eps)): what the gradient needs
     besides x.  gamma, beta [C] float32 or x's type.  An image's bits do not depend on n."""
-    _need_cuda(x, gamma, beta)
+    dev = _gpu(x, gamma, beta)
     code, act = _dtype_code(x, "group_norm_act"), _act_code(act)
     t, ldn, ldp, n, pixels, C = _as_images(x, "group_norm_act")
     groups = int(groups)
@@ -1072,20 +1106,19 @@ def group_norm_act(x, groups, gamma=None, beta=None, eps=1e-5, act=ACT_ELU, want
     beta, bcode = _affine("group_norm_act beta", beta, C, x)
     if gamma is not None and beta is not None and gcode != bcode:
         raise BitswapHipError("group_norm_act: gamma and beta of one type")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = (torch.empty if x.numel() else torch.zeros)((n, groups, 2), dtype=torch.float32, device=x.device) if want_stats else None
-    L = load()
-    nb = L.bs_group_norm_workspace(code, n, pixels, C, groups, 0)
-    ws = _workspace(nb, x.device)
-    _check(L.bs_group_norm_act(_ptr(t), ldn, ldp, _ptr(gamma), _ptr(beta), gcode if gamma is not None else bcode, float(eps), act, code,
-                               n, pixels, C, groups, _ptr(y), _ptr(stats), _ptr(ws), nb, _stream()), "bs_group_norm_act")
+    y = x.new_empty(x.shape)
+    stats = (x.new_empty if x.numel() else x.new_zeros)((n, groups, 2), dtype=torch.float32) if want_stats else None
+    nb = _workspace_bytes("bs_group_norm_workspace", code, n, pixels, C, groups, 0)
+    ws = _scratch(x, nb)
+    _check(load().bs_group_norm_act(_at(t), ldn, ldp, _at(gamma), _at(beta), gcode if gamma is not None else bcode, float(eps), act, code,
+                               n, pixels, C, groups, _at(y), _at(stats), _at(ws), nb, _raw_stream(dev)), "bs_group_norm_act")
     return y, stats, pack8(x) if want_pack else None
 
 
 def group_norm_act_grad(x, stats, groups, g, gamma=None, beta=None, act=ACT_ELU, want_affine=True):
     """Gradients of group_norm_act -> (dx, dgamma float32 [C] | None, dbeta float32 [C] | None) from the saved input x (whole or as
     Packed8), the stats of the forward call and the gradient g of its y."""
-    _need_cuda(stats, g, gamma, beta)
+    dev = _gpu(stats, g, gamma, beta)
     code, act = _dtype_code(g, "group_norm_act_grad"), _act_code(act)
     gt, ldgn, ldgp, n, pixels, C = _as_images(g, "group_norm_act_grad")
     groups = int(groups)
@@ -1097,23 +1130,22 @@ def group_norm_act_grad(x, stats, groups, g, gamma=None, beta=None, act=ACT_ELU,
         raise BitswapHipError(f"group_norm_act_grad: stats must be float32 [{n}, {groups}, 2]")
     stats = stats.contiguous()
     if isinstance(x, Packed8):
-        _need_cuda(x.codes, x.exps)
+        _gpu(x.codes, x.exps)
         xt, xe, ldn, ldp = x.codes, x.exps, pixels * C, C
     else:
-        _need_cuda(x)
+        _gpu(x)
         (xt, ldn, ldp), xe = _as_images(x, "group_norm_act_grad")[:3], None
     gamma, gcode = _affine("group_norm_act_grad gamma", gamma, C, g)
     beta, bcode = _affine("group_norm_act_grad beta", beta, C, g)
     if gamma is not None and beta is not None and gcode != bcode:
         raise BitswapHipError("group_norm_act_grad: gamma and beta of one type")
-    dx = torch.empty(g.shape, dtype=g.dtype, device=g.device)
-    dgamma, dbeta = (torch.empty(C, dtype=torch.float32, device=g.device) if want_affine else None for _ in range(2))
-    L = load()
-    nb = L.bs_group_norm_workspace(code, n, pixels, C, groups, 1)
-    ws = _workspace(nb, g.device)
-    _check(L.bs_group_norm_act_grad(_ptr(gt), ldgn, ldgp, _ptr(xt), _ptr(xe), ldn, ldp, _ptr(stats), _ptr(gamma), _ptr(beta),
-                                    gcode if gamma is not None else bcode, act, code, n, pixels, C, groups, _ptr(dx), _ptr(dgamma),
-                                    _ptr(dbeta), _ptr(ws), nb, _stream()), "bs_group_norm_act_grad")
+    dx = g.new_empty(g.shape)
+    dgamma, dbeta = (g.new_empty(C, dtype=torch.float32) if want_affine else None for _ in range(2))
+    nb = _workspace_bytes("bs_group_norm_workspace", code, n, pixels, C, groups, 1)
+    ws = _scratch(g, nb)
+    _check(load().bs_group_norm_act_grad(_at(gt), ldgn, ldgp, _at(xt), _at(xe), ldn, ldp, _at(stats), _at(gamma), _at(beta),
+                                    gcode if gamma is not None else bcode, act, code, n, pixels, C, groups, _at(dx), _at(dgamma),
+                                    _at(dbeta), _at(ws), nb, _raw_stream(dev)), "bs_group_norm_act_grad")
     return dx, dgamma, dbeta
 
 
