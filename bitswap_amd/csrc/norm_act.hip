@@ -23,7 +23,7 @@ struct NormArgs {
     float eps;
     int64_t n, pixels;
     int C, G, per;
-    int pl_log2;                        // pixel lanes of a workgroup
+    int pl;                             // pixel lanes of a workgroup
     int cl;                             // lanes along the channels
     int gs;                             // groups of a workgroup
     int slabs;
@@ -95,20 +95,51 @@ struct SlabSum {
 };
 
 // ---- images that fit -------------------------------------------------------------------------------------------------------
-template <int DT>
+// Sums of N values over a group where its channels are whole lanes (per % V == 0) and lanes and groups are powers of two: exchanges
+// within the wavefront, one barrier, and every thread adds up what the wavefronts left for its group.
+template <int N>
+struct LaneSum {
+    int cl, cpg, CL, gs, rows, row, lane;           // lanes per group and of the slab; wavefronts that hold pixels of one lane
+    __device__ __forceinline__ void run(float (&v)[N], float* red) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            for (int o = 1; o < cpg; o *= 2) v[n] += __shfl_xor(v[n], o);
+            for (int o = CL; o < 64; o *= 2) v[n] += __shfl_xor(v[n], o);
+        }
+        const int g = cl / cpg;
+        if ((cl & (cpg - 1)) == 0 && (CL >= 64 || lane < CL)) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) red[(n * rows + row) * gs + g] = v[n];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            v[n] = 0.0f;
+            for (int r = 0; r < rows; ++r) v[n] += red[(n * rows + r) * gs + g];
+        }
+    }
+};
+template <int N>
+__device__ __forceinline__ LaneSum<N> lane_sum(const NormArgs& a, int cl, int V, int tid) {
+    LaneSum<N> s;
+    s.cl = cl; s.cpg = a.per / V; s.CL = a.cl; s.gs = a.gs; s.lane = tid & 63;
+    const int wpr = a.cl > 64 ? a.cl / 64 : 1;                       // wavefronts a pixel takes
+    const int waves = (a.pl * a.cl + 63) / 64;
+    s.rows = waves / wpr;
+    s.row = (tid >> 6) / wpr;
+    return s;
+}
+
+template <int DT, bool LANES>
 __global__ __launch_bounds__(1024) void k_norm(const NormArgs a) {
     constexpr int V = vlen(DT), R = 32 / V, ES = esize(DT);
     extern __shared__ __align__(16) float sh[];
-    const int PL = 1 << a.pl_log2, CL = a.cl, tid = threadIdx.x;
+    const int PL = a.pl, CL = a.cl, tid = threadIdx.x;
     const int64_t img = blockIdx.x / a.slabs;
     const int slab = blockIdx.x % a.slabs, c0 = slab * a.gs * a.per;
     const int width = min(a.gs * a.per, a.C - c0);               // channels of this slab
     const int pl = tid / CL, cl = tid - pl * CL, k = cl * V, left = width - k;
     const bool live = pl < PL && left > 0;
-    SlabSum ss;
-    ss.ch = CL * V; ss.PL = PL; ss.Q = max(1, PL / V); ss.gs = min(a.gs, a.G - slab * a.gs); ss.per = a.per;
-    ss.nthr = blockDim.x; ss.tid = tid;
-    ss.red = sh; ss.part = sh + PL * ss.ch; ss.out = ss.part + ss.Q * ss.ch;
 
     float f[R][V];
     const char* const xp = a.x + (img * a.ldn + c0 + k) * ES;
@@ -119,42 +150,72 @@ __global__ __launch_bounds__(1024) void k_norm(const NormArgs a) {
         const int64_t p = pl + (int64_t)r * PL;
         if (live && p < a.pixels) load_vec<DT>(xp + p * a.ldp * ES, left, f[r]);
     }
+    float ga[V], be[V];
+    affine<DT>(a.gamma, a.aff_f32, c0 + k, live ? left : 0, 1.0f, ga);
+    affine<DT>(a.beta, a.aff_f32, c0 + k, live ? left : 0, 0.0f, be);
     const float inv = 1.0f / ((float)a.pixels * (float)a.per);
-    float s[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        s[i] = 0.0f;
-#pragma unroll
-        for (int r = 0; r < R; ++r) s[i] += f[r][i];
-    }
-    ss.run<V>(s, pl, k, live, nullptr, 0, c0, a.C, DT, nullptr);
-    float m[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) m[i] = i < left ? ss.out[(k + i) / a.per] * inv : 0.0f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        s[i] = 0.0f;
+    float m[V], rs[V], s[V];
+    if (LANES) {
+        const LaneSum<1> sum = lane_sum<1>(a, cl, V, tid);
+        float t[1] = {0.0f};
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            if (pl + r * PL < a.pixels) {
-                const float d = f[r][i] - m[i];
-                s[i] = fmaf(d, d, s[i]);
-            }
-    }
-    float* const mean_sh = ss.out;                               // the means move on: out is written again
-    ss.out += ss.gs;
-    ss.run<V>(s, pl, k, live, nullptr, 0, c0, a.C, DT, nullptr);
-    float rs[V], ga[V], be[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) rs[i] = i < left ? 1.0f / sqrtf(ss.out[(k + i) / a.per] * inv + a.eps) : 0.0f;
-    if (a.stats && tid < ss.gs) {
-        float* const o = a.stats + (img * a.G + slab * a.gs + tid) * 2;
-        o[0] = mean_sh[tid] * inv;
-        o[1] = 1.0f / sqrtf(ss.out[tid] * inv + a.eps);
+            for (int i = 0; i < V; ++i) t[0] += f[r][i];
+        sum.run(t, sh);
+        const float mean = t[0] * inv;
+        t[0] = 0.0f;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (live && pl + r * PL < a.pixels) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) t[0] = fmaf(f[r][i] - mean, f[r][i] - mean, t[0]);
+            }
+        sum.run(t, sh + 16 * a.gs);
+        const float rstd = 1.0f / sqrtf(t[0] * inv + a.eps);
+        if (a.stats && live && pl == 0 && k % a.per == 0) {
+            float* const o = a.stats + (img * a.G + (c0 + k) / a.per) * 2;
+            o[0] = mean;
+            o[1] = rstd;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            m[i] = mean;
+            rs[i] = rstd;
+        }
+    } else {
+        SlabSum ss;
+        ss.ch = CL * V; ss.PL = PL; ss.Q = max(1, PL / V); ss.gs = min(a.gs, a.G - slab * a.gs); ss.per = a.per;
+        ss.nthr = blockDim.x; ss.tid = tid;
+        ss.red = sh; ss.part = sh + PL * ss.ch; ss.out = ss.part + ss.Q * ss.ch;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            s[i] = 0.0f;
+#pragma unroll
+            for (int r = 0; r < R; ++r) s[i] += f[r][i];
+        }
+        ss.run<V>(s, pl, k, live, nullptr, 0, c0, a.C, DT, nullptr);
+#pragma unroll
+        for (int i = 0; i < V; ++i) m[i] = i < left ? ss.out[(k + i) / a.per] * inv : 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            s[i] = 0.0f;
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (pl + r * PL < a.pixels) s[i] = fmaf(f[r][i] - m[i], f[r][i] - m[i], s[i]);
+        }
+        float* const mean_sh = ss.out;                               // the means stay: the next sums go behind them
+        ss.out += ss.gs;
+        ss.run<V>(s, pl, k, live, nullptr, 0, c0, a.C, DT, nullptr);
+#pragma unroll
+        for (int i = 0; i < V; ++i) rs[i] = i < left ? 1.0f / sqrtf(ss.out[(k + i) / a.per] * inv + a.eps) : 0.0f;
+        if (a.stats && tid < ss.gs) {
+            float* const o = a.stats + (img * a.G + slab * a.gs + tid) * 2;
+            o[0] = mean_sh[tid] * inv;
+            o[1] = 1.0f / sqrtf(ss.out[tid] * inv + a.eps);
+        }
     }
     if (!live) return;
-    affine<DT>(a.gamma, a.aff_f32, c0 + k, left, 1.0f, ga);
-    affine<DT>(a.beta, a.aff_f32, c0 + k, left, 0.0f, be);
     char* const yp = a.y + (img * a.pixels * a.C + c0 + k) * ES;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -178,11 +239,11 @@ __device__ __forceinline__ void load_x(const NormArgs& a, int64_t img, int64_t p
     }
 }
 
-template <int DT, bool SAVED8>
-__global__ __launch_bounds__(1024) void k_norm_grad(const NormArgs a) {
+template <int DT, bool SAVED8, bool LANES>
+__global__ __launch_bounds__(512) void k_norm_grad(const NormArgs a) {
     constexpr int V = vlen(DT), R = 32 / V, ES = esize(DT);
     extern __shared__ __align__(16) float sh[];
-    const int PL = 1 << a.pl_log2, CL = a.cl, tid = threadIdx.x;
+    const int PL = a.pl, CL = a.cl, tid = threadIdx.x;
     const int64_t img = blockIdx.x / a.slabs;
     const int slab = blockIdx.x % a.slabs, c0 = slab * a.gs * a.per;
     const int width = min(a.gs * a.per, a.C - c0);
@@ -204,20 +265,29 @@ __global__ __launch_bounds__(1024) void k_norm_grad(const NormArgs a) {
             load_vec<DT>(a.g + (img * a.ldgn + p * a.ldgp + c0 + k) * ES, left, d[r]);
         }
     }
+    if (LANES) {                                                     // the lane's channels are of one group
+        const float* const st = a.stats + (img * a.G + (c0 + min(k, width - 1)) / a.per) * 2;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const float* const st = a.stats + (img * a.G + (c0 + min(k + i, width - 1)) / a.per) * 2;
-        m[i] = st[0];
-        rs[i] = st[1];
+        for (int i = 0; i < V; ++i) {
+            m[i] = st[0];
+            rs[i] = st[1];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float* const st = a.stats + (img * a.G + (c0 + min(k + i, width - 1)) / a.per) * 2;
+            m[i] = st[0];
+            rs[i] = st[1];
+        }
     }
-    affine<DT>(a.gamma, a.aff_f32, c0 + k, left, 1.0f, ga);
-    affine<DT>(a.beta, a.aff_f32, c0 + k, left, 0.0f, be);
+    affine<DT>(a.gamma, a.aff_f32, c0 + k, live ? left : 0, 1.0f, ga);
+    affine<DT>(a.beta, a.aff_f32, c0 + k, live ? left : 0, 0.0f, be);
     float s1[V], s2[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.0f;
 #pragma unroll
     for (int r = 0; r < R; ++r)
-        if (pl + r * PL < a.pixels) {
+        if (live && pl + r * PL < a.pixels) {
             float u[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -232,27 +302,65 @@ __global__ __launch_bounds__(1024) void k_norm_grad(const NormArgs a) {
             }
         }
     float* const po = a.parts ? a.parts + img * 2 * a.C + c0 : nullptr;
-    ss.run<V>(s2, pl, k, live, a.gamma, a.aff_f32, c0, a.C, DT, po);
-    const float* const two = ss.out;
-    ss.out += ss.gs;
-    ss.run<V>(s1, pl, k, live, a.gamma, a.aff_f32, c0, a.C, DT, po ? po + a.C : nullptr);
-    if (!live) return;
     const float inv = 1.0f / ((float)a.pixels * (float)a.per);
     float m1[V], m2[V];
+    if (LANES) {
+        const LaneSum<2> sum = lane_sum<2>(a, cl, V, tid);
+        float t[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int g = min(k + i, width - 1) / a.per;
-        m1[i] = ss.out[g] * inv;
-        m2[i] = two[g] * inv;
+        for (int i = 0; i < V; ++i) {
+            t[0] = fmaf(ga[i], s1[i], t[0]);
+            t[1] = fmaf(ga[i], s2[i], t[1]);
+        }
+        sum.run(t, ss.out);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            m1[i] = t[0] * inv;
+            m2[i] = t[1] * inv;
+        }
+    } else {
+        ss.run<V>(s2, pl, k, live, a.gamma, a.aff_f32, c0, a.C, DT, po);
+        const float* const two = ss.out;
+        ss.out += ss.gs;
+        ss.run<V>(s1, pl, k, live, a.gamma, a.aff_f32, c0, a.C, DT, po ? po + a.C : nullptr);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int g = min(k + i, width - 1) / a.per;
+            m1[i] = ss.out[g] * inv;
+            m2[i] = two[g] * inv;
+        }
     }
-    char* const yp = a.y + (img * a.pixels * a.C + c0 + k) * ES;
+    if (live) {
+        char* const yp = a.y + (img * a.pixels * a.C + c0 + k) * ES;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int64_t p = pl + (int64_t)r * PL;
-        if (p >= a.pixels) break;
+        for (int r = 0; r < R; ++r) {
+            const int64_t p = pl + (int64_t)r * PL;
+            if (p >= a.pixels) break;
 #pragma unroll
-        for (int i = 0; i < V; ++i) d[r][i] = rs[i] * (fmaf(d[r][i], ga[i], -m1[i]) - h[r][i] * m2[i]);
-        store_vec<DT>(yp + p * a.C * ES, left, d[r]);
+            for (int i = 0; i < V; ++i) d[r][i] = rs[i] * (fmaf(d[r][i], ga[i], -m1[i]) - h[r][i] * m2[i]);
+            store_vec<DT>(yp + p * a.C * ES, left, d[r]);
+        }
+    }
+    if (LANES && po) {                                               // the channels' sums over the pixels, while dx is on its way out
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            if (live)
+#pragma unroll
+                for (int i = 0; i < V; ++i) ss.red[pl * ss.ch + k + i] = n ? s1[i] : s2[i];
+            __syncthreads();
+            for (int i = tid; i < ss.ch * ss.Q; i += ss.nthr) {
+                const int q = i / ss.ch, c = i - q * ss.ch;
+                float t = 0.0f;
+                for (int p = q; p < PL; p += ss.Q) t += ss.red[p * ss.ch + c];
+                ss.part[i] = t;
+            }
+            __syncthreads();
+            for (int c = tid; c < width; c += ss.nthr) {
+                float t = 0.0f;
+                for (int q = 0; q < ss.Q; ++q) t += ss.part[q * ss.ch + c];
+                po[n * a.C + c] = t;
+            }
+        }
     }
 }
 
@@ -432,36 +540,40 @@ __global__ __launch_bounds__(256) void k_apply(const NormArgs a, const float* __
 
 // ---- which way, and how it is cut --------------------------------------------------------------------------------------------
 struct Plan {
-    bool fits;
-    int pl_log2, cl, gs, slabs, threads, lds;
+    bool fits, lanes;
+    int pl, cl, gs, slabs, threads, lds;
     int runs;
     int64_t run;
     int cly;              // split: workgroups along the channels
 };
 
-Plan plan(int dtype, int64_t n, int64_t pixels, int C, int G, int outs) {
+Plan plan(int dtype, int64_t pixels, int C, int G, int grad) {
     Plan p = {};
-    const int V = dtype == BS_DT_F32 ? 4 : 8, R = 32 / V, per = C / G;
-    int64_t need = (pixels + R - 1) / R;
-    while ((1 << p.pl_log2) < need && p.pl_log2 < 10) ++p.pl_log2;
-    const int PL = 1 << p.pl_log2, cap = 1024 / PL;
-    const int one = (per + V - 1) / V;                  // lanes that one group takes
-    p.fits = need <= 256 && one <= cap;
+    const int V = dtype == BS_DT_F32 ? 4 : 8, R = 32 / V, per = C / G, cap = grad ? 512 : 1024;
+    const int64_t need = (pixels + R - 1) / R;              // pixel lanes
+    const int one = (per + V - 1) / V;                      // channel lanes of a group
+    p.fits = need <= 256 && need * one <= cap;             // (longer columns would leave a row of the workgroup under 64 bytes)
     if (p.fits) {
-        // as many groups as give rows of 256 bytes, or 512 threads; fewer when there are few images (neither changes a bit)
+        auto pow2 = [](int64_t v) { return (v & (v - 1)) == 0; };
+        int64_t up = 1;
+        while (up < need) up *= 2;
+        p.lanes = per % V == 0 && pow2(one) && one <= 64 && up * one <= cap;
+        p.pl = (int)(p.lanes ? up : need);
+        // groups of a workgroup: until a row of it is 256 bytes long or the workgroup has 512 threads
         int gs = 1;
-        while (gs < G) {
-            const int lanes = (2 * gs * per + V - 1) / V;
-            if (lanes > cap || lanes * PL > 512 || gs * per * 16 / V >= 256) break;
-            if (n * ((G + 2 * gs - 1) / (2 * gs)) < 512) break;
-            gs *= 2;
+        auto lanes_of = [&](int g) { return (g * per + V - 1) / V; };
+        while (gs < G && lanes_of(gs) < 16) {
+            const int next = p.lanes ? 2 * gs : gs + 1;
+            if (next > G || lanes_of(next) * p.pl > 512) break;
+            gs = next;
         }
         p.gs = gs;
-        p.cl = (gs * per + V - 1) / V;
+        p.cl = lanes_of(gs);
         p.slabs = (G + gs - 1) / gs;
-        p.threads = (PL * p.cl + 63) / 64 * 64;
-        const int ch = p.cl * V, Q = PL / V > 1 ? PL / V : 1;
-        p.lds = (PL * ch + Q * ch + 2 * gs) * 4;
+        p.threads = (p.pl * p.cl + 63) / 64 * 64;
+        const int ch = p.cl * V, Q = p.pl / V > 1 ? p.pl / V : 1;
+        const int sums = p.lanes ? 32 * gs : 2 * gs;
+        p.lds = (p.lanes && !grad ? sums : p.pl * ch + Q * ch + sums) * 4;
         return p;
     }
     const int chunks = (C + V - 1) / V;
@@ -479,7 +591,7 @@ int bad_norm(int dtype, int64_t n, int64_t pixels, int channels, int groups, int
 }
 
 void fill(NormArgs* a, const Plan& p) {
-    a->pl_log2 = p.pl_log2; a->cl = p.cl; a->gs = p.gs; a->slabs = p.slabs; a->runs = p.runs; a->run = p.run;
+    a->pl = p.pl; a->cl = p.cl; a->gs = p.gs; a->slabs = p.slabs; a->runs = p.runs; a->run = p.run;
 }
 
 }  // namespace
@@ -488,7 +600,7 @@ extern "C" {
 
 int64_t bs_group_norm_workspace(int dtype, int64_t n, int64_t pixels, int channels, int groups, int grad) {
     if (bad_norm(dtype, n, pixels, channels, groups, 0)) return BS_EINVAL;
-    const Plan p = plan(dtype, n, pixels, channels, groups, grad);
+    const Plan p = plan(dtype, pixels, channels, groups, grad);
     if (p.fits) return grad ? n * 2 * channels * 4 : 0;
     return (n * p.runs * 2 * channels + n * groups * 2) * 4;
 }
@@ -500,7 +612,7 @@ int bs_group_norm_act(const void* x, int64_t ldn, int64_t ldp, const void* gamma
     if (n == 0 || pixels == 0) return BS_OK;
     if (!x || !y || ldp < channels || ldn < 0) return BS_EINVAL;
     if ((gamma || beta) && affine_dtype != BS_DT_F32 && affine_dtype != dtype) return BS_EINVAL;
-    const Plan p = plan(dtype, n, pixels, channels, groups, 0);
+    const Plan p = plan(dtype, pixels, channels, groups, 0);
     const int64_t need = bs_group_norm_workspace(dtype, n, pixels, channels, groups, 0);
     if (need > 0 && (!workspace || workspace_bytes < need)) return BS_EINVAL;
     NormArgs a = {};
@@ -512,7 +624,8 @@ int bs_group_norm_act(const void* x, int64_t ldn, int64_t ldp, const void* gamma
     const int64_t blocks = p.fits ? n * p.slabs : n * p.runs;
     if (blocks > 0x7fffffff || n * groups > 0x7fffffff) return BS_EINVAL;
     if (p.fits) {
-#define GO(DT) hipLaunchKernelGGL(k_norm<DT>, dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a)
+#define GO(DT) do { if (p.lanes) hipLaunchKernelGGL((k_norm<DT, true>), dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a); \
+                    else hipLaunchKernelGGL((k_norm<DT, false>), dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a); } while (0)
         if (dtype == BS_DT_F32) GO(BS_DT_F32);
         else if (dtype == BS_DT_BF16) GO(BS_DT_BF16);
         else GO(BS_DT_F16);
@@ -546,7 +659,7 @@ int bs_group_norm_act_grad(const void* g, int64_t ldgn, int64_t ldgp, const void
     }
     if (!g || !x || !stats || !dx || ldgp < channels || ldgn < 0 || (!x_exps && (ldp < channels || ldn < 0))) return BS_EINVAL;
     if ((gamma || beta) && affine_dtype != BS_DT_F32 && affine_dtype != dtype) return BS_EINVAL;
-    const Plan p = plan(dtype, n, pixels, channels, groups, 1);
+    const Plan p = plan(dtype, pixels, channels, groups, 1);
     const int64_t need = bs_group_norm_workspace(dtype, n, pixels, channels, groups, 1);
     if (!workspace || workspace_bytes < need) return BS_EINVAL;
     NormArgs a = {};
@@ -560,12 +673,14 @@ int bs_group_norm_act_grad(const void* g, int64_t ldgn, int64_t ldgp, const void
     if (blocks > 0x7fffffff || n * groups > 0x7fffffff) return BS_EINVAL;
     if (p.fits) {
         if (!dgamma && !dbeta) a.parts = nullptr;
-#define GO(DT) do { if (x_exps) hipLaunchKernelGGL((k_norm_grad<DT, true>), dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a); \
-                    else hipLaunchKernelGGL((k_norm_grad<DT, false>), dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a); } while (0)
+#define FIT(DT, P8) do { if (p.lanes) hipLaunchKernelGGL((k_norm_grad<DT, P8, true>), dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a); \
+                         else hipLaunchKernelGGL((k_norm_grad<DT, P8, false>), dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a); } while (0)
+#define GO(DT) do { if (x_exps) FIT(DT, true); else FIT(DT, false); } while (0)
         if (dtype == BS_DT_F32) GO(BS_DT_F32);
         else if (dtype == BS_DT_BF16) GO(BS_DT_BF16);
         else GO(BS_DT_F16);
 #undef GO
+#undef FIT
     } else {
         float* const means = a.parts + n * p.runs * 2 * channels;
         const dim3 grid((unsigned)blocks, (unsigned)p.cly);
