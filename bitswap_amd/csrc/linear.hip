@@ -127,19 +127,15 @@ __device__ __forceinline__ void load_bias(const RowsArgs& a, int64_t p, float* b
     if (!a.bias || p >= a.N) return;
     if (DT != BS_DT_F32 && a.bias_f32) {
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-            if (p + e < a.N) b[e] = reinterpret_cast<const float*>(a.bias)[p + e];
+        for (int e = 0; e < V; e += 4)
+            if (p + e < a.N) load_vec<BS_DT_F32>(a.bias + (p + e) * 4, a.N - p - e < 4 ? (int)(a.N - p - e) : 4, b + e);
     } else {
         load_vec<DT>(a.bias + p * esize(DT), a.N - p < V ? (int)(a.N - p) : V, b);
     }
 }
 template <int DT>
 __device__ __forceinline__ u32x4 residual(const RowsArgs& a, int64_t q, int64_t p, int n) {
-    constexpr int V = vlen(DT);
-    if (n >= V) return load16(a.res + (q * a.ldr + p) * esize(DT));
-    float t[V];
-    load_vec<DT>(a.res + (q * a.ldr + p) * esize(DT), n, t);
-    return pack16<DT>(t);
+    return load_raw<DT>(a.res + (q * a.ldr + p) * esize(DT), n);
 }
 
 // A wavefront's 32 rows x 64 channels from the registers of the matrix instruction to rows of memory, by way of its own piece of
@@ -238,18 +234,7 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_rows(const RowsA
             constexpr int V = vlen(DT);
             const int k = s * BK + (u % UPR) * V, left = a.K - k;
             const char* const src = a.x + (q * a.ldx + k) * ES;
-            if (left >= V) {
-                xr[n] = load16(src);
-            } else {
-                u32x4 v = {0, 0, 0, 0};
-#pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if (e < left) {
-                        if (DT == BS_DT_F32) v[e % 4] = *reinterpret_cast<const uint32_t*>(src + e * 4);
-                        else v[e / 2] |= (uint32_t) * reinterpret_cast<const uint16_t*>(src + e * 2) << (16 * (e % 2));
-                    }
-                xr[n] = v;
-            }
+            xr[n] = left > 0 ? load_raw<DT>(src, left) : u32x4{0, 0, 0, 0};
         }
     };
     auto store_x = [&](char* st) {
@@ -537,19 +522,9 @@ __global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {
     constexpr int RAW = DT == BS_DT_F32 ? 2 : 1;
     auto fetch = [&](const char* base, int k, u32x4* r) {          // 8 values from k on, zero behind K
         const int left = a.K - k;
-        if (left >= 8) {
-            r[0] = load16(base + (int64_t)k * ES);
-            if (RAW == 2) r[RAW - 1] = load16(base + (int64_t)k * ES + 16);
-        } else {
-#pragma unroll
-            for (int n = 0; n < RAW; ++n) r[n] = u32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (e < left) {
-                    if (DT == BS_DT_F32) r[(e / 4) % RAW][e % 4] = *reinterpret_cast<const uint32_t*>(base + (int64_t)(k + e) * ES);
-                    else r[0][e / 2] |= (uint32_t) * reinterpret_cast<const uint16_t*>(base + (int64_t)(k + e) * ES) << (16 * (e % 2));
-                }
-        }
+        const char* const at = base + (int64_t)k * ES;
+        r[0] = left > 0 ? load_raw<DT>(at, left) : u32x4{0, 0, 0, 0};
+        if (RAW == 2) r[RAW - 1] = left > 4 ? load_raw<DT>(at + 16, left - 4) : u32x4{0, 0, 0, 0};
     };
     auto split = [&](const u32x4* r, u32x4* l) {
         if (DT == BS_DT_F32) {
@@ -711,21 +686,19 @@ struct Strip {
             if (k + row < ke && left > 0) {
                 const char* const src = base + ((k + row) * ld + ch) * ES;
                 if (SRC == S_P8) step[n % (SRC == S_P8 ? N : 1)] = p8_pow2(a.exps[(k + row) * a.nb + ch / P8_BLOCK]);
-                if (left >= V) {
-                    if (SRC == S_P8) {
+                if (SRC == S_P8) {
+                    if (left >= V) {
                         const u32x2 t = load8(src);
                         v[0] = t[0]; v[1] = t[1];
                     } else {
-                        v = load16(src);
+                        uint32_t c[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) c[e] = *reinterpret_cast<const uint8_t*>(src + min(e, left - 1));
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e / 4] |= e < left ? c[e] << (8 * (e % 4)) : 0u;
                     }
                 } else {
-#pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        if (e < left) {
-                            if (SRC == S_P8) v[e / 4] |= (uint32_t) * reinterpret_cast<const uint8_t*>(src + e) << (8 * (e % 4));
-                            else if (DT == BS_DT_F32) v[e % 4] = *reinterpret_cast<const uint32_t*>(src + e * 4);
-                            else v[e / 2] |= (uint32_t) * reinterpret_cast<const uint16_t*>(src + e * 2) << (16 * (e % 2));
-                        }
+                    v = load_raw<DT>(src, left);
                 }
             }
             raw[n] = v;

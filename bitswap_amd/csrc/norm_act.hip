@@ -39,8 +39,15 @@ template <int DT>
 __device__ __forceinline__ void affine(const char* p, int f32, int c, int left, float fill, float* v) {
     constexpr int V = vlen(DT);
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-        v[i] = (p && i < left) ? (f32 ? reinterpret_cast<const float*>(p)[c + i] : load1<DT>(p + (int64_t)(c + i) * esize(DT))) : fill;
+    for (int i = 0; i < V; ++i) v[i] = fill;
+    if (!p || left <= 0) return;
+    if (f32) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4)
+            if (left > i) load_vec<BS_DT_F32>(p + (int64_t)(c + i) * 4, left - i, v + i);
+    } else {
+        load_vec<DT>(p + (int64_t)c * esize(DT), left, v);
+    }
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
@@ -547,7 +554,7 @@ struct Plan {
     int cly;              // split: workgroups along the channels
 };
 
-Plan plan(int dtype, int64_t pixels, int C, int G, int grad) {
+Plan plan(int dtype, int64_t n, int64_t pixels, int C, int G, int grad) {
     Plan p = {};
     const int V = dtype == BS_DT_F32 ? 4 : 8, R = 32 / V, per = C / G, cap = grad ? 512 : 1024;
     const int64_t need = (pixels + R - 1) / R;              // pixel lanes
@@ -567,6 +574,7 @@ Plan plan(int dtype, int64_t pixels, int C, int G, int grad) {
             if (next > G || lanes_of(next) * p.pl > 512) break;
             gs = next;
         }
+        while (!p.lanes && gs > 1 && n * ((G + gs - 1) / gs) < 512) --gs;       // (changes no bit: no sum here crosses channel lanes)
         p.gs = gs;
         p.cl = lanes_of(gs);
         p.slabs = (G + gs - 1) / gs;
@@ -600,7 +608,7 @@ extern "C" {
 
 int64_t bs_group_norm_workspace(int dtype, int64_t n, int64_t pixels, int channels, int groups, int grad) {
     if (bad_norm(dtype, n, pixels, channels, groups, 0)) return BS_EINVAL;
-    const Plan p = plan(dtype, pixels, channels, groups, grad);
+    const Plan p = plan(dtype, n, pixels, channels, groups, grad);
     if (p.fits) return grad ? n * 2 * channels * 4 : 0;
     return (n * p.runs * 2 * channels + n * groups * 2) * 4;
 }
@@ -612,7 +620,7 @@ int bs_group_norm_act(const void* x, int64_t ldn, int64_t ldp, const void* gamma
     if (n == 0 || pixels == 0) return BS_OK;
     if (!x || !y || ldp < channels || ldn < 0) return BS_EINVAL;
     if ((gamma || beta) && affine_dtype != BS_DT_F32 && affine_dtype != dtype) return BS_EINVAL;
-    const Plan p = plan(dtype, pixels, channels, groups, 0);
+    const Plan p = plan(dtype, n, pixels, channels, groups, 0);
     const int64_t need = bs_group_norm_workspace(dtype, n, pixels, channels, groups, 0);
     if (need > 0 && (!workspace || workspace_bytes < need)) return BS_EINVAL;
     NormArgs a = {};
@@ -659,7 +667,7 @@ int bs_group_norm_act_grad(const void* g, int64_t ldgn, int64_t ldgp, const void
     }
     if (!g || !x || !stats || !dx || ldgp < channels || ldgn < 0 || (!x_exps && (ldp < channels || ldn < 0))) return BS_EINVAL;
     if ((gamma || beta) && affine_dtype != BS_DT_F32 && affine_dtype != dtype) return BS_EINVAL;
-    const Plan p = plan(dtype, pixels, channels, groups, 1);
+    const Plan p = plan(dtype, n, pixels, channels, groups, 1);
     const int64_t need = bs_group_norm_workspace(dtype, n, pixels, channels, groups, 1);
     if (!workspace || workspace_bytes < need) return BS_EINVAL;
     NormArgs a = {};

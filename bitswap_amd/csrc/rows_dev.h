@@ -86,17 +86,30 @@ __device__ __forceinline__ u32x4 pack16(const float* f) {
     }
     return r;
 }
-// the first n elements of such a vector (0 < n; all of them when n >= vlen), the others zero
+// the first n elements of such a vector (0 < n; all of them when n >= vlen), the others zero.  The end of a row is gathered by
+// loads that are all on their way at once (behind its last element they repeat that one): a branch per element would wait for
+// each of them in turn, and the whole wavefront with it.
 template <int DT>
-__device__ __forceinline__ void load_vec(const char* p, int n, float* f) {
+__device__ __forceinline__ u32x4 load_raw(const char* p, int n) {
     constexpr int V = vlen(DT);
-    if (n >= V) {
-        unpack16<DT>(load16(p), f);
-    } else {
+    if (n >= V) return load16(p);
+    u32x4 r;
+    if (DT == BS_DT_F32) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = i < n ? load1<DT>(p + i * esize(DT)) : 0.0f;
+        for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const uint32_t*>(p + min(i, n - 1) * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = i < n ? r[i] : 0u;
+    } else {
+        uint32_t u[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] = *reinterpret_cast<const uint16_t*>(p + min(i, n - 1) * 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = (2 * i < n ? u[2 * i] : 0u) | (2 * i + 1 < n ? u[2 * i + 1] << 16 : 0u);
     }
+    return r;
 }
+template <int DT>
+__device__ __forceinline__ void load_vec(const char* p, int n, float* f) { unpack16<DT>(load_raw<DT>(p, n), f); }
 template <int DT>
 __device__ __forceinline__ void store_vec(char* p, int n, const float* f) {
     constexpr int V = vlen(DT);
@@ -223,9 +236,11 @@ __device__ __forceinline__ void load_codes(const int8_t* __restrict__ codes, con
             w[0] = t[0]; w[1] = t[1];
         }
     } else {
+        uint32_t u[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i < n) w[i / 4] |= (uint32_t)(uint8_t)codes[c + i] << (8 * (i % 4));
+        for (int i = 0; i < V; ++i) u[i] = (uint8_t)codes[c + min(i, n - 1)];
+#pragma unroll
+        for (int i = 0; i < V; ++i) w[i / 4] |= i < n ? u[i] << (8 * (i % 4)) : 0u;
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) f[i] = p8_value((int)(int8_t)(w[i / 4] >> (8 * (i % 4))), (c + i) / P8_BLOCK == b0 ? s0 : s1);
