@@ -56,46 +56,67 @@ __device__ __forceinline__ float wave_sum(float v) {
     return v;
 }
 
-// Sums per thread and channel -> sums per group, known to every thread of the workgroup.
-//   a: this thread's sums of its channels, added up over its pixels; slot [pixel lane][channel of the slab] in `red`
-//   out[g] for the gs groups of the slab.  weight (null: 1) multiplies a channel's sum.  chan_out (nullable): the channel sums.
+// Workgroups of one XCD (blockIdx % 8) take a run of the work: the slabs of an image, whose rows share cache lines where a slab is no
+// multiple of them, go through one L2.  -1: nothing left (the grid is a multiple of 8).
+__device__ __forceinline__ int64_t xcd_run(int64_t total) {
+    const int64_t at = (blockIdx.x % 8) * ((total + 7) / 8) + blockIdx.x / 8;
+    return at < total ? at : -1;
+}
+
+// N sums per thread and channel -> sums per group, known to every thread of the workgroup (any channels per group).
+//   add_up: over the pixel lanes, in Q parts a channel (red -> part).  groups: over a group's parts, each channel's times its weight
+//   (null: 1), a wavefront a group.  channels: a channel's sum, out to memory.
 struct SlabSum {
     float *red, *part, *out;
-    int ch, PL, Q, gs, per, nthr, tid;           // ch: channels of the slab (chunks x V); Q: parts the pixel lanes are added in
-    template <int NV>
-    __device__ __forceinline__ void run(const float* a, int pl, int c, bool live, const char* weight, int w_f32, int c0, int C, int dt,
-                                        float* chan_out) const {
+    int ch, PL, Q, gs, per, nthr, tid;           // ch: channels of the slab (lanes x V)
+    template <int N, int V>
+    __device__ __forceinline__ void add_up(const float (&a)[N][V], int pl, int c, bool live) const {
         if (live)
 #pragma unroll
-            for (int i = 0; i < NV; ++i) red[pl * ch + c + i] = a[i];
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int i = 0; i < V; ++i) red[(n * PL + pl) * ch + c + i] = a[n][i];
         __syncthreads();
         for (int i = tid; i < ch * Q; i += nthr) {
             const int q = i / ch, k = i - q * ch;
-            float s = 0.0f;
-            for (int p = q; p < PL; p += Q) s += red[p * ch + k];
-            part[i] = s;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                float s = 0.0f;
+#pragma unroll 4
+                for (int p = q; p < PL; p += Q) s += red[(n * PL + p) * ch + k];
+                part[n * Q * ch + i] = s;
+            }
         }
         __syncthreads();
-        if (chan_out)
-            for (int k = tid; k < ch; k += nthr)
-                if (k < gs * per && c0 + k < C) {
-                    float s = 0.0f;
-                    for (int q = 0; q < Q; ++q) s += part[q * ch + k];
-                    chan_out[k] = s;
-                }
-        for (int g = tid >> 6; g < gs; g += nthr >> 6) {
-            float s = 0.0f;
-            for (int k = tid & 63; k < per; k += 64) {
-                float t = 0.0f;
-                for (int q = 0; q < Q; ++q) t += part[q * ch + g * per + k];
-                const int c_ = c0 + g * per + k;
-                if (weight && c_ < C)
-                    t *= w_f32 ? reinterpret_cast<const float*>(weight)[c_]
-                               : dt == BS_DT_BF16 ? load1<BS_DT_BF16>(weight + 2 * (int64_t)c_) : load1<BS_DT_F16>(weight + 2 * (int64_t)c_);
-                s += t;
+    }
+    template <int N>
+    __device__ __forceinline__ void channels(int width, int64_t C, float* to) const {
+        for (int k = tid; k < width; k += nthr)
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                float s = 0.0f;
+#pragma unroll 4
+                for (int q = 0; q < Q; ++q) s += part[(n * Q + q) * ch + k];
+                to[n * C + k] = s;
             }
-            s = wave_sum(s);
-            if ((tid & 63) == 0) out[g] = s;
+    }
+    template <int N>
+    __device__ __forceinline__ void groups(const float* weight) const {
+        for (int g = tid >> 6; g < gs; g += nthr >> 6) {
+            float s[N];
+#pragma unroll
+            for (int n = 0; n < N; ++n) s[n] = 0.0f;
+            for (int j = tid & 63; j < per * Q; j += 64) {
+                const int q = j / per, k = g * per + j - q * per;
+                const float w = weight ? weight[k] : 1.0f;
+#pragma unroll
+                for (int n = 0; n < N; ++n) s[n] = fmaf(part[(n * Q + q) * ch + k], w, s[n]);
+            }
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                s[n] = wave_sum(s[n]);
+                if ((tid & 63) == 0) out[n * gs + g] = s[n];
+            }
         }
         __syncthreads();
     }
@@ -142,8 +163,10 @@ __global__ __launch_bounds__(1024) void k_norm(const NormArgs a) {
     constexpr int V = vlen(DT), R = 32 / V, ES = esize(DT);
     extern __shared__ __align__(16) float sh[];
     const int PL = a.pl, CL = a.cl, tid = threadIdx.x;
-    const int64_t img = blockIdx.x / a.slabs;
-    const int slab = blockIdx.x % a.slabs, c0 = slab * a.gs * a.per;
+    const int64_t at = xcd_run(a.n * a.slabs);
+    if (at < 0) return;
+    const int64_t img = at / a.slabs;
+    const int slab = (int)(at % a.slabs), c0 = slab * a.gs * a.per;
     const int width = min(a.gs * a.per, a.C - c0);               // channels of this slab
     const int pl = tid / CL, cl = tid - pl * CL, k = cl * V, left = width - k;
     const bool live = pl < PL && left > 0;
@@ -161,7 +184,7 @@ __global__ __launch_bounds__(1024) void k_norm(const NormArgs a) {
     affine<DT>(a.gamma, a.aff_f32, c0 + k, live ? left : 0, 1.0f, ga);
     affine<DT>(a.beta, a.aff_f32, c0 + k, live ? left : 0, 0.0f, be);
     const float inv = 1.0f / ((float)a.pixels * (float)a.per);
-    float m[V], rs[V], s[V];
+    float m[V], rs[V];
     if (LANES) {
         const LaneSum<1> sum = lane_sum<1>(a, cl, V, tid);
         float t[1] = {0.0f};
@@ -195,27 +218,33 @@ __global__ __launch_bounds__(1024) void k_norm(const NormArgs a) {
         ss.ch = CL * V; ss.PL = PL; ss.Q = max(1, PL / V); ss.gs = min(a.gs, a.G - slab * a.gs); ss.per = a.per;
         ss.nthr = blockDim.x; ss.tid = tid;
         ss.red = sh; ss.part = sh + PL * ss.ch; ss.out = ss.part + ss.Q * ss.ch;
+        float t[1][V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            s[i] = 0.0f;
+            t[0][i] = 0.0f;
 #pragma unroll
-            for (int r = 0; r < R; ++r) s[i] += f[r][i];
+            for (int r = 0; r < R; ++r) t[0][i] += f[r][i];
         }
-        ss.run<V>(s, pl, k, live, nullptr, 0, c0, a.C, DT, nullptr);
+        int g[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) m[i] = i < left ? ss.out[(k + i) / a.per] * inv : 0.0f;
+        for (int i = 0; i < V; ++i) g[i] = min(k + i, width - 1) / a.per;
+        ss.add_up<1, V>(t, pl, k, live);
+        ss.groups<1>(nullptr);
+#pragma unroll
+        for (int i = 0; i < V; ++i) m[i] = i < left ? ss.out[g[i]] * inv : 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            s[i] = 0.0f;
+            t[0][i] = 0.0f;
 #pragma unroll
             for (int r = 0; r < R; ++r)
-                if (pl + r * PL < a.pixels) s[i] = fmaf(f[r][i] - m[i], f[r][i] - m[i], s[i]);
+                if (pl + r * PL < a.pixels) t[0][i] = fmaf(f[r][i] - m[i], f[r][i] - m[i], t[0][i]);
         }
         float* const mean_sh = ss.out;                               // the means stay: the next sums go behind them
         ss.out += ss.gs;
-        ss.run<V>(s, pl, k, live, nullptr, 0, c0, a.C, DT, nullptr);
+        ss.add_up<1, V>(t, pl, k, live);
+        ss.groups<1>(nullptr);
 #pragma unroll
-        for (int i = 0; i < V; ++i) rs[i] = i < left ? 1.0f / sqrtf(ss.out[(k + i) / a.per] * inv + a.eps) : 0.0f;
+        for (int i = 0; i < V; ++i) rs[i] = i < left ? 1.0f / sqrtf(ss.out[g[i]] * inv + a.eps) : 0.0f;
         if (a.stats && tid < ss.gs) {
             float* const o = a.stats + (img * a.G + slab * a.gs + tid) * 2;
             o[0] = mean_sh[tid] * inv;
@@ -251,15 +280,18 @@ __global__ __launch_bounds__(512) void k_norm_grad(const NormArgs a) {
     constexpr int V = vlen(DT), R = 32 / V, ES = esize(DT);
     extern __shared__ __align__(16) float sh[];
     const int PL = a.pl, CL = a.cl, tid = threadIdx.x;
-    const int64_t img = blockIdx.x / a.slabs;
-    const int slab = blockIdx.x % a.slabs, c0 = slab * a.gs * a.per;
+    const int64_t at = xcd_run(a.n * a.slabs);
+    if (at < 0) return;
+    const int64_t img = at / a.slabs;
+    const int slab = (int)(at % a.slabs), c0 = slab * a.gs * a.per;
     const int width = min(a.gs * a.per, a.C - c0);
     const int pl = tid / CL, cl = tid - pl * CL, k = cl * V, left = width - k;
     const bool live = pl < PL && left > 0;
     SlabSum ss;
     ss.ch = CL * V; ss.PL = PL; ss.Q = max(1, PL / V); ss.gs = min(a.gs, a.G - slab * a.gs); ss.per = a.per;
     ss.nthr = blockDim.x; ss.tid = tid;
-    ss.red = sh; ss.part = sh + PL * ss.ch; ss.out = ss.part + ss.Q * ss.ch;
+    ss.red = sh; ss.part = sh + 2 * PL * ss.ch; ss.out = ss.part + 2 * ss.Q * ss.ch;
+    float* const weight = ss.out + 32 * a.gs;
 
     float h[R][V], d[R][V], m[V], rs[V], ga[V], be[V];
 #pragma unroll
@@ -289,9 +321,9 @@ __global__ __launch_bounds__(512) void k_norm_grad(const NormArgs a) {
     }
     affine<DT>(a.gamma, a.aff_f32, c0 + k, live ? left : 0, 1.0f, ga);
     affine<DT>(a.beta, a.aff_f32, c0 + k, live ? left : 0, 0.0f, be);
-    float s1[V], s2[V];
+    float s[2][V];                                                   // sums of du h and of du
 #pragma unroll
-    for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.0f;
+    for (int i = 0; i < V; ++i) s[0][i] = s[1][i] = 0.0f;
 #pragma unroll
     for (int r = 0; r < R; ++r)
         if (live && pl + r * PL < a.pixels) {
@@ -304,8 +336,8 @@ __global__ __launch_bounds__(512) void k_norm_grad(const NormArgs a) {
             act_slopes<V>(a.act, u, d[r]);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                s1[i] += d[r][i];
-                s2[i] = fmaf(d[r][i], h[r][i], s2[i]);
+                s[0][i] = fmaf(d[r][i], h[r][i], s[0][i]);
+                s[1][i] += d[r][i];
             }
         }
     float* const po = a.parts ? a.parts + img * 2 * a.C + c0 : nullptr;
@@ -316,25 +348,27 @@ __global__ __launch_bounds__(512) void k_norm_grad(const NormArgs a) {
         float t[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            t[0] = fmaf(ga[i], s1[i], t[0]);
-            t[1] = fmaf(ga[i], s2[i], t[1]);
+            t[0] = fmaf(ga[i], s[0][i], t[0]);
+            t[1] = fmaf(ga[i], s[1][i], t[1]);
         }
         sum.run(t, ss.out);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            m1[i] = t[0] * inv;
-            m2[i] = t[1] * inv;
+            m2[i] = t[0] * inv;
+            m1[i] = t[1] * inv;
         }
     } else {
-        ss.run<V>(s2, pl, k, live, a.gamma, a.aff_f32, c0, a.C, DT, po);
-        const float* const two = ss.out;
-        ss.out += ss.gs;
-        ss.run<V>(s1, pl, k, live, a.gamma, a.aff_f32, c0, a.C, DT, po ? po + a.C : nullptr);
+        if (live && pl == 0)
+#pragma unroll
+            for (int i = 0; i < V; ++i) weight[k + i] = ga[i];
+        ss.add_up<2, V>(s, pl, k, live);
+        if (po) ss.channels<2>(width, a.C, po);
+        ss.groups<2>(weight);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int g = min(k + i, width - 1) / a.per;
-            m1[i] = ss.out[g] * inv;
-            m2[i] = two[g] * inv;
+            m2[i] = ss.out[g] * inv;
+            m1[i] = ss.out[ss.gs + g] * inv;
         }
     }
     if (live) {
@@ -349,25 +383,8 @@ __global__ __launch_bounds__(512) void k_norm_grad(const NormArgs a) {
         }
     }
     if (LANES && po) {                                               // the channels' sums over the pixels, while dx is on its way out
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            if (live)
-#pragma unroll
-                for (int i = 0; i < V; ++i) ss.red[pl * ss.ch + k + i] = n ? s1[i] : s2[i];
-            __syncthreads();
-            for (int i = tid; i < ss.ch * ss.Q; i += ss.nthr) {
-                const int q = i / ss.ch, c = i - q * ss.ch;
-                float t = 0.0f;
-                for (int p = q; p < PL; p += ss.Q) t += ss.red[p * ss.ch + c];
-                ss.part[i] = t;
-            }
-            __syncthreads();
-            for (int c = tid; c < width; c += ss.nthr) {
-                float t = 0.0f;
-                for (int q = 0; q < ss.Q; ++q) t += ss.part[q * ss.ch + c];
-                po[n * a.C + c] = t;
-            }
-        }
+        ss.add_up<2, V>(s, pl, k, live);
+        ss.channels<2>(width, a.C, po);
     }
 }
 
@@ -580,8 +597,7 @@ Plan plan(int dtype, int64_t n, int64_t pixels, int C, int G, int grad) {
         p.slabs = (G + gs - 1) / gs;
         p.threads = (p.pl * p.cl + 63) / 64 * 64;
         const int ch = p.cl * V, Q = p.pl / V > 1 ? p.pl / V : 1;
-        const int sums = p.lanes ? 32 * gs : 2 * gs;
-        p.lds = (p.lanes && !grad ? sums : p.pl * ch + Q * ch + sums) * 4;
+        p.lds = ((p.lanes && !grad ? 0 : (grad ? 2 : 1) * (p.pl + Q) * ch) + 32 * gs + (grad ? ch : 0)) * 4;
         return p;
     }
     const int chunks = (C + V - 1) / V;
@@ -629,7 +645,7 @@ int bs_group_norm_act(const void* x, int64_t ldn, int64_t ldp, const void* gamma
     a.C = channels; a.G = groups; a.per = channels / groups; a.y = (char*)y; a.stats = stats;
     fill(&a, p);
     hipStream_t st = rows_stream(stream);
-    const int64_t blocks = p.fits ? n * p.slabs : n * p.runs;
+    const int64_t blocks = p.fits ? (n * p.slabs + 7) / 8 * 8 : n * p.runs;
     if (blocks > 0x7fffffff || n * groups > 0x7fffffff) return BS_EINVAL;
     if (p.fits) {
 #define GO(DT) do { if (p.lanes) hipLaunchKernelGGL((k_norm<DT, true>), dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a); \
@@ -677,7 +693,7 @@ int bs_group_norm_act_grad(const void* g, int64_t ldgn, int64_t ldgp, const void
     a.n = n; a.pixels = pixels; a.C = channels; a.G = groups; a.per = channels / groups;
     a.y = (char*)dx; a.stats = (float*)stats; a.parts = (float*)workspace;
     fill(&a, p);
-    const int64_t blocks = p.fits ? n * p.slabs : n * p.runs;
+    const int64_t blocks = p.fits ? (n * p.slabs + 7) / 8 * 8 : n * p.runs;
     if (blocks > 0x7fffffff || n * groups > 0x7fffffff) return BS_EINVAL;
     if (p.fits) {
         if (!dgamma && !dbeta) a.parts = nullptr;
