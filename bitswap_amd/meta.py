@@ -29,6 +29,8 @@ CDF_SPECS = (1, 2, 3, 4)
 DEFAULT_GEMM_ARITH = "bf16x3"
 ROUTE_REV = 3    # bump when a kernel or route change alters the float32 bits of (mu, scale) or the integer tables
 
+POINT_REV = 1    # the same for the pointwise layers of Model(npoint=k): group norm and products on channels-last activations
+
 
 class StreamMismatch(RuntimeError):
     """The stream was written with settings this receiver does not reproduce."""
@@ -39,6 +41,8 @@ def route(model):
     fused = bool(getattr(model, "fused", False))
     own = bool(getattr(model, "own_gemm", False))
     r = {"rev": ROUTE_REV, "fused": fused, "nn_batch": getattr(model, "nn_batch", None)}
+    if getattr(model, "npoint", 0):      # pointwise layers (csrc/linear.hip, norm_act.hip): their own revision
+        r["point"] = {"layers": int(model.npoint), "rev": POINT_REV}
     if fused:
         r.update({"conv_algo": model.conv_algo, "wino_inputs": bool(model.wino_inputs), "wino_in5": bool(model.wino_in5),
                   "fused_inputs": bool(model.fused_inputs), "pad_channels": bool(model.pad_channels),

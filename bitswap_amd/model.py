@@ -215,7 +215,11 @@ class _WinoOperand:
 
 class Model(nn.Module):
     def __init__(self, xs=(3, 32, 32), nz=1, zchannels=16, nprocessing=1, kernel_size=3, resdepth=2,
-                 reswidth=256, dropout_p=0., tag='', root_process=True, conditional_gen_std=False, nn_batch=None):
+                 reswidth=256, dropout_p=0., tag='', root_process=True, conditional_gen_std=False, nn_batch=None, npoint=0,
+                 save8=False):
+        """Beyond the reference's arguments: nn_batch (above); npoint pointwise residual layers (layers.PointwiseResNetLayer,
+        group norm + 1x1 convolutions on channels-last activations) close each of the 2 nz conv stacks in front of its heads --
+        0, the reference's architecture, by default; save8 keeps their activations in 8 bits for the backward pass."""
         super().__init__()
         self.compressing = False
         self.xs, self.nz, self.zchannels, self.nprocessing = tuple(xs), nz, zchannels, nprocessing
@@ -327,6 +331,12 @@ class Model(nn.Module):
             self.gen_std = nn.Sequential(head(X4, 0.1), UnSqueeze2d(2))
         else:                     # mnist_train.py:306-308
             self.gen_std = nn.Parameter(torch.zeros(*self.xs))
+        self.npoint = int(npoint)
+        if self.npoint:           # (drawn behind everything else: the other parameters do not depend on it)
+            from .layers import PointwiseResNetLayer
+            self.point_infer, self.point_gen = (
+                nn.ModuleList([nn.Sequential(*[PointwiseResNetLayer(W, save8=save8) for _ in range(self.npoint)]) for _ in range(nz)])
+                for _ in range(2))
 
     # ----------------------------------------------------------------------------------------
     def load_state_dict(self, *a, **k):
@@ -614,17 +624,21 @@ class Model(nn.Module):
     def _infer_stack_fused(self, i, h):
         from . import hip
         hv = f"infer{i}" in self._heads_u
+        last = hv and not self.npoint
         if i == 0:
-            h = self._fused_res(self.infer_res1, self._fused_res(self.infer_res0, self._fused_in(self.infer_in, h, self.infer_res0)), hv)
+            h = self._fused_res(self.infer_res1, self._fused_res(self.infer_res0, self._fused_in(self.infer_in, h, self.infer_res0)), last)
         else:
-            h = self._fused_res(self.deepinfer_res[i - 1], self._fused_in(self.deepinfer_in[i - 1], h, self.deepinfer_res[i - 1]), hv)
+            h = self._fused_res(self.deepinfer_res[i - 1], self._fused_in(self.deepinfer_in[i - 1], h, self.deepinfer_res[i - 1]), last)
+        h = self._point_fused("point_infer", i, h, hv)
         return self._fused_head(f"infer{i}", h, hip.HEAD_SIGMOID)
 
     def _gen_stack_fused(self, i, h):
         from . import hip
         if i == 0:
             hv = self._gen_mu_u is not None
-            h = self._fused_res(self.gen_res0, self._fused_res(self.gen_res1, self._fused_in(self.gen_in, h, self.gen_res1)), hv)
+            h = self._fused_res(self.gen_res0, self._fused_res(self.gen_res1, self._fused_in(self.gen_in, h, self.gen_res1)),
+                                hv and not self.npoint)
+            h = self._point_fused("point_gen", 0, h, hv)
             if isinstance(h, _WinoOperand) and self.conditional_gen_std:
                 c = self.gen_mu[0].out_dim
                 x = hip.wino_fused(self._bmm(self._gen_mu_u, h.v), (h.shape[0], 2 * c) + h.shape[2:], 6, self._gen_b2,
@@ -642,9 +656,29 @@ class Model(nn.Module):
             else:
                 scale = self._gen_scale
             return mu, scale
-        h = self._fused_res(self.deepgen_res[i - 1], self._fused_in(self.deepgen_in[i - 1], h, self.deepgen_res[i - 1]),
-                            f"gen{i}" in self._heads_u)
+        hv = f"gen{i}" in self._heads_u
+        h = self._fused_res(self.deepgen_res[i - 1], self._fused_in(self.deepgen_in[i - 1], h, self.deepgen_res[i - 1]), hv and not self.npoint)
+        h = self._point_fused("point_gen", i, h, hv)
         return self._fused_head(f"gen{i}", h, hip.HEAD_SOFTPLUS)
+
+    def _point(self, which, i, h):
+        """The pointwise layers that close stack i: NCHW in and out, channels last between."""
+        if not self.npoint:
+            return h
+        return getattr(self, which)[i](h.permute(0, 2, 3, 1).contiguous()).permute(0, 3, 1, 2).contiguous()
+
+    def _point_fused(self, which, i, h, want_v):
+        """_point behind a fused stack; want_v: as the Winograd operand of the 3x3 head convolutions (channels padded again)."""
+        if not self.npoint:
+            return h
+        from . import hip
+        h = self._point(which, i, self._unpad(h))
+        if not want_v:
+            return h
+        extra = self._cp - h.shape[1]
+        if extra:
+            h = torch.cat([h, h.new_zeros((h.shape[0], extra) + tuple(h.shape[2:]))], 1)
+        return _WinoOperand(hip.wino_fused(h, tuple(h.shape), 0, None, None, False, ts_out=6)[2], h.shape)
 
     def _use_fused(self, h):
         return self.fused and self.compressing and h.is_cuda and not torch.is_grad_enabled()
@@ -655,11 +689,11 @@ class Model(nn.Module):
             with _blas(self.gemm_backend if self.conv_algo == "winograd" else None):
                 return self._infer_stack_fused(i, h.contiguous())
         if i == 0:
-            h = self.infer_res1(self.infer_res0(self.infer_in(h)))
+            h = self._point("point_infer", 0, self.infer_res1(self.infer_res0(self.infer_in(h))))
             mu = self.infer_mu(h)
             scale = 0.1 + 0.9 * self.sigmoid(self.infer_std(h) + 2.)
         else:
-            h = self.deepinfer_res[i - 1](self.deepinfer_in[i - 1](h))
+            h = self._point("point_infer", i, self.deepinfer_res[i - 1](self.deepinfer_in[i - 1](h)))
             mu = self.deepinfer_mu[i - 1](h)
             scale = 0.1 + 0.9 * self.sigmoid(self.deepinfer_std[i - 1](h) + 2.)
         return mu, scale
@@ -669,12 +703,12 @@ class Model(nn.Module):
             with _blas(self.gemm_backend if self.conv_algo == "winograd" else None):
                 return self._gen_stack_fused(i, h.contiguous())
         if i == 0:
-            h = self.gen_res0(self.gen_res1(self.gen_in(h)))
+            h = self._point("point_gen", 0, self.gen_res0(self.gen_res1(self.gen_in(h))))
             mu = self.gen_mu(h)
             std = self.gen_std(h) if self.conditional_gen_std else self.gen_std
             scale = ((2. / 255.) / 8.) + softplus(std)
         else:
-            h = self.deepgen_res[i - 1](self.deepgen_in[i - 1](h))
+            h = self._point("point_gen", i, self.deepgen_res[i - 1](self.deepgen_in[i - 1](h)))
             mu = self.deepgen_mu[i - 1](h)
             scale = 0.1 + 0.9 * softplus(self.deepgen_std[i - 1](h) + np.log(np.exp(1.) - 1.))
         return mu, scale

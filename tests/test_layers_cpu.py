@@ -105,3 +105,41 @@ def test_rows_and_images_are_read_in_place_where_their_strides_allow():
         t, ldn, ldp, n, pixels, c = hip._as_images(v, "x")
         assert (t.data_ptr() == v.data_ptr()) == inplace
         assert torch.equal(torch.as_strided(t, (n, pixels, c), (ldn, ldp, 1)), v.reshape(n, pixels, c))
+
+
+def test_layers_on_the_cpu_and_the_models_option():
+    """The plain path: gradients against differences; Model(npoint=0) is the reference's architecture, npoint > 0 adds parameters
+    and changes no other one."""
+    from bitswap_amd.layers import PointwiseResNetLayer, groups_for
+    from bitswap_amd.model import Model
+    assert [groups_for(c) for c in (256, 252, 254, 255, 64, 61, 16)] == [32, 28, 2, 17, 32, 1, 16]
+    torch.manual_seed(3)
+    for act in ("none", "elu", "silu", "gelu"):
+        layer = PointwiseResNetLayer(6, hidden=5, groups=3, act=act).double()
+        x = torch.randn(2, 3, 2, 6, dtype=torch.float64, requires_grad=True)
+        assert torch.autograd.gradcheck(lambda *a: layer(a[0]), (x,) + tuple(layer.parameters()), atol=1e-6)
+    kw = dict(xs=(1, 32, 32), nz=2, zchannels=1, nprocessing=1, resdepth=2, reswidth=12)
+    torch.manual_seed(5)
+    plain = Model(**kw)
+    torch.manual_seed(5)
+    point = Model(npoint=2, **kw)
+    a, b = plain.state_dict(), point.state_dict()
+    assert all(torch.equal(a[k], b[k]) for k in a)
+    more = set(b) - set(a)
+    assert len(more) == 4 * 2 * 6 and all(k.startswith(("point_infer.", "point_gen.")) for k in more)
+    torch.manual_seed(6)
+    lr, ld, le, _ = point.loss(torch.randint(0, 256, (2, 1, 32, 32)).float())
+    (-lr + (le - ld).sum()).backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in point.parameters() if p.requires_grad)
+    assert point.point_gen[0][1].w2.grad.abs().sum() > 0 and point.point_infer[1][0].gamma.grad.abs().sum() > 0
+
+
+def test_stream_record_names_the_pointwise_layers():
+    from bitswap_amd import meta
+    from bitswap_amd.model import Model
+    kw = dict(xs=(1, 32, 32), nz=2, zchannels=1, nprocessing=1, resdepth=2, reswidth=12)
+    assert "point" not in meta.route(Model(**kw))
+    r = meta.route(Model(npoint=2, **kw))
+    assert r["point"] == {"layers": 2, "rev": meta.POINT_REV}
+    with pytest.raises(meta.StreamMismatch):
+        meta.check({"conv_route": r}, {"conv_route": meta.route(Model(**kw))})

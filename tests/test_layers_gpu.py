@@ -607,3 +607,154 @@ def test_refusals(hip):
                 lambda: hip.pack8(x.long()), lambda: hip.unpack8(x), lambda: hip.pack8(x[:, :0])):
         with pytest.raises(Err):
             bad()
+
+
+# ---- run together, as a layer and in the model ------------------------------------------------------------------------------------
+def make_layer(c, hidden, act, dtype, save8=False, seed=1):
+    from bitswap_amd.layers import PointwiseResNetLayer
+    torch.manual_seed(seed)
+    layer = PointwiseResNetLayer(c, hidden=hidden, act=act, save8=save8)
+    with torch.no_grad():
+        for p in layer.parameters():
+            p.add_(0.2 * torch.randn_like(p) / math.sqrt(max(1, p.shape[-1] if p.dim() > 1 else 1)))
+    return layer.to("cuda", dtype)
+
+
+@pytest.mark.parametrize("act", ["elu", "silu", "gelu"])
+@pytest.mark.parametrize("n,c,hidden", [(3, 64, 64), (1, 61, 122), (30, 252, 96)])
+def test_layer_forward(hip, n, c, hidden, act):
+    """float32, every stage's bound carried through the next one."""
+    layer = make_layer(c, hidden, act, torch.float32)
+    x = randn((n, 16, 16, c), torch.float32, 2)
+    with torch.no_grad():
+        y = layer(x)
+    code = {"elu": 1, "silu": 2, "gelu": 3}[act]
+    p = {k: v.detach().double() for k, v in layer.named_parameters()}
+    mean, rstd, h0, u = norm64(x, layer.groups, p["gamma"], p["beta"], 1e-5)
+    eu = norm_bounds(x, mean, rstd, h0, u, p["gamma"], layer.groups)[2]
+    h = act64(u, code)
+    eh = 1.13 * eu + 16 * E * (u.abs() + 1)
+    s = h @ p["w1"].t() + p["b1"]
+    es = eh @ p["w1"].abs().t() + (c + 8) * E * (h.abs() @ p["w1"].abs().t() + p["b1"].abs())
+    t = act64(s, code)
+    et = 1.13 * es + 16 * E * (s.abs() + 1)
+    want = t @ p["w2"].t() + p["b2"] + x.double().view(n, -1, c)
+    mag = t.abs() @ p["w2"].abs().t() + p["b2"].abs() + x.double().abs().view(n, -1, c)
+    close(y.view(n, -1, c), want, et @ p["w2"].abs().t() + (hidden + 8) * E * mag + E * want.abs())
+
+
+@pytest.mark.parametrize("save8", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_layer_gradients_are_the_operators_chained(hip, dtype, save8):
+    n, c, hidden = 5, 60, 44
+    layer = make_layer(c, hidden, "silu", dtype, save8)
+    x, g = randn((n, 12, 10, c), dtype, 2).requires_grad_(), randn((n, 12, 10, c), dtype, 3)
+    names = [k for k, _ in layer.named_parameters()]
+    got = dict(zip(["x"] + names, torch.autograd.grad(layer(x), [x] + list(layer.parameters()), g)))
+    with torch.no_grad():
+        put = hip.pack8 if save8 else (lambda v: v)
+        h, st, _ = hip.group_norm_act(x, layer.groups, layer.gamma, layer.beta, act=2, want_stats=True)
+        s1, t = hip.linear_act(h, layer.w1, layer.b1, act=2, want_sum=True)
+        dt, dw2, db2, dres = hip.linear_act_grad(put(t), layer.w2, g_sum=g, want_res=True)
+        dh, dw1, db1, _ = hip.linear_act_grad(put(h), layer.w1, put(s1), act=2, g_act=dt)
+        dx, dgamma, dbeta = hip.group_norm_act_grad(put(x.detach()), st, layer.groups, dh, layer.gamma, layer.beta, act=2)
+        want = {"x": dx + dres, "gamma": dgamma.to(dtype), "beta": dbeta.to(dtype), "w1": dw1, "b1": db1.to(dtype), "w2": dw2, "b2": db2.to(dtype)}
+    for k, v in want.items():
+        assert got[k].dtype == dtype and torch.equal(got[k], v), k
+
+
+@pytest.mark.parametrize("act", ["elu", "gelu"])
+def test_layer_gradients_against_the_cpu_in_64_bits(hip, act):
+    """float32: a relative error of the whole gradient of 2^-24 times the longest sum's terms (3 x 16 x 16 x 61 values a group, added
+    in runs of 32 and lanes: 300) times a condition of at most 30 for such layers: 5e-4."""
+    layer = make_layer(61, 40, act, torch.float32)
+    x, g = randn((3, 16, 16, 61), torch.float32, 2).requires_grad_(), randn((3, 16, 16, 61), torch.float32, 3)
+    got = torch.autograd.grad(layer(x), [x] + list(layer.parameters()), g)
+    import copy
+    ref = copy.deepcopy(layer).cpu().double()
+    x64 = x.detach().cpu().double().requires_grad_()
+    want = torch.autograd.grad(ref(x64), [x64] + list(ref.parameters()), g.cpu().double())
+    for a, b in zip(got, want):
+        assert float((a.cpu().double() - b).norm() / b.norm()) < 5e-4
+
+
+def test_saved8_takes_less_memory_and_keeps_the_forward(hip):
+    used = []
+    for save8 in (False, True):
+        layer = make_layer(256, 256, "elu", torch.float32, save8)
+        x = randn((100, 16, 16, 256), torch.float32, 2).requires_grad_()
+        before = torch.cuda.memory_allocated()
+        y = layer(x)
+        kept = torch.cuda.memory_allocated() - before - y.numel() * 4
+        used.append((y.detach(), kept))
+    assert torch.equal(used[0][0], used[1][0])
+    # whole: x is the caller's; h, s, t of 26 MB each.  8 bits: x, h, s, t of 6.8 MB each
+    assert used[1][1] < 0.55 * used[0][1]
+
+
+def test_training_step_in_a_graph(hip):
+    """Forward and gradients captured, replayed between eager steps of the same leaves: the same bits."""
+    layer = make_layer(64, 64, "silu", torch.bfloat16, True)
+    x, g = randn((4, 16, 16, 64), torch.bfloat16, 2).requires_grad_(), randn((4, 16, 16, 64), torch.bfloat16, 3)
+    leaves = [x] + list(layer.parameters())
+
+    def step():
+        return torch.autograd.grad(layer(x), leaves, g)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = step()
+    for k in range(3):
+        with torch.no_grad():
+            x.copy_(randn(tuple(x.shape), torch.bfloat16, 40 + k))
+        gr.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+
+
+def test_model_trains_with_pointwise_layers(hip):
+    from bitswap_amd.model import Model
+    torch.manual_seed(4)
+    kw = dict(xs=(1, 32, 32), nz=2, zchannels=1, nprocessing=1, resdepth=2, reswidth=12, npoint=1)
+    for save8 in (False, True):
+        m = Model(save8=save8, **kw).cuda()
+        lr, ld, le, _ = m.loss(torch.randint(0, 256, (2, 1, 32, 32), device="cuda").float())
+        (-lr + (le - ld).sum()).backward()
+        assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in m.parameters() if p.requires_grad)
+        assert m.point_gen[1][0].w1.grad.abs().sum() > 0
+
+
+@pytest.mark.parametrize("small", [16, 60])          # 60: run at 64 channels by the convolutions, at 60 by the pointwise layers
+def test_codec_with_pointwise_layers_is_lossless_and_batch_invariant(hip, small):
+    """The layers on the coding path: (mu, scale) of a chain do not depend on how many are coded together, so streams written by four
+    chains at once are read one chain at a time."""
+    from bitswap_amd import workload
+    from bitswap_amd.codec import BitSwapCodec
+    from bitswap_amd.model import Model
+    base, zend, zcen = workload.build("mnist2", torch.device("cuda"), quantbits=8, small=small)
+    m = Model(xs=base.xs, nz=base.nz, zchannels=base.zchannels, nprocessing=1, kernel_size=3, resdepth=2, reswidth=small, npoint=2)
+    missing = m.load_state_dict(base.cpu().state_dict(), strict=False)
+    assert not missing.unexpected_keys and all(k.startswith("point_") for k in missing.missing_keys)
+    m = m.cuda().eval().fold().fuse()
+    m.compress(True)
+    z = randn((4, base.zdim_flat), torch.float32, 8)
+    with torch.no_grad():
+        whole = m.generate(1)(given=z)
+        for b in range(4):
+            one = m.generate(1)(given=z[b:b + 1])
+            assert all(torch.equal(u[b:b + 1], v) for u, v in zip(whole, one))
+    images = workload.synthetic_blocks(4 * 2, m.xs, seed=3).view(4, 2, -1).to(torch.int32)
+    codec = BitSwapCodec(m, zend, zcen, quantbits=8, bitswap=True)
+    state, _ = codec.compress(images, nwords=2000)
+    words = state.to_lists()
+    from bitswap_amd import hip as h
+    for b in range(4):
+        one = h.RansState.from_lists([words[b]], cap=state.cap)
+        out = codec.decompress(one, 2)
+        assert torch.equal(out.cpu()[0], images[b])
