@@ -112,7 +112,7 @@ __device__ __forceinline__ void finish(const RowsArgs& a, int64_t q, int64_t p, 
         }
         if (a.sum) store_vec<DT>(a.sum + at, n, v);
         if (a.act_out) {
-            act_values<V>(a.act, v, t);
+            act_values<DT, V>(a.act, v, t);
             store_vec<DT>(a.act_out + at, n, t);
         }
     } else {
@@ -195,8 +195,8 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_rows(const RowsA
     constexpr int SL = BK / 8, RB = BK * 2;                    // chunks and bytes of a row
     constexpr int XB = L * BQ * RB, WB = L * BP * RB, STAGE = XB + WB;
     constexpr int NP = WP / 32, NQ = WQ / 32;
-    static_assert(2 * STAGE <= 160 * 1024 && NW * TURN <= 2 * STAGE && (NP == 2 || NP == 4), "shared memory");
-    __shared__ __align__(16) char lds[2 * STAGE];
+    static_assert(2 * STAGE <= 160 * 1024 && NP % 2 == 0, "shared memory");
+    __shared__ __align__(16) char lds[2 * STAGE > NW * TURN ? 2 * STAGE : NW * TURN];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wp = wave % (BP / WP), wq = wave / (BP / WP);
     auto swz = [](int row, int c) { return SL == 8 ? (c ^ ((row >> 1) & 7)) : SL == 4 ? (c ^ ((row >> 2) & 3)) : (c ^ ((row >> 3) & 1)); };
@@ -503,8 +503,9 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64, PER_SIMD) void k_rows_d
 }
 
 // ---- forward and dx, few rows -------------------------------------------------------------------------------------------------
-// One 32x32 tile a workgroup.  Its four wavefronts hold four runs of k in registers, loaded at once straight from memory, and pass
-// the sums on from run to run (a relay): the order of k_rows, at the latency of about one load.
+// One 32x32 tile a workgroup.  Its four wavefronts hold four runs of k in registers, loaded at once straight from memory (the next
+// four while these are multiplied), and pass the sums on from run to run (a relay): the order of k_rows, at the latency of about
+// one load.
 template <int DT, int EPI, bool WL>
 __global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {
     constexpr int L = limbs_of(DT), NS = DT == BS_DT_F32 ? 4 : 8, ES = esize(DT), RUN = NS * 16;
@@ -539,12 +540,11 @@ __global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {
             l[0] = r[0];
         }
     };
-    for (int k0 = 0; k0 < a.K; k0 += 4 * RUN) {
-        u32x4 xr[NS][RAW], wr[NS][WL ? L : RAW];
-        const int kb = k0 + wave * RUN + 8 * (lane >> 5);
+    u32x4 xr[NS][RAW], wr[NS][WL ? L : RAW];
+    auto ask = [&](int k0) {
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
-            const int k = kb + n * 16;
+            const int k = k0 + wave * RUN + 8 * (lane >> 5) + n * 16;
             fetch(xp, k, xr[n]);
             if (WL) {
 #pragma unroll
@@ -554,8 +554,24 @@ __global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {
                 fetch(wp, k, wr[n]);
             }
         }
+    };
+    ask(0);
+    for (int k0 = 0; k0 < a.K; k0 += 4 * RUN) {
+        u32x4 fp[NS][1][L], fq[NS][1][L];
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            if (WL) {
+#pragma unroll
+                for (int l = 0; l < L; ++l) fp[n][0][l] = wr[n][l % (WL ? L : RAW)];
+            } else {
+                split(wr[n], fp[n][0]);
+            }
+            split(xr[n], fq[n][0]);
+        }
+        if (k0 + 4 * RUN < a.K) ask(k0 + 4 * RUN);                  // on its way while the others take their turns
         for (int turn = 0; turn < 4; ++turn) {
             if (turn == wave && k0 + wave * RUN < a.K) {
+                f32x16 one[1][1];
                 if (k0 + turn > 0) {
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) {
@@ -563,20 +579,10 @@ __global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {
                         acc[e] = t[0]; acc[e + 1] = t[1]; acc[e + 2] = t[2]; acc[e + 3] = t[3];
                     }
                 }
+                one[0][0] = acc;
 #pragma unroll
-                for (int n = 0; n < NS; ++n) {
-                    u32x4 fp[1][L], fq[1][L];
-                    if (WL) {
-#pragma unroll
-                        for (int l = 0; l < L; ++l) fp[0][l] = wr[n][l % (WL ? L : RAW)];
-                    } else {
-                        split(wr[n], fp[0]);
-                    }
-                    split(xr[n], fq[0]);
-                    f32x16 one[1][1] = {{acc}};
-                    multiply<DT, L, L, 1, 1>(fp, fq, one);
-                    acc = one[0][0];
-                }
+                for (int n = 0; n < NS; ++n) multiply<DT, L, L, 1, 1>(fp[n], fq[n], one);
+                acc = one[0][0];
 #pragma unroll
                 for (int e = 0; e < 16; e += 4)
                     *reinterpret_cast<f32x4*>(lds + (e * 64 + lane * 4) * 4) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
@@ -1141,31 +1147,36 @@ __global__ __launch_bounds__(256) void k_lay_steps(const int8_t* __restrict__ ex
     for (int b = 0; b < nb; ++b) out[b * ld + i] = i < rows ? p8_pow2(exps[i * nb + b]) : 0.0f;
 }
 
-// parts [nparts][n] float32 -> their sum in dtype; 64 threads of four neighbours x 4 lanes over the parts
+// parts [nparts][n] float32 -> their sum in dtype; 16 threads of four neighbours x 16 lanes over the parts
 template <int DT>
 __global__ __launch_bounds__(256) void k_add_parts(const float* __restrict__ parts, int nparts, int64_t n, char* __restrict__ out) {
     __shared__ __align__(16) f32x4 red[256];
-    const int64_t i = ((int64_t)blockIdx.x * 64 + (threadIdx.x & 63)) * 4;
-    const int l = threadIdx.x >> 6;
+    const int tx = threadIdx.x & 15, l = threadIdx.x >> 4;
+    const int64_t i = ((int64_t)blockIdx.x * 16 + tx) * 4;
     f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (i + 4 <= n) {
-        for (int k = l; k < nparts; k += 4) {
-            const f32x4 v = __builtin_bit_cast(f32x4, load16((const char*)(parts + k * n + i)));
+    if (i < n) {
+        const int left = n - i < 4 ? (int)(n - i) : 4;
+#pragma unroll 4
+        for (int k = l; k < nparts; k += 16) {
+            const f32x4 v = __builtin_bit_cast(f32x4, load_raw<BS_DT_F32>((const char*)(parts + k * n + i), left));
             s[0] += v[0]; s[1] += v[1]; s[2] += v[2]; s[3] += v[3];
         }
-    } else if (i < n) {
-        for (int k = l; k < nparts; k += 4)
-            for (int e = 0; e < n - i; ++e) s[e] += parts[k * n + i + e];
     }
     red[threadIdx.x] = s;
     __syncthreads();
     if (l || i >= n) return;
-    const f32x4 *r = red + threadIdx.x;
-    for (int e = 0; e < 4 && i + e < n; ++e) store1<DT>(out + (i + e) * esize(DT), (r[0][e] + r[64][e]) + (r[128][e] + r[192][e]));
+    float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] += red[k * 16 + tx][e];
+    for (int e = 0; e < 4 && i + e < n; ++e) store1<DT>(out + (i + e) * esize(DT), t[e]);
 }
 
 // ---- which way --------------------------------------------------------------------------------------------------------------------
-bool few(int64_t rows, int N) { return (rows + 31) / 32 * ((N + 31) / 32) <= 1024; }
+constexpr int RELAY_TILES = 256, MID_TILES = 256, BIG_TILES = 384;
+int64_t tiles_of(int64_t rows, int N, int bq, int bp) { return (rows + bq - 1) / bq * ((N + bp - 1) / bp); }
+bool few(int64_t rows, int N) { return tiles_of(rows, N, 32, 32) <= RELAY_TILES; }
 
 int64_t lay_bytes(int dtype, int K, int P) { return (int64_t)limbs_of(dtype) * P * ((K + 63) / 64 * 64) * 2; }
 
@@ -1173,9 +1184,13 @@ int64_t lay_bytes(int dtype, int K, int P) { return (int64_t)limbs_of(dtype) * P
 template <int DT, int EPI>
 int launch_rows(RowsArgs a, void* workspace, int64_t bytes, hipStream_t st) {
     const int kp = (a.K + 63) / 64 * 64;
-    const bool small = few(a.rows, a.N);
+    constexpr int CK = 16 / esize(DT);
+    const bool chunks = a.K % CK == 0 && a.ldx % CK == 0 && ((uintptr_t)a.x & 15) == 0 && a.ldx * esize(DT) < (1 << 22);
+    // (rows that DMA cannot take: the relay is ahead of k_rows up to four times as many tiles of few k)
+    const bool small = few(a.rows, a.N) || (!chunks && a.K <= 256 && tiles_of(a.rows, a.N, 32, 32) <= 4 * RELAY_TILES);
     const bool as_is = DT != BS_DT_F32 && !a.wt && a.K % 64 == 0 && a.ldw % 8 == 0 && ((uintptr_t)a.w & 15) == 0;
-    const bool lay = a.wt || !small; (void)as_is;
+    const bool big = DT != BS_DT_F32 && tiles_of(a.rows, a.N, 256, 256) >= BIG_TILES;
+    const bool lay = a.wt || (!small && (big || !as_is));
     if (lay) {
         if (!workspace || bytes < lay_bytes(DT, a.K, a.N)) return BS_EINVAL;
         const dim3 grid((unsigned)(kp / 64), (unsigned)((a.N + 31) / 32));
@@ -1195,23 +1210,22 @@ int launch_rows(RowsArgs a, void* workspace, int64_t bytes, hipStream_t st) {
         return rows_rc();
     }
     // rows of whole aligned chunks, tiles within 31 bits of their first byte: both operands by DMA
-    constexpr int CK = 16 / esize(DT);
-    const bool dma = a.K % CK == 0 && a.ldx % CK == 0 && ((uintptr_t)a.x & 15) == 0 && a.ldx * esize(DT) < (1 << 22) &&
-                     (a.sl * limbs_of(DT) + a.sp * 256 + a.sk * 2) * 2 < 0x7fffffff;
-    auto tiles = [&](int bq, int bp) {
-        a.tp = (a.N + bp - 1) / bp;
-        a.tiles = (a.rows + bq - 1) / bq * a.tp;
-        return (a.tiles + 7) / 8 * 8;
-    };
-#define ROWS(KERNEL, BQ, BP, NT) do { const int64_t blocks = tiles(BQ, BP); if (blocks > 0x7fffffff) return BS_EINVAL; \
+    const bool dma = chunks && (a.sl * limbs_of(DT) + a.sp * 256 + a.sk * 2) * 2 < 0x7fffffff;
+#define ROWS(KERNEL, BQ, BP, NT) do { a.tp = (a.N + BP - 1) / BP; a.tiles = tiles_of(a.rows, a.N, BQ, BP); \
+        const int64_t blocks = (a.tiles + 7) / 8 * 8; if (blocks > 0x7fffffff) return BS_EINVAL; \
         hipLaunchKernelGGL((KERNEL), dim3((unsigned)blocks), dim3(NT), 0, st, a); } while (0)
 #define K_(...) __VA_ARGS__
     if constexpr (DT == BS_DT_F32) {
-        if (dma) ROWS(K_(k_rows_dma<DT, EPI, 64, 128, 32, 64, 16, 3, 3>), 64, 128, 256);
-        else ROWS(K_(k_rows<DT, EPI, 128, 128, 64, 64, 16>), 128, 128, 256);
+        if (dma && tiles_of(a.rows, a.N, 64, 128) >= MID_TILES && a.N > 64) ROWS(K_(k_rows_dma<DT, EPI, 64, 128, 32, 64, 16, 3, 3>), 64, 128, 256);
+        else if (dma) ROWS(K_(k_rows_dma<DT, EPI, 64, 64, 32, 64, 16, 6, 1>), 64, 64, 128);
+        else if (tiles_of(a.rows, a.N, 128, 128) >= MID_TILES && a.N > 64) ROWS(K_(k_rows<DT, EPI, 128, 128, 64, 64, 16>), 128, 128, 256);
+        else ROWS(K_(k_rows<DT, EPI, 64, 64, 32, 64, 16>), 64, 64, 128);
     } else {
-        if (dma) ROWS(K_(k_rows_dma<DT, EPI, 256, 256, 128, 64, 32, 4, 1>), 256, 256, 512);
-        else ROWS(K_(k_rows<DT, EPI, 128, 128, 64, 64, 64>), 128, 128, 256);
+        if (dma && big) ROWS(K_(k_rows_dma<DT, EPI, 256, 256, 128, 64, 32, 4, 1>), 256, 256, 512);
+        else if (dma && tiles_of(a.rows, a.N, 128, 128) >= MID_TILES && a.N > 64) ROWS(K_(k_rows_dma<DT, EPI, 128, 128, 64, 64, 32, 4, 1>), 128, 128, 256);
+        else if (dma) ROWS(K_(k_rows_dma<DT, EPI, 64, 64, 32, 64, 32, 4, 1>), 64, 64, 128);
+        else if (tiles_of(a.rows, a.N, 128, 128) >= MID_TILES && a.N > 64) ROWS(K_(k_rows<DT, EPI, 128, 128, 64, 64, 64>), 128, 128, 256);
+        else ROWS(K_(k_rows<DT, EPI, 64, 64, 32, 64, 64>), 64, 64, 128);
     }
 #undef K_
 #undef ROWS
@@ -1219,13 +1233,14 @@ int launch_rows(RowsArgs a, void* workspace, int64_t bytes, hipStream_t st) {
 }
 
 // How a weight gradient is cut: tiles of BQ x 128 outputs (256 channels of ds where there are that many), and the rows into as many
-// parts as give the chip two workgroups a compute unit, none under 256 rows.
-int over_bq(int dtype, int N) { return dtype != BS_DT_F32 && N > 128 ? 256 : 128; }
+// parts as give the chip two workgroups a compute unit, none under 128 rows.
+int over_bq(int dtype, int64_t rows, int K, int N) {
+    return dtype != BS_DT_F32 && N > 128 && tiles_of(N, K, 256, 128) * ((rows + 255) / 256) >= 512 ? 256 : 128;
+}
 void split_rows(int dtype, int64_t rows, int K, int N, int64_t* part, int64_t* parts) {
-    const int bq = over_bq(dtype, N);
-    const int64_t tiles = (int64_t)((K + 127) / 128) * ((N + bq - 1) / bq);
+    const int64_t tiles = tiles_of(N, K, over_bq(dtype, rows, K, N), 128);
     int64_t want = (512 + tiles - 1) / tiles;
-    const int64_t most = (rows + 255) / 256;
+    const int64_t most = (rows + 127) / 128;
     if (want > most) want = most;
     if (want < 1) want = 1;
     *part = ((rows + want - 1) / want + 63) / 64 * 64;
@@ -1236,7 +1251,7 @@ int64_t steps_bytes(int64_t rows, int K) { return (int64_t)((K + 31) / 32) * ((r
 
 template <int DT>
 int launch_over(OverArgs a, char* steps, hipStream_t st) {
-    constexpr int BK = DT == BS_DT_F32 ? 16 : 64, CK = 16 / esize(DT);
+    constexpr int BK = DT == BS_DT_F32 ? 16 : 32, CK = 16 / esize(DT);
     auto go = [&](int bq) {
         a.tp = (a.K + 127) / 128;
         a.tiles = (int64_t)a.tp * ((a.N + bq - 1) / bq) * a.parts;
@@ -1255,11 +1270,11 @@ int launch_over(OverArgs a, char* steps, hipStream_t st) {
             const int nb = (a.K + 31) / 32;
             hipLaunchKernelGGL(k_lay_steps, dim3((unsigned)((ld + 255) / 256)), dim3(256), 0, st, a.exps, a.rows, nb, (float*)steps, ld);
             if constexpr (DT == BS_DT_F32) OVER(true, 128, 64, 32, 3);
-            else if (over_bq(DT, a.N) == 256) OVER(true, 256, 128, 32, 3);
+            else if (over_bq(DT, a.rows, a.K, a.N) == 256) OVER(true, 256, 128, 32, 3);
             else OVER(true, 128, 64, 32, 4);
         } else {
             if constexpr (DT == BS_DT_F32) OVER(false, 128, 64, 16, 4);
-            else if (over_bq(DT, a.N) == 256) OVER(false, 256, 128, 32, 3);
+            else if (over_bq(DT, a.rows, a.K, a.N) == 256) OVER(false, 256, 128, 32, 3);
             else OVER(false, 128, 64, 32, 4);
         }
         return rows_rc();
@@ -1351,7 +1366,7 @@ int bs_linear_grad_w(const void* ds, int64_t ldds, const void* x, const int8_t* 
         parts = 0;                                            // the sum of no parts
     }
     const float* ws = (const float*)((const char*)workspace + before);
-    const dim3 blocks((unsigned)((n + 255) / 256));
+    const dim3 blocks((unsigned)((n + 63) / 64));
     if (dtype == BS_DT_F32) hipLaunchKernelGGL(k_add_parts<BS_DT_F32>, blocks, dim3(256), 0, st, ws, (int)parts, n, (char*)dw);
     else if (dtype == BS_DT_BF16) hipLaunchKernelGGL(k_add_parts<BS_DT_BF16>, blocks, dim3(256), 0, st, ws, (int)parts, n, (char*)dw);
     else hipLaunchKernelGGL(k_add_parts<BS_DT_F16>, blocks, dim3(256), 0, st, ws, (int)parts, n, (char*)dw);

@@ -259,7 +259,7 @@ __global__ __launch_bounds__(1024) void k_norm(const NormArgs a) {
         if (p >= a.pixels) break;
 #pragma unroll
         for (int i = 0; i < V; ++i) f[r][i] = fmaf((f[r][i] - m[i]) * rs[i], ga[i], be[i]);
-        act_values<V>(a.act, f[r], f[r]);
+        act_values<DT, V>(a.act, f[r], f[r]);
         store_vec<DT>(yp + p * a.C * ES, left, f[r]);
     }
 }
@@ -556,7 +556,7 @@ __global__ __launch_bounds__(256) void k_apply(const NormArgs a, const float* __
 #pragma unroll
             for (int i = 0; i < V; ++i) f[i] = rs[i] * (fmaf(g[i], ga[i], -m1[i]) - f[i] * m2[i]);
         } else {
-            act_values<V>(a.act, u, f);
+            act_values<DT, V>(a.act, u, f);
         }
         store_vec<DT>(a.y + ((img * a.pixels + p) * a.C + c) * ES, left, f);
     }
