@@ -1,9 +1,9 @@
 // linear.hip -- products over rows of channels (channels-last activations): s = x w^T + bias (+ res) with its activation, and the
 // two products of its backward pass, on the bf16 / f16 matrix cores (v_mfma_f32_32x32x16), float32 sums.
 //
-//   forward  out[q][p] = sum_k w[p][k] x[q][k]          k = K, the contiguous axis of both: k_rows / k_relay
+//   forward  out[q][p] = sum_k w[p][k] x[q][k]          k = K, the contiguous axis of both: k_rows_dma / k_relay
 //   dx       out[q][p] = sum_k w[k][p] ds[q][k]         k = N; w is small and is turned round first (k_lay_w), then as the forward
-//   dw       out[q][p] = sum_k x[k][p] ds[k][q]         k = rows, the strided axis of both: k_over_rows, cut into parts of the rows
+//   dw       out[q][p] = sum_k x[k][p] ds[k][q]         k = rows, the strided axis of both: k_over_dma, cut into parts of the rows
 //
 // float32 operands are split into three bfloat16 limbs (their sum is the float exactly) and multiplied as the six limb products of
 // total order <= 2; what is left out is of relative size 2^-24.  Limb products of an infinity or of a value that rounds to one are
@@ -64,11 +64,14 @@ __device__ __forceinline__ void multiply(const u32x4 (&fp)[NP][LP], const u32x4 
 struct RowsArgs {
     const char *x, *w;                 // operands as the caller holds them
     int64_t ldx, ldw;
+    const char* xd;                    // x as DMA takes it (rows of whole chunks): x itself or its copy
+    int64_t ldxd;
     const char* wl;                    // w as the kernel reads it, 16-bit: laid out (k_lay_w), or w itself
     int64_t sp, sk, sl;                // element (limb, p, k) is at limb sl + p sp + k / KB sk + k % KB
     int kp;                            // k it has, a multiple of 64; zero behind K
     int64_t rows;
     int K, N;
+    int Kx;                            // k that rows of x hold in whole 16-byte chunks, zero from K on
     int wt;                            // w is [K, N] (the gradient of x)
     int tp;
     int64_t tiles;
@@ -186,130 +189,12 @@ __device__ __forceinline__ void turn_and_finish(const RowsArgs& a, const f32x16&
 }
 
 // ---- forward and dx, many rows ------------------------------------------------------------------------------------------------
-// Tile of BQ rows x BP channels, BK deep steps through two buffers of shared memory.  Rows of BK k lie there as 16-byte chunks of 8,
-// chunk c in slot c ^ f(row), f such that the 16 lanes a 16-byte read serves together (0-3, 12-15, 20-27; the others) touch all 64 banks.  w comes by DMA (laid out
-// for it: whole steps, zero behind K), x through registers, where float32 is split: rows of any alignment and length.
-template <int DT, int EPI, int BQ, int BP, int WQ, int WP, int BK>
-__global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_rows(const RowsArgs a) {
-    constexpr int NW = (BQ / WQ) * (BP / WP), NT = NW * 64, L = limbs_of(DT), ES = esize(DT);
-    constexpr int SL = BK / 8, RB = BK * 2;                    // chunks and bytes of a row
-    constexpr int XB = L * BQ * RB, WB = L * BP * RB, STAGE = XB + WB;
-    constexpr int NP = WP / 32, NQ = WQ / 32;
-    static_assert(2 * STAGE <= 160 * 1024 && NP % 2 == 0, "shared memory");
-    __shared__ __align__(16) char lds[2 * STAGE > NW * TURN ? 2 * STAGE : NW * TURN];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wp = wave % (BP / WP), wq = wave / (BP / WP);
-    auto swz = [](int row, int c) { return SL == 8 ? (c ^ ((row >> 1) & 7)) : SL == 4 ? (c ^ ((row >> 2) & 3)) : (c ^ ((row >> 3) & 1)); };
-
-    // workgroups of one XCD (blockIdx % 8) take a run of tiles, channels fastest: rows that several tiles read are in its L2
-    const int64_t per = (a.tiles + 7) / 8;
-    const int64_t t = (blockIdx.x % 8) * per + blockIdx.x / 8;
-    if (t >= a.tiles) return;
-    const int64_t q0 = t / a.tp * BQ;
-    const int p0 = (int)(t % a.tp) * BP;
-    const int steps = (a.K + BK - 1) / BK;
-
-    // DMA: a wavefront's instruction fills 1 KB, 64 / SL rows
-    constexpr int WI = WB / 1024;
-    auto dma_w = [&](int s, char* st) {
-#pragma unroll
-        for (int n = 0; n < (WI + NW - 1) / NW; ++n) {
-            const int i = wave + n * NW;
-            if (WI % NW != 0 && i >= WI) break;
-            const int r = i * (64 / SL) + lane / SL, limb = r / BP, row = r % BP;
-            const int p = p0 + row < a.N ? p0 + row : a.N - 1;         // channels behind the last: not stored
-            const int k = s * BK + swz(row, lane % SL) * 8;
-            const char* const src = a.wl + (limb * a.sl + p * a.sp + k / kb_of(DT) * a.sk + k % kb_of(DT)) * 2;
-            __builtin_amdgcn_global_load_lds(src, (lds_ptr)(st + XB + i * 1024), 16, 0, 0);
-        }
-    };
-    // registers: float32 four values a unit (8 units a row: 128 bytes side by side), 16-bit eight
-    constexpr int UPR = DT == BS_DT_F32 ? BK / 4 : SL, UNITS = BQ * UPR, XN = UNITS / NT;
-    u32x4 xr[XN];
-    auto load_x = [&](int s) {
-#pragma unroll
-        for (int n = 0; n < XN; ++n) {
-            const int u = tid + n * NT, row = u / UPR;
-            const int64_t q = q0 + row < a.rows ? q0 + row : a.rows - 1;
-            constexpr int V = vlen(DT);
-            const int k = s * BK + (u % UPR) * V, left = a.K - k;
-            const char* const src = a.x + (q * a.ldx + k) * ES;
-            xr[n] = left > 0 ? load_raw<DT>(src, left) : u32x4{0, 0, 0, 0};
-        }
-    };
-    auto store_x = [&](char* st) {
-#pragma unroll
-        for (int n = 0; n < XN; ++n) {
-            const int u = tid + n * NT, row = u / UPR, c = u % UPR;
-            if (DT == BS_DT_F32) {
-                uint32_t lo[3], hi[3];
-                limbs2(bits_f32(xr[n][0]), bits_f32(xr[n][1]), lo);
-                limbs2(bits_f32(xr[n][2]), bits_f32(xr[n][3]), hi);
-#pragma unroll
-                for (int l = 0; l < L; ++l)
-                    *reinterpret_cast<u32x2*>(st + (l * BQ + row) * RB + swz(row, c / 2) * 16 + (c & 1) * 8) = u32x2{lo[l % 3], hi[l % 3]};
-            } else {
-                *reinterpret_cast<u32x4*>(st + row * RB + swz(row, c) * 16) = xr[n];
-            }
-        }
-    };
-
-    f32x16 acc[NP][NQ];
-#pragma unroll
-    for (int i = 0; i < NP; ++i)
-#pragma unroll
-        for (int j = 0; j < NQ; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-
-    load_x(0);
-    dma_w(0, lds);
-    store_x(lds);
-    for (int s = 0; s < steps; ++s) {
-        char* const cur = lds + (s & 1) * STAGE;
-        char* const nxt = lds + ((s & 1) ^ 1) * STAGE;
-        __syncthreads();                        // this step has landed; the other buffer's readers are done
-        const bool more = s + 1 < steps;
-        if (more) {
-            load_x(s + 1);
-            dma_w(s + 1, nxt);
-        }
-#pragma unroll
-        for (int b = 0; b < BK / 16; ++b) {
-            u32x4 fp[NP][L], fq[NQ][L];
-            const int c = 2 * b + (lane >> 5);
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const int row = wp * WP + i * 32 + (lane & 31);
-#pragma unroll
-                for (int l = 0; l < L; ++l) fp[i][l] = *reinterpret_cast<const u32x4*>(cur + XB + (l * BP + row) * RB + swz(row, c) * 16);
-            }
-#pragma unroll
-            for (int j = 0; j < NQ; ++j) {
-                const int row = wq * WQ + j * 32 + (lane & 31);
-#pragma unroll
-                for (int l = 0; l < L; ++l) fq[j][l] = *reinterpret_cast<const u32x4*>(cur + (l * BQ + row) * RB + swz(row, c) * 16);
-            }
-            multiply<DT, L, L, NP, NQ>(fp, fq, acc);
-        }
-        if (more) store_x(nxt);
-    }
-    __syncthreads();
-    float* const mine = reinterpret_cast<float*>(lds + wave * TURN);
-#pragma unroll
-    for (int i = 0; i < NP; i += 2) {
-        const int p = p0 + wp * WP + i * 32;
-        float bias[vlen(DT)];
-        if (EPI == E_LAYER) load_bias<DT>(a, p + lane % (64 / vlen(DT)) * vlen(DT), bias);
-#pragma unroll
-        for (int j = 0; j < NQ; ++j) turn_and_finish<DT, EPI>(a, acc[i][j], acc[i + 1][j], mine, lane, q0 + wq * WQ + j * 32, p, bias);
-    }
-}
-
-// ---- ... whose rows are whole aligned 16-byte chunks --------------------------------------------------------------------------------
-// Both operands come by DMA through a ring of NS buffers with one barrier a step; fragments are read one 16-deep block ahead of
+// Tile of BQ rows x BP channels, BK deep steps.  Both operands come by DMA (rows of x that are no whole aligned 16-byte chunks are
+// copied to such first, k_pad) through a ring of NS buffers with one barrier a step; fragments are read one 16-deep block ahead of
 // the matrix instructions.  float32 rows lie in shared memory as they are and are split into limbs after the read, between the
-// matrix instructions of the block before: 32 bytes a fragment instead of 48, and nothing goes back to shared memory.
+// matrix instructions of the block before: 32 bytes a fragment instead of 48, and nothing goes back to shared memory.  Rows of BK k
+// lie there as 16-byte chunks, chunk c in slot c ^ f(row), f such that the 16 lanes a 16-byte read serves together (0-3, 12-15, 20-27;
+// the others) touch all 64 banks.
 __device__ __forceinline__ constexpr int wait_vm(int v) { return (v & 15) | (7 << 4) | ((v >> 4) << 14); }      // vmcnt(v), lgkmcnt(0)
 
 template <int DT, int EPI, int BQ, int BP, int WQ, int WP, int BK, int NS, int PER_SIMD>
@@ -330,7 +215,7 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64, PER_SIMD) void k_rows_d
     const int64_t q0 = t / a.tp * BQ;
     const int p0 = (int)(t % a.tp) * BP;
     const int steps = (a.K + BK - 1) / BK;
-    const char* const xb = a.x + q0 * a.ldx * ES;
+    const char* const xb = a.xd + q0 * a.ldxd * ES;
     const char* const wb = a.wl + p0 * a.sp * 2;
     constexpr int KB = kb_of(DT);
     static_assert(BK % KB == 0, "");
@@ -340,8 +225,8 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64, PER_SIMD) void k_rows_d
     for (int n = 0; n < XI; ++n) {
         const int row = (wave * XI + n) * (64 / XS) + lane / XS, c = swz(XS, row, lane % XS);
         const int64_t r = q0 + row < a.rows ? row : a.rows - 1 - q0;            // rows behind the last: not stored
-        xo[n] = (uint32_t)(r * a.ldx * ES + c * 16);
-        xk[n] = a.K - c * CK;
+        xo[n] = (uint32_t)(r * a.ldxd * ES + c * 16);
+        xk[n] = a.Kx - c * CK;
     }
 #pragma unroll
     for (int n = 0; n < WI; ++n) {
@@ -367,7 +252,7 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64, PER_SIMD) void k_rows_d
         }
     };
     auto issue = [&](int s, int slot) {
-        if ((s + 1) * BK <= a.K) return issue_whole(s, slot);
+        if ((s + 1) * BK <= a.Kx) return issue_whole(s, slot);
         char* const st = lds + slot * STAGE;
         const char* const xs = xb + (int64_t)s * BK * ES;
         const char* const ws = wb + (int64_t)s * (BK / KB) * a.sk * 2;
@@ -432,7 +317,7 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64, PER_SIMD) void k_rows_d
 #pragma unroll
     for (int s = 0; s < NS; ++s)
         if (s < steps) issue(s, s);
-    if (NS <= a.K / BK) __builtin_amdgcn_s_waitcnt(wait_vm((NS - 1) * (XI + WI)));      // NS whole steps are on their way
+    if (NS <= a.Kx / BK) __builtin_amdgcn_s_waitcnt(wait_vm((NS - 1) * (XI + WI)));      // NS whole steps are on their way
     else __builtin_amdgcn_s_waitcnt(wait_vm(0));
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -485,7 +370,7 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64, PER_SIMD) void k_rows_d
         }
         slot = next;
     };
-    const int whole = a.K / BK;                               // steps s with s + NS < whole have a whole step NS ahead
+    const int whole = a.Kx / BK;                               // steps s with s + NS < whole have a whole step NS ahead
     int s = 0;
 #pragma unroll SB == 1 ? 2 : 1
     for (; s + NS < whole; ++s) step(s, std::true_type{});
@@ -623,134 +508,45 @@ __global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {
 // zero from K to kp
 template <int DT, bool TURNED>
 __global__ __launch_bounds__(256) void k_lay_w(const char* __restrict__ w, int64_t ldw, int P, int K, int kp, char* __restrict__ out) {
-    constexpr int ES = esize(DT), L = limbs_of(DT);
+    constexpr int ES = esize(DT), L = limbs_of(DT), KB = kb_of(DT);
     __shared__ uint32_t tile[32][33];
-    const int p0 = blockIdx.y * 32, k0 = blockIdx.x * 64;
+    const int p0 = blockIdx.y * 32, k0 = blockIdx.x * 32;                // 32 p x 32 k
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    uint32_t v[4];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {                       // 32 p x 32 k at a time
-        const int kb = k0 + half * 32;
-        __syncthreads();
-        for (int r = ty; r < 32; r += 8) {
-            const int p = TURNED ? p0 + tx : p0 + r, k = TURNED ? kb + r : kb + tx;
-            uint32_t v = 0;
-            if (p < P && k < K) {
-                const char* const src = w + (TURNED ? (int64_t)k * ldw + p : (int64_t)p * ldw + k) * ES;
-                v = DT == BS_DT_F32 ? *reinterpret_cast<const uint32_t*>(src) : *reinterpret_cast<const uint16_t*>(src);
-            }
-            tile[TURNED ? tx : r][TURNED ? r : tx] = v;
-        }
-        __syncthreads();
-        // two k a thread: words of a row side by side
-        for (int u = threadIdx.x; u < 32 * 16; u += 256) {
-            const int r = u >> 4, k2 = (u & 15) * 2, p = p0 + r;
-            if (p >= P || kb + k2 >= kp) continue;
-            uint32_t l[3];
-            if (DT == BS_DT_F32) limbs2(bits_f32(tile[r][k2]), bits_f32(tile[r][k2 + 1]), l);
-            else l[0] = tile[r][k2] | (tile[r][k2 + 1] << 16);
+    for (int n = 0; n < 4; ++n) {                                        // (all loads at once: outside, any element, then zero)
+        const int r = ty + 8 * n, p = p0 + (TURNED ? tx : r), k = k0 + (TURNED ? r : tx);
+        const int pc = min(p, P - 1), kc = min(k, K - 1);
+        const char* const src = w + (TURNED ? (int64_t)kc * ldw + pc : (int64_t)pc * ldw + kc) * ES;
+        v[n] = DT == BS_DT_F32 ? *reinterpret_cast<const uint32_t*>(src) : *reinterpret_cast<const uint16_t*>(src);
+        if (k >= K) v[n] = 0;
+    }
 #pragma unroll
-            for (int b = 0; b < L; ++b) {
-                constexpr int KB = kb_of(DT);
-                *reinterpret_cast<uint32_t*>(out + ((((int64_t)(kb + k2) / KB * L + b) * P + p) * KB + (kb + k2) % KB) * 2) = l[b];
-            }
-        }
+    for (int n = 0; n < 4; ++n) tile[TURNED ? tx : ty + 8 * n][TURNED ? ty + 8 * n : tx] = v[n];
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {                                        // two k a thread: words of a row side by side
+        const int u = threadIdx.x + n * 256, r = u >> 4, k2 = (u & 15) * 2, p = p0 + r, k = k0 + k2;
+        if (p >= P) continue;
+        uint32_t l[3];
+        if (DT == BS_DT_F32) limbs2(bits_f32(tile[r][k2]), bits_f32(tile[r][k2 + 1]), l);
+        else l[0] = tile[r][k2] | (tile[r][k2 + 1] << 16);
+#pragma unroll
+        for (int b = 0; b < L; ++b) *reinterpret_cast<uint32_t*>(out + ((((int64_t)k / KB * L + b) * P + p) * KB + k % KB) * 2) = l[b];
     }
 }
 
 // ---- dw -------------------------------------------------------------------------------------------------------------------------
 struct OverArgs {
-    const char *x, *ds;
+    const char *x, *ds;                // as the caller holds them
+    const char *xd, *dd;               // as DMA takes them
     const int8_t* exps;
-    int64_t ldx, ldds, rows, part;
+    int64_t ldx, ldds, ldxd, lddd, rows, part;
     int K, N, nb, parts;
     int tp;
     int64_t tiles;                     // tiles x parts
     char* out;
 };
-enum { S_REG = 1, S_P8 = 2 };
-
-// One operand's tile of BK rows x 128 channels as it lies in memory; 16-byte chunk c of row r in slot c ^ 4 (r & 3), so that the
-// four rows a transposing read takes 64 bytes of (32 lanes together) lie in different banks.
-template <int DT, int SRC, int BK>
-struct Strip {
-    static constexpr int L = (DT == BS_DT_F32 && SRC != S_P8) ? 3 : 1;
-    static constexpr int BYTES = L * BK * 256;
-    static constexpr int ES = SRC == S_P8 ? 1 : esize(DT);
-    static constexpr int V = SRC == S_P8 ? 8 : vlen(DT);                         // channels of a unit
-    static constexpr int UPR = 128 / V, UNITS = BK * UPR, N = UNITS / 256;
-    u32x4 raw[N];
-    float step[SRC == S_P8 ? N : 1];
-
-    static __device__ __forceinline__ int at(int limb, int row, int c) { return (limb * BK + row) * 256 + ((c ^ (4 * (row & 3))) * 16); }
-
-    __device__ __forceinline__ void load(const OverArgs& a, const char* base, int64_t ld, int ni, int i0, int64_t k, int64_t ke, int tid) {
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int u = tid + n * 256, row = u / UPR, ch = i0 + (u % UPR) * V, left = ni - ch;
-            u32x4 v = {0, 0, 0, 0};
-            if (SRC == S_P8) step[n % (SRC == S_P8 ? N : 1)] = 0.0f;
-            if (k + row < ke && left > 0) {
-                const char* const src = base + ((k + row) * ld + ch) * ES;
-                if (SRC == S_P8) step[n % (SRC == S_P8 ? N : 1)] = p8_pow2(a.exps[(k + row) * a.nb + ch / P8_BLOCK]);
-                if (SRC == S_P8) {
-                    if (left >= V) {
-                        const u32x2 t = load8(src);
-                        v[0] = t[0]; v[1] = t[1];
-                    } else {
-                        uint32_t c[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) c[e] = *reinterpret_cast<const uint8_t*>(src + min(e, left - 1));
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e / 4] |= e < left ? c[e] << (8 * (e % 4)) : 0u;
-                    }
-                } else {
-                    v = load_raw<DT>(src, left);
-                }
-            }
-            raw[n] = v;
-        }
-    }
-    __device__ __forceinline__ void store(char* st, int tid) const {
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int u = tid + n * 256, row = u / UPR, g = u % UPR;
-            if (SRC == S_P8) {
-                const float s = step[n % (SRC == S_P8 ? N : 1)];
-                u32x4 v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t w = raw[n][e / 2] >> (16 * (e & 1));
-                    const float f0 = p8_value((int)(int8_t)w, s), f1 = p8_value((int)(int8_t)(w >> 8), s);
-                    v[e] = DT == BS_DT_F16 ? pk_f16(f0, f1) : pk_bf16(f0, f1);
-                }
-                *reinterpret_cast<u32x4*>(st + at(0, row, g)) = v;
-            } else if (DT == BS_DT_F32) {
-                uint32_t lo[3], hi[3];
-                limbs2(bits_f32(raw[n][0]), bits_f32(raw[n][1]), lo);
-                limbs2(bits_f32(raw[n][2]), bits_f32(raw[n][3]), hi);
-#pragma unroll
-                for (int l = 0; l < L; ++l) *reinterpret_cast<u32x2*>(st + at(l, row, g / 2) + (g & 1) * 8) = u32x2{lo[l % 3], hi[l % 3]};
-            } else {
-                *reinterpret_cast<u32x4*>(st + at(0, row, g)) = raw[n];
-            }
-        }
-    }
-    // the fragment of 32 channels from c0 on and 16 rows from r0 on: lane's channel c0 + lane % 32, rows r0 + 8 (lane / 32) + 0..7.
-    // A transposing read hands each 16 lanes 16 channels of 4 rows; lane i of them points at row i / 4, channels 4 (i % 4).
-    static __device__ __forceinline__ u32x4 fragment(const char* st, int limb, int r0, int c0, int lane) {
-        u32x4 v;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int row = r0 + 8 * (lane >> 5) + 4 * h + ((lane & 15) >> 2), ch = c0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-            const s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(st + at(limb, row, ch >> 3) + (ch & 4) * 2));
-            const u32x2 w = __builtin_bit_cast(u32x2, t);
-            v[2 * h] = w[0];
-            v[2 * h + 1] = w[1];
-        }
-        return v;
-    }
-};
-
 // sums over rows kb..ke that did not come out finite once more, in float32 arithmetic
 template <int DT, bool P8>
 __device__ __forceinline__ void again_over(const OverArgs& a, int64_t kb, int64_t ke, int p, int q, int n, f32x4& v) {
@@ -771,83 +567,6 @@ __device__ __forceinline__ void again_over(const OverArgs& a, int64_t kb, int64_
         }
 }
 
-template <int DT, int XS, int DS, int BK>
-__global__ __launch_bounds__(256) void k_over_rows(const OverArgs a) {
-    typedef Strip<DT, XS, BK> TX;
-    typedef Strip<DT, DS, BK> TD;
-    constexpr int STAGE = TX::BYTES + TD::BYTES;
-    __shared__ __align__(16) char lds[2 * STAGE];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wp = wave & 1, wq = wave >> 1;
-    const int64_t per = (a.tiles + 7) / 8;
-    const int64_t t = (blockIdx.x % 8) * per + blockIdx.x / 8;        // an XCD takes whole runs of tiles of the same rows
-    if (t >= a.tiles) return;
-    const int64_t tiles = a.tiles / a.parts;
-    const int part = (int)(t / tiles), tile = (int)(t % tiles);
-    const int p0 = tile % a.tp * 128, q0 = tile / a.tp * 128;
-    const int64_t kb = part * a.part, ke = kb + a.part < a.rows ? kb + a.part : a.rows;
-    TX tx;
-    TD td;
-    f32x16 acc[2][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-    auto begin = [&](int64_t k) {
-        tx.load(a, a.x, a.ldx, a.K, p0, k, ke, tid);
-        td.load(a, a.ds, a.ldds, a.N, q0, k, ke, tid);
-    };
-    auto end = [&](char* st) {
-        tx.store(st, tid);
-        td.store(st + TX::BYTES, tid);
-    };
-    begin(kb);
-    end(lds);
-    int buf = 0;
-    for (int64_t k = kb; k < ke; k += BK) {
-        char* const cur = lds + buf * STAGE;
-        char* const nxt = lds + (buf ^ 1) * STAGE;
-        __syncthreads();
-        const bool more = k + BK < ke;
-        if (more) begin(k + BK);
-#pragma unroll
-        for (int b = 0; b < BK / 16; ++b) {
-            u32x4 fp[2][TX::L], fq[2][TD::L];
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int l = 0; l < TX::L; ++l) fp[i][l] = TX::fragment(cur, l, b * 16, wp * 64 + i * 32, lane);
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int l = 0; l < TD::L; ++l) fq[j][l] = TD::fragment(cur + TX::BYTES, l, b * 16, wq * 64 + j * 32, lane);
-            multiply<DT, TX::L, TD::L, 2, 2>(fp, fq, acc);
-        }
-        if (more) end(nxt);
-        buf ^= 1;
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int q = q0 + wq * 64 + j * 32 + (lane & 31);
-        if (q >= a.N) continue;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int p = p0 + wp * 64 + i * 32 + 8 * g + 4 * (lane >> 5), n = a.K - p;
-                if (n <= 0) continue;
-                f32x4 v = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-                if (DT == BS_DT_F32) again_over<DT, XS == S_P8>(a, kb, ke, p, q, n, v);
-                float* const o = reinterpret_cast<float*>(a.out) + ((int64_t)part * a.N + q) * a.K + p;
-                if (n >= 4) store16((char*)o, __builtin_bit_cast(u32x4, v));
-                else
-                    for (int e = 0; e < n; ++e) o[e] = v[e];
-            }
-    }
-}
-
-// ---- ... whose rows are whole aligned 16-byte chunks ---------------------------------------------------------------------------------
 // x and ds by DMA through a ring, as in k_rows_dma, every tile as it lies in memory: [BK rows][channels].  The transposition that the
 // matrix instruction wants (8 rows of one channel side by side) happens in the read from shared memory: transposing reads for 16-bit
 // values (4 rows) and for codes (8 rows, turned into bfloat16 / float16 in registers: exact), dword reads along the channels and a
@@ -876,8 +595,8 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
     const int p0 = tile % a.tp * BP, q0 = tile / a.tp * BQ;
     const int64_t kb = part * a.part, ke = kb + a.part < a.rows ? kb + a.part : a.rows;
     const int nk = (int)(ke - kb), count = (nk + BK - 1) / BK;
-    const char* const xb = a.x + (kb * a.ldx + p0) * XE;
-    const char* const db = a.ds + (kb * a.ldds + q0) * ES;
+    const char* const xb = a.xd + (kb * a.ldxd + p0) * XE;
+    const char* const db = a.dd + (kb * a.lddd + q0) * ES;
     uint32_t xo[XI], dof[DI];
     int xr[XI], dr[DI];
 #pragma unroll
@@ -885,14 +604,14 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
         constexpr int CH = XR / 16;
         const int u = (wave * XI + n) * 64 + lane, row = u / CH, c = (u % CH) ^ sx(row);
         xr[n] = row;
-        xo[n] = (uint32_t)((int64_t)row * a.ldx * XE + (p0 + c * (16 / XE) < a.K ? c * 16 : 0));        // channels behind the last: not stored
+        xo[n] = (uint32_t)((int64_t)row * a.ldxd * XE + (p0 + c * (16 / XE) < a.K ? c * 16 : 0));        // channels behind the last: not stored
     }
 #pragma unroll
     for (int n = 0; n < DI; ++n) {
         constexpr int CH = DR / 16;
         const int u = (wave * DI + n) * 64 + lane, row = u / CH, c = (u % CH) ^ sd(row);
         dr[n] = row;
-        dof[n] = (uint32_t)((int64_t)row * a.ldds * ES + (q0 + c * (16 / ES) < a.N ? c * 16 : 0));
+        dof[n] = (uint32_t)((int64_t)row * a.lddd * ES + (q0 + c * (16 / ES) < a.N ? c * 16 : 0));
     }
     const float* sp = nullptr;
     if constexpr (P8) {
@@ -901,8 +620,8 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
     }
     auto issue_whole = [&](int s, int slot) {                             // all its rows exist: no branch among the loads
         char* const st = lds + slot * STAGE;
-        const char* const xs = xb + (int64_t)s * BK * a.ldx * XE;
-        const char* const ds = db + (int64_t)s * BK * a.ldds * ES;
+        const char* const xs = xb + (int64_t)s * BK * a.ldxd * XE;
+        const char* const ds = db + (int64_t)s * BK * a.lddd * ES;
 #pragma unroll
         for (int n = 0; n < XI; ++n) {
             const char* const src = xs + xo[n];
@@ -921,8 +640,8 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
     auto issue = [&](int s, int slot) {
         if ((s + 1) * BK <= nk) return issue_whole(s, slot);
         char* const st = lds + slot * STAGE;
-        const char* const xs = xb + (int64_t)s * BK * a.ldx * XE;
-        const char* const ds = db + (int64_t)s * BK * a.ldds * ES;
+        const char* const xs = xb + (int64_t)s * BK * a.ldxd * XE;
+        const char* const ds = db + (int64_t)s * BK * a.lddd * ES;
         const int left = nk - s * BK;
 #pragma unroll
         for (int n = 0; n < XI; ++n) {
@@ -1140,6 +859,42 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
         }
 }
 
+// rows of K elements of ES bytes (1, 2, 4) -> rows of whole 16-byte chunks, zero behind K.  2^lanes_log2 threads a row (a power of two:
+// no division); the last chunk of a row comes as its last 16 bytes, moved down.
+template <int ES>
+__global__ __launch_bounds__(256) void k_pad(const char* __restrict__ in, int64_t ld, int64_t rows, int K, char* __restrict__ out, int chunks, int lanes_log2) {
+    constexpr int V = 16 / ES;
+    const int64_t row = (int64_t)blockIdx.x * (256 >> lanes_log2) + (threadIdx.x >> lanes_log2);
+    if (row >= rows) return;
+    for (int c = threadIdx.x & ((1 << lanes_log2) - 1); c < chunks; c += 1 << lanes_log2) {
+        const int left = K - c * V;
+        const char* const src = in + (row * ld + (int64_t)c * V) * ES;
+        u32x4 v;
+        if (left >= V) {
+            v = load16(src);
+        } else if (c > 0) {
+            const int down = (V - left) * ES;                            // bytes of the chunk before
+            const u32x4 t = load16(src - down);
+            const uint64_t lo = t[0] | (uint64_t)t[1] << 32, hi = t[2] | (uint64_t)t[3] << 32;
+            const int bits = down * 8;                                   // 8 .. 120
+            const uint64_t l = bits < 64 ? (lo >> bits) | (hi << (64 - bits)) : bits == 64 ? hi : hi >> (bits - 64);
+            const uint64_t h = bits < 64 ? hi >> bits : 0;
+            v = u32x4{(uint32_t)l, (uint32_t)(l >> 32), (uint32_t)h, (uint32_t)(h >> 32)};
+        } else {
+            uint8_t u[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) u[e] = *reinterpret_cast<const uint8_t*>(src + min(e, left * ES - 1));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = 0;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) v[e] |= 4 * e + b < left * ES ? (uint32_t)u[4 * e + b] << (8 * b) : 0u;
+            }
+        }
+        *reinterpret_cast<u32x4*>(out + (row * chunks + c) * 16) = v;
+    }
+}
+
 // exponents [rows, nb] -> 2^e as floats [nb][ld], zero from rows to ld
 __global__ __launch_bounds__(256) void k_lay_steps(const int8_t* __restrict__ exps, int64_t rows, int nb, float* __restrict__ out, int64_t ld) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -1178,25 +933,48 @@ constexpr int RELAY_TILES = 256, MID_TILES = 256, BIG_TILES = 384;
 int64_t tiles_of(int64_t rows, int N, int bq, int bp) { return (rows + bq - 1) / bq * ((N + bp - 1) / bp); }
 bool few(int64_t rows, int N) { return tiles_of(rows, N, 32, 32) <= RELAY_TILES; }
 
-int64_t lay_bytes(int dtype, int K, int P) { return (int64_t)limbs_of(dtype) * P * ((K + 63) / 64 * 64) * 2; }
+int64_t lay_bytes(int dtype, int K, int P) { return ((int64_t)limbs_of(dtype) * P * ((K + 63) / 64 * 64) * 2 + 255) / 256 * 256; }
+int64_t pad_bytes(int es, int64_t rows, int K) { return (rows * (((int64_t)K * es + 15) / 16) * 16 + 255) / 256 * 256; }
 
-// out [rows, N] over K: w [N, K], or [K, N] when turned
+// rows that DMA can take: aligned chunks, whole or ended with zeros (zeros), tiles within 31 bits of their first byte
+bool whole_rows(const void* p, int64_t ld, int K, int es, int zeros) {
+    return ((uintptr_t)p & 15) == 0 && ld * es % 16 == 0 && ((int64_t)K * es % 16 == 0 || (zeros && ld * es >= ((int64_t)K * es + 15) / 16 * 16)) &&
+           ld * es < (1 << 22);
+}
+int pad(int es, const void* in, int64_t ld, int64_t rows, int K, char* out, hipStream_t st) {
+    const int chunks = (int)(((int64_t)K * es + 15) / 16);
+    int log2 = 0;
+    while ((1 << log2) < chunks && log2 < 8) ++log2;
+    const int64_t blocks = (rows + (256 >> log2) - 1) / (256 >> log2);
+    if (blocks > 0x7fffffff) return BS_EINVAL;
+    const dim3 grid((unsigned)blocks);
+    if (es == 4) hipLaunchKernelGGL(k_pad<4>, grid, dim3(256), 0, st, (const char*)in, ld, rows, K, out, chunks, log2);
+    else if (es == 2) hipLaunchKernelGGL(k_pad<2>, grid, dim3(256), 0, st, (const char*)in, ld, rows, K, out, chunks, log2);
+    else hipLaunchKernelGGL(k_pad<1>, grid, dim3(256), 0, st, (const char*)in, ld, rows, K, out, chunks, log2);
+    return BS_OK;
+}
+
+// out [rows, N] over K: w [N, K], or [K, N] when turned; zeros: rows of x end in zeros up to whole chunks
+int64_t rows_bytes(int dtype, int64_t rows, int K, int N, bool turned, bool whole) {
+    const bool small = few(rows, N);
+    return (turned || !small ? lay_bytes(dtype, K, N) : 0) + (small || whole ? 0 : pad_bytes(esize(dtype), rows, K));
+}
 template <int DT, int EPI>
-int launch_rows(RowsArgs a, void* workspace, int64_t bytes, hipStream_t st) {
+int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream_t st) {
+    constexpr int ES = esize(DT), CK = 16 / ES;
     const int kp = (a.K + 63) / 64 * 64;
-    constexpr int CK = 16 / esize(DT);
-    const bool chunks = a.K % CK == 0 && a.ldx % CK == 0 && ((uintptr_t)a.x & 15) == 0 && a.ldx * esize(DT) < (1 << 22);
-    // (rows that DMA cannot take: the relay is ahead of k_rows up to four times as many tiles of few k)
-    const bool small = few(a.rows, a.N) || (!chunks && a.K <= 256 && tiles_of(a.rows, a.N, 32, 32) <= 4 * RELAY_TILES);
-    const bool as_is = DT != BS_DT_F32 && !a.wt && a.K % 64 == 0 && a.ldw % 8 == 0 && ((uintptr_t)a.w & 15) == 0;
+    const bool small = few(a.rows, a.N), whole = whole_rows(a.x, a.ldx, a.K, ES, zeros);
     const bool big = DT != BS_DT_F32 && tiles_of(a.rows, a.N, 256, 256) >= BIG_TILES;
+    const bool as_is = DT != BS_DT_F32 && !a.wt && a.K % 64 == 0 && a.ldw % 8 == 0 && ((uintptr_t)a.w & 15) == 0 && a.ldw < (1 << 21);
+    const int64_t need = rows_bytes(DT, a.rows, a.K, a.N, a.wt, whole);
+    if (need > 0 && (!workspace || bytes < need)) return BS_EINVAL;
     const bool lay = a.wt || (!small && (big || !as_is));
     if (lay) {
-        if (!workspace || bytes < lay_bytes(DT, a.K, a.N)) return BS_EINVAL;
-        const dim3 grid((unsigned)(kp / 64), (unsigned)((a.N + 31) / 32));
+        const dim3 grid((unsigned)(kp / 32), (unsigned)((a.N + 31) / 32));
+        constexpr int KB = kb_of(DT);
+        if (a.N > (1 << 21)) return BS_EINVAL;                       // (grid, and 31-bit offsets into w)
         if (a.wt) hipLaunchKernelGGL((k_lay_w<DT, true>), grid, dim3(256), 0, st, a.w, a.ldw, a.N, a.K, kp, (char*)workspace);
         else hipLaunchKernelGGL((k_lay_w<DT, false>), grid, dim3(256), 0, st, a.w, a.ldw, a.N, a.K, kp, (char*)workspace);
-        constexpr int KB = kb_of(DT);
         a.wl = (const char*)workspace; a.sp = KB; a.sl = (int64_t)a.N * KB; a.sk = a.sl * limbs_of(DT);
     } else {
         a.wl = a.w; a.sp = a.ldw; a.sl = 0; a.sk = kb_of(DT);
@@ -1209,25 +987,25 @@ int launch_rows(RowsArgs a, void* workspace, int64_t bytes, hipStream_t st) {
         else hipLaunchKernelGGL((k_relay<DT, EPI, false>), dim3(blocks), dim3(256), 0, st, a);
         return rows_rc();
     }
-    // rows of whole aligned chunks, tiles within 31 bits of their first byte: both operands by DMA
-    const bool dma = chunks && (a.sl * limbs_of(DT) + a.sp * 256 + a.sk * 2) * 2 < 0x7fffffff;
-#define ROWS(KERNEL, BQ, BP, NT) do { a.tp = (a.N + BP - 1) / BP; a.tiles = tiles_of(a.rows, a.N, BQ, BP); \
-        const int64_t blocks = (a.tiles + 7) / 8 * 8; if (blocks > 0x7fffffff) return BS_EINVAL; \
-        hipLaunchKernelGGL((KERNEL), dim3((unsigned)blocks), dim3(NT), 0, st, a); } while (0)
-#define K_(...) __VA_ARGS__
-    if constexpr (DT == BS_DT_F32) {
-        if (dma && tiles_of(a.rows, a.N, 64, 128) >= MID_TILES && a.N > 64) ROWS(K_(k_rows_dma<DT, EPI, 64, 128, 32, 64, 16, 3, 3>), 64, 128, 256);
-        else if (dma) ROWS(K_(k_rows_dma<DT, EPI, 64, 64, 32, 64, 16, 6, 1>), 64, 64, 128);
-        else if (tiles_of(a.rows, a.N, 128, 128) >= MID_TILES && a.N > 64) ROWS(K_(k_rows<DT, EPI, 128, 128, 64, 64, 16>), 128, 128, 256);
-        else ROWS(K_(k_rows<DT, EPI, 64, 64, 32, 64, 16>), 64, 64, 128);
-    } else {
-        if (dma && big) ROWS(K_(k_rows_dma<DT, EPI, 256, 256, 128, 64, 32, 4, 1>), 256, 256, 512);
-        else if (dma && tiles_of(a.rows, a.N, 128, 128) >= MID_TILES && a.N > 64) ROWS(K_(k_rows_dma<DT, EPI, 128, 128, 64, 64, 32, 4, 1>), 128, 128, 256);
-        else if (dma) ROWS(K_(k_rows_dma<DT, EPI, 64, 64, 32, 64, 32, 4, 1>), 64, 64, 128);
-        else if (tiles_of(a.rows, a.N, 128, 128) >= MID_TILES && a.N > 64) ROWS(K_(k_rows<DT, EPI, 128, 128, 64, 64, 64>), 128, 128, 256);
-        else ROWS(K_(k_rows<DT, EPI, 64, 64, 32, 64, 64>), 64, 64, 128);
+    a.Kx = (a.K + CK - 1) / CK * CK;
+    a.xd = a.x; a.ldxd = a.ldx;
+    if (!whole) {
+        char* const to = (char*)workspace + lay_bytes(DT, a.K, a.N);
+        if (pad(ES, a.x, a.ldx, a.rows, a.K, to, st) != BS_OK) return BS_EINVAL;
+        a.xd = to; a.ldxd = a.Kx;
     }
-#undef K_
+#define ROWS(BQ, BP, WQ, WP, BK, NS, PS) do { a.tp = (a.N + BP - 1) / BP; a.tiles = tiles_of(a.rows, a.N, BQ, BP); \
+        const int64_t blocks = (a.tiles + 7) / 8 * 8; if (blocks > 0x7fffffff) return BS_EINVAL; \
+        hipLaunchKernelGGL((k_rows_dma<DT, EPI, BQ, BP, WQ, WP, BK, NS, PS>), dim3((unsigned)blocks), dim3((BQ / WQ) * (BP / WP) * 64), 0, st, a); } while (0)
+    if constexpr (DT == BS_DT_F32) {
+        if (tiles_of(a.rows, a.N, 64, 128) >= MID_TILES && a.N > 64) ROWS(64, 128, 32, 64, 16, 3, 3);
+        else ROWS(64, 64, 32, 64, 16, 4, 1);
+    } else {
+        if (big) ROWS(256, 256, 128, 64, 32, 4, 1);
+        else if (tiles_of(a.rows, a.N, 128, 128) >= MID_TILES && a.N > 64) ROWS(128, 128, 64, 64, 32, 4, 1);
+        else if (tiles_of(a.rows, a.N, 128, 64) >= 2 * MID_TILES && a.N <= 64) ROWS(128, 64, 32, 64, 32, 4, 1);
+        else ROWS(64, 64, 32, 64, 32, 4, 1);
+    }
 #undef ROWS
     return rows_rc();
 }
@@ -1248,43 +1026,32 @@ void split_rows(int dtype, int64_t rows, int K, int N, int64_t* part, int64_t* p
     *parts = rows ? (rows + *part - 1) / *part : 1;
 }
 int64_t steps_bytes(int64_t rows, int K) { return (int64_t)((K + 31) / 32) * ((rows + 63) / 64 * 64) * 4; }
+struct OverBytes {
+    int64_t steps, x, ds, parts;
+    int64_t all() const { return steps + x + ds + parts; }
+};
+OverBytes over_bytes(int dtype, int64_t rows, int K, int N, bool codes, bool x_whole, bool ds_whole) {
+    int64_t part, parts;
+    split_rows(dtype, rows, K, N, &part, &parts);
+    return {codes ? steps_bytes(rows, K) : 0, x_whole ? 0 : pad_bytes(codes ? 1 : esize(dtype), rows, K), ds_whole ? 0 : pad_bytes(esize(dtype), rows, N),
+            parts > 1 || dtype != BS_DT_F32 ? parts * K * N * 4 : 0};
+}
 
 template <int DT>
-int launch_over(OverArgs a, char* steps, hipStream_t st) {
-    constexpr int BK = DT == BS_DT_F32 ? 16 : 32, CK = 16 / esize(DT);
-    auto go = [&](int bq) {
-        a.tp = (a.K + 127) / 128;
-        a.tiles = (int64_t)a.tp * ((a.N + bq - 1) / bq) * a.parts;
-        return (a.tiles + 7) / 8 * 8;
-    };
-    auto whole = [](const void* p, int64_t ld, int n, int ck, int es) {
-        return n % ck == 0 && ld % ck == 0 && ((uintptr_t)p & 15) == 0 && ld * es < (1 << 22);
-    };
-    const bool dd = whole(a.ds, a.ldds, a.N, CK, esize(DT));
-    const bool xd = a.exps ? whole(a.x, a.ldx, a.K, 16, 1) : whole(a.x, a.ldx, a.K, CK, esize(DT));
-    const int64_t ld = (a.rows + 63) / 64 * 64;
-#define OVER(P8, BQ, WQ, BK_, NS) do { const int64_t blocks = go(BQ); if (blocks > 0x7fffffff) return BS_EINVAL; \
-        hipLaunchKernelGGL((k_over_dma<DT, P8, BQ, 128, WQ, 64, BK_, NS>), dim3((unsigned)blocks), dim3(256), 0, st, a, (const float*)steps, ld); } while (0)
-    if (xd && dd && a.rows < (1 << 30)) {
-        if (a.exps) {
-            const int nb = (a.K + 31) / 32;
-            hipLaunchKernelGGL(k_lay_steps, dim3((unsigned)((ld + 255) / 256)), dim3(256), 0, st, a.exps, a.rows, nb, (float*)steps, ld);
-            if constexpr (DT == BS_DT_F32) OVER(true, 128, 64, 32, 3);
-            else if (over_bq(DT, a.rows, a.K, a.N) == 256) OVER(true, 256, 128, 32, 3);
-            else OVER(true, 128, 64, 32, 4);
-        } else {
-            if constexpr (DT == BS_DT_F32) OVER(false, 128, 64, 16, 4);
-            else if (over_bq(DT, a.rows, a.K, a.N) == 256) OVER(false, 256, 128, 32, 3);
-            else OVER(false, 128, 64, 32, 4);
-        }
-        return rows_rc();
+int launch_over(OverArgs a, const float* steps, int64_t ld, hipStream_t st) {
+#define OVER(P8, BQ, WQ, BK_, NS) do { a.tp = (a.K + 127) / 128; a.tiles = tiles_of(a.N, a.K, BQ, 128) * a.parts; \
+        const int64_t blocks = (a.tiles + 7) / 8 * 8; if (blocks > 0x7fffffff) return BS_EINVAL; \
+        hipLaunchKernelGGL((k_over_dma<DT, P8, BQ, 128, WQ, 64, BK_, NS>), dim3((unsigned)blocks), dim3(256), 0, st, a, steps, ld); } while (0)
+    if (a.exps) {
+        if constexpr (DT == BS_DT_F32) OVER(true, 128, 64, 32, 3);
+        else if (over_bq(DT, a.rows, a.K, a.N) == 256) OVER(true, 256, 128, 32, 3);
+        else OVER(true, 128, 64, 32, 4);
+    } else {
+        if constexpr (DT == BS_DT_F32) OVER(false, 128, 64, 16, 4);
+        else if (over_bq(DT, a.rows, a.K, a.N) == 256) OVER(false, 256, 128, 32, 3);
+        else OVER(false, 128, 64, 32, 4);
     }
 #undef OVER
-    const int64_t blocks = go(128);
-    if (blocks > 0x7fffffff) return BS_EINVAL;
-    const dim3 grid((unsigned)blocks);
-    if (a.exps) hipLaunchKernelGGL((k_over_rows<DT, S_P8, S_REG, BK>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_over_rows<DT, S_REG, S_REG, BK>), grid, dim3(256), 0, st, a);
     return rows_rc();
 }
 
@@ -1292,9 +1059,9 @@ int launch_over(OverArgs a, char* steps, hipStream_t st) {
 
 extern "C" {
 
-int64_t bs_linear_workspace(int dtype, int64_t rows, int K, int N) {
+int64_t bs_linear_workspace(int dtype, int64_t rows, int K, int N, int whole) {
     if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1) return BS_EINVAL;
-    return few(rows, N) ? 0 : lay_bytes(dtype, K, N);
+    return rows_bytes(dtype, rows, K, N, false, whole != 0);
 }
 
 int bs_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype, const void* res,
@@ -1310,17 +1077,17 @@ int bs_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const 
     a.res = (const char*)res; a.ldr = ldr;
     a.sum = (char*)sum_out; a.act_out = (char*)act_out; a.act = act;
     hipStream_t st = rows_stream(stream);
-    if (dtype == BS_DT_F32) return launch_rows<BS_DT_F32, E_LAYER>(a, workspace, workspace_bytes, st);
-    if (dtype == BS_DT_BF16) return launch_rows<BS_DT_BF16, E_LAYER>(a, workspace, workspace_bytes, st);
-    return launch_rows<BS_DT_F16, E_LAYER>(a, workspace, workspace_bytes, st);
+    if (dtype == BS_DT_F32) return launch_rows<BS_DT_F32, E_LAYER>(a, 0, workspace, workspace_bytes, st);
+    if (dtype == BS_DT_BF16) return launch_rows<BS_DT_BF16, E_LAYER>(a, 0, workspace, workspace_bytes, st);
+    return launch_rows<BS_DT_F16, E_LAYER>(a, 0, workspace, workspace_bytes, st);
 }
 
-int64_t bs_linear_grad_x_workspace(int dtype, int64_t rows, int K, int N) {
+int64_t bs_linear_grad_x_workspace(int dtype, int64_t rows, int K, int N, int whole) {
     if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1) return BS_EINVAL;
-    return lay_bytes(dtype, N, K);
+    return rows_bytes(dtype, rows, N, K, true, whole != 0);
 }
 
-int bs_linear_grad_x(const void* ds, int64_t ldds, const void* w, int64_t ldw, void* dx, int dtype, int64_t rows, int K, int N,
+int bs_linear_grad_x(const void* ds, int64_t ldds, int zeros, const void* w, int64_t ldw, void* dx, int dtype, int64_t rows, int K, int N,
                      void* workspace, int64_t workspace_bytes, void* stream) {
     if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1) return BS_EINVAL;
     if (rows == 0) return BS_OK;
@@ -1329,47 +1096,57 @@ int bs_linear_grad_x(const void* ds, int64_t ldds, const void* w, int64_t ldw, v
     a.x = (const char*)ds; a.ldx = ldds; a.w = (const char*)w; a.ldw = ldw; a.rows = rows; a.K = N; a.N = K; a.wt = 1;
     a.sum = (char*)dx;
     hipStream_t st = rows_stream(stream);
-    if (dtype == BS_DT_F32) return launch_rows<BS_DT_F32, E_PLAIN>(a, workspace, workspace_bytes, st);
-    if (dtype == BS_DT_BF16) return launch_rows<BS_DT_BF16, E_PLAIN>(a, workspace, workspace_bytes, st);
-    return launch_rows<BS_DT_F16, E_PLAIN>(a, workspace, workspace_bytes, st);
+    if (dtype == BS_DT_F32) return launch_rows<BS_DT_F32, E_PLAIN>(a, zeros, workspace, workspace_bytes, st);
+    if (dtype == BS_DT_BF16) return launch_rows<BS_DT_BF16, E_PLAIN>(a, zeros, workspace, workspace_bytes, st);
+    return launch_rows<BS_DT_F16, E_PLAIN>(a, zeros, workspace, workspace_bytes, st);
 }
 
-int64_t bs_linear_grad_w_workspace(int dtype, int64_t rows, int K, int N, int codes) {
+int64_t bs_linear_grad_w_workspace(int dtype, int64_t rows, int K, int N, int codes, int x_whole, int ds_whole) {
     if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1) return BS_EINVAL;
-    int64_t part, parts;
-    split_rows(dtype, rows, K, N, &part, &parts);
-    return (codes ? steps_bytes(rows, K) : 0) + (parts > 1 || dtype != BS_DT_F32 ? parts * K * N * 4 : 0);
+    return over_bytes(dtype, rows, K, N, codes != 0, x_whole != 0, ds_whole != 0).all();
 }
 
-int bs_linear_grad_w(const void* ds, int64_t ldds, const void* x, const int8_t* x_exps, int64_t ldx, void* dw, int dtype,
+int bs_linear_grad_w(const void* ds, int64_t ldds, int zeros, const void* x, const int8_t* x_exps, int64_t ldx, void* dw, int dtype,
                      int64_t rows, int K, int N, void* workspace, int64_t workspace_bytes, void* stream) {
-    if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1 || !dw) return BS_EINVAL;
+    if (bad_type(dtype) || rows < 0 || rows > (1 << 30) || K < 1 || N < 1 || !dw) return BS_EINVAL;
     if (rows > 0 && (!ds || !x || ldds < N || ldx < K)) return BS_EINVAL;
     hipStream_t st = rows_stream(stream);
     const int64_t n = (int64_t)K * N;
+    const int es = esize(dtype), xe = x_exps ? 1 : es;
+    const bool x_whole = whole_rows(x, ldx, K, xe, 0), ds_whole = whole_rows(ds, ldds, N, es, zeros);
+    const OverBytes b = over_bytes(dtype, rows, K, N, x_exps != nullptr, x_whole, ds_whole);
     int64_t part, parts;
     split_rows(dtype, rows, K, N, &part, &parts);
-    const bool joined = parts > 1 || dtype != BS_DT_F32;
-    const int64_t before = x_exps ? steps_bytes(rows, K) : 0;           // workspace: steps of the codes, then the parts
-    const int64_t need = before + (joined ? parts * n * 4 : 0);
-    if (need > 0 && rows > 0 && (!workspace || workspace_bytes < need)) return BS_EINVAL;
-    int rc = BS_OK;
+    if (rows > 0 && b.all() > 0 && (!workspace || workspace_bytes < b.all())) return BS_EINVAL;
+    char* const ws = (char*)workspace;                       // steps of the codes | copy of x | copy of ds | parts
+    const bool joined = b.parts > 0;
     if (rows > 0) {
         OverArgs a = {};
         a.x = (const char*)x; a.exps = x_exps; a.ldx = ldx; a.ds = (const char*)ds; a.ldds = ldds; a.rows = rows; a.part = part;
         a.K = K; a.N = N; a.nb = (K + P8_BLOCK - 1) / P8_BLOCK; a.parts = (int)parts;
-        char* const ws = (char*)workspace;
-        a.out = joined ? ws + before : (char*)dw;
-        rc = dtype == BS_DT_F32 ? launch_over<BS_DT_F32>(a, ws, st) : dtype == BS_DT_BF16 ? launch_over<BS_DT_BF16>(a, ws, st) : launch_over<BS_DT_F16>(a, ws, st);
+        a.xd = a.x; a.ldxd = ldx; a.dd = a.ds; a.lddd = ldds;
+        a.out = joined ? ws + b.steps + b.x + b.ds : (char*)dw;
+        const int64_t ld = (rows + 63) / 64 * 64;
+        if (x_exps) hipLaunchKernelGGL(k_lay_steps, dim3((unsigned)((ld + 255) / 256)), dim3(256), 0, st, x_exps, rows, a.nb, (float*)ws, ld);
+        if (!x_whole) {
+            if (pad(xe, x, ldx, rows, K, ws + b.steps, st) != BS_OK) return BS_EINVAL;
+            a.xd = ws + b.steps; a.ldxd = (K + 16 / xe - 1) / (16 / xe) * (16 / xe);
+        }
+        if (!ds_whole) {
+            if (pad(es, ds, ldds, rows, N, ws + b.steps + b.x, st) != BS_OK) return BS_EINVAL;
+            a.dd = ws + b.steps + b.x; a.lddd = (N + 16 / es - 1) / (16 / es) * (16 / es);
+        }
+        const int rc = dtype == BS_DT_F32 ? launch_over<BS_DT_F32>(a, (float*)ws, ld, st) : dtype == BS_DT_BF16 ? launch_over<BS_DT_BF16>(a, (float*)ws, ld, st)
+                                                                                              : launch_over<BS_DT_F16>(a, (float*)ws, ld, st);
         if (rc != BS_OK || !joined) return rc;
     } else {
         parts = 0;                                            // the sum of no parts
     }
-    const float* ws = (const float*)((const char*)workspace + before);
+    const float* const from = (const float*)(ws + b.steps + b.x + b.ds);
     const dim3 blocks((unsigned)((n + 63) / 64));
-    if (dtype == BS_DT_F32) hipLaunchKernelGGL(k_add_parts<BS_DT_F32>, blocks, dim3(256), 0, st, ws, (int)parts, n, (char*)dw);
-    else if (dtype == BS_DT_BF16) hipLaunchKernelGGL(k_add_parts<BS_DT_BF16>, blocks, dim3(256), 0, st, ws, (int)parts, n, (char*)dw);
-    else hipLaunchKernelGGL(k_add_parts<BS_DT_F16>, blocks, dim3(256), 0, st, ws, (int)parts, n, (char*)dw);
+    if (dtype == BS_DT_F32) hipLaunchKernelGGL(k_add_parts<BS_DT_F32>, blocks, dim3(256), 0, st, from, (int)parts, n, (char*)dw);
+    else if (dtype == BS_DT_BF16) hipLaunchKernelGGL(k_add_parts<BS_DT_BF16>, blocks, dim3(256), 0, st, from, (int)parts, n, (char*)dw);
+    else hipLaunchKernelGGL(k_add_parts<BS_DT_F16>, blocks, dim3(256), 0, st, from, (int)parts, n, (char*)dw);
     return rows_rc();
 }
 

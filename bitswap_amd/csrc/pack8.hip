@@ -68,6 +68,7 @@ struct ActGradArgs {
     int64_t ldgs, ldga, lds, rows, part;
     int N, nb, act;
     char* ds;
+    int64_t ldds;
     float* parts;             // [parts][N]
 };
 
@@ -105,7 +106,7 @@ __global__ __launch_bounds__(256) void k_act_grad(const ActGradArgs a, int cl_lo
 #pragma unroll
                 for (int i = 0; i < V; ++i) d[i] += g[i];
             }
-            if (a.ds) store_vec<DT>(a.ds + (r * a.N + c) * ES, left, d);
+            if (a.ds) store_vec<DT>(a.ds + (r * a.ldds + c) * ES, c + V <= a.ldds ? V : left, d);      // (d is 0 behind the last channel)
 #pragma unroll
             for (int i = 0; i < V; ++i) sum[i] += d[i];
         }
@@ -176,13 +177,13 @@ int64_t bs_act_grad_workspace(int64_t rows, int N) {
 }
 
 int bs_act_grad(const void* g_sum, int64_t ldgs, const void* g_act, int64_t ldga, const void* s, const int8_t* s_exps, int64_t lds,
-                int act, int dtype, int64_t rows, int N, void* ds_out, float* db_out, void* workspace, int64_t workspace_bytes,
-                void* stream) {
+                int act, int dtype, int64_t rows, int N, void* ds_out, int64_t ldds, float* db_out, void* workspace,
+                int64_t workspace_bytes, void* stream) {
     if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || N < 1 || N > (1 << 30) || act < BS_ACT_NONE || act > BS_ACT_GELU) return BS_EINVAL;
     hipStream_t st = rows_stream(stream);
     if (rows > 0 && ((!g_sum && !g_act) || (g_sum && ldgs < N) || (g_act && ldga < N) ||
                      (g_act && act != BS_ACT_NONE && (!s || lds < N)))) return BS_EINVAL;
-    if (!ds_out && !db_out) return BS_EINVAL;
+    if ((!ds_out && !db_out) || (ds_out && ldds < N)) return BS_EINVAL;
     if (rows == 0 && !db_out) return BS_OK;
     int64_t part, parts;
     split_rows(rows, N, &part, &parts);
@@ -190,7 +191,7 @@ int bs_act_grad(const void* g_sum, int64_t ldgs, const void* g_act, int64_t ldga
     ActGradArgs a = {};
     a.g_sum = (const char*)g_sum; a.g_act = (const char*)g_act; a.s = (const char*)s; a.exps = s_exps;
     a.ldgs = ldgs; a.ldga = ldga; a.lds = lds; a.rows = rows; a.part = part;
-    a.N = N; a.nb = (N + P8_BLOCK - 1) / P8_BLOCK; a.act = act; a.ds = (char*)ds_out;
+    a.N = N; a.nb = (N + P8_BLOCK - 1) / P8_BLOCK; a.act = act; a.ds = (char*)ds_out; a.ldds = ldds;
     a.parts = db_out ? (parts > 1 ? (float*)workspace : db_out) : nullptr;
     const int V = dtype == BS_DT_F32 ? 4 : 8, chunks = (N + V - 1) / V;
     int cl = 0;

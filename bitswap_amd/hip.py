@@ -85,13 +85,13 @@ def load():
     L.bs_wino_gemm_bf16x3.argtypes = [p, p, p, i32, i32, i32, i64, i32, p]
     L.bs_conv3_wino_f32.argtypes = [p, p, p, i32, p, p, i32, i64, i32, i32, i32, i32, p]
     L.bs_wino_out_f32.argtypes = [p, p, p, p, p, i64, i32, i32, i32, i32, i32, p]
-    L.bs_linear_workspace.argtypes = L.bs_linear_grad_x_workspace.argtypes = [i32, i64, i32, i32]
+    L.bs_linear_workspace.argtypes = L.bs_linear_grad_x_workspace.argtypes = [i32, i64, i32, i32, i32]
     L.bs_linear_act.argtypes = [p, i64, p, i64, p, i32, p, i64, p, p, i32, i32, i64, i32, i32, p, i64, p]
     L.bs_act_grad_workspace.argtypes = [i64, i32]
-    L.bs_act_grad.argtypes = [p, i64, p, i64, p, p, i64, i32, i32, i64, i32, p, p, p, i64, p]
-    L.bs_linear_grad_x.argtypes = [p, i64, p, i64, p, i32, i64, i32, i32, p, i64, p]
-    L.bs_linear_grad_w_workspace.argtypes = [i32, i64, i32, i32, i32]
-    L.bs_linear_grad_w.argtypes = [p, i64, p, p, i64, p, i32, i64, i32, i32, p, i64, p]
+    L.bs_act_grad.argtypes = [p, i64, p, i64, p, p, i64, i32, i32, i64, i32, p, i64, p, p, i64, p]
+    L.bs_linear_grad_x.argtypes = [p, i64, i32, p, i64, p, i32, i64, i32, i32, p, i64, p]
+    L.bs_linear_grad_w_workspace.argtypes = [i32, i64, i32, i32, i32, i32, i32]
+    L.bs_linear_grad_w.argtypes = [p, i64, i32, p, p, i64, p, i32, i64, i32, i32, p, i64, p]
     L.bs_group_norm_workspace.argtypes = [i32, i64, i64, i32, i32, i32]
     L.bs_group_norm_act.argtypes = [p, i64, i64, p, p, i32, C.c_float, i32, i32, i64, i64, i32, i32, p, p, p, i64, p]
     L.bs_group_norm_act_grad.argtypes = [p, i64, i64, p, p, i64, i64, p, p, p, i32, i32, i32, i64, i64, i32, i32, p, p, p, p, i64, p]
@@ -862,6 +862,11 @@ def _raw_stream(dev):
     return torch._C._cuda_getCurrentRawStream(dev)
 
 
+def _whole(t, ld, width, es):
+    """Rows of whole aligned 16-byte chunks, which the kernels read as they lie (include/bitswap_hip.h, workspaces)."""
+    return int(not (t.data_ptr() | ld * es | width * es) & 15 and ld * es < 1 << 22)
+
+
 def _scratch(like, nbytes):
     return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
@@ -997,7 +1002,7 @@ def linear_act(x, w, bias=None, res=None, act=ACT_ELU, want_sum=False, want_act=
         rt, ldr, _ = _as_rows(res, N, "linear_act res")
     s = x.new_empty(shape) if want_sum else None
     y = x.new_empty(shape) if want_act else None
-    nb = _workspace_bytes("bs_linear_workspace", code, rows, K, N)
+    nb = _workspace_bytes("bs_linear_workspace", code, rows, K, N, _whole(xt, ldx, K, x.element_size()))
     ws = _scratch(x, nb)
     _check(load().bs_linear_act(_at(xt), ldx, _at(wt), ldw, _at(bias), bcode, _at(rt), ldr, _at(s), _at(y), act, code, rows, K, N,
                            _at(ws), nb, _raw_stream(dev)), "bs_linear_act")
@@ -1041,29 +1046,35 @@ def linear_act_grad(x, w, s=None, act=ACT_NONE, g_sum=None, g_act=None, want_x=T
     # one gradient and no slope: it is ds already
     made = sloped or (g_sum is not None and g_act is not None)
     need_ds = want_x or want_w or want_res
-    ds = w.new_empty(g0.shape) if made and need_ds else None
+    es = w.element_size()
+    ds, ldd = None, -(-N * es // 16) * 16 // es           # ds in rows of whole 16-byte chunks (a strided view where N is not one)
+    if made and need_ds:
+        ds = w.new_empty(tuple(g0.shape[:-1]) + (ldd,))
+        ds = ds if ldd == N else ds[..., :N]
     db = w.new_empty(N, dtype=torch.float32) if want_bias else None
     if ds is not None or db is not None:
         nb = _workspace_bytes("bs_act_grad_workspace", rows, N) if want_bias else 0
         ws = _scratch(w, nb)
         _check(L.bs_act_grad(_at(gs[0][0]), gs[0][1], _at(gs[1][0]), gs[1][1], _at(st), _at(se), lds, act, code, rows, N, _at(ds),
-                             _at(db), _at(ws), nb, _raw_stream(dev)), "bs_act_grad")
+                             ldd, _at(db), _at(ws), nb, _raw_stream(dev)), "bs_act_grad")
     if ds is not None:
-        dt, ldd = ds, N
+        dt, zeros, ds_whole = ds, 1, 1
     else:
         dt, ldd = gs[0] if g_sum is not None else gs[1]
+        zeros, ds_whole = 0, _whole(dt, ldd, N, es)
     dx = dw = None
     if want_x:
         wt, ldw, _ = _as_rows(w, K, "linear_act_grad w")
         dx = w.new_empty(tuple(g0.shape[:-1]) + (K,))
-        nb = _workspace_bytes("bs_linear_grad_x_workspace", code, rows, K, N)
+        nb = _workspace_bytes("bs_linear_grad_x_workspace", code, rows, K, N, ds_whole)
         ws = _scratch(w, nb)
-        _check(L.bs_linear_grad_x(_at(dt), ldd, _at(wt), ldw, _at(dx), code, rows, K, N, _at(ws), nb, _raw_stream(dev)), "bs_linear_grad_x")
+        _check(L.bs_linear_grad_x(_at(dt), ldd, zeros, _at(wt), ldw, _at(dx), code, rows, K, N, _at(ws), nb, _raw_stream(dev)), "bs_linear_grad_x")
     if want_w:
         dw = w.new_empty((N, K))
-        nb = _workspace_bytes("bs_linear_grad_w_workspace", code, rows, K, N, int(xe is not None))
+        nb = _workspace_bytes("bs_linear_grad_w_workspace", code, rows, K, N, int(xe is not None),
+                              _whole(xt, ldx, K, es if xe is None else 1), ds_whole)
         ws = _scratch(w, nb)
-        _check(L.bs_linear_grad_w(_at(dt), ldd, _at(xt), _at(xe), ldx, _at(dw), code, rows, K, N, _at(ws), nb, _raw_stream(dev)),
+        _check(L.bs_linear_grad_w(_at(dt), ldd, zeros, _at(xt), _at(xe), ldx, _at(dw), code, rows, K, N, _at(ws), nb, _raw_stream(dev)),
                "bs_linear_grad_w")
     return dx, dw, db, ((ds if ds is not None else g0) if want_res else None)
 

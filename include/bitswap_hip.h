@@ -356,16 +356,21 @@ int bs_wino_out_f32(const float* M, const float* bias, const float* res, float* 
  *   sum_out = s, act_out = a, contiguous [rows, N] (each nullable, at least one).  act sees s before its rounding.  float32
  *   operands are split into three bfloat16 limbs and multiplied as six limb products (as bs_wino_gemm_bf16x3); a sum that does
  *   not come out finite is added up again in float32, so infinities and NaN arrive as they do in float32 arithmetic.  A row's
- *   bits do not depend on `rows`.  workspace: bs_linear_workspace bytes (0 for few rows), in which w is laid out for the kernel.
+ *   bits do not depend on `rows`.
  *
- * bs_act_grad -- ds = g_sum + g_act act'(s) (either gradient nullable, not both), rows [rows, N]: ds_out contiguous (nullable),
+ * Workspaces: the *_workspace functions give the bytes a call needs (0: none) for w laid out for the kernel, copies of rows that are
+ *   not whole, partial sums.  whole: the operand's address, row stride and row are multiples of 16 bytes and the stride is under 4
+ *   MiB; rows that are not are copied first.  zeros (of ds): the rows end in zeros up to the next multiple of 16 bytes, which lies
+ *   within their stride, as bs_act_grad writes them -- such rows count as whole.
+ *
+ * bs_act_grad -- ds = g_sum + g_act act'(s) (either gradient nullable, not both), rows [rows, N]: ds_out (row stride ldds, nullable; where ldds has the room its rows end in zeros up to the next multiple of 16 bytes),
  *   db_out [N] float32 = sum over the rows of ds before its rounding (nullable; workspace of bs_act_grad_workspace bytes then).
  *   s: [rows, N] of dtype (row stride lds), or, if s_exps is given, int8 codes [rows, N] with their exponents (bs_pack8).
  *   act BS_ACT_NONE: s is not read and may be null.
- * bs_linear_grad_x -- dx [rows, K] = ds w;  ds [rows, N] (row stride ldds), w [N, K].  workspace: bs_linear_grad_x_workspace bytes.
+ * bs_linear_grad_x -- dx [rows, K] = ds w;  ds [rows, N] (row stride ldds), w [N, K].
  * bs_linear_grad_w -- dw [N, K] = ds^T x;  x [rows, K] of dtype (row stride ldx) or, if x_exps is given, codes of bs_pack8.  The
  *   rows are split over the chip into parts of a size fixed by (rows, N, K) and the parts added in order: the same call gives the
- *   same bits.  workspace: bs_linear_grad_w_workspace bytes (may be 0; codes: whether x is in 8 bits).
+ *   same bits.  rows <= 2^30.
  *
  * bs_group_norm_act -- x [n, pixels, channels] (strides ldn, ldp), groups dividing channels: mean and biased variance over the
  *   pixels and channels of a group, u = (x - mean) / sqrt(var + eps) * gamma + beta, y = act(u), y contiguous; stats
@@ -389,19 +394,19 @@ int bs_wino_out_f32(const float* M, const float* bias, const float* res, float* 
 #define BS_ACT_ELU 1
 #define BS_ACT_SILU 2
 #define BS_ACT_GELU 3
-int64_t bs_linear_workspace(int dtype, int64_t rows, int K, int N);
+int64_t bs_linear_workspace(int dtype, int64_t rows, int K, int N, int whole);
 int bs_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype, const void* res,
                   int64_t ldr, void* sum_out, void* act_out, int act, int dtype, int64_t rows, int K, int N, void* workspace,
                   int64_t workspace_bytes, void* stream);
 int64_t bs_act_grad_workspace(int64_t rows, int N);
 int bs_act_grad(const void* g_sum, int64_t ldgs, const void* g_act, int64_t ldga, const void* s, const int8_t* s_exps, int64_t lds,
-                int act, int dtype, int64_t rows, int N, void* ds_out, float* db_out, void* workspace, int64_t workspace_bytes,
-                void* stream);
-int64_t bs_linear_grad_x_workspace(int dtype, int64_t rows, int K, int N);
-int bs_linear_grad_x(const void* ds, int64_t ldds, const void* w, int64_t ldw, void* dx, int dtype, int64_t rows, int K, int N,
+                int act, int dtype, int64_t rows, int N, void* ds_out, int64_t ldds, float* db_out, void* workspace,
+                int64_t workspace_bytes, void* stream);
+int64_t bs_linear_grad_x_workspace(int dtype, int64_t rows, int K, int N, int whole);
+int bs_linear_grad_x(const void* ds, int64_t ldds, int zeros, const void* w, int64_t ldw, void* dx, int dtype, int64_t rows, int K, int N,
                      void* workspace, int64_t workspace_bytes, void* stream);
-int64_t bs_linear_grad_w_workspace(int dtype, int64_t rows, int K, int N, int codes);
-int bs_linear_grad_w(const void* ds, int64_t ldds, const void* x, const int8_t* x_exps, int64_t ldx, void* dw, int dtype,
+int64_t bs_linear_grad_w_workspace(int dtype, int64_t rows, int K, int N, int codes, int x_whole, int ds_whole);
+int bs_linear_grad_w(const void* ds, int64_t ldds, int zeros, const void* x, const int8_t* x_exps, int64_t ldx, void* dw, int dtype,
                      int64_t rows, int K, int N, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t bs_group_norm_workspace(int dtype, int64_t n, int64_t pixels, int channels, int groups, int grad);
 int bs_group_norm_act(const void* x, int64_t ldn, int64_t ldp, const void* gamma, const void* beta, int affine_dtype, float eps,

@@ -27,20 +27,21 @@ def test_null_operands_sizes_types_and_strides_are_refused(L):
                 dict(dt=-1), dict(rows=-1), dict(rows=1 << 41), dict(K=0), dict(N=0), dict(bias=p, bt=1), dict(rows=100000)):
         assert ok(**bad) == E, bad
     assert ok(rows=0, x=None) == hip.OK                                     # no rows: nothing to do
-    n = L.bs_linear_grad_x_workspace(0, 4, 8, 8)
-    assert L.bs_linear_grad_x(None, 8, p, 8, p, 0, 4, 8, 8, p, n, None) == E
-    assert L.bs_linear_grad_x(p, 7, p, 8, p, 0, 4, 8, 8, p, n, None) == E
-    assert L.bs_linear_grad_x(p, 8, p, 8, p, 0, 4, 8, 8, p, n - 1, None) == E
-    assert L.bs_linear_grad_w(p, 8, None, None, 8, p, 0, 4, 8, 8, None, 0, None) == E
-    assert L.bs_linear_grad_w(p, 8, p, None, 8, None, 0, 4, 8, 8, None, 0, None) == E
-    n = L.bs_linear_grad_w_workspace(0, 100000, 8, 8, 0)
-    assert n > 0 and L.bs_linear_grad_w(p, 8, p, None, 8, p, 0, 100000, 8, 8, p, n - 1, None) == E
-    assert L.bs_linear_grad_w(p, 8, p, None, 8, p, 0, 100000, 8, 8, None, n, None) == E
-    assert L.bs_act_grad(None, 8, None, 8, None, None, 8, 1, 0, 4, 8, p, None, None, 0, None) == E           # no gradient
-    assert L.bs_act_grad(None, 8, p, 8, None, None, 8, 1, 0, 4, 8, p, None, None, 0, None) == E              # no sum
-    assert L.bs_act_grad(p, 8, None, 8, None, None, 8, 1, 0, 4, 8, None, None, None, 0, None) == E           # nothing asked
+    n = L.bs_linear_grad_x_workspace(0, 4, 8, 8, 1)
+    assert L.bs_linear_grad_x(None, 8, 0, p, 8, p, 0, 4, 8, 8, p, n, None) == E
+    assert L.bs_linear_grad_x(p, 7, 0, p, 8, p, 0, 4, 8, 8, p, n, None) == E
+    assert L.bs_linear_grad_x(p, 8, 0, p, 8, p, 0, 4, 8, 8, p, n - 1, None) == E
+    assert L.bs_linear_grad_w(p, 8, 0, None, None, 8, p, 0, 4, 8, 8, None, 0, None) == E
+    assert L.bs_linear_grad_w(p, 8, 0, p, None, 8, None, 0, 4, 8, 8, None, 0, None) == E
+    n = L.bs_linear_grad_w_workspace(0, 100000, 8, 8, 0, 1, 1)
+    assert n > 0 and L.bs_linear_grad_w(p, 8, 0, p, None, 8, p, 0, 100000, 8, 8, p, n - 1, None) == E
+    assert L.bs_linear_grad_w(p, 8, 0, p, None, 8, p, 0, 100000, 8, 8, None, n, None) == E
+    assert L.bs_act_grad(None, 8, None, 8, None, None, 8, 1, 0, 4, 8, p, 8, None, None, 0, None) == E           # no gradient
+    assert L.bs_act_grad(None, 8, p, 8, None, None, 8, 1, 0, 4, 8, p, 8, None, None, 0, None) == E              # no sum
+    assert L.bs_act_grad(p, 8, None, 8, None, None, 8, 1, 0, 4, 8, None, 8, None, None, 0, None) == E
+    assert L.bs_act_grad(p, 8, None, 8, None, None, 8, 0, 0, 4, 8, p, 7, None, None, 0, None) == E           # nothing asked
     n = L.bs_act_grad_workspace(100000, 8)
-    assert n > 0 and L.bs_act_grad(p, 8, None, 8, None, None, 8, 0, 0, 100000, 8, None, p, p, n - 1, None) == E
+    assert n > 0 and L.bs_act_grad(p, 8, None, 8, None, None, 8, 0, 0, 100000, 8, None, 8, p, p, n - 1, None) == E
     assert L.bs_group_norm_act(p, 64, 8, None, None, 0, 1e-5, 0, 0, 2, 8, 8, 3, p, None, None, 0, None) == E  # 3 groups of 8 channels
     assert L.bs_group_norm_act(p, 64, 7, None, None, 0, 1e-5, 0, 0, 2, 8, 8, 2, p, None, None, 0, None) == E
     assert L.bs_group_norm_act(p, 64, 8, p, None, 2, 1e-5, 0, 0, 2, 8, 8, 2, p, None, None, 0, None) == E     # gamma of a third type
@@ -56,12 +57,13 @@ def test_null_operands_sizes_types_and_strides_are_refused(L):
 def test_workspaces(L):
     for rows in (0, 1, 63, 64, 65, 1000, 102400, 1 << 33):
         for k, n in ((1, 1), (61, 130), (2048, 2048)):
-            assert 0 <= L.bs_linear_grad_w_workspace(1, rows, k, n, 0) < 1 << 28
+            assert 0 <= L.bs_linear_grad_w_workspace(1, rows, k, n, 0, 1, 1) < 1 << 28
             assert 0 <= L.bs_act_grad_workspace(rows, n) < 1 << 26
-    assert L.bs_linear_grad_w_workspace(1, 1000, 100, 8, 1) == L.bs_linear_grad_w_workspace(1, 1000, 100, 8, 0) + 4 * 1024 * 4
-    assert L.bs_linear_grad_w_workspace(0, 1, 8, 8, 0) == 0 and L.bs_linear_workspace(0, 256, 256, 256) == 0
+    assert L.bs_linear_grad_w_workspace(1, 1000, 100, 8, 1, 1, 1) == L.bs_linear_grad_w_workspace(1, 1000, 100, 8, 0, 1, 1) + 4 * 1024 * 4
+    assert L.bs_linear_grad_w_workspace(1, 1000, 100, 8, 0, 0, 1) >= L.bs_linear_grad_w_workspace(1, 1000, 100, 8, 0, 1, 1) + 1000 * 104 * 2
+    assert L.bs_linear_grad_w_workspace(0, 1, 8, 8, 0, 1, 1) == 0 and L.bs_linear_workspace(0, 256, 256, 256, 0) == 0
     for bad in ((3, 8, 8, 8), (1, -1, 8, 8), (1, 8, 0, 8), (1, 8, 8, 0)):
-        assert L.bs_linear_grad_w_workspace(*bad, 0) < 0 and L.bs_linear_workspace(*bad) < 0 and L.bs_linear_grad_x_workspace(*bad) < 0
+        assert L.bs_linear_grad_w_workspace(*bad, 0, 0, 0) < 0 and L.bs_linear_workspace(*bad, 1) < 0 and L.bs_linear_grad_x_workspace(*bad, 1) < 0
     assert L.bs_group_norm_workspace(0, 3, 256, 256, 32, 0) == 0
     assert L.bs_group_norm_workspace(0, 3, 1 << 20, 64, 32, 1) > 0
     assert L.bs_group_norm_workspace(0, 3, 256, 256, 33, 0) < 0
