@@ -144,11 +144,12 @@ __device__ __forceinline__ u32x4 residual(const RowsArgs& a, int64_t q, int64_t 
 // A wavefront's 32 rows x 64 channels from the registers of the matrix instruction to rows of memory, by way of its own piece of
 // shared memory (row stride 68 floats: 16 lanes of a 16-byte access touch all banks): whole 16-byte accesses, 128 or 256 bytes of a
 // row side by side.
-constexpr int TURN = 32 * 68 * 4;
-template <int DT, int EPI>
+constexpr int turn_bytes(int cols) { return 32 * (cols + 4) * 4; }
+// COLS: 64, or 32 where a wavefront has one 32x32 tile across
+template <int DT, int EPI, int COLS>
 __device__ __forceinline__ void turn_and_finish(const RowsArgs& a, const f32x16& a0, const f32x16& a1, float* mine, int lane, int64_t q0,
                                                 int64_t p0, const float* bias) {
-    constexpr int V = vlen(DT), LPR = 64 / V, RI = 64 / LPR, NI = 32 / RI;      // lanes per row of 64 channels, rows at a time
+    constexpr int V = vlen(DT), LPR = COLS / V, RI = 64 / LPR, NI = 32 / RI, ST = COLS + 4;      // lanes per row, rows at a time
     const int c = (lane % LPR) * V;
     const int64_t p = p0 + c, left = a.N - p;
     const int n = left < V ? (int)left : V;
@@ -162,11 +163,9 @@ __device__ __forceinline__ void turn_and_finish(const RowsArgs& a, const f32x16&
     }
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-        const f32x4 v0 = {a0[4 * g], a0[4 * g + 1], a0[4 * g + 2], a0[4 * g + 3]};
-        const f32x4 v1 = {a1[4 * g], a1[4 * g + 1], a1[4 * g + 2], a1[4 * g + 3]};
-        float* const at = mine + (lane & 31) * 68 + 8 * g + 4 * (lane >> 5);
-        *reinterpret_cast<f32x4*>(at) = v0;
-        *reinterpret_cast<f32x4*>(at + 32) = v1;
+        float* const at = mine + (lane & 31) * ST + 8 * g + 4 * (lane >> 5);
+        *reinterpret_cast<f32x4*>(at) = f32x4{a0[4 * g], a0[4 * g + 1], a0[4 * g + 2], a0[4 * g + 3]};
+        if (COLS == 64) *reinterpret_cast<f32x4*>(at + 32) = f32x4{a1[4 * g], a1[4 * g + 1], a1[4 * g + 2], a1[4 * g + 3]};
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -178,7 +177,7 @@ __device__ __forceinline__ void turn_and_finish(const RowsArgs& a, const f32x16&
             float v[V];
 #pragma unroll
             for (int e = 0; e < V; e += 4) {
-                const f32x4 t = *reinterpret_cast<const f32x4*>(mine + r * 68 + c + e);
+                const f32x4 t = *reinterpret_cast<const f32x4*>(mine + r * ST + c + e);
                 v[e] = t[0]; v[e + 1] = t[1]; v[e + 2] = t[2]; v[e + 3] = t[3];
             }
             finish<DT, EPI>(a, q0 + r, p, n, v, bias, res[i]);
@@ -204,7 +203,8 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64, PER_SIMD) void k_rows_d
     constexpr int XB = BQ * BK * ES, WB = L * BP * BK * 2, STAGE = XB + WB;
     constexpr int XI = XB / 1024 / NW, WI = WB / 1024 / NW;
     constexpr int NP = WP / 32, NQ = WQ / 32;
-    static_assert(XB % (1024 * NW) == 0 && WB % (1024 * NW) == 0 && NS * STAGE <= 160 * 1024 && NP % 2 == 0, "");
+    static_assert(XB % (1024 * NW) == 0 && WB % (1024 * NW) == 0 && NS * STAGE <= 160 * 1024 && (NP == 1 || NP % 2 == 0), "");
+    constexpr int COLS = NP == 1 ? 32 : 64, TURN = turn_bytes(COLS);
     __shared__ __align__(16) char lds[NS * STAGE > NW * TURN ? NS * STAGE : NW * TURN];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wp = wave % (BP / WP), wq = wave / (BP / WP);
@@ -378,12 +378,13 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64, PER_SIMD) void k_rows_d
     __syncthreads();
     float* const mine = reinterpret_cast<float*>(lds + wave * TURN);
 #pragma unroll
-    for (int i = 0; i < NP; i += 2) {
+    for (int i = 0; i < NP; i += COLS / 32) {
         const int p = p0 + wp * WP + i * 32;
         float bias[vlen(DT)];
-        if (EPI == E_LAYER) load_bias<DT>(a, p + lane % (64 / vlen(DT)) * vlen(DT), bias);
+        if (EPI == E_LAYER) load_bias<DT>(a, p + lane % (COLS / vlen(DT)) * vlen(DT), bias);
 #pragma unroll
-        for (int j = 0; j < NQ; ++j) turn_and_finish<DT, EPI>(a, acc[i][j], acc[i + 1][j], mine, lane, q0 + wq * WQ + j * 32, p, bias);
+        for (int j = 0; j < NQ; ++j)
+            turn_and_finish<DT, EPI, COLS>(a, acc[i][j], acc[i + COLS / 32 - 1][j], mine, lane, q0 + wq * WQ + j * 32, p, bias);
     }
 }
 
@@ -394,7 +395,7 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64, PER_SIMD) void k_rows_d
 template <int DT, int EPI, bool WL>
 __global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {
     constexpr int L = limbs_of(DT), NS = DT == BS_DT_F32 ? 4 : 8, ES = esize(DT), RUN = NS * 16;
-    __shared__ __align__(16) char lds[TURN];
+    __shared__ __align__(16) char lds[turn_bytes(64)];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t q0 = blockIdx.x / a.tp * 32;
     const int p0 = (int)(blockIdx.x % a.tp) * 32;
@@ -543,6 +544,7 @@ struct OverArgs {
     const int8_t* exps;
     int64_t ldx, ldds, ldxd, lddd, rows, part;
     int K, N, nb, parts;
+    int64_t pstride;                   // floats of a part: N K, rounded up to whole 16 bytes
     int tp;
     int64_t tiles;                     // tiles x parts
     char* out;
@@ -579,7 +581,7 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
     constexpr int XB = BK * XR, DB = BK * DR, SB = P8 ? BP / 32 * BK * 4 : 0, STAGE = XB + DB + SB;
     constexpr int XI = XB / 1024 / NW, DI = DB / 1024 / NW, SI = P8 ? 1 : 0;
     constexpr int NP = WP / 32, NQ = WQ / 32;
-    static_assert(XB % (1024 * NW) == 0 && DB % (1024 * NW) == 0 && NS * STAGE <= 160 * 1024 && NW * TURN <= NS * STAGE, "shared memory");
+    static_assert(XB % (1024 * NW) == 0 && DB % (1024 * NW) == 0 && NS * STAGE <= 160 * 1024 && NW * turn_bytes(64) <= NS * STAGE, "shared memory");
     static_assert(!P8 || (SB % 256 == 0 && SB / 256 <= NW), "steps: one dword a lane");
     __shared__ __align__(16) char lds[NS * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -829,7 +831,7 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
     for (; s + NS < whole; ++s) step(s, std::true_type{});
     for (; s < count; ++s) step(s, std::false_type{});
     __syncthreads();
-    float* const mine = reinterpret_cast<float*>(lds + wave * TURN);
+    float* const mine = reinterpret_cast<float*>(lds + wave * turn_bytes(64));
 #pragma unroll
     for (int j = 0; j < NQ; ++j)
 #pragma unroll
@@ -849,7 +851,7 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
                     if (q >= a.N) break;
                     f32x4 v = *reinterpret_cast<const f32x4*>(mine + r * 68 + lane % 16 * 4);
                     if (DT == BS_DT_F32) again_over<DT, P8>(a, kb, ke, p, q, n, v);
-                    float* const o = reinterpret_cast<float*>(a.out) + ((int64_t)part * a.N + q) * a.K + p;
+                    float* const o = reinterpret_cast<float*>(a.out) + part * a.pstride + (int64_t)q * a.K + p;
                     if (n >= 4) store16((char*)o, __builtin_bit_cast(u32x4, v));
                     else
                         for (int e = 0; e < n; ++e) o[e] = v[e];
@@ -902,7 +904,7 @@ __global__ __launch_bounds__(256) void k_lay_steps(const int8_t* __restrict__ ex
     for (int b = 0; b < nb; ++b) out[b * ld + i] = i < rows ? p8_pow2(exps[i * nb + b]) : 0.0f;
 }
 
-// parts [nparts][n] float32 -> their sum in dtype; 16 threads of four neighbours x 16 lanes over the parts
+// parts [nparts][n, rounded up to whole 16 bytes] float32 -> their sum in dtype; 16 threads of four neighbours x 16 lanes over the parts
 template <int DT>
 __global__ __launch_bounds__(256) void k_add_parts(const float* __restrict__ parts, int nparts, int64_t n, char* __restrict__ out) {
     __shared__ __align__(16) f32x4 red[256];
@@ -910,10 +912,10 @@ __global__ __launch_bounds__(256) void k_add_parts(const float* __restrict__ par
     const int64_t i = ((int64_t)blockIdx.x * 16 + tx) * 4;
     f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
     if (i < n) {
-        const int left = n - i < 4 ? (int)(n - i) : 4;
+        const int64_t stride = (n + 3) / 4 * 4;
 #pragma unroll 4
         for (int k = l; k < nparts; k += 16) {
-            const f32x4 v = __builtin_bit_cast(f32x4, load_raw<BS_DT_F32>((const char*)(parts + k * n + i), left));
+            const f32x4 v = *reinterpret_cast<const f32x4*>(parts + k * stride + i);
             s[0] += v[0]; s[1] += v[1]; s[2] += v[2]; s[3] += v[3];
         }
     }
@@ -964,7 +966,7 @@ int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream
     constexpr int ES = esize(DT), CK = 16 / ES;
     const int kp = (a.K + 63) / 64 * 64;
     const bool small = few(a.rows, a.N), whole = whole_rows(a.x, a.ldx, a.K, ES, zeros);
-    const bool big = DT != BS_DT_F32 && tiles_of(a.rows, a.N, 256, 256) >= BIG_TILES;
+    const bool big = DT != BS_DT_F32 && a.N > 128 && tiles_of(a.rows, a.N, 256, 256) >= BIG_TILES;
     const bool as_is = DT != BS_DT_F32 && !a.wt && a.K % 64 == 0 && a.ldw % 8 == 0 && ((uintptr_t)a.w & 15) == 0 && a.ldw < (1 << 21);
     const int64_t need = rows_bytes(DT, a.rows, a.K, a.N, a.wt, whole);
     if (need > 0 && (!workspace || bytes < need)) return BS_EINVAL;
@@ -999,7 +1001,7 @@ int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream
         hipLaunchKernelGGL((k_rows_dma<DT, EPI, BQ, BP, WQ, WP, BK, NS, PS>), dim3((unsigned)blocks), dim3((BQ / WQ) * (BP / WP) * 64), 0, st, a); } while (0)
     if constexpr (DT == BS_DT_F32) {
         if (tiles_of(a.rows, a.N, 64, 128) >= MID_TILES && a.N > 64) ROWS(64, 128, 32, 64, 16, 3, 3);
-        else ROWS(64, 64, 32, 64, 16, 4, 1);
+        else ROWS(64, 64, 32, 32, 32, 4, 1);
     } else {
         if (big) ROWS(256, 256, 128, 64, 32, 4, 1);
         else if (tiles_of(a.rows, a.N, 128, 128) >= MID_TILES && a.N > 64) ROWS(128, 128, 64, 64, 32, 4, 1);
@@ -1034,7 +1036,7 @@ OverBytes over_bytes(int dtype, int64_t rows, int K, int N, bool codes, bool x_w
     int64_t part, parts;
     split_rows(dtype, rows, K, N, &part, &parts);
     return {codes ? steps_bytes(rows, K) : 0, x_whole ? 0 : pad_bytes(codes ? 1 : esize(dtype), rows, K), ds_whole ? 0 : pad_bytes(esize(dtype), rows, N),
-            parts > 1 || dtype != BS_DT_F32 ? parts * K * N * 4 : 0};
+            parts > 1 || dtype != BS_DT_F32 ? parts * (((int64_t)K * N + 3) / 4 * 4) * 4 : 0};
 }
 
 template <int DT>
@@ -1124,7 +1126,7 @@ int bs_linear_grad_w(const void* ds, int64_t ldds, int zeros, const void* x, con
         OverArgs a = {};
         a.x = (const char*)x; a.exps = x_exps; a.ldx = ldx; a.ds = (const char*)ds; a.ldds = ldds; a.rows = rows; a.part = part;
         a.K = K; a.N = N; a.nb = (K + P8_BLOCK - 1) / P8_BLOCK; a.parts = (int)parts;
-        a.xd = a.x; a.ldxd = ldx; a.dd = a.ds; a.lddd = ldds;
+        a.xd = a.x; a.ldxd = ldx; a.dd = a.ds; a.lddd = ldds; a.pstride = (n + 3) / 4 * 4;
         a.out = joined ? ws + b.steps + b.x + b.ds : (char*)dw;
         const int64_t ld = (rows + 63) / 64 * 64;
         if (x_exps) hipLaunchKernelGGL(k_lay_steps, dim3((unsigned)((ld + 255) / 256)), dim3(256), 0, st, x_exps, rows, a.nb, (float*)ws, ld);
