@@ -587,8 +587,11 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wp = wave % (BP / WP), wq = wave / (BP / WP);
     // chunk c of row r lies in slot c ^ sx(r): rows that one transposing read gathers then lie in different banks
-    auto sd = [](int r) { return ES == 2 ? 4 * (r & 3) : 8 * ((r >> 3) & 1); };
-    auto sx = [&](int r) { return P8 ? 2 * ((r >> 1) & 3) : sd(r); };
+    // (swap: RB bytes a row; 64 channels of 16 bits are 128 bytes, two rows on the 64 banks)
+    auto swap = [](int RB, int r) { return ES == 4 ? 8 * ((r >> 3) & 1) : RB >= 256 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); };
+    auto sd = [&](int r) { return swap(DR, r); };
+    auto sx = [&](int r) { return P8 ? 2 * ((r >> 1) & 3) : swap(XR, r); };
+    static_assert(XR >= 128 && DR >= 128 && (ES == 2 || DR >= 256), "a row takes its swaps");
     const int64_t per = (a.tiles + 7) / 8;
     const int64_t t = (blockIdx.x % 8) * per + blockIdx.x / 8;        // an XCD takes runs of tiles over the same rows
     if (t >= a.tiles) return;
@@ -678,13 +681,13 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int row = r0 + 8 * (lane >> 5) + e, ch = c0 + (lane & 31);
-                r.f[e] = *reinterpret_cast<const float*>(base + row * RB + ((ch >> 2) ^ sd(row)) * 16 + (ch & 3) * 4);
+                r.f[e] = *reinterpret_cast<const float*>(base + row * RB + ((ch >> 2) ^ swap(RB, row)) * 16 + (ch & 3) * 4);
             }
         } else {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int row = r0 + 8 * (lane >> 5) + 4 * h + ((lane & 15) >> 2), ch = c0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-                const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(base + row * RB + (((ch >> 3) ^ sd(row)) * 16) + (ch & 4) * 2));
+                const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(base + row * RB + (((ch >> 3) ^ swap(RB, row)) * 16) + (ch & 4) * 2));
                 const u32x2 w2 = __builtin_bit_cast(u32x2, w);
                 r.v[2 * h] = w2[0];
                 r.v[2 * h + 1] = w2[1];
@@ -811,7 +814,8 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 if (m * RM < R) __builtin_amdgcn_sched_group_barrier(0x100, RM, 0);
                 if (RUN && b == SBK - 1 && m >= M - D) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-                if ((P8 || DT == BS_DT_F32) && m >= M / 2) __builtin_amdgcn_sched_group_barrier(0x002, P8 && LD == 1 ? 16 : 8, 0);
+                if (P8 && LD == 1 && m >= M / 2) __builtin_amdgcn_sched_group_barrier(0x002, 16, 0);
+                if (DT == BS_DT_F32 && m >= M / 4) __builtin_amdgcn_sched_group_barrier(0x002, 10, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
             mend(xn, pn);
@@ -851,6 +855,14 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
                     if (q >= a.N) break;
                     f32x4 v = *reinterpret_cast<const f32x4*>(mine + r * 68 + lane % 16 * 4);
                     if (DT == BS_DT_F32) again_over<DT, P8>(a, kb, ke, p, q, n, v);
+                    if (DT != BS_DT_F32 && a.parts == 1) {                       // nothing to be joined with: rounded here
+                        char* const o = a.out + ((int64_t)q * a.K + p) * ES;
+                        const u32x2 w = DT == BS_DT_F16 ? u32x2{pk_f16(v[0], v[1]), pk_f16(v[2], v[3])} : u32x2{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3])};
+                        if (n >= 4) store8(o, w);
+                        else
+                            for (int e = 0; e < n; ++e) store1<DT>(o + e * ES, v[e]);
+                        continue;
+                    }
                     float* const o = reinterpret_cast<float*>(a.out) + part * a.pstride + (int64_t)q * a.K + p;
                     if (n >= 4) store16((char*)o, __builtin_bit_cast(u32x4, v));
                     else
@@ -1012,10 +1024,11 @@ int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream
     return rows_rc();
 }
 
-// How a weight gradient is cut: tiles of BQ x 128 outputs (256 channels of ds where there are that many), and the rows into as many
-// parts as give the chip two workgroups a compute unit, none under 128 rows.
+// How a weight gradient is cut: tiles of 256 x 128 outputs (16-bit, where there are enough) or 64 x 128, and the rows into as many parts as
+// give the chip two workgroups a compute unit, none under 128 rows.
 int over_bq(int dtype, int64_t rows, int K, int N) {
-    return dtype != BS_DT_F32 && N > 128 && tiles_of(N, K, 256, 128) * ((rows + 255) / 256) >= 512 ? 256 : 128;
+    if (dtype == BS_DT_F32) return 64;
+    return N > 128 && tiles_of(N, K, 256, 128) * ((rows + 255) / 256) >= 512 ? 256 : 64;
 }
 void split_rows(int dtype, int64_t rows, int K, int N, int64_t* part, int64_t* parts) {
     const int64_t tiles = tiles_of(N, K, over_bq(dtype, rows, K, N), 128);
@@ -1036,7 +1049,7 @@ OverBytes over_bytes(int dtype, int64_t rows, int K, int N, bool codes, bool x_w
     int64_t part, parts;
     split_rows(dtype, rows, K, N, &part, &parts);
     return {codes ? steps_bytes(rows, K) : 0, x_whole ? 0 : pad_bytes(codes ? 1 : esize(dtype), rows, K), ds_whole ? 0 : pad_bytes(esize(dtype), rows, N),
-            parts > 1 || dtype != BS_DT_F32 ? parts * (((int64_t)K * N + 3) / 4 * 4) * 4 : 0};
+            parts > 1 ? parts * (((int64_t)K * N + 3) / 4 * 4) * 4 : 0};
 }
 
 template <int DT>
@@ -1045,13 +1058,13 @@ int launch_over(OverArgs a, const float* steps, int64_t ld, hipStream_t st) {
         const int64_t blocks = (a.tiles + 7) / 8 * 8; if (blocks > 0x7fffffff) return BS_EINVAL; \
         hipLaunchKernelGGL((k_over_dma<DT, P8, BQ, 128, WQ, 64, BK_, NS>), dim3((unsigned)blocks), dim3(256), 0, st, a, steps, ld); } while (0)
     if (a.exps) {
-        if constexpr (DT == BS_DT_F32) OVER(true, 128, 64, 32, 3);
+        if constexpr (DT == BS_DT_F32) OVER(true, 64, 32, 32, 3);
         else if (over_bq(DT, a.rows, a.K, a.N) == 256) OVER(true, 256, 128, 32, 3);
-        else OVER(true, 128, 64, 32, 4);
+        else OVER(true, 64, 32, 32, 4);
     } else {
-        if constexpr (DT == BS_DT_F32) OVER(false, 128, 64, 16, 4);
+        if constexpr (DT == BS_DT_F32) OVER(false, 64, 32, 16, 3);
         else if (over_bq(DT, a.rows, a.K, a.N) == 256) OVER(false, 256, 128, 32, 3);
-        else OVER(false, 128, 64, 32, 4);
+        else OVER(false, 64, 32, 32, 4);
     }
 #undef OVER
     return rows_rc();
@@ -1121,7 +1134,7 @@ int bs_linear_grad_w(const void* ds, int64_t ldds, int zeros, const void* x, con
     split_rows(dtype, rows, K, N, &part, &parts);
     if (rows > 0 && b.all() > 0 && (!workspace || workspace_bytes < b.all())) return BS_EINVAL;
     char* const ws = (char*)workspace;                       // steps of the codes | copy of x | copy of ds | parts
-    const bool joined = b.parts > 0;
+    const bool joined = parts > 1;
     if (rows > 0) {
         OverArgs a = {};
         a.x = (const char*)x; a.exps = x_exps; a.ldx = ldx; a.ds = (const char*)ds; a.ldds = ldds; a.rows = rows; a.part = part;
