@@ -359,7 +359,6 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64, PER_SIMD) void k_rows_d
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                                       // one matrix instruction
                 if (m < (R + 1) / 2) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);                  // two LDS reads
                 else if (RUN && b == SB - 1 && m < (R + 1) / 2 + D) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-                if (L == 3 && m >= M / 2) __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
             f = g;
@@ -814,8 +813,6 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 if (m * RM < R) __builtin_amdgcn_sched_group_barrier(0x100, RM, 0);
                 if (RUN && b == SBK - 1 && m >= M - D) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-                if (P8 && LD == 1 && m >= M / 2) __builtin_amdgcn_sched_group_barrier(0x002, 16, 0);
-                if (DT == BS_DT_F32 && m >= M / 4) __builtin_amdgcn_sched_group_barrier(0x002, 10, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
             mend(xn, pn);
@@ -943,7 +940,7 @@ __global__ __launch_bounds__(256) void k_add_parts(const float* __restrict__ par
 }
 
 // ---- which way --------------------------------------------------------------------------------------------------------------------
-constexpr int RELAY_TILES = 256, MID_TILES = 256, BIG_TILES = 384;
+constexpr int RELAY_TILES = 256, MID_TILES = 256, BIG_TILES = 384, DEEP_K = 512;
 int64_t tiles_of(int64_t rows, int N, int bq, int bp) { return (rows + bq - 1) / bq * ((N + bp - 1) / bp); }
 bool few(int64_t rows, int N) { return tiles_of(rows, N, 32, 32) <= RELAY_TILES; }
 
@@ -1012,7 +1009,8 @@ int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream
         const int64_t blocks = (a.tiles + 7) / 8 * 8; if (blocks > 0x7fffffff) return BS_EINVAL; \
         hipLaunchKernelGGL((k_rows_dma<DT, EPI, BQ, BP, WQ, WP, BK, NS, PS>), dim3((unsigned)blocks), dim3((BQ / WQ) * (BP / WP) * 64), 0, st, a); } while (0)
     if constexpr (DT == BS_DT_F32) {
-        if (tiles_of(a.rows, a.N, 64, 128) >= MID_TILES && a.N > 64) ROWS(64, 128, 32, 64, 16, 3, 3);
+        if (a.K >= DEEP_K && a.N > 64 && tiles_of(a.rows, a.N, 128, 128) >= MID_TILES) ROWS(128, 128, 64, 64, 16, 3, 2);
+        else if (tiles_of(a.rows, a.N, 64, 128) >= MID_TILES && a.N > 64) ROWS(64, 128, 32, 64, 16, 3, 3);
         else ROWS(64, 64, 32, 32, 32, 4, 1);
     } else {
         if (big) ROWS(256, 256, 128, 64, 32, 4, 1);
@@ -1024,11 +1022,11 @@ int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream
     return rows_rc();
 }
 
-// How a weight gradient is cut: tiles of 256 x 128 outputs (16-bit, where there are enough) or 64 x 128, and the rows into as many parts as
+// How a weight gradient is cut: tiles of 256 x 128 (16-bit) or 128 x 128 (float32) outputs where there are enough, else 64 x 128, and the rows into as many parts as
 // give the chip two workgroups a compute unit, none under 128 rows.
 int over_bq(int dtype, int64_t rows, int K, int N) {
-    if (dtype == BS_DT_F32) return 64;
-    return N > 128 && tiles_of(N, K, 256, 128) * ((rows + 255) / 256) >= 512 ? 256 : 64;
+    const int big = dtype == BS_DT_F32 ? 128 : 256;
+    return 2 * N > big && tiles_of(N, K, big, 128) * ((rows + 255) / 256) >= 512 ? big : 64;
 }
 void split_rows(int dtype, int64_t rows, int K, int N, int64_t* part, int64_t* parts) {
     const int64_t tiles = tiles_of(N, K, over_bq(dtype, rows, K, N), 128);
@@ -1058,12 +1056,16 @@ int launch_over(OverArgs a, const float* steps, int64_t ld, hipStream_t st) {
         const int64_t blocks = (a.tiles + 7) / 8 * 8; if (blocks > 0x7fffffff) return BS_EINVAL; \
         hipLaunchKernelGGL((k_over_dma<DT, P8, BQ, 128, WQ, 64, BK_, NS>), dim3((unsigned)blocks), dim3(256), 0, st, a, steps, ld); } while (0)
     if (a.exps) {
-        if constexpr (DT == BS_DT_F32) OVER(true, 64, 32, 32, 3);
-        else if (over_bq(DT, a.rows, a.K, a.N) == 256) OVER(true, 256, 128, 32, 3);
+        if constexpr (DT == BS_DT_F32) {
+            if (over_bq(DT, a.rows, a.K, a.N) == 128) OVER(true, 128, 64, 32, 3);
+            else OVER(true, 64, 32, 32, 3);
+        } else if (over_bq(DT, a.rows, a.K, a.N) == 256) OVER(true, 256, 128, 32, 3);
         else OVER(true, 64, 32, 32, 4);
     } else {
-        if constexpr (DT == BS_DT_F32) OVER(false, 64, 32, 16, 3);
-        else if (over_bq(DT, a.rows, a.K, a.N) == 256) OVER(false, 256, 128, 32, 3);
+        if constexpr (DT == BS_DT_F32) {
+            if (over_bq(DT, a.rows, a.K, a.N) == 128) OVER(false, 128, 64, 16, 3);
+            else OVER(false, 64, 32, 16, 3);
+        } else if (over_bq(DT, a.rows, a.K, a.N) == 256) OVER(false, 256, 128, 32, 3);
         else OVER(false, 64, 32, 32, 4);
     }
 #undef OVER

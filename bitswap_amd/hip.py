@@ -828,6 +828,7 @@ def wino_fused(src, shape, ts_in=0, bias=None, res=None, act=True, want_sum=Fals
 
 # ---- channels-last layers: products, group norm, 8-bit saves (linear.hip, norm_act.hip, pack8.hip) ------------------------------
 ACT_NONE, ACT_ELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3
+_ACTS = (ACT_NONE, ACT_ELU, ACT_SILU, ACT_GELU)
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # BS_DT_*
 PACK8_BLOCK = 32
 
@@ -839,9 +840,11 @@ def _gpu(*ts):
     for t in ts:
         if t is not None:
             d = t.get_device()
-            if cur is None:
-                cur = torch._C._cuda_getDevice() if d >= 0 else -1
-            if d < 0 or d != cur:
+            if d != cur or d < 0:
+                if cur is None and d >= 0:
+                    cur = torch._C._cuda_getDevice()
+                    if d == cur:
+                        continue
                 _need_cuda(t)
     return cur
 
@@ -873,13 +876,14 @@ def _scratch(like, nbytes):
 
 
 def _dtype_code(t, what):
-    if t.dtype not in _DTYPES:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
         raise BitswapHipError(f"{what}: float32, bfloat16 or float16, got {t.dtype}")
-    return _DTYPES[t.dtype]
+    return code
 
 
 def _act_code(act):
-    if act not in (ACT_NONE, ACT_ELU, ACT_SILU, ACT_GELU):
+    if act not in _ACTS:
         raise BitswapHipError(f"unknown activation {act!r}")
     return int(act)
 
@@ -887,12 +891,13 @@ def _act_code(act):
 def _as_rows(t, width, what):
     """[..., width] as rows of channels -> (tensor that owns the memory, row stride in elements, rows).  Leading axes that do not
     collapse to one stride, rows that overlap (an expanded gradient) or strided channels are copied."""
-    if t.dim() < 1 or t.shape[-1] != width:
-        raise BitswapHipError(f"{what}: expected [..., {width}], got {tuple(t.shape)}")
+    shape = t.shape
+    if not shape or shape[-1] != width:
+        raise BitswapHipError(f"{what}: expected [..., {width}], got {tuple(shape)}")
     if t.is_contiguous():
         return t, width, t.numel() // width
     rows = 1
-    for n in t.shape[:-1]:
+    for n in shape[:-1]:
         rows *= n
     axes = [(n, st) for n, st in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
     ld = axes[-1][1] if axes else width
@@ -907,9 +912,10 @@ def _as_rows(t, width, what):
 def _affine(name, v, n, like):
     if v is None:
         return None, 0
-    if tuple(v.shape) != (n,) or v.dtype not in (torch.float32, like.dtype):
-        raise BitswapHipError(f"{name}: expected [{n}] of float32 or {like.dtype}, got {tuple(v.shape)} {v.dtype}")
-    return v.contiguous(), _DTYPES[v.dtype]
+    dtype = v.dtype
+    if v.shape != (n,) or (dtype != torch.float32 and dtype != like.dtype):
+        raise BitswapHipError(f"{name}: expected [{n}] of float32 or {like.dtype}, got {tuple(v.shape)} {dtype}")
+    return v.contiguous(), _DTYPES[dtype]
 
 
 class Packed8:
@@ -986,20 +992,21 @@ def linear_act(x, w, bias=None, res=None, act=ACT_ELU, want_sum=False, want_act=
     there are (include/bitswap_hip.h, bs_linear_act)."""
     dev = _gpu(x, w, bias, res)
     code, act = _dtype_code(x, "linear_act"), _act_code(act)
-    if w.dim() != 2 or w.dtype != x.dtype or w.shape[0] < 1 or w.shape[1] < 1:
-        raise BitswapHipError(f"linear_act: w must be [N, K] of {x.dtype}, got {tuple(w.shape)} {w.dtype}")
+    dtype, wshape = x.dtype, w.shape
+    if len(wshape) != 2 or w.dtype != dtype or 0 in wshape:
+        raise BitswapHipError(f"linear_act: w must be [N, K] of {dtype}, got {tuple(wshape)} {w.dtype}")
     if not (want_sum or want_act):
         raise BitswapHipError("linear_act: nothing is asked for")
-    N, K = w.shape
+    N, K = wshape
     xt, ldx, rows = _as_rows(x, K, "linear_act x")
-    wt, ldw, _ = _as_rows(w, K, "linear_act w")
+    wt, ldw = (w, K) if w.is_contiguous() else _as_rows(w, K, "linear_act w")[:2]
     bias, bcode = _affine("linear_act bias", bias, N, x)
-    shape = tuple(x.shape[:-1]) + (N,)
+    shape = (*x.shape[:-1], N)
     rt, ldr = None, 0
     if res is not None:
-        if tuple(res.shape) != shape or res.dtype != x.dtype:
-            raise BitswapHipError(f"linear_act: res must be {shape} of {x.dtype}, got {tuple(res.shape)} {res.dtype}")
-        rt, ldr, _ = _as_rows(res, N, "linear_act res")
+        if res.shape != shape or res.dtype != dtype:
+            raise BitswapHipError(f"linear_act: res must be {shape} of {dtype}, got {tuple(res.shape)} {res.dtype}")
+        rt, ldr = (res, N) if res.is_contiguous() else _as_rows(res, N, "linear_act res")[:2]
     s = x.new_empty(shape) if want_sum else None
     y = x.new_empty(shape) if want_act else None
     nb = _workspace_bytes("bs_linear_workspace", code, rows, K, N, _whole(xt, ldx, K, x.element_size()))
@@ -1081,14 +1088,15 @@ def linear_act_grad(x, w, s=None, act=ACT_NONE, g_sum=None, g_act=None, want_x=T
 
 def _as_images(t, what):
     """[n, ..., C] channels last -> (tensor that owns the memory, image stride, pixel stride, n, pixels, C)."""
-    if t.dim() < 2 or t.shape[-1] < 1:
-        raise BitswapHipError(f"{what}: expected [n, ..., C], got {tuple(t.shape)}")
-    n, C = t.shape[0], t.shape[-1]
+    shape = t.shape
+    if len(shape) < 2 or shape[-1] < 1:
+        raise BitswapHipError(f"{what}: expected [n, ..., C], got {tuple(shape)}")
+    n, C = shape[0], shape[-1]
     if t.is_contiguous() and n:
         pixels = t.numel() // (n * C)
         return t, pixels * C, C, n, pixels, C
     pixels = 1
-    for k in t.shape[1:-1]:
+    for k in shape[1:-1]:
         pixels *= k
     axes = [(k, st) for k, st in zip(t.shape[1:-1], t.stride()[1:-1]) if k != 1]
     ldp = axes[-1][1] if axes else C
