@@ -536,6 +536,14 @@ __global__ __launch_bounds__(256) void k_lay_w(const char* __restrict__ w, int64
     }
 }
 
+// the same for 16-bit w [P, K] in whole aligned chunks: nothing to turn, a thread moves one chunk of 8 k
+__global__ __launch_bounds__(256) void k_lay_chunks(const char* __restrict__ w, int64_t ldw, int P, int K, char* __restrict__ out) {
+    constexpr int KB = kb_of(BS_DT_BF16);
+    const int p = blockIdx.y * 32 + (threadIdx.x >> 3), k = blockIdx.x * 64 + (threadIdx.x & 7) * 8;
+    if (p >= P) return;
+    *reinterpret_cast<u32x4*>(out + (((int64_t)k / KB * P + p) * KB + k % KB) * 2) = k < K ? load16(w + (p * ldw + k) * 2) : u32x4{0, 0, 0, 0};
+}
+
 // ---- dw -------------------------------------------------------------------------------------------------------------------------
 struct OverArgs {
     const char *x, *ds;                // as the caller holds them
@@ -940,6 +948,7 @@ __global__ __launch_bounds__(256) void k_add_parts(const float* __restrict__ par
 }
 
 // ---- which way --------------------------------------------------------------------------------------------------------------------
+constexpr int MAX_WIDTH = 1 << 20;
 constexpr int RELAY_TILES = 256, MID_TILES = 256, BIG_TILES = 384, DEEP_K = 512;
 int64_t tiles_of(int64_t rows, int N, int bq, int bp) { return (rows + bq - 1) / bq * ((N + bp - 1) / bp); }
 bool few(int64_t rows, int N) { return tiles_of(rows, N, 32, 32) <= RELAY_TILES; }
@@ -979,12 +988,14 @@ int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream
     const bool as_is = DT != BS_DT_F32 && !a.wt && a.K % 64 == 0 && a.ldw % 8 == 0 && ((uintptr_t)a.w & 15) == 0 && a.ldw < (1 << 21);
     const int64_t need = rows_bytes(DT, a.rows, a.K, a.N, a.wt, whole);
     if (need > 0 && (!workspace || bytes < need)) return BS_EINVAL;
+    if (a.K > MAX_WIDTH || a.N > MAX_WIDTH) return BS_EINVAL;          // 31-bit offsets into a tile's rows, and the grids below
     const bool lay = a.wt || (!small && (big || !as_is));
     if (lay) {
         const dim3 grid((unsigned)(kp / 32), (unsigned)((a.N + 31) / 32));
         constexpr int KB = kb_of(DT);
-        if (a.N > (1 << 21)) return BS_EINVAL;                       // (grid, and 31-bit offsets into w)
-        if (a.wt) hipLaunchKernelGGL((k_lay_w<DT, true>), grid, dim3(256), 0, st, a.w, a.ldw, a.N, a.K, kp, (char*)workspace);
+        const bool chunks = DT != BS_DT_F32 && !a.wt && a.K % 8 == 0 && a.ldw % 8 == 0 && ((uintptr_t)a.w & 15) == 0;
+        if (chunks) hipLaunchKernelGGL(k_lay_chunks, dim3((unsigned)(kp / 64), (unsigned)((a.N + 31) / 32)), dim3(256), 0, st, a.w, a.ldw, a.N, a.K, (char*)workspace);
+        else if (a.wt) hipLaunchKernelGGL((k_lay_w<DT, true>), grid, dim3(256), 0, st, a.w, a.ldw, a.N, a.K, kp, (char*)workspace);
         else hipLaunchKernelGGL((k_lay_w<DT, false>), grid, dim3(256), 0, st, a.w, a.ldw, a.N, a.K, kp, (char*)workspace);
         a.wl = (const char*)workspace; a.sp = KB; a.sl = (int64_t)a.N * KB; a.sk = a.sl * limbs_of(DT);
     } else {
@@ -1077,7 +1088,7 @@ int launch_over(OverArgs a, const float* steps, int64_t ld, hipStream_t st) {
 extern "C" {
 
 int64_t bs_linear_workspace(int dtype, int64_t rows, int K, int N, int whole) {
-    if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1) return BS_EINVAL;
+    if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1 || K > MAX_WIDTH || N > MAX_WIDTH) return BS_EINVAL;
     return rows_bytes(dtype, rows, K, N, false, whole != 0);
 }
 
@@ -1100,7 +1111,7 @@ int bs_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const 
 }
 
 int64_t bs_linear_grad_x_workspace(int dtype, int64_t rows, int K, int N, int whole) {
-    if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1) return BS_EINVAL;
+    if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1 || K > MAX_WIDTH || N > MAX_WIDTH) return BS_EINVAL;
     return rows_bytes(dtype, rows, N, K, true, whole != 0);
 }
 
@@ -1119,16 +1130,17 @@ int bs_linear_grad_x(const void* ds, int64_t ldds, int zeros, const void* w, int
 }
 
 int64_t bs_linear_grad_w_workspace(int dtype, int64_t rows, int K, int N, int codes, int x_whole, int ds_whole) {
-    if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1) return BS_EINVAL;
+    if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1 || K > MAX_WIDTH || N > MAX_WIDTH) return BS_EINVAL;
     return over_bytes(dtype, rows, K, N, codes != 0, x_whole != 0, ds_whole != 0).all();
 }
 
 int bs_linear_grad_w(const void* ds, int64_t ldds, int zeros, const void* x, const int8_t* x_exps, int64_t ldx, void* dw, int dtype,
                      int64_t rows, int K, int N, void* workspace, int64_t workspace_bytes, void* stream) {
-    if (bad_type(dtype) || rows < 0 || rows > (1 << 30) || K < 1 || N < 1 || !dw) return BS_EINVAL;
+    if (bad_type(dtype) || rows < 0 || rows > (1 << 30) || K < 1 || N < 1 || K > MAX_WIDTH || N > MAX_WIDTH || !dw) return BS_EINVAL;
     if (rows > 0 && (!ds || !x || ldds < N || ldx < K)) return BS_EINVAL;
     hipStream_t st = rows_stream(stream);
     const int64_t n = (int64_t)K * N;
+    if ((n + 63) / 64 > 0x7fffffff) return BS_EINVAL;
     const int es = esize(dtype), xe = x_exps ? 1 : es;
     const bool x_whole = whole_rows(x, ldx, K, xe, 0), ds_whole = whole_rows(ds, ldds, N, es, zeros);
     const OverBytes b = over_bytes(dtype, rows, K, N, x_exps != nullptr, x_whole, ds_whole);

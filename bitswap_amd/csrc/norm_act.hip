@@ -610,7 +610,7 @@ Plan plan(int dtype, int64_t n, int64_t pixels, int C, int G, int grad) {
 }
 
 int bad_norm(int dtype, int64_t n, int64_t pixels, int channels, int groups, int act) {
-    return bad_type(dtype) || n < 0 || n > MAX_ROWS || pixels < 0 || pixels > MAX_ROWS || channels < 1 || channels > (1 << 24) || groups < 1 ||
+    return bad_type(dtype) || n < 0 || n > MAX_ROWS || pixels < 0 || pixels > MAX_ROWS || channels < 1 || channels > (1 << 20) || n > MAX_ROWS / channels || groups < 1 ||
            channels % groups || act < BS_ACT_NONE || act > BS_ACT_GELU;
 }
 

@@ -142,6 +142,7 @@ int bs_pack8(const void* x, int64_t ldx, int8_t* codes, int8_t* exps, int dtype,
     if (rows == 0) return BS_OK;
     if (!x || !codes || !exps || ldx < channels) return BS_EINVAL;
     const int nb = (channels + P8_BLOCK - 1) / P8_BLOCK;
+    if (rows > MAX_ROWS / nb) return BS_EINVAL;
     const int64_t threads = rows * nb * (dtype == BS_DT_F32 ? 8 : 4), blocks = (threads + 255) / 256;
     if (blocks > 0x7fffffff) return BS_EINVAL;
     hipStream_t st = rows_stream(stream);
@@ -158,6 +159,7 @@ int bs_unpack8(const int8_t* codes, const int8_t* exps, void* x, int dtype, int6
     if (rows == 0) return BS_OK;
     if (!x || !codes || !exps) return BS_EINVAL;
     const int nb = (channels + P8_BLOCK - 1) / P8_BLOCK, V = dtype == BS_DT_F32 ? 4 : 8, cpr = (channels + V - 1) / V;
+    if (rows > MAX_ROWS / cpr) return BS_EINVAL;
     const int64_t blocks = (rows * cpr + 255) / 256;
     if (blocks > 0x7fffffff) return BS_EINVAL;
     hipStream_t st = rows_stream(stream);

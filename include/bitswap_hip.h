@@ -356,15 +356,16 @@ int bs_wino_out_f32(const float* M, const float* bias, const float* res, float* 
  *   sum_out = s, act_out = a, contiguous [rows, N] (each nullable, at least one).  act sees s before its rounding.  float32
  *   operands are split into three bfloat16 limbs and multiplied as six limb products (as bs_wino_gemm_bf16x3); a sum that does
  *   not come out finite is added up again in float32, so infinities and NaN arrive as they do in float32 arithmetic.  A row's
- *   bits do not depend on `rows`.
+ *   bits do not depend on `rows`.  K, N <= 2^20, here and in the gradients.
  *
  * Workspaces: the *_workspace functions give the bytes a call needs (0: none) for w laid out for the kernel, copies of rows that are
  *   not whole, partial sums.  whole: the operand's address, row stride and row are multiples of 16 bytes and the stride is under 4
  *   MiB; rows that are not are copied first.  zeros (of ds): the rows end in zeros up to the next multiple of 16 bytes, which lies
  *   within their stride, as bs_act_grad writes them -- such rows count as whole.
  *
- * bs_act_grad -- ds = g_sum + g_act act'(s) (either gradient nullable, not both), rows [rows, N]: ds_out (row stride ldds, nullable; where ldds has the room its rows end in zeros up to the next multiple of 16 bytes),
- *   db_out [N] float32 = sum over the rows of ds before its rounding (nullable; workspace of bs_act_grad_workspace bytes then).
+ * bs_act_grad -- ds = g_sum + g_act act'(s) (either gradient nullable, not both), rows [rows, N]: ds_out (row stride ldds,
+ *   nullable; where ldds has the room its rows end in zeros up to the next multiple of 16 bytes), db_out [N] float32 = sum over
+ *   the rows of ds before its rounding (nullable; workspace of bs_act_grad_workspace bytes then).
  *   s: [rows, N] of dtype (row stride lds), or, if s_exps is given, int8 codes [rows, N] with their exponents (bs_pack8).
  *   act BS_ACT_NONE: s is not read and may be null.
  * bs_linear_grad_x -- dx [rows, K] = ds w;  ds [rows, N] (row stride ldds), w [N, K].
@@ -375,14 +376,15 @@ int bs_wino_out_f32(const float* M, const float* bias, const float* res, float* 
  * bs_group_norm_act -- x [n, pixels, channels] (strides ldn, ldp), groups dividing channels: mean and biased variance over the
  *   pixels and channels of a group, u = (x - mean) / sqrt(var + eps) * gamma + beta, y = act(u), y contiguous; stats
  *   [n, groups, 2] float32 = (mean, 1 / sqrt(var + eps)) (nullable).  An image's bits do not depend on n.
- *   workspace: bs_group_norm_workspace bytes (0 for images that fit a workgroup's registers).
+ *   channels <= 2^20.  workspace: bs_group_norm_workspace bytes (0 for images that fit a workgroup's registers).
  * bs_group_norm_act_grad -- with h = (x - mean) rstd, du = g act'(h gamma + beta), t = du gamma:
  *   dx = rstd (t - mean_g(t) - h mean_g(t h)), dgamma = sum du h, dbeta = sum du (float32 [channels], each nullable).
  *   x [n, pixels, channels] of dtype, or codes of bs_pack8 over [n * pixels, channels] if x_exps is given.
  *
  * bs_pack8 -- x [rows, channels] -> codes int8 [rows, channels] and exps int8 [rows, ceil(channels / 32)]: 32 channels of a row
  *   share 2^e, e the smallest integer >= -126 with max|x| <= 127 2^e, at most 121 (float16: 9: 127 2^e stays a value of the type);
- *   code = rint(x 2^-e) (ties to even) within +-127; -128 marks a value that is not finite (left out of the maximum).  bs_unpack8 -- x = code 2^e, exact in every dtype that held x; -128 gives NaN.
+ *   code = rint(x 2^-e) (ties to even) within +-127; -128 marks a value that is not finite (left out of the maximum).
+ *   bs_unpack8 -- x = code 2^e, exact in every dtype that held x; -128 gives NaN.
  *
  * All of them: BS_EINVAL for null operands, negative sizes, strides below the row length, unknown types or activations, a
  * workspace that is too small; rows == 0 or n == 0 is a call without rows (gradients of parameters are then zero).

@@ -145,3 +145,19 @@ def test_stream_record_names_the_pointwise_layers():
     assert r["point"] == {"layers": 2, "rev": meta.POINT_REV}
     with pytest.raises(meta.StreamMismatch):
         meta.check({"conv_route": r}, {"conv_route": meta.route(Model(**kw))})
+
+
+def test_rows_wider_than_the_kernels_offsets_are_refused(L):
+    from bitswap_amd import hip
+    keep, p = buf()
+    E, wide = hip.EINVAL, (1 << 20) + 1
+    for k, n in ((wide, 8), (8, wide)):
+        assert L.bs_linear_workspace(0, 4, k, n, 1) < 0 and L.bs_linear_grad_x_workspace(0, 4, k, n, 1) < 0
+        assert L.bs_linear_grad_w_workspace(0, 4, k, n, 0, 1, 1) < 0
+        assert L.bs_linear_act(p, k, p, k, None, 0, None, 0, p, None, 0, 0, 4, k, n, p, 1 << 40, None) == E
+        assert L.bs_linear_grad_x(p, n, 0, p, k, p, 0, 4, k, n, p, 1 << 40, None) == E
+        assert L.bs_linear_grad_w(p, n, 0, p, None, k, p, 0, 4, k, n, p, 1 << 40, None) == E
+    assert L.bs_linear_workspace(0, 4, 1 << 20, 8, 1) >= 0
+    assert L.bs_group_norm_workspace(0, 1, 8, wide, 1, 0) < 0 and L.bs_group_norm_workspace(0, 1 << 40, 8, 8, 1, 1) < 0
+    assert L.bs_pack8(p, 1 << 30, p, p, 0, 1 << 40, 1 << 30, None) == E and L.bs_unpack8(p, p, p, 0, 1 << 40, 1 << 30, None) == E
+    del keep

@@ -758,3 +758,30 @@ def test_codec_with_pointwise_layers_is_lossless_and_batch_invariant(hip, small)
         one = h.RansState.from_lists([words[b]], cap=state.cap)
         out = codec.decompress(one, 2)
         assert torch.equal(out.cpu()[0], images[b])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,n", [(8300, 520, 500), (8300, 517, 500), (24700, 72, 1010)])
+def test_linear_act_in_the_largest_tiles(hip, rows, k, n, dtype):
+    x, w, b, r = randn((rows, k), dtype, 1), randn((n, k), dtype, 2, k ** -0.5), randn((n,), dtype, 3), randn((rows, n), dtype, 4)
+    check_linear(hip, x, w, b, r, 2)
+    check_linear(hip, x, randn((n, k + 8), dtype, 2, k ** -0.5)[:, 8:], None, None, 1, want_sum=False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k,n", [(600, 500), (72, 1010), (1030, 300)])
+def test_linear_act_row_bits_through_every_tile(hip, k, n, dtype):
+    """One row, a few, and as many as fill each size of tile: the same bits wherever a row lies."""
+    x, w, b = randn((24700, k), dtype, 1), randn((n, k), dtype, 2, k ** -0.5), randn((n,), dtype, 3)
+    whole = hip.linear_act(x, w, b, act=1)[1]
+    for rows in (1, 40, 700, 2100, 4200, 9000, 17000):
+        assert torch.equal(hip.linear_act(x[:rows], w, b, act=1)[1], whole[:rows]), rows
+        assert torch.equal(hip.linear_act(x[-rows:], w, b, act=1)[1], whole[-rows:]), rows
+
+
+@pytest.mark.parametrize("saved8", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,n", [(24000, 300, 300), (24001, 304, 260)])
+def test_linear_act_grad_in_the_largest_tiles(hip, rows, k, n, dtype, saved8):
+    check_linear_grad(hip, randn((rows, k), dtype, 1), randn((n, k), dtype, 2, k ** -0.5), randn((rows, n), dtype, 5), 1, randn((rows, n), dtype, 6),
+                      randn((rows, n), dtype, 7), saved8)
