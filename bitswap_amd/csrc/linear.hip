@@ -984,7 +984,7 @@ int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream
     constexpr int ES = esize(DT), CK = 16 / ES;
     const int kp = (a.K + 63) / 64 * 64;
     const bool small = few(a.rows, a.N), whole = whole_rows(a.x, a.ldx, a.K, ES, zeros);
-    const bool big = DT != BS_DT_F32 && a.N > 128 && tiles_of(a.rows, a.N, 256, 256) >= BIG_TILES;
+    const bool big = DT != BS_DT_F32 && a.K >= DEEP_K && a.N > 128 && tiles_of(a.rows, a.N, 256, 256) >= BIG_TILES;
     const bool as_is = DT != BS_DT_F32 && !a.wt && a.K % 64 == 0 && a.ldw % 8 == 0 && ((uintptr_t)a.w & 15) == 0 && a.ldw < (1 << 21);
     const int64_t need = rows_bytes(DT, a.rows, a.K, a.N, a.wt, whole);
     if (need > 0 && (!workspace || bytes < need)) return BS_EINVAL;
@@ -1025,9 +1025,9 @@ int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream
         else ROWS(64, 64, 32, 32, 32, 4, 1);
     } else {
         if (big) ROWS(256, 256, 128, 64, 32, 4, 1);
-        else if (tiles_of(a.rows, a.N, 128, 128) >= MID_TILES && a.N > 64) ROWS(128, 128, 64, 64, 32, 4, 1);
+        else if (tiles_of(a.rows, a.N, 128, 128) >= MID_TILES && a.N > 64) ROWS(128, 128, 32, 64, 32, 3, 4);
         else if (tiles_of(a.rows, a.N, 128, 64) >= 2 * MID_TILES && a.N <= 64) ROWS(128, 64, 32, 64, 32, 4, 1);
-        else ROWS(64, 64, 32, 64, 32, 4, 1);
+        else ROWS(64, 64, 32, 32, 32, 4, 1);
     }
 #undef ROWS
     return rows_rc();
