@@ -113,13 +113,13 @@ __device__ __forceinline__ void finish(const RowsArgs& a, int64_t q, int64_t p, 
 #pragma unroll
             for (int e = 0; e < V; ++e) v[e] += t[e];
         }
-        if (a.sum) store_vec<DT>(a.sum + at, n, v);
+        if (a.sum) store_out<DT>(a.sum + at, n, v, a.N);
         if (a.act_out) {
             act_values<DT, V>(a.act, v, t);
-            store_vec<DT>(a.act_out + at, n, t);
+            store_out<DT>(a.act_out + at, n, t, a.N);
         }
     } else {
-        store_vec<DT>(a.sum + at, n, v);
+        store_out<DT>(a.sum + at, n, v, a.N);
     }
 }
 template <int DT>

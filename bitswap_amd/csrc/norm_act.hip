@@ -260,7 +260,7 @@ __global__ __launch_bounds__(1024) void k_norm(const NormArgs a) {
 #pragma unroll
         for (int i = 0; i < V; ++i) f[r][i] = fmaf((f[r][i] - m[i]) * rs[i], ga[i], be[i]);
         act_values<DT, V>(a.act, f[r], f[r]);
-        store_vec<DT>(yp + p * a.C * ES, left, f[r]);
+        store_out<DT>(yp + p * a.C * ES, left, f[r], a.C);
     }
 }
 
@@ -379,7 +379,7 @@ __global__ __launch_bounds__(512) void k_norm_grad(const NormArgs a) {
             if (p >= a.pixels) break;
 #pragma unroll
             for (int i = 0; i < V; ++i) d[r][i] = rs[i] * (fmaf(d[r][i], ga[i], -m1[i]) - h[r][i] * m2[i]);
-            store_vec<DT>(yp + p * a.C * ES, left, d[r]);
+            store_out<DT>(yp + p * a.C * ES, left, d[r], a.C);
         }
     }
     if (LANES && po) {                                               // the channels' sums over the pixels, while dx is on its way out
@@ -558,7 +558,7 @@ __global__ __launch_bounds__(256) void k_apply(const NormArgs a, const float* __
         } else {
             act_values<DT, V>(a.act, u, f);
         }
-        store_vec<DT>(a.y + ((img * a.pixels + p) * a.C + c) * ES, left, f);
+        store_out<DT>(a.y + ((img * a.pixels + p) * a.C + c) * ES, left, f, a.C);
     }
 }
 

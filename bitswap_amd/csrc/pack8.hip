@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256) void k_unpack8(const int8_t* __restrict__ code
     const int c = (int)(t - row * cpr) * V;
     float f[V];
     load_codes<V>(codes + row * C, exps + row * nb, c, C - c, f);
-    store_vec<DT>(x + (row * C + c) * esize(DT), C - c, f);
+    store_out<DT>(x + (row * C + c) * esize(DT), C - c, f, C);
 }
 
 struct ActGradArgs {

@@ -122,6 +122,17 @@ __device__ __forceinline__ void store_vec(char* p, int n, const float* f) {
     }
 }
 
+// store_vec for an output that its launch does not read again, rows of `width` channels: past the L2 (nontemporal), where the inputs
+// that are read again stay.  Not for 16-bit rows that are no multiple of 64 bytes: lines written in two pieces cost more than is won
+// (25600x256 -> 264 bf16: 21.5 us kept, 23.5 us past; -> 288: 20.8 and 18.4; float32 102400x256 -> 256 131 and 110, -> 257 still 22.7
+// and 21.2).
+template <int DT>
+__device__ __forceinline__ void store_out(char* p, int n, const float* f, int width) {
+    typedef uint32_t u32x4_e __attribute__((ext_vector_type(4), aligned(2)));
+    if (n >= vlen(DT) && (DT == BS_DT_F32 || width % 32 == 0)) __builtin_nontemporal_store((u32x4_e)pack16<DT>(f), reinterpret_cast<u32x4_e*>(p));
+    else store_vec<DT>(p, n, f);
+}
+
 // ---- activations ----------------------------------------------------------------------------------------------------------
 // A layer's epilogue has tens of millions of these beside a product that is bound elsewhere; the library's expm1f and erff cost
 // more than the product itself (16384 x 2048 x 2048 with GELU: 226 us, 96 of them the product).  Here: one v_exp_f32 where a ratio
