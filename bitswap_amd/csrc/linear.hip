@@ -949,9 +949,28 @@ __global__ __launch_bounds__(256) void k_add_parts(const float* __restrict__ par
 
 // ---- which way --------------------------------------------------------------------------------------------------------------------
 constexpr int MAX_WIDTH = 1 << 20;
-constexpr int RELAY_TILES = 256, MID_TILES = 256, BIG_TILES = 384, DEEP_K = 512;
 int64_t tiles_of(int64_t rows, int N, int bq, int bp) { return (rows + bq - 1) / bq * ((N + bp - 1) / bp); }
-bool few(int64_t rows, int N) { return tiles_of(rows, N, 32, 32) <= RELAY_TILES; }
+// The tile of a product goes by how many tiles of a size there are for 256 compute units, and by K.  Both sides, in us, at
+// (rows, K, N):
+//   k_relay up to 256 tiles of 32x32 (16-bit) or 512 (float32), as its workgroups, a tile each, then have the chip for themselves:
+//     bf16  (256, 256, 256) 4.6, k_rows_dma 5.2   (512, 512, 512) 6.0 and 6.2    beyond: (1024, 256, 512) 5.9 and 5.4
+//     f32   (256, 1024, 1024) 18.6 and 27.3       (1024, 256, 512) 9.4 and 12.0  beyond: (2048, 256, 512) 15.9 and 12.6
+bool few(int dtype, int64_t rows, int N) { return tiles_of(rows, N, 32, 32) <= (dtype == BS_DT_F32 ? 512 : 256); }
+//   128 channels across (16-bit 128x128, float32 64x128) from 256 tiles on, 64x64 below and for N <= 64:
+//     bf16  (8192, 512, 512), 256 tiles, 10.9 and 12.6      (2048, 256, 512), 64 tiles, 8.3 and 5.7
+//     f32   (4096, 512, 1024), 512 tiles, 38.3 and 40.4     (1024, 512, 512), 64 tiles, 21.7 and 16.0
+bool enough(int64_t rows, int N, int bq, int bp) { return tiles_of(rows, N, bq, bp) >= 256; }
+//   the largest tile (16-bit 256x256, one workgroup a compute unit; float32 128x128, two) where K is long enough to pay for its
+//   start and end, which nothing covers:
+//     bf16  (16384, 2048, 2048) 145 and 168                 (102400, 256, 256) 50 and 43
+//     f32   (4942, 832, 1168) 74 and 84                     (102400, 256, 256) 105 and 103,  (8192, 256, 512) 24.3 and 21.4
+constexpr int DEEP_K = 512;
+//   and, 16-bit, where its tiles fill four fifths of the rounds that they take:
+//     (16384, 1024, 1024), 256 tiles, 46 and 50             (12288, 512, 1024), 192 tiles, 29 and 23
+bool fills(int64_t rows, int N) {
+    const int64_t tiles = tiles_of(rows, N, 256, 256), rounds = (tiles + 255) / 256;
+    return N > 128 && tiles * 5 >= rounds * 256 * 4;
+}
 
 int64_t lay_bytes(int dtype, int K, int P) { return ((int64_t)limbs_of(dtype) * P * ((K + 63) / 64 * 64) * 2 + 255) / 256 * 256; }
 int64_t pad_bytes(int es, int64_t rows, int K) { return (rows * (((int64_t)K * es + 15) / 16) * 16 + 255) / 256 * 256; }
@@ -976,20 +995,20 @@ int pad(int es, const void* in, int64_t ld, int64_t rows, int K, char* out, hipS
 
 // out [rows, N] over K: w [N, K], or [K, N] when turned; zeros: rows of x end in zeros up to whole chunks
 int64_t rows_bytes(int dtype, int64_t rows, int K, int N, bool turned, bool whole) {
-    const bool small = few(rows, N);
+    const bool small = few(dtype, rows, N);
     return (turned || !small ? lay_bytes(dtype, K, N) : 0) + (small || whole ? 0 : pad_bytes(esize(dtype), rows, K));
 }
 template <int DT, int EPI>
 int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream_t st) {
     constexpr int ES = esize(DT), CK = 16 / ES;
     const int kp = (a.K + 63) / 64 * 64;
-    const bool small = few(a.rows, a.N), whole = whole_rows(a.x, a.ldx, a.K, ES, zeros);
-    const bool big = DT != BS_DT_F32 && a.K >= DEEP_K && a.N > 128 && tiles_of(a.rows, a.N, 256, 256) >= BIG_TILES;
+    const bool small = few(DT, a.rows, a.N), whole = whole_rows(a.x, a.ldx, a.K, ES, zeros);
+    const bool big = DT != BS_DT_F32 && a.K >= DEEP_K && fills(a.rows, a.N);
     const bool as_is = DT != BS_DT_F32 && !a.wt && a.K % 64 == 0 && a.ldw % 8 == 0 && ((uintptr_t)a.w & 15) == 0 && a.ldw < (1 << 21);
     const int64_t need = rows_bytes(DT, a.rows, a.K, a.N, a.wt, whole);
     if (need > 0 && (!workspace || bytes < need)) return BS_EINVAL;
     if (a.K > MAX_WIDTH || a.N > MAX_WIDTH) return BS_EINVAL;          // 31-bit offsets into a tile's rows, and the grids below
-    const bool lay = a.wt || (!small && (big || !as_is));
+    const bool lay = a.wt || (!small && !as_is);
     if (lay) {
         const dim3 grid((unsigned)(kp / 32), (unsigned)((a.N + 31) / 32));
         constexpr int KB = kb_of(DT);
@@ -1020,28 +1039,33 @@ int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream
         const int64_t blocks = (a.tiles + 7) / 8 * 8; if (blocks > 0x7fffffff) return BS_EINVAL; \
         hipLaunchKernelGGL((k_rows_dma<DT, EPI, BQ, BP, WQ, WP, BK, NS, PS>), dim3((unsigned)blocks), dim3((BQ / WQ) * (BP / WP) * 64), 0, st, a); } while (0)
     if constexpr (DT == BS_DT_F32) {
-        if (a.K >= DEEP_K && a.N > 64 && tiles_of(a.rows, a.N, 128, 128) >= MID_TILES) ROWS(128, 128, 64, 64, 16, 3, 2);
-        else if (tiles_of(a.rows, a.N, 64, 128) >= MID_TILES && a.N > 64) ROWS(64, 128, 32, 64, 16, 3, 3);
+        if (a.K >= DEEP_K && a.N > 64 && enough(a.rows, a.N, 128, 128)) ROWS(128, 128, 64, 64, 16, 3, 2);
+        else if (a.N > 64 && enough(a.rows, a.N, 64, 128)) ROWS(64, 128, 32, 64, 16, 3, 3);
         else ROWS(64, 64, 32, 32, 32, 4, 1);
     } else {
         if (big) ROWS(256, 256, 128, 64, 32, 4, 1);
-        else if (tiles_of(a.rows, a.N, 128, 128) >= MID_TILES && a.N > 64) ROWS(128, 128, 32, 64, 32, 3, 4);
-        else if (tiles_of(a.rows, a.N, 128, 64) >= 2 * MID_TILES && a.N <= 64) ROWS(128, 64, 32, 64, 32, 4, 1);
+        else if (a.N > 64 && enough(a.rows, a.N, 128, 128)) ROWS(128, 128, 32, 64, 32, 3, 4);
         else ROWS(64, 64, 32, 32, 32, 4, 1);
     }
 #undef ROWS
     return rows_rc();
 }
 
-// How a weight gradient is cut: tiles of 256 x 128 (16-bit) or 128 x 128 (float32) outputs where there are enough, else 64 x 128, and the rows into as many parts as
-// give the chip two workgroups a compute unit, none under 128 rows.
+// How a weight gradient is cut: tiles of 256 x 128 (16-bit) or 128 x 128 (float32) outputs where these and parts of 256 rows come to
+// two workgroups a compute unit, else of 64 x 128; the rows into as many parts as give a compute unit two (large tiles) or one (small
+// ones: what more parts win the join of them costs again), none under 128 rows.  Both sides, in us, at (rows, K, N):
+//   large tiles   bf16 from codes (65536, 512, 1024) 102 and 179    f32 (8192, 1024, 1024) 113 and 124
+//                 below: bf16 (8192, 512, 512) 30 and 22            f32 (2048, 256, 256) 16.5 and 12.8
+//   parts, large  two a compute unit 102, one 126, four 126 (bf16 from codes (65536, 512, 1024))
+//   parts, small  one a compute unit 12.7, two 17.2 (bf16 (8192, 256, 256)); under 512 rows allowed 12.7, not allowed 22.2 (f32 (2048, 256, 256))
 int over_bq(int dtype, int64_t rows, int K, int N) {
     const int big = dtype == BS_DT_F32 ? 128 : 256;
     return 2 * N > big && tiles_of(N, K, big, 128) * ((rows + 255) / 256) >= 512 ? big : 64;
 }
 void split_rows(int dtype, int64_t rows, int K, int N, int64_t* part, int64_t* parts) {
-    const int64_t tiles = tiles_of(N, K, over_bq(dtype, rows, K, N), 128);
-    int64_t want = (512 + tiles - 1) / tiles;
+    const int bq = over_bq(dtype, rows, K, N);
+    const int64_t tiles = tiles_of(N, K, bq, 128), groups = bq == 64 ? 256 : 512;
+    int64_t want = (groups + tiles - 1) / tiles;
     const int64_t most = (rows + 127) / 128;
     if (want > most) want = most;
     if (want < 1) want = 1;
