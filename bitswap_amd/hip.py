@@ -1050,10 +1050,12 @@ def linear_act_grad(x, w, s=None, act=ACT_NONE, g_sum=None, g_act=None, want_x=T
             raise BitswapHipError("linear_act_grad: the gradient of w needs the saved input x")
         xt, xe, ldx = _saved_rows(x, K, w.dtype, rows, "linear_act_grad x")
     L = load()
-    # one gradient and no slope: it is ds already
-    made = sloped or (g_sum is not None and g_act is not None)
-    need_ds = want_x or want_w or want_res
     es = w.element_size()
+    # one gradient and no slope: it is ds already.  But dw needs whole rows of it, and dx takes those too: where they are not, the
+    # launch that adds up db copies them
+    changed = sloped or (g_sum is not None and g_act is not None)
+    made = changed or (want_w and not _whole(*next(g for g in gs if g[0] is not None), N, es))
+    need_ds = want_x or want_w or (want_res and changed)
     ds, ldd = None, -(-N * es // 16) * 16 // es           # ds in rows of whole 16-byte chunks (a strided view where N is not one)
     if made and need_ds:
         ds = w.new_empty(tuple(g0.shape[:-1]) + (ldd,))
@@ -1065,7 +1067,7 @@ def linear_act_grad(x, w, s=None, act=ACT_NONE, g_sum=None, g_act=None, want_x=T
         _check(L.bs_act_grad(_at(gs[0][0]), gs[0][1], _at(gs[1][0]), gs[1][1], _at(st), _at(se), lds, act, code, rows, N, _at(ds),
                              ldd, _at(db), _at(ws), nb, _raw_stream(dev)), "bs_act_grad")
     if ds is not None:
-        dt, zeros, ds_whole = ds, 1, 1
+        dt, zeros, ds_whole = ds, 1, int(ldd * es < 1 << 22)
     else:
         dt, ldd = gs[0] if g_sum is not None else gs[1]
         zeros, ds_whole = 0, _whole(dt, ldd, N, es)
@@ -1083,7 +1085,7 @@ def linear_act_grad(x, w, s=None, act=ACT_NONE, g_sum=None, g_act=None, want_x=T
         ws = _scratch(w, nb)
         _check(L.bs_linear_grad_w(_at(dt), ldd, zeros, _at(xt), _at(xe), ldx, _at(dw), code, rows, K, N, _at(ws), nb, _raw_stream(dev)),
                "bs_linear_grad_w")
-    return dx, dw, db, ((ds if ds is not None else g0) if want_res else None)
+    return dx, dw, db, ((ds if changed else g0) if want_res else None)
 
 
 def _as_images(t, what):

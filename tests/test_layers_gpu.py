@@ -785,3 +785,16 @@ def test_linear_act_row_bits_through_every_tile(hip, k, n, dtype):
 def test_linear_act_grad_in_the_largest_tiles(hip, rows, k, n, dtype, saved8):
     check_linear_grad(hip, randn((rows, k), dtype, 1), randn((n, k), dtype, 2, k ** -0.5), randn((rows, n), dtype, 5), 1, randn((rows, n), dtype, 6),
                       randn((rows, n), dtype, 7), saved8)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_act_grad_of_one_plain_gradient_in_rows_that_are_not_whole(hip, dtype):
+    """No slope and one gradient: ds is the gradient, which comes back as dres itself however its rows lie."""
+    for rows, k, n in ((2151, 25, 57), (40, 16, 61), (1, 8, 1)):
+        x, w = randn((rows, k), dtype, 1), randn((n, k), dtype, 2)
+        for g in (randn((rows, n), dtype, 3), randn((rows, n + 5), dtype, 3)[:, 2:2 + n], randn((1, n), dtype, 3).expand(rows, n)):
+            dr = check_linear_grad(hip, x, w, randn((rows, n), dtype, 4), 0, g, None, False)[3]
+            assert dr is g
+            dx, dw, db, dr = hip.linear_act_grad(x, w, g_sum=g, want_x=False, want_bias=False)
+            assert dx is None and db is None and dr is None
+            close(dw, g.double().t() @ x.double(), (rows + 8 + 2 / E * U[dtype]) * E * (g.double().abs().t() @ x.double().abs()) + TINY[dtype], "dw")
