@@ -6,10 +6,15 @@
 //
 // Bound by memory: x (and g) in, y (dx) out.  Where the pixels of a few whole groups fit a workgroup's registers (k_norm,
 // k_norm_grad) everything is read once: a thread keeps 32 elements (V neighbouring channels of 32 / V pixels), sums go over its
-// pixels, then over the workgroup's pixel lanes and a group's channels through shared memory, the variance as the mean squared
-// distance from the mean already known.  Larger images (k_part_* / k_stats / k_apply*) are cut into runs of pixels whose
-// per-channel sums are joined in a second launch and applied in a third.  Which way is taken, and every order of addition, follows
-// from (pixels, channels, groups, type) alone: an image's bits do not depend on how many there are.
+// pixels, then over the workgroup's pixel lanes and a group's channels, by exchanges between lanes where channels and pixels divide
+// into powers of two, else through shared memory; the variance is the mean squared distance from the mean already known.  Larger
+// images (k_part, k_join, k_apply) are cut into runs of pixels whose per-channel sums are joined in a second launch and applied in a
+// third.  Which way is taken, and every order of addition, follows from (pixels, channels, groups, type) alone: an image's bits do
+// not depend on how many there are.
+//
+// Measured (256 x 256 images in 32 groups; the bytes in and out at 4.9 TB/s in brackets): bfloat16, 400 images 23.8 us [21.5];
+// float32, 100 images 9.3 us, their gradient 16.7 us and 3 for the parameters' [17]; one image 6.3 us, bound by the one workgroup's
+// load, reduction and store one after the other.
 #include "rows_dev.h"
 
 namespace {
@@ -275,8 +280,8 @@ __device__ __forceinline__ void load_x(const NormArgs& a, int64_t img, int64_t p
     }
 }
 
-template <int DT, bool SAVED8, bool LANES>
-__global__ __launch_bounds__(512) void k_norm_grad(const NormArgs a) {
+template <int DT, bool SAVED8, bool LANES, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_norm_grad(const NormArgs a) {
     constexpr int V = vlen(DT), R = 32 / V, ES = esize(DT);
     extern __shared__ __align__(16) float sh[];
     const int PL = a.pl, CL = a.cl, tid = threadIdx.x;
@@ -563,6 +568,14 @@ __global__ __launch_bounds__(256) void k_apply(const NormArgs a, const float* __
 }
 
 // ---- which way, and how it is cut --------------------------------------------------------------------------------------------
+// Both sides, in us, at (images, pixels, channels, groups); forward | gradient:
+//   registers against three launches   (400, 256, 256, 32) bf16 24 and 66 | 60 and 74    (1, 256, 256, 32) f32 6.3 and 29 | 10 and 34
+//     up to 1024 threads               (16, 1024, 256, 8) f32 gradient 17 and 44
+//     and 256 pixel lanes, a row of the workgroup under 64 bytes beyond:  (50, 3000, 32, 8) bf16 55 and 16 | 103 and 23
+//   exchanges against shared memory    (400, 256, 256, 32) bf16 24 and 39 | 60 and 70    (100, 1024, 64, 8) f32 12 and 26 | 20 and 35
+//   groups of a workgroup, until a row of it is 256 bytes or it has 512 threads:
+//     256 threads                      (400, 225, 60, 6) f32 16 and 11 | 24 and 19       (37, 289, 252, 28) f32 13 and 11.5 | 18 and 16.5
+//     1024 threads                     (400, 256, 256, 32) bf16 32 and 24                (1, 256, 256, 32) bf16 8.2 and 6.3
 struct Plan {
     bool fits, lanes;
     int pl, cl, gs, slabs, threads, lds;
@@ -573,7 +586,7 @@ struct Plan {
 
 Plan plan(int dtype, int64_t n, int64_t pixels, int C, int G, int grad) {
     Plan p = {};
-    const int V = dtype == BS_DT_F32 ? 4 : 8, R = 32 / V, per = C / G, cap = grad ? 512 : 1024;
+    const int V = dtype == BS_DT_F32 ? 4 : 8, R = 32 / V, per = C / G, cap = 1024;
     const int64_t need = (pixels + R - 1) / R;              // pixel lanes
     const int one = (per + V - 1) / V;                      // channel lanes of a group
     p.fits = need <= 256 && need * one <= cap;             // (longer columns would leave a row of the workgroup under 64 bytes)
@@ -583,7 +596,6 @@ Plan plan(int dtype, int64_t n, int64_t pixels, int C, int G, int grad) {
         while (up < need) up *= 2;
         p.lanes = per % V == 0 && pow2(one) && one <= 64 && up * one <= cap;
         p.pl = (int)(p.lanes ? up : need);
-        // groups of a workgroup: until a row of it is 256 bytes long or the workgroup has 512 threads
         int gs = 1;
         auto lanes_of = [&](int g) { return (g * per + V - 1) / V; };
         while (gs < G && lanes_of(gs) < 16) {
@@ -591,7 +603,6 @@ Plan plan(int dtype, int64_t n, int64_t pixels, int C, int G, int grad) {
             if (next > G || lanes_of(next) * p.pl > 512) break;
             gs = next;
         }
-        while (!p.lanes && gs > 1 && n * ((G + gs - 1) / gs) < 512) --gs;       // (changes no bit: no sum here crosses channel lanes)
         p.gs = gs;
         p.cl = lanes_of(gs);
         p.slabs = (G + gs - 1) / gs;
@@ -697,14 +708,17 @@ int bs_group_norm_act_grad(const void* g, int64_t ldgn, int64_t ldgp, const void
     if (blocks > 0x7fffffff || n * groups > 0x7fffffff) return BS_EINVAL;
     if (p.fits) {
         if (!dgamma && !dbeta) a.parts = nullptr;
-#define FIT(DT, P8) do { if (p.lanes) hipLaunchKernelGGL((k_norm_grad<DT, P8, true>), dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a); \
-                         else hipLaunchKernelGGL((k_norm_grad<DT, P8, false>), dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a); } while (0)
+        // (two builds: with the registers that 1024 threads leave, 512 of them take 25 us instead of 16, bfloat16, 37 images of 289 x 252)
+#define FIT_T(DT, P8, T) do { if (p.lanes) hipLaunchKernelGGL((k_norm_grad<DT, P8, true, T>), dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a); \
+                              else hipLaunchKernelGGL((k_norm_grad<DT, P8, false, T>), dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a); } while (0)
+#define FIT(DT, P8) do { if (p.threads > 512) FIT_T(DT, P8, 1024); else FIT_T(DT, P8, 512); } while (0)
 #define GO(DT) do { if (x_exps) FIT(DT, true); else FIT(DT, false); } while (0)
         if (dtype == BS_DT_F32) GO(BS_DT_F32);
         else if (dtype == BS_DT_BF16) GO(BS_DT_BF16);
         else GO(BS_DT_F16);
 #undef GO
 #undef FIT
+#undef FIT_T
     } else {
         float* const means = a.parts + n * p.runs * 2 * channels;
         const dim3 grid((unsigned)blocks, (unsigned)p.cly);

@@ -798,3 +798,18 @@ def test_linear_act_grad_of_one_plain_gradient_in_rows_that_are_not_whole(hip, d
             dx, dw, db, dr = hip.linear_act_grad(x, w, g_sum=g, want_x=False, want_bias=False)
             assert dx is None and db is None and dr is None
             close(dw, g.double().t() @ x.double(), (rows + 8 + 2 / E * U[dtype]) * E * (g.double().abs().t() @ x.double().abs()) + TINY[dtype], "dw")
+
+
+@pytest.mark.parametrize("saved8", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,pixels,c,groups", [(2, 1024, 256, 8), (2, 784, 100, 5), (1, 1000, 90, 3), (2, 256, 512, 8), (9, 225, 60, 6)])
+def test_group_norm_in_the_largest_workgroups(hip, n, pixels, c, groups, dtype, saved8):
+    """Groups that take more than 512 threads, and as many groups as 512 threads hold, in power-of-two lanes and in others."""
+    x, g = randn((n, pixels, c), dtype, 1), randn((n, pixels, c), dtype, 4)
+    gamma, beta = randn((c,), torch.float32, 2), randn((c,), torch.float32, 3)
+    check_norm_grad(hip, x, groups, gamma, beta, 2, g, saved8)
+    y = hip.group_norm_act(x, groups, gamma, beta, act=1)[0]
+    assert torch.equal(hip.group_norm_act(x[-1:], groups, gamma, beta, act=1)[0], y[-1:])
+    dx = [hip.group_norm_act_grad(x[i:], hip.group_norm_act(x[i:], groups, gamma, beta, act=1, want_stats=True)[1], groups, g[i:], gamma, beta, act=1)[0]
+          for i in (0, n - 1)]
+    assert torch.equal(dx[0][-1:], dx[1])
