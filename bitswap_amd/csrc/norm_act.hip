@@ -569,10 +569,10 @@ __global__ __launch_bounds__(256) void k_apply(const NormArgs a, const float* __
 
 // ---- which way, and how it is cut --------------------------------------------------------------------------------------------
 // Both sides, in us, at (images, pixels, channels, groups); forward | gradient:
-//   registers against three launches   (400, 256, 256, 32) bf16 24 and 66 | 60 and 74    (1, 256, 256, 32) f32 6.3 and 29 | 10 and 34
+//   registers against three launches   (400, 256, 256, 32) bf16 24 and 66 | 48 and 74    (1, 256, 256, 32) f32 6.3 and 29 | 10 and 34
 //     up to 1024 threads               (16, 1024, 256, 8) f32 gradient 17 and 44
 //     and 256 pixel lanes, a row of the workgroup under 64 bytes beyond:  (50, 3000, 32, 8) bf16 55 and 16 | 103 and 23
-//   exchanges against shared memory    (400, 256, 256, 32) bf16 24 and 39 | 60 and 70    (100, 1024, 64, 8) f32 12 and 26 | 20 and 35
+//   exchanges against shared memory    (400, 256, 256, 32) bf16 24 and 39 | 48 and 70    (100, 1024, 64, 8) f32 12 and 26 | 20 and 35
 //   groups of a workgroup, until a row of it is 256 bytes or it has 512 threads:
 //     256 threads                      (400, 225, 60, 6) f32 16 and 11 | 24 and 19       (37, 289, 252, 28) f32 13 and 11.5 | 18 and 16.5
 //     1024 threads                     (400, 256, 256, 32) bf16 32 and 24                (1, 256, 256, 32) bf16 8.2 and 6.3
@@ -708,10 +708,12 @@ int bs_group_norm_act_grad(const void* g, int64_t ldgn, int64_t ldgp, const void
     if (blocks > 0x7fffffff || n * groups > 0x7fffffff) return BS_EINVAL;
     if (p.fits) {
         if (!dgamma && !dbeta) a.parts = nullptr;
-        // (two builds: with the registers that 1024 threads leave, 512 of them take 25 us instead of 16, bfloat16, 37 images of 289 x 252)
-#define FIT_T(DT, P8, T) do { if (p.lanes) hipLaunchKernelGGL((k_norm_grad<DT, P8, true, T>), dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a); \
-                              else hipLaunchKernelGGL((k_norm_grad<DT, P8, false, T>), dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a); } while (0)
-#define FIT(DT, P8) do { if (p.threads > 512) FIT_T(DT, P8, 1024); else FIT_T(DT, P8, 512); } while (0)
+        // Builds by the registers that a number of threads leaves, in us at (images, pixels, channels, groups), bf16.  Exchanges: 128,
+        // which lets two workgroups of 512 threads share a compute unit, at the cost of a few spilled: (400, 256, 256, 32) 48, 61 with
+        // the 131 that it would take; (1, 256, 256, 32) 11.6 and 10.4.  Shared memory: 128 spill 50 to 90, (37, 289, 252, 28) 25, 16
+        // with 153; only where 1024 threads leave no more.
+#define FIT_T(DT, P8, L, T) hipLaunchKernelGGL((k_norm_grad<DT, P8, L, T>), dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a)
+#define FIT(DT, P8) do { if (p.lanes) FIT_T(DT, P8, true, 1024); else if (p.threads > 512) FIT_T(DT, P8, false, 1024); else FIT_T(DT, P8, false, 512); } while (0)
 #define GO(DT) do { if (x_exps) FIT(DT, true); else FIT(DT, false); } while (0)
         if (dtype == BS_DT_F32) GO(BS_DT_F32);
         else if (dtype == BS_DT_BF16) GO(BS_DT_BF16);
