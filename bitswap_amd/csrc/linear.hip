@@ -5,6 +5,10 @@
 //   dx       out[q][p] = sum_k w[k][p] ds[q][k]         k = N; w is small and is turned round first (k_lay_w), then as the forward
 //   dw       out[q][p] = sum_k x[k][p] ds[k][q]         k = rows, the strided axis of both: k_over_dma, cut into parts of the rows
 //
+// What bounds them: the bytes of x, residual and outputs where K is a few hundred (a copy runs at 4.9 TB/s here), the matrix cores
+// where it is long (a library product reaches 1420 TFLOP/s in bfloat16 at 16384 x 2048 x 2048; float32 costs six such products), and
+// below some hundred rows the latency of one load, a chain of matrix instructions and one store.
+//
 // float32 operands are split into three bfloat16 limbs (their sum is the float exactly) and multiplied as the six limb products of
 // total order <= 2; what is left out is of relative size 2^-24.  Limb products of an infinity or of a value that rounds to one are
 // NaN, so a sum that does not come out finite is added up again in float32.
@@ -194,6 +198,14 @@ __device__ __forceinline__ void turn_and_finish(const RowsArgs& a, const f32x16&
 // matrix instructions of the block before: 32 bytes a fragment instead of 48, and nothing goes back to shared memory.  Rows of BK k
 // lie there as 16-byte chunks, chunk c in slot c ^ f(row), f such that the 16 lanes a 16-byte read serves together (0-3, 12-15, 20-27;
 // the others) touch all 64 banks.
+//
+// Measured: bfloat16 16384 x 2048 x 2048 with GELU, both outputs 134 us (1025 TFLOP/s; the library's product alone 97 us, what is more
+// is the epilogue, which nothing covers with one workgroup a compute unit: 256 x 128 tiles, two of them, 156 us); float32
+// 102400 x 256 x 256 with residual and both outputs 118 us (3.5 TB/s of 419 MB; 55 us of matrix instructions, 86 of traffic, one
+// partly behind the other); bfloat16 25600 x 256 x 256 11.8 us.  Kept after trying the other way: the compiler places the limb splits
+// (places given to them: 105 us against 100 for 102400 x 256 x 256); a third block of reads ahead, six buffers or steps twice as
+// deep change nothing or cost; 16-bit 128x128 tiles over eight wavefronts of 32 rows, not four of 64 (102400 x 256 x 256 43 and 49 us);
+// 64x64 over four of 32x32, not two of 32x64 (4096 x 256 x 256 5.6 and 6.7 us).
 __device__ __forceinline__ constexpr int wait_vm(int v) { return (v & 15) | (7 << 4) | ((v >> 4) << 14); }      // vmcnt(v), lgkmcnt(0)
 
 template <int DT, int EPI, int BQ, int BP, int WQ, int WP, int BK, int NS, int PER_SIMD>
@@ -389,8 +401,9 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64, PER_SIMD) void k_rows_d
 
 // ---- forward and dx, few rows -------------------------------------------------------------------------------------------------
 // One 32x32 tile a workgroup.  Its four wavefronts hold four runs of k in registers, loaded at once straight from memory (the next
-// four while these are multiplied), and pass the sums on from run to run (a relay): the order of k_rows, at the latency of about
-// one load.
+// four while these are multiplied), and pass the sums on from run to run (a relay): the order of k_rows_dma, at the latency of
+// about one load.  w comes as the caller holds it (dx: turned round).  Measured: 1 x 512 x 512 float16 7.2 us, 256 x 256 x 256 float32
+// 7.5 us with a residual; bound by that latency (an empty launch takes 2 us).
 template <int DT, int EPI, bool WL>
 __global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {
     constexpr int L = limbs_of(DT), NS = DT == BS_DT_F32 ? 4 : 8, ES = esize(DT), RUN = NS * 16;
@@ -505,7 +518,9 @@ __global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {
 
 // ---- w laid out for the kernels above -------------------------------------------------------------------------------------------
 // out [kp / KB][limb][P][KB] 16-bit: a DMA of neighbouring rows reads whole kilobytes.  w [P, K], or with TURNED w [K, P] turned round;
-// zero from K to kp
+// zero from K to kp.  16-bit w whose rows are whole aligned multiples of 64 k is read as it lies instead (8192 x 512 x 512 bfloat16
+// 11.0 us, laid out first 13.5).  Once per call, not kept from call to call: a caller that trains changes w.  256 x 256 float32 2.7 us,
+// 1024 x 512 bfloat16 turned 4.8 us, the better part of each the launch.
 template <int DT, bool TURNED>
 __global__ __launch_bounds__(256) void k_lay_w(const char* __restrict__ w, int64_t ldw, int P, int K, int kp, char* __restrict__ out) {
     constexpr int ES = esize(DT), L = limbs_of(DT), KB = kb_of(DT);
@@ -536,7 +551,8 @@ __global__ __launch_bounds__(256) void k_lay_w(const char* __restrict__ w, int64
     }
 }
 
-// the same for 16-bit w [P, K] in whole aligned chunks: nothing to turn, a thread moves one chunk of 8 k
+// the same for 16-bit w [P, K] in whole aligned chunks: nothing to turn, a thread moves one chunk of 8 k (2048 x 2048: 6 us, by single
+// elements 9)
 __global__ __launch_bounds__(256) void k_lay_chunks(const char* __restrict__ w, int64_t ldw, int P, int K, char* __restrict__ out) {
     constexpr int KB = kb_of(BS_DT_BF16);
     const int p = blockIdx.y * 32 + (threadIdx.x >> 3), k = blockIdx.x * 64 + (threadIdx.x & 7) * 8;
@@ -580,6 +596,11 @@ __device__ __forceinline__ void again_over(const OverArgs& a, int64_t kb, int64_
 // matrix instruction wants (8 rows of one channel side by side) happens in the read from shared memory: transposing reads for 16-bit
 // values (4 rows) and for codes (8 rows, turned into bfloat16 / float16 in registers: exact), dword reads along the channels and a
 // split into limbs for float32.  steps: 2^e of the codes, laid out [blocks of 32 channels][rows] beforehand (k_lay_steps).
+// A part's sums go to the workspace in float32 and are joined in order (k_add_parts); a single part is rounded here.
+//
+// Measured: bfloat16 x as codes, 65536 x 512 x 1024 100 us (687 TFLOP/s; as bfloat16 85: the codes' conversion, 16 instructions per 8
+// values, goes beside the matrix instructions but not for nothing); float32 25600 x 256 x 256 32 us, 8192 x 1024 x 1024 113 us (six
+// products: 912 TFLOP/s), bound by the reads from shared memory, dwords here as no transposing read takes 32 bits.
 template <int DT, bool P8, int BQ, int BP, int WQ, int WP, int BK, int NS>
 __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const OverArgs a, const float* __restrict__ steps, int64_t ldsteps) {
     constexpr int NW = (BQ / WQ) * (BP / WP), ES = esize(DT), XE = P8 ? 1 : ES;
@@ -879,7 +900,9 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
 }
 
 // rows of K elements of ES bytes (1, 2, 4) -> rows of whole 16-byte chunks, zero behind K.  2^lanes_log2 threads a row (a power of two:
-// no division); the last chunk of a row comes as its last 16 bytes, moved down.
+// no division); the last chunk of a row comes as its last 16 bytes, moved down.  A copy: 7919 x 252 bfloat16 3 us, 20567 x 963 float32
+// 24 us (6.6 TB/s).  The products that went without it, by single elements through registers into shared memory, took 17 us for
+// 7919 x 252 x 505 in bfloat16 and 28 for its dw; copied first 16 and 25, and one kernel less of each kind.
 template <int ES>
 __global__ __launch_bounds__(256) void k_pad(const char* __restrict__ in, int64_t ld, int64_t rows, int K, char* __restrict__ out, int chunks, int lanes_log2) {
     constexpr int V = 16 / ES;
@@ -914,14 +937,16 @@ __global__ __launch_bounds__(256) void k_pad(const char* __restrict__ in, int64_
     }
 }
 
-// exponents [rows, nb] -> 2^e as floats [nb][ld], zero from rows to ld
+// exponents [rows, nb] -> 2^e as floats [nb][ld], zero from rows to ld (65536 x 16: 5.3 us; the products would read each a byte at a
+// time, a row apart)
 __global__ __launch_bounds__(256) void k_lay_steps(const int8_t* __restrict__ exps, int64_t rows, int nb, float* __restrict__ out, int64_t ld) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= ld) return;
     for (int b = 0; b < nb; ++b) out[b * ld + i] = i < rows ? p8_pow2(exps[i * nb + b]) : 0.0f;
 }
 
-// parts [nparts][n, rounded up to whole 16 bytes] float32 -> their sum in dtype; 16 threads of four neighbours x 16 lanes over the parts
+// parts [nparts][n, rounded up to whole 16 bytes] float32 -> their sum in dtype; 16 threads of four neighbours x 16 lanes over the parts,
+// always the same order.  64 parts of 256 x 256 4.7 us, 32 of 512 x 1024 11 us (6.1 TB/s, from the caches)
 template <int DT>
 __global__ __launch_bounds__(256) void k_add_parts(const float* __restrict__ parts, int nparts, int64_t n, char* __restrict__ out) {
     __shared__ __align__(16) f32x4 red[256];

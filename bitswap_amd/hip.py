@@ -1061,28 +1061,27 @@ def linear_act_grad(x, w, s=None, act=ACT_NONE, g_sum=None, g_act=None, want_x=T
         ds = w.new_empty(tuple(g0.shape[:-1]) + (ldd,))
         ds = ds if ldd == N else ds[..., :N]
     db = w.new_empty(N, dtype=torch.float32) if want_bias else None
-    if ds is not None or db is not None:
-        nb = _workspace_bytes("bs_act_grad_workspace", rows, N) if want_bias else 0
-        ws = _scratch(w, nb)
-        _check(L.bs_act_grad(_at(gs[0][0]), gs[0][1], _at(gs[1][0]), gs[1][1], _at(st), _at(se), lds, act, code, rows, N, _at(ds),
-                             ldd, _at(db), _at(ws), nb, _raw_stream(dev)), "bs_act_grad")
     if ds is not None:
         dt, zeros, ds_whole = ds, 1, int(ldd * es < 1 << 22)
     else:
         dt, ldd = gs[0] if g_sum is not None else gs[1]
         zeros, ds_whole = 0, _whole(dt, ldd, N, es)
+    # one workspace: the launches that use it follow each other on the stream
+    nb = max(_workspace_bytes("bs_act_grad_workspace", rows, N) if want_bias else 0,
+             _workspace_bytes("bs_linear_grad_x_workspace", code, rows, K, N, ds_whole) if want_x else 0,
+             _workspace_bytes("bs_linear_grad_w_workspace", code, rows, K, N, int(xe is not None), _whole(xt, ldx, K, es if xe is None else 1),
+                              ds_whole) if want_w else 0)
+    ws = _scratch(w, nb)
+    if ds is not None or db is not None:
+        _check(L.bs_act_grad(_at(gs[0][0]), gs[0][1], _at(gs[1][0]), gs[1][1], _at(st), _at(se), lds, act, code, rows, N, _at(ds),
+                             ldd, _at(db), _at(ws), nb, _raw_stream(dev)), "bs_act_grad")
     dx = dw = None
     if want_x:
         wt, ldw, _ = _as_rows(w, K, "linear_act_grad w")
         dx = w.new_empty(tuple(g0.shape[:-1]) + (K,))
-        nb = _workspace_bytes("bs_linear_grad_x_workspace", code, rows, K, N, ds_whole)
-        ws = _scratch(w, nb)
         _check(L.bs_linear_grad_x(_at(dt), ldd, zeros, _at(wt), ldw, _at(dx), code, rows, K, N, _at(ws), nb, _raw_stream(dev)), "bs_linear_grad_x")
     if want_w:
         dw = w.new_empty((N, K))
-        nb = _workspace_bytes("bs_linear_grad_w_workspace", code, rows, K, N, int(xe is not None),
-                              _whole(xt, ldx, K, es if xe is None else 1), ds_whole)
-        ws = _scratch(w, nb)
         _check(L.bs_linear_grad_w(_at(dt), ldd, zeros, _at(xt), _at(xe), ldx, _at(dw), code, rows, K, N, _at(ws), nb, _raw_stream(dev)),
                "bs_linear_grad_w")
     return dx, dw, db, ((ds if changed else g0) if want_res else None)
