@@ -402,7 +402,7 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64, PER_SIMD) void k_rows_d
 // ---- forward and dx, few rows -------------------------------------------------------------------------------------------------
 // One 32x32 tile a workgroup.  Its four wavefronts hold four runs of k in registers, loaded at once straight from memory (the next
 // four while these are multiplied), and pass the sums on from run to run (a relay): the order of k_rows_dma, at the latency of
-// about one load.  w comes as the caller holds it (dx: turned round).  Measured: 1 x 512 x 512 float16 7.2 us, 256 x 256 x 256 float32
+// about one load.  w comes as the caller holds it (dx: turned round).  Measured: 1 x 1024 x 1024 float16 7.2 us, 256 x 256 x 256 float32
 // 7.5 us with a residual; bound by that latency (an empty launch takes 2 us).
 template <int DT, int EPI, bool WL>
 __global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {

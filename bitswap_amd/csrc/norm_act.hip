@@ -609,7 +609,8 @@ Plan plan(int dtype, int64_t n, int64_t pixels, int C, int G, int grad) {
         p.threads = (p.pl * p.cl + 63) / 64 * 64;
         const int ch = p.cl * V, Q = p.pl / V > 1 ? p.pl / V : 1;
         p.lds = ((p.lanes && !grad ? 0 : (grad ? 2 : 1) * (p.pl + Q) * ch) + 32 * gs + (grad ? ch : 0)) * 4;
-        return p;
+        if (p.lds <= 160 * 1024) return p;
+        p = {};                                             // (over 1020 lanes of 16-bit channels to a pixel lane: the gradient's sums)
     }
     const int chunks = (C + V - 1) / V;
     p.cl = chunks < 32 ? chunks : 32;

@@ -802,7 +802,8 @@ def test_linear_act_grad_of_one_plain_gradient_in_rows_that_are_not_whole(hip, d
 
 @pytest.mark.parametrize("saved8", [False, True])
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("n,pixels,c,groups", [(2, 1024, 256, 8), (2, 784, 100, 5), (1, 1000, 90, 3), (2, 256, 512, 8), (9, 225, 60, 6)])
+@pytest.mark.parametrize("n,pixels,c,groups", [(2, 1024, 256, 8), (2, 784, 100, 5), (1, 1000, 90, 3), (2, 256, 512, 8), (9, 225, 60, 6),
+                                               (2, 3, 8192, 1), (3, 1, 8192, 1), (1, 4, 8150, 1), (1, 2, 4096, 1)])
 def test_group_norm_in_the_largest_workgroups(hip, n, pixels, c, groups, dtype, saved8):
     """Groups that take more than 512 threads, and as many groups as 512 threads hold, in power-of-two lanes and in others."""
     x, g = randn((n, pixels, c), dtype, 1), randn((n, pixels, c), dtype, 4)
