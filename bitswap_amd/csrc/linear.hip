@@ -2,7 +2,7 @@
 // two products of its backward pass, on the bf16 / f16 matrix cores (v_mfma_f32_32x32x16), float32 sums.
 //
 //   forward  out[q][p] = sum_k w[p][k] x[q][k]          k = K, the contiguous axis of both: k_rows_dma / k_relay
-//   dx       out[q][p] = sum_k w[k][p] ds[q][k]         k = N; w is small and is turned round first (k_lay_w), then as the forward
+//   dx       out[q][p] = sum_k w[k][p] ds[q][k]         k = N; as the forward, w turned round first (k_lay_w) where rows are many
 //   dw       out[q][p] = sum_k x[k][p] ds[k][q]         k = rows, the strided axis of both: k_over_dma, cut into parts of the rows
 //
 // What bounds them: the bytes of x, residual and outputs where K is a few hundred (a copy runs at 4.9 TB/s here), the matrix cores
@@ -72,7 +72,6 @@ struct RowsArgs {
     int64_t ldxd;
     const char* wl;                    // w as the kernel reads it, 16-bit: laid out (k_lay_w), or w itself
     int64_t sp, sk, sl;                // element (limb, p, k) is at limb sl + p sp + k / KB sk + k % KB
-    int kp;                            // k it has, a multiple of 64; zero behind K
     int64_t rows;
     int K, N;
     int Kx;                            // k that rows of x hold in whole 16-byte chunks, zero from K on
@@ -402,9 +401,10 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64, PER_SIMD) void k_rows_d
 // ---- forward and dx, few rows -------------------------------------------------------------------------------------------------
 // One 32x32 tile a workgroup.  Its four wavefronts hold four runs of k in registers, loaded at once straight from memory (the next
 // four while these are multiplied), and pass the sums on from run to run (a relay): the order of k_rows_dma, at the latency of
-// about one load.  w comes as the caller holds it (dx: turned round).  Measured: 1 x 1024 x 1024 float16 7.2 us, 256 x 256 x 256 float32
-// 7.5 us with a residual; bound by that latency (an empty launch takes 2 us).
-template <int DT, int EPI, bool WL>
+// about one load.  w comes as the caller holds it; dx (WT) gathers 8 rows of it a fragment, a launch less than turning it round first.
+// Measured: 1 x 1024 x 1024 float16 7.2 us, 256 x 256 x 256 float32 7.5 us with a residual; bound by that latency (an empty launch
+// takes 2 us).
+template <int DT, int EPI, bool WT>
 __global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {
     constexpr int L = limbs_of(DT), NS = DT == BS_DT_F32 ? 4 : 8, ES = esize(DT), RUN = NS * 16;
     __shared__ __align__(16) char lds[turn_bytes(64)];
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {
     const int64_t q = q0 + (lane & 31) < a.rows ? q0 + (lane & 31) : a.rows - 1;
     const int p = p0 + (lane & 31) < a.N ? p0 + (lane & 31) : a.N - 1;
     const char* const xp = a.x + q * a.ldx * ES;
-    const char* const wp = WL ? a.wl + p * a.sp * 2 : a.w + (int64_t)p * a.ldw * ES;
+    const char* const wp = a.w + (WT ? p : (int64_t)p * a.ldw) * ES;
     f32x16 acc;
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
@@ -438,19 +438,32 @@ __global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {
             l[0] = r[0];
         }
     };
-    u32x4 xr[NS][RAW], wr[NS][WL ? L : RAW];
+    auto fetch_turned = [&](int k, u32x4* r) {                     // the same of a column of w [K, N]: neighbouring lanes, neighbouring values
+        uint32_t u[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const char* const at = wp + (int64_t)min(k + e, a.K - 1) * a.ldw * ES;
+            u[e] = DT == BS_DT_F32 ? *reinterpret_cast<const uint32_t*>(at) : *reinterpret_cast<const uint16_t*>(at);
+            if (k + e >= a.K) u[e] = 0;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (DT == BS_DT_F32) {
+                r[0][e] = u[e];
+                r[RAW - 1][e] = u[4 + e];
+            } else {
+                r[0][e] = u[2 * e] | u[2 * e + 1] << 16;
+            }
+        }
+    };
+    u32x4 xr[NS][RAW], wr[NS][RAW];
     auto ask = [&](int k0) {
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
             const int k = k0 + wave * RUN + 8 * (lane >> 5) + n * 16;
             fetch(xp, k, xr[n]);
-            if (WL) {
-#pragma unroll
-                for (int l = 0; l < L; ++l)
-                    wr[n][l] = k < a.kp ? load16(wp + (l * a.sl + k / kb_of(DT) * a.sk + k % kb_of(DT)) * 2) : u32x4{0, 0, 0, 0};
-            } else {
-                fetch(wp, k, wr[n]);
-            }
+            if (WT) fetch_turned(k, wr[n]);
+            else fetch(wp, k, wr[n]);
         }
     };
     ask(0);
@@ -458,12 +471,7 @@ __global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {
         u32x4 fp[NS][1][L], fq[NS][1][L];
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
-            if (WL) {
-#pragma unroll
-                for (int l = 0; l < L; ++l) fp[n][0][l] = wr[n][l % (WL ? L : RAW)];
-            } else {
-                split(wr[n], fp[n][0]);
-            }
+            split(wr[n], fp[n][0]);
             split(xr[n], fq[n][0]);
         }
         if (k0 + 4 * RUN < a.K) ask(k0 + 4 * RUN);                  // on its way while the others take their turns
@@ -1018,10 +1026,9 @@ int pad(int es, const void* in, int64_t ld, int64_t rows, int K, char* out, hipS
     return BS_OK;
 }
 
-// out [rows, N] over K: w [N, K], or [K, N] when turned; zeros: rows of x end in zeros up to whole chunks
-int64_t rows_bytes(int dtype, int64_t rows, int K, int N, bool turned, bool whole) {
-    const bool small = few(dtype, rows, N);
-    return (turned || !small ? lay_bytes(dtype, K, N) : 0) + (small || whole ? 0 : pad_bytes(esize(dtype), rows, K));
+// out [rows, N] over K; whole: rows of x that DMA can take
+int64_t rows_bytes(int dtype, int64_t rows, int K, int N, bool whole) {
+    return few(dtype, rows, N) ? 0 : lay_bytes(dtype, K, N) + (whole ? 0 : pad_bytes(esize(dtype), rows, K));
 }
 template <int DT, int EPI>
 int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream_t st) {
@@ -1030,10 +1037,10 @@ int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream
     const bool small = few(DT, a.rows, a.N), whole = whole_rows(a.x, a.ldx, a.K, ES, zeros);
     const bool big = DT != BS_DT_F32 && a.K >= DEEP_K && fills(a.rows, a.N);
     const bool as_is = DT != BS_DT_F32 && !a.wt && a.K % 64 == 0 && a.ldw % 8 == 0 && ((uintptr_t)a.w & 15) == 0 && a.ldw < (1 << 21);
-    const int64_t need = rows_bytes(DT, a.rows, a.K, a.N, a.wt, whole);
+    const int64_t need = rows_bytes(DT, a.rows, a.K, a.N, whole);
     if (need > 0 && (!workspace || bytes < need)) return BS_EINVAL;
     if (a.K > MAX_WIDTH || a.N > MAX_WIDTH) return BS_EINVAL;          // 31-bit offsets into a tile's rows, and the grids below
-    const bool lay = a.wt || (!small && !as_is);
+    const bool lay = !small && !as_is;
     if (lay) {
         const dim3 grid((unsigned)(kp / 32), (unsigned)((a.N + 31) / 32));
         constexpr int KB = kb_of(DT);
@@ -1045,12 +1052,10 @@ int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream
     } else {
         a.wl = a.w; a.sp = a.ldw; a.sl = 0; a.sk = kb_of(DT);
     }
-    a.kp = kp;
     if (small) {
         a.tp = (a.N + 31) / 32;
         const unsigned blocks = (unsigned)((a.rows + 31) / 32 * a.tp);
-        if (lay) hipLaunchKernelGGL((k_relay<DT, EPI, true>), dim3(blocks), dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((k_relay<DT, EPI, false>), dim3(blocks), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_relay<DT, EPI, EPI == E_PLAIN>), dim3(blocks), dim3(256), 0, st, a);      // (E_PLAIN: dx, w [K, N])
         return rows_rc();
     }
     a.Kx = (a.K + CK - 1) / CK * CK;
@@ -1091,7 +1096,7 @@ void split_rows(int dtype, int64_t rows, int K, int N, int64_t* part, int64_t* p
     const int bq = over_bq(dtype, rows, K, N);
     const int64_t tiles = tiles_of(N, K, bq, 128), groups = bq == 64 ? 256 : 512;
     int64_t want = (groups + tiles - 1) / tiles;
-    const int64_t most = (rows + 127) / 128;
+    const int64_t most = rows <= 256 ? 1 : (rows + 127) / 128;      // (so few: the launch that joins two parts costs more)
     if (want > most) want = most;
     if (want < 1) want = 1;
     *part = ((rows + want - 1) / want + 63) / 64 * 64;
@@ -1138,7 +1143,7 @@ extern "C" {
 
 int64_t bs_linear_workspace(int dtype, int64_t rows, int K, int N, int whole) {
     if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1 || K > MAX_WIDTH || N > MAX_WIDTH) return BS_EINVAL;
-    return rows_bytes(dtype, rows, K, N, false, whole != 0);
+    return rows_bytes(dtype, rows, K, N, whole != 0);
 }
 
 int bs_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype, const void* res,
@@ -1161,7 +1166,7 @@ int bs_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const 
 
 int64_t bs_linear_grad_x_workspace(int dtype, int64_t rows, int K, int N, int whole) {
     if (bad_type(dtype) || rows < 0 || rows > MAX_ROWS || K < 1 || N < 1 || K > MAX_WIDTH || N > MAX_WIDTH) return BS_EINVAL;
-    return rows_bytes(dtype, rows, N, K, true, whole != 0);
+    return rows_bytes(dtype, rows, N, K, whole != 0);
 }
 
 int bs_linear_grad_x(const void* ds, int64_t ldds, int zeros, const void* w, int64_t ldw, void* dx, int dtype, int64_t rows, int K, int N,

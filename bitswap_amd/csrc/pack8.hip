@@ -134,7 +134,9 @@ __global__ __launch_bounds__(256) void k_act_grad(const ActGradArgs a, int cl_lo
 void split_rows(int64_t rows, int N, int64_t* part, int64_t* parts) {
     const int slabs = (N + 127) / 128;
     int64_t want = (2048 + slabs - 1) / slabs;
-    const int64_t most = (rows + 31) / 32;
+    int lanes = 1;                                            // along the channels, at most (k_act_grad)
+    while (lanes < 32 && lanes * 4 < N) lanes *= 2;
+    const int64_t most = rows <= 8 * (256 / lanes) ? 1 : (rows + 31) / 32;     // (eight rows a thread: sooner done than joined)
     if (want > most) want = most;
     if (want < 1) want = 1;
     *part = (rows + want - 1) / want;

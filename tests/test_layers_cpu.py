@@ -27,10 +27,12 @@ def test_null_operands_sizes_types_and_strides_are_refused(L):
                 dict(dt=-1), dict(rows=-1), dict(rows=1 << 41), dict(K=0), dict(N=0), dict(bias=p, bt=1), dict(rows=100000)):
         assert ok(**bad) == E, bad
     assert ok(rows=0, x=None) == hip.OK                                     # no rows: nothing to do
-    n = L.bs_linear_grad_x_workspace(0, 4, 8, 8, 1)
-    assert L.bs_linear_grad_x(None, 8, 0, p, 8, p, 0, 4, 8, 8, p, n, None) == E
-    assert L.bs_linear_grad_x(p, 7, 0, p, 8, p, 0, 4, 8, 8, p, n, None) == E
-    assert L.bs_linear_grad_x(p, 8, 0, p, 8, p, 0, 4, 8, 8, p, n - 1, None) == E
+    n = L.bs_linear_grad_x_workspace(0, 100000, 8, 8, 1)
+    assert n > 0 and L.bs_linear_grad_x_workspace(0, 4, 8, 8, 1) == 0
+    assert L.bs_linear_grad_x(None, 8, 0, p, 8, p, 0, 4, 8, 8, None, 0, None) == E
+    assert L.bs_linear_grad_x(p, 7, 0, p, 8, p, 0, 4, 8, 8, None, 0, None) == E
+    assert L.bs_linear_grad_x(p, 8, 0, p, 8, p, 0, 100000, 8, 8, p, n - 1, None) == E
+    assert L.bs_linear_grad_x(p, 8, 0, p, 8, p, 0, 100000, 8, 8, None, n, None) == E
     assert L.bs_linear_grad_w(p, 8, 0, None, None, 8, p, 0, 4, 8, 8, None, 0, None) == E
     assert L.bs_linear_grad_w(p, 8, 0, p, None, 8, None, 0, 4, 8, 8, None, 0, None) == E
     n = L.bs_linear_grad_w_workspace(0, 100000, 8, 8, 0, 1, 1)
