@@ -204,7 +204,9 @@ __device__ __forceinline__ void turn_and_finish(const RowsArgs& a, const f32x16&
 // partly behind the other); bfloat16 25600 x 256 x 256 11.8 us.  Kept after trying the other way: the compiler places the limb splits
 // (places given to them: 105 us against 100 for 102400 x 256 x 256); a third block of reads ahead, six buffers or steps twice as
 // deep change nothing or cost; 16-bit 128x128 tiles over eight wavefronts of 32 rows, not four of 64 (102400 x 256 x 256 43 and 49 us);
-// 64x64 over four of 32x32, not two of 32x64 (4096 x 256 x 256 5.6 and 6.7 us).
+// 64x64 over four of 32x32, not two of 32x64 (4096 x 256 x 256 5.6 and 6.7 us); float32
+// 128x128 over four wavefronts of 32 rows x 128 channels, which split a row into limbs once, not of 64x64 (16384 x 1024 x 1024 187 and 192 us).
+// Residuals asked for before the sums change nothing (115 and 112 us).
 __device__ __forceinline__ constexpr int wait_vm(int v) { return (v & 15) | (7 << 4) | ((v >> 4) << 14); }      // vmcnt(v), lgkmcnt(0)
 
 template <int DT, int EPI, int BQ, int BP, int WQ, int WP, int BK, int NS, int PER_SIMD>
@@ -996,7 +998,7 @@ bool enough(int64_t rows, int N, int bq, int bp) { return tiles_of(rows, N, bq, 
 //   the largest tile (16-bit 256x256, one workgroup a compute unit; float32 128x128, two) where K is long enough to pay for its
 //   start and end, which nothing covers:
 //     bf16  (16384, 2048, 2048) 145 and 168                 (102400, 256, 256) 50 and 43
-//     f32   (4942, 832, 1168) 74 and 84                     (102400, 256, 256) 105 and 103,  (8192, 256, 512) 24.3 and 21.4
+//     f32   (4942, 832, 1168) 72 and 84                     (40000, 256, 256) 54 and 45,  (8192, 256, 512) 25.5 and 22.3
 constexpr int DEEP_K = 512;
 //   and, 16-bit, where its tiles fill four fifths of the rounds that they take:
 //     (16384, 1024, 1024), 256 tiles, 46 and 50             (12288, 512, 1024), 192 tiles, 29 and 23
@@ -1069,7 +1071,7 @@ int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream
         const int64_t blocks = (a.tiles + 7) / 8 * 8; if (blocks > 0x7fffffff) return BS_EINVAL; \
         hipLaunchKernelGGL((k_rows_dma<DT, EPI, BQ, BP, WQ, WP, BK, NS, PS>), dim3((unsigned)blocks), dim3((BQ / WQ) * (BP / WP) * 64), 0, st, a); } while (0)
     if constexpr (DT == BS_DT_F32) {
-        if (a.K >= DEEP_K && a.N > 64 && enough(a.rows, a.N, 128, 128)) ROWS(128, 128, 64, 64, 16, 3, 2);
+        if (a.K >= DEEP_K && a.N > 64 && enough(a.rows, a.N, 128, 128)) ROWS(128, 128, 32, 128, 16, 3, 2);
         else if (a.N > 64 && enough(a.rows, a.N, 64, 128)) ROWS(64, 128, 32, 64, 16, 3, 3);
         else ROWS(64, 64, 32, 32, 32, 4, 1);
     } else {
