@@ -610,7 +610,8 @@ __device__ __forceinline__ void again_over(const OverArgs& a, int64_t kb, int64_
 //
 // Measured: bfloat16 x as codes, 65536 x 512 x 1024 100 us (687 TFLOP/s; as bfloat16 85: the codes' conversion, 16 instructions per 8
 // values, goes beside the matrix instructions but not for nothing); float32 25600 x 256 x 256 32 us, 8192 x 1024 x 1024 113 us (six
-// products: 912 TFLOP/s), bound by the reads from shared memory, dwords here as no transposing read takes 32 bits.
+// products: 912 TFLOP/s), bound by the limb splits, 44 instructions a fragment beside its matrix instructions (reads are dwords: no
+// transposing read takes 32 bits).
 template <int DT, bool P8, int BQ, int BP, int WQ, int WP, int BK, int NS>
 __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const OverArgs a, const float* __restrict__ steps, int64_t ldsteps) {
     constexpr int NW = (BQ / WQ) * (BP / WP), ES = esize(DT), XE = P8 ? 1 : ES;
@@ -1084,19 +1085,20 @@ int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream
 }
 
 // How a weight gradient is cut: tiles of 256 x 128 (16-bit) or 128 x 128 (float32) outputs where these and parts of 256 rows come to
-// two workgroups a compute unit, else of 64 x 128; the rows into as many parts as give a compute unit two (large tiles) or one (small
-// ones: what more parts win the join of them costs again), none under 128 rows.  Both sides, in us, at (rows, K, N):
+// two workgroups a compute unit, else of 64 x 128; the rows into as many parts as give a compute unit two, or one where tiles are small
+// and 16-bit (what more parts win the join of them costs again), none under 128 rows.  Both sides, in us, at (rows, K, N):
 //   large tiles   bf16 from codes (65536, 512, 1024) 102 and 179    f32 (8192, 1024, 1024) 113 and 124
 //                 below: bf16 (8192, 512, 512) 30 and 22            f32 (2048, 256, 256) 16.5 and 12.8
 //   parts, large  two a compute unit 102, one 126, four 126 (bf16 from codes (65536, 512, 1024))
-//   parts, small  one a compute unit 12.7, two 17.2 (bf16 (8192, 256, 256)); under 512 rows allowed 12.7, not allowed 22.2 (f32 (2048, 256, 256))
+//   parts, small  one a compute unit 12.7, two 17.2 (bf16 (8192, 256, 256)); 40 and 37 (f32 (25600, 256, 256), both launches); parts
+//                 under 512 rows 12.7, none 22.2 (f32 (2048, 256, 256))
 int over_bq(int dtype, int64_t rows, int K, int N) {
     const int big = dtype == BS_DT_F32 ? 128 : 256;
     return 2 * N > big && tiles_of(N, K, big, 128) * ((rows + 255) / 256) >= 512 ? big : 64;
 }
 void split_rows(int dtype, int64_t rows, int K, int N, int64_t* part, int64_t* parts) {
     const int bq = over_bq(dtype, rows, K, N);
-    const int64_t tiles = tiles_of(N, K, bq, 128), groups = bq == 64 ? 256 : 512;
+    const int64_t tiles = tiles_of(N, K, bq, 128), groups = bq == 64 && dtype != BS_DT_F32 ? 256 : 512;
     int64_t want = (groups + tiles - 1) / tiles;
     const int64_t most = rows <= 256 ? 1 : (rows + 127) / 128;      // (so few: the launch that joins two parts costs more)
     if (want > most) want = most;
