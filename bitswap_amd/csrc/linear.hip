@@ -2,7 +2,7 @@
 // two products of its backward pass, on the bf16 / f16 matrix cores (v_mfma_f32_32x32x16), float32 sums.
 //
 //   forward  out[q][p] = sum_k w[p][k] x[q][k]          k = K, the contiguous axis of both: k_rows_dma / k_relay
-//   dx       out[q][p] = sum_k w[k][p] ds[q][k]         k = N; as the forward, w turned round first (k_lay_w) where rows are many
+//   dx       out[q][p] = sum_k w[k][p] ds[q][k]         k = N; as the forward, w turned round first (k_prepare) where rows are many
 //   dw       out[q][p] = sum_k x[k][p] ds[k][q]         k = rows, the strided axis of both: k_over_dma, cut into parts of the rows
 //
 // What bounds them: the bytes of x, residual and outputs where K is a few hundred (a copy runs at 4.9 TB/s here), the matrix cores
@@ -70,7 +70,7 @@ struct RowsArgs {
     int64_t ldx, ldw;
     const char* xd;                    // x as DMA takes it (rows of whole chunks): x itself or its copy
     int64_t ldxd;
-    const char* wl;                    // w as the kernel reads it, 16-bit: laid out (k_lay_w), or w itself
+    const char* wl;                    // w as the kernel reads it, 16-bit: laid out (k_prepare), or w itself
     int64_t sp, sk, sl;                // element (limb, p, k) is at limb sl + p sp + k / KB sk + k % KB
     int64_t rows;
     int K, N;
@@ -192,7 +192,7 @@ __device__ __forceinline__ void turn_and_finish(const RowsArgs& a, const f32x16&
 
 // ---- forward and dx, many rows ------------------------------------------------------------------------------------------------
 // Tile of BQ rows x BP channels, BK deep steps.  Both operands come by DMA (rows of x that are no whole aligned 16-byte chunks are
-// copied to such first, k_pad) through a ring of NS buffers with one barrier a step; fragments are read one 16-deep block ahead of
+// copied to such first, k_prepare) through a ring of NS buffers with one barrier a step; fragments are read one 16-deep block ahead of
 // the matrix instructions.  float32 rows lie in shared memory as they are and are split into limbs after the read, between the
 // matrix instructions of the block before: 32 bytes a fragment instead of 48, and nothing goes back to shared memory.  Rows of BK k
 // lie there as 16-byte chunks, chunk c in slot c ^ f(row), f such that the 16 lanes a 16-byte read serves together (0-3, 12-15, 20-27;
@@ -531,11 +531,23 @@ __global__ __launch_bounds__(256) void k_relay(const RowsArgs a) {
 // zero from K to kp.  16-bit w whose rows are whole aligned multiples of 64 k is read as it lies instead (8192 x 512 x 512 bfloat16
 // 11.0 us, laid out first 13.5).  Once per call, not kept from call to call: a caller that trains changes w.  256 x 256 float32 2.7 us,
 // 1024 x 512 bfloat16 turned 4.8 us, the better part of each the launch.
+struct LayJob {
+    const char* w;
+    int64_t ldw;
+    int P, K;
+    char* out;
+    int across, blocks;                // blocks along k, all of them
+    int chunks;                        // by chunks
+};
 template <int DT, bool TURNED>
-__global__ __launch_bounds__(256) void k_lay_w(const char* __restrict__ w, int64_t ldw, int P, int K, int kp, char* __restrict__ out) {
+__device__ __forceinline__ void lay_tile(const LayJob& j, int bx, int by) {
     constexpr int ES = esize(DT), L = limbs_of(DT), KB = kb_of(DT);
+    const char* const w = j.w;
+    const int64_t ldw = j.ldw;
+    const int P = j.P, K = j.K;
+    char* const out = j.out;
     __shared__ uint32_t tile[32][33];
-    const int p0 = blockIdx.y * 32, k0 = blockIdx.x * 32;                // 32 p x 32 k
+    const int p0 = by * 32, k0 = bx * 32;                                // 32 p x 32 k
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     uint32_t v[4];
 #pragma unroll
@@ -563,11 +575,71 @@ __global__ __launch_bounds__(256) void k_lay_w(const char* __restrict__ w, int64
 
 // the same for 16-bit w [P, K] in whole aligned chunks: nothing to turn, a thread moves one chunk of 8 k (2048 x 2048: 6 us, by single
 // elements 9)
-__global__ __launch_bounds__(256) void k_lay_chunks(const char* __restrict__ w, int64_t ldw, int P, int K, char* __restrict__ out) {
+__device__ __forceinline__ void lay_chunks(const LayJob& j, int bx, int by) {
     constexpr int KB = kb_of(BS_DT_BF16);
-    const int p = blockIdx.y * 32 + (threadIdx.x >> 3), k = blockIdx.x * 64 + (threadIdx.x & 7) * 8;
-    if (p >= P) return;
-    *reinterpret_cast<u32x4*>(out + (((int64_t)k / KB * P + p) * KB + k % KB) * 2) = k < K ? load16(w + (p * ldw + k) * 2) : u32x4{0, 0, 0, 0};
+    const int p = by * 32 + (threadIdx.x >> 3), k = bx * 64 + (threadIdx.x & 7) * 8;
+    if (p >= j.P) return;
+    *reinterpret_cast<u32x4*>(j.out + (((int64_t)k / KB * j.P + p) * KB + k % KB) * 2) = k < j.K ? load16(j.w + (p * j.ldw + k) * 2) : u32x4{0, 0, 0, 0};
+}
+
+// rows of K elements of ES bytes (1, 2, 4) -> rows of whole 16-byte chunks, zero behind K.  2^lanes_log2 threads a row (a power of two:
+// no division); the last chunk of a row comes as its last 16 bytes, moved down.  A copy: 7919 x 252 bfloat16 3 us, 20567 x 963 float32
+// 24 us (6.6 TB/s).  The products that went without it, by single elements through registers into shared memory, took 17 us for
+// 7919 x 252 x 505 in bfloat16 and 28 for its dw; copied first 16 and 25, and one kernel less of each kind.
+struct PadJob {
+    const char* in;
+    int64_t ld, rows;
+    int K;
+    char* out;
+    int chunks, lanes_log2;
+    int64_t blocks;
+};
+template <int ES>
+__device__ __forceinline__ void pad_rows(const PadJob& j, int64_t block) {
+    constexpr int V = 16 / ES;
+    const char* const in = j.in;
+    const int64_t ld = j.ld, rows = j.rows;
+    const int K = j.K, chunks = j.chunks, lanes_log2 = j.lanes_log2;
+    char* const out = j.out;
+    const int64_t row = block * (256 >> lanes_log2) + (threadIdx.x >> lanes_log2);
+    if (row >= rows) return;
+    for (int c = threadIdx.x & ((1 << lanes_log2) - 1); c < chunks; c += 1 << lanes_log2) {
+        const int left = K - c * V;
+        const char* const src = in + (row * ld + (int64_t)c * V) * ES;
+        u32x4 v;
+        if (left >= V) {
+            v = load16(src);
+        } else if (c > 0) {
+            const int down = (V - left) * ES;                            // bytes of the chunk before
+            const u32x4 t = load16(src - down);
+            const uint64_t lo = t[0] | (uint64_t)t[1] << 32, hi = t[2] | (uint64_t)t[3] << 32;
+            const int bits = down * 8;                                   // 8 .. 120
+            const uint64_t l = bits < 64 ? (lo >> bits) | (hi << (64 - bits)) : bits == 64 ? hi : hi >> (bits - 64);
+            const uint64_t h = bits < 64 ? hi >> bits : 0;
+            v = u32x4{(uint32_t)l, (uint32_t)(l >> 32), (uint32_t)h, (uint32_t)(h >> 32)};
+        } else {
+            uint8_t u[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) u[e] = *reinterpret_cast<const uint8_t*>(src + min(e, left * ES - 1));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = 0;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) v[e] |= 4 * e + b < left * ES ? (uint32_t)u[4 * e + b] << (8 * b) : 0u;
+            }
+        }
+        *reinterpret_cast<u32x4*>(out + (row * chunks + c) * 16) = v;
+    }
+}
+
+// What a product over rows needs first, one launch: w laid out, x in whole rows (either may have no blocks).  bfloat16 7919 x 252 and
+// 505 x 252 4.8 us; in two launches 4.5 + 2.9, the whole call 18.5 us instead of 15.5.
+template <int DT, bool TURNED>
+__global__ __launch_bounds__(256) void k_prepare(const LayJob l, const PadJob x) {
+    const int b = blockIdx.x;
+    if (b >= l.blocks) pad_rows<esize(DT)>(x, b - l.blocks);
+    else if (l.chunks) lay_chunks(l, b % l.across, b / l.across);
+    else lay_tile<DT, TURNED>(l, b % l.across, b / l.across);
 }
 
 // ---- dw -------------------------------------------------------------------------------------------------------------------------
@@ -605,7 +677,7 @@ __device__ __forceinline__ void again_over(const OverArgs& a, int64_t kb, int64_
 // x and ds by DMA through a ring, as in k_rows_dma, every tile as it lies in memory: [BK rows][channels].  The transposition that the
 // matrix instruction wants (8 rows of one channel side by side) happens in the read from shared memory: transposing reads for 16-bit
 // values (4 rows) and for codes (8 rows, turned into bfloat16 / float16 in registers: exact), dword reads along the channels and a
-// split into limbs for float32.  steps: 2^e of the codes, laid out [blocks of 32 channels][rows] beforehand (k_lay_steps).
+// split into limbs for float32.  steps: 2^e of the codes, laid out [blocks of 32 channels][rows] beforehand (k_prepare_over).
 // A part's sums go to the workspace in float32 and are joined in order (k_add_parts); a single part is rounded here.
 //
 // Measured: bfloat16 x as codes, 65536 x 512 x 1024 100 us (687 TFLOP/s; as bfloat16 85: the codes' conversion, 16 instructions per 8
@@ -910,50 +982,27 @@ __global__ __launch_bounds__((BQ / WQ) * (BP / WP) * 64) void k_over_dma(const O
         }
 }
 
-// rows of K elements of ES bytes (1, 2, 4) -> rows of whole 16-byte chunks, zero behind K.  2^lanes_log2 threads a row (a power of two:
-// no division); the last chunk of a row comes as its last 16 bytes, moved down.  A copy: 7919 x 252 bfloat16 3 us, 20567 x 963 float32
-// 24 us (6.6 TB/s).  The products that went without it, by single elements through registers into shared memory, took 17 us for
-// 7919 x 252 x 505 in bfloat16 and 28 for its dw; copied first 16 and 25, and one kernel less of each kind.
-template <int ES>
-__global__ __launch_bounds__(256) void k_pad(const char* __restrict__ in, int64_t ld, int64_t rows, int K, char* __restrict__ out, int chunks, int lanes_log2) {
-    constexpr int V = 16 / ES;
-    const int64_t row = (int64_t)blockIdx.x * (256 >> lanes_log2) + (threadIdx.x >> lanes_log2);
-    if (row >= rows) return;
-    for (int c = threadIdx.x & ((1 << lanes_log2) - 1); c < chunks; c += 1 << lanes_log2) {
-        const int left = K - c * V;
-        const char* const src = in + (row * ld + (int64_t)c * V) * ES;
-        u32x4 v;
-        if (left >= V) {
-            v = load16(src);
-        } else if (c > 0) {
-            const int down = (V - left) * ES;                            // bytes of the chunk before
-            const u32x4 t = load16(src - down);
-            const uint64_t lo = t[0] | (uint64_t)t[1] << 32, hi = t[2] | (uint64_t)t[3] << 32;
-            const int bits = down * 8;                                   // 8 .. 120
-            const uint64_t l = bits < 64 ? (lo >> bits) | (hi << (64 - bits)) : bits == 64 ? hi : hi >> (bits - 64);
-            const uint64_t h = bits < 64 ? hi >> bits : 0;
-            v = u32x4{(uint32_t)l, (uint32_t)(l >> 32), (uint32_t)h, (uint32_t)(h >> 32)};
-        } else {
-            uint8_t u[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) u[e] = *reinterpret_cast<const uint8_t*>(src + min(e, left * ES - 1));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[e] = 0;
-#pragma unroll
-                for (int b = 0; b < 4; ++b) v[e] |= 4 * e + b < left * ES ? (uint32_t)u[4 * e + b] << (8 * b) : 0u;
-            }
-        }
-        *reinterpret_cast<u32x4*>(out + (row * chunks + c) * 16) = v;
-    }
-}
-
 // exponents [rows, nb] -> 2^e as floats [nb][ld], zero from rows to ld (65536 x 16: 5.3 us; the products would read each a byte at a
 // time, a row apart)
-__global__ __launch_bounds__(256) void k_lay_steps(const int8_t* __restrict__ exps, int64_t rows, int nb, float* __restrict__ out, int64_t ld) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= ld) return;
-    for (int b = 0; b < nb; ++b) out[b * ld + i] = i < rows ? p8_pow2(exps[i * nb + b]) : 0.0f;
+struct StepsJob {
+    const int8_t* exps;
+    int64_t rows;
+    int nb;
+    float* out;
+    int64_t ld, blocks;
+};
+__device__ __forceinline__ void lay_steps(const StepsJob& j, int64_t block) {
+    const int64_t i = block * 256 + threadIdx.x;
+    if (i >= j.ld) return;
+    for (int b = 0; b < j.nb; ++b) j.out[b * j.ld + i] = i < j.rows ? p8_pow2(j.exps[i * j.nb + b]) : 0.0f;
+}
+// What a weight gradient needs first, one launch: the steps of codes, x (codes: bytes) and ds in whole rows.
+template <int DT, bool P8>
+__global__ __launch_bounds__(256) void k_prepare_over(const StepsJob s, const PadJob x, const PadJob ds) {
+    const int64_t b = blockIdx.x;
+    if (P8 && b < s.blocks) lay_steps(s, b);
+    else if (b < s.blocks + x.blocks) pad_rows<P8 ? 1 : esize(DT)>(x, b - s.blocks);
+    else pad_rows<esize(DT)>(ds, b - s.blocks - x.blocks);
 }
 
 // parts [nparts][n, rounded up to whole 16 bytes] float32 -> their sum in dtype; 16 threads of four neighbours x 16 lanes over the parts,
@@ -1016,17 +1065,11 @@ bool whole_rows(const void* p, int64_t ld, int K, int es, int zeros) {
     return ((uintptr_t)p & 15) == 0 && ld * es % 16 == 0 && ((int64_t)K * es % 16 == 0 || (zeros && ld * es >= ((int64_t)K * es + 15) / 16 * 16)) &&
            ld * es < (1 << 22);
 }
-int pad(int es, const void* in, int64_t ld, int64_t rows, int K, char* out, hipStream_t st) {
-    const int chunks = (int)(((int64_t)K * es + 15) / 16);
-    int log2 = 0;
-    while ((1 << log2) < chunks && log2 < 8) ++log2;
-    const int64_t blocks = (rows + (256 >> log2) - 1) / (256 >> log2);
-    if (blocks > 0x7fffffff) return BS_EINVAL;
-    const dim3 grid((unsigned)blocks);
-    if (es == 4) hipLaunchKernelGGL(k_pad<4>, grid, dim3(256), 0, st, (const char*)in, ld, rows, K, out, chunks, log2);
-    else if (es == 2) hipLaunchKernelGGL(k_pad<2>, grid, dim3(256), 0, st, (const char*)in, ld, rows, K, out, chunks, log2);
-    else hipLaunchKernelGGL(k_pad<1>, grid, dim3(256), 0, st, (const char*)in, ld, rows, K, out, chunks, log2);
-    return BS_OK;
+PadJob pad_job(int es, const void* in, int64_t ld, int64_t rows, int K, char* out) {
+    PadJob j = {(const char*)in, ld, rows, K, out, (int)(((int64_t)K * es + 15) / 16), 0, 0};
+    while ((1 << j.lanes_log2) < j.chunks && j.lanes_log2 < 8) ++j.lanes_log2;
+    j.blocks = (rows + (256 >> j.lanes_log2) - 1) / (256 >> j.lanes_log2);
+    return j;
 }
 
 // out [rows, N] over K; whole: rows of x that DMA can take
@@ -1043,31 +1086,32 @@ int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream
     const int64_t need = rows_bytes(DT, a.rows, a.K, a.N, whole);
     if (need > 0 && (!workspace || bytes < need)) return BS_EINVAL;
     if (a.K > MAX_WIDTH || a.N > MAX_WIDTH) return BS_EINVAL;          // 31-bit offsets into a tile's rows, and the grids below
-    const bool lay = !small && !as_is;
-    if (lay) {
-        const dim3 grid((unsigned)(kp / 32), (unsigned)((a.N + 31) / 32));
-        constexpr int KB = kb_of(DT);
-        const bool chunks = DT != BS_DT_F32 && !a.wt && a.K % 8 == 0 && a.ldw % 8 == 0 && ((uintptr_t)a.w & 15) == 0;
-        if (chunks) hipLaunchKernelGGL(k_lay_chunks, dim3((unsigned)(kp / 64), (unsigned)((a.N + 31) / 32)), dim3(256), 0, st, a.w, a.ldw, a.N, a.K, (char*)workspace);
-        else if (a.wt) hipLaunchKernelGGL((k_lay_w<DT, true>), grid, dim3(256), 0, st, a.w, a.ldw, a.N, a.K, kp, (char*)workspace);
-        else hipLaunchKernelGGL((k_lay_w<DT, false>), grid, dim3(256), 0, st, a.w, a.ldw, a.N, a.K, kp, (char*)workspace);
-        a.wl = (const char*)workspace; a.sp = KB; a.sl = (int64_t)a.N * KB; a.sk = a.sl * limbs_of(DT);
-    } else {
-        a.wl = a.w; a.sp = a.ldw; a.sl = 0; a.sk = kb_of(DT);
-    }
     if (small) {
         a.tp = (a.N + 31) / 32;
         const unsigned blocks = (unsigned)((a.rows + 31) / 32 * a.tp);
         hipLaunchKernelGGL((k_relay<DT, EPI, EPI == E_PLAIN>), dim3(blocks), dim3(256), 0, st, a);      // (E_PLAIN: dx, w [K, N])
         return rows_rc();
     }
+    LayJob l = {};
+    PadJob x = {};
     a.Kx = (a.K + CK - 1) / CK * CK;
     a.xd = a.x; a.ldxd = a.ldx;
-    if (!whole) {
-        char* const to = (char*)workspace + lay_bytes(DT, a.K, a.N);
-        if (pad(ES, a.x, a.ldx, a.rows, a.K, to, st) != BS_OK) return BS_EINVAL;
-        a.xd = to; a.ldxd = a.Kx;
+    if (as_is) {
+        a.wl = a.w; a.sp = a.ldw; a.sl = 0; a.sk = kb_of(DT);
+    } else {
+        constexpr int KB = kb_of(DT);
+        l = {a.w, a.ldw, a.N, a.K, (char*)workspace, kp / 32, 0, DT != BS_DT_F32 && !a.wt && a.K % 8 == 0 && a.ldw % 8 == 0 && ((uintptr_t)a.w & 15) == 0};
+        if (l.chunks) l.across = kp / 64;
+        l.blocks = l.across * ((a.N + 31) / 32);
+        a.wl = (const char*)workspace; a.sp = KB; a.sl = (int64_t)a.N * KB; a.sk = a.sl * limbs_of(DT);
     }
+    if (!whole) {
+        x = pad_job(ES, a.x, a.ldx, a.rows, a.K, (char*)workspace + lay_bytes(DT, a.K, a.N));
+        a.xd = x.out; a.ldxd = a.Kx;
+    }
+    if (l.blocks + x.blocks > 0x7fffffff) return BS_EINVAL;
+    if (l.blocks + x.blocks > 0)
+        hipLaunchKernelGGL((k_prepare<DT, EPI == E_PLAIN>), dim3((unsigned)(l.blocks + x.blocks)), dim3(256), 0, st, l, x);
 #define ROWS(BQ, BP, WQ, WP, BK, NS, PS) do { a.tp = (a.N + BP - 1) / BP; a.tiles = tiles_of(a.rows, a.N, BQ, BP); \
         const int64_t blocks = (a.tiles + 7) / 8 * 8; if (blocks > 0x7fffffff) return BS_EINVAL; \
         hipLaunchKernelGGL((k_rows_dma<DT, EPI, BQ, BP, WQ, WP, BK, NS, PS>), dim3((unsigned)blocks), dim3((BQ / WQ) * (BP / WP) * 64), 0, st, a); } while (0)
@@ -1214,14 +1258,26 @@ int bs_linear_grad_w(const void* ds, int64_t ldds, int zeros, const void* x, con
         a.xd = a.x; a.ldxd = ldx; a.dd = a.ds; a.lddd = ldds; a.pstride = (n + 3) / 4 * 4;
         a.out = joined ? ws + b.steps + b.x + b.ds : (char*)dw;
         const int64_t ld = (rows + 63) / 64 * 64;
-        if (x_exps) hipLaunchKernelGGL(k_lay_steps, dim3((unsigned)((ld + 255) / 256)), dim3(256), 0, st, x_exps, rows, a.nb, (float*)ws, ld);
+        StepsJob sj = {};
+        PadJob xj = {}, dj = {};
+        if (x_exps) sj = {x_exps, rows, a.nb, (float*)ws, ld, (ld + 255) / 256};
         if (!x_whole) {
-            if (pad(xe, x, ldx, rows, K, ws + b.steps, st) != BS_OK) return BS_EINVAL;
-            a.xd = ws + b.steps; a.ldxd = (K + 16 / xe - 1) / (16 / xe) * (16 / xe);
+            xj = pad_job(xe, x, ldx, rows, K, ws + b.steps);
+            a.xd = xj.out; a.ldxd = (K + 16 / xe - 1) / (16 / xe) * (16 / xe);
         }
         if (!ds_whole) {
-            if (pad(es, ds, ldds, rows, N, ws + b.steps + b.x, st) != BS_OK) return BS_EINVAL;
-            a.dd = ws + b.steps + b.x; a.lddd = (N + 16 / es - 1) / (16 / es) * (16 / es);
+            dj = pad_job(es, ds, ldds, rows, N, ws + b.steps + b.x);
+            a.dd = dj.out; a.lddd = (N + 16 / es - 1) / (16 / es) * (16 / es);
+        }
+        const int64_t first = sj.blocks + xj.blocks + dj.blocks;
+        if (first > 0x7fffffff) return BS_EINVAL;
+        if (first > 0) {
+#define PREPARE(DT) do { if (x_exps) hipLaunchKernelGGL((k_prepare_over<DT, true>), dim3((unsigned)first), dim3(256), 0, st, sj, xj, dj); \
+                         else hipLaunchKernelGGL((k_prepare_over<DT, false>), dim3((unsigned)first), dim3(256), 0, st, sj, xj, dj); } while (0)
+            if (dtype == BS_DT_F32) PREPARE(BS_DT_F32);
+            else if (dtype == BS_DT_BF16) PREPARE(BS_DT_BF16);
+            else PREPARE(BS_DT_F16);
+#undef PREPARE
         }
         const int rc = dtype == BS_DT_F32 ? launch_over<BS_DT_F32>(a, (float*)ws, ld, st) : dtype == BS_DT_BF16 ? launch_over<BS_DT_BF16>(a, (float*)ws, ld, st)
                                                                                               : launch_over<BS_DT_F16>(a, (float*)ws, ld, st);
