@@ -1050,6 +1050,10 @@ bool enough(int64_t rows, int N, int bq, int bp) { return tiles_of(rows, N, bq, 
 //     bf16  (16384, 2048, 2048) 145 and 168                 (102400, 256, 256) 50 and 43
 //     f32   (4942, 832, 1168) 72 and 84                     (40000, 256, 256) 54 and 45,  (8192, 256, 512) 25.5 and 22.3
 constexpr int DEEP_K = 512;
+//   or, float32, where it saves a round: 512 of its tiles are on the chip at once, 768 of 64x128, a round of which costs 3/4 as much
+//     (25600, 256, 256), a round of 400 against two of 800, 35 and 41;   (50000, 64, 128), 391, 23 and 25;   (7400, 300, 1000), 464, 48
+//     and 44;   (16384, 256, 512), 512, 39 and 39;   no round saved: (40000, 256, 256), 54 and 45
+bool fewer_rounds(int64_t rows, int N) { return 4 * ((tiles_of(rows, N, 128, 128) + 511) / 512) < 3 * ((tiles_of(rows, N, 64, 128) + 767) / 768); }
 //   and, 16-bit, where its tiles fill four fifths of the rounds that they take:
 //     (16384, 1024, 1024), 256 tiles, 46 and 50             (12288, 512, 1024), 192 tiles, 29 and 23
 bool fills(int64_t rows, int N) {
@@ -1116,7 +1120,7 @@ int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream
         const int64_t blocks = (a.tiles + 7) / 8 * 8; if (blocks > 0x7fffffff) return BS_EINVAL; \
         hipLaunchKernelGGL((k_rows_dma<DT, EPI, BQ, BP, WQ, WP, BK, NS, PS>), dim3((unsigned)blocks), dim3((BQ / WQ) * (BP / WP) * 64), 0, st, a); } while (0)
     if constexpr (DT == BS_DT_F32) {
-        if (a.K >= DEEP_K && a.N > 64 && enough(a.rows, a.N, 128, 128)) ROWS(128, 128, 32, 128, 16, 3, 2);
+        if (a.N > 64 && enough(a.rows, a.N, 128, 128) && (a.K >= DEEP_K || fewer_rounds(a.rows, a.N))) ROWS(128, 128, 32, 128, 16, 3, 2);
         else if (a.N > 64 && enough(a.rows, a.N, 64, 128)) ROWS(64, 128, 32, 64, 16, 3, 3);
         else ROWS(64, 64, 32, 32, 32, 4, 1);
     } else {
