@@ -874,7 +874,6 @@ def _scratch(like, nbytes):
     return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
-
 def _dtype_code(t, what):
     code = _DTYPES.get(t.dtype)
     if code is None:
