@@ -946,25 +946,28 @@ class Packed8:
 def pack8(x):
     """x [..., C] float32 / bfloat16 / float16 -> Packed8."""
     dev = _gpu(x)
-    code = _dtype_code(x, "pack8")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise BitswapHipError(f"pack8: expected [..., C], got {tuple(x.shape)}")
-    width = x.shape[-1]
+    code, shape = _dtype_code(x, "pack8"), x.shape
+    if not shape or shape[-1] < 1:
+        raise BitswapHipError(f"pack8: expected [..., C], got {tuple(shape)}")
+    width = shape[-1]
     t, ld, rows = _as_rows(x, width, "pack8")
     codes = x.new_empty((rows, width), dtype=torch.int8)
     exps = x.new_empty((rows, -(-width // PACK8_BLOCK)), dtype=torch.int8)
-    _check(load().bs_pack8(_at(t), ld, _at(codes), _at(exps), code, rows, width, _raw_stream(dev)), "bs_pack8")
-    return Packed8(codes, exps, x.shape, x.dtype)
+    _check(load().bs_pack8(t.data_ptr(), ld, codes.data_ptr(), exps.data_ptr(), code, rows, width, _raw_stream(dev)), "bs_pack8")
+    p = object.__new__(Packed8)                      # its parts need no checks here
+    p.codes, p.exps, p.shape, p.dtype = codes, exps, tuple(shape), x.dtype
+    return p
 
 
 def unpack8(p):
     """Packed8 -> the values it holds, contiguous, in the type it was packed from."""
     if not isinstance(p, Packed8):
         raise BitswapHipError("unpack8 takes the Packed8 that pack8() returns")
-    dev = _gpu(p.codes, p.exps)
-    x = p.codes.new_empty(p.shape, dtype=p.dtype)
-    _check(load().bs_unpack8(_at(p.codes), _at(p.exps), _at(x), _DTYPES[p.dtype], p.codes.shape[0], p.codes.shape[1], _raw_stream(dev)),
-           "bs_unpack8")
+    codes = p.codes
+    dev = _gpu(codes, p.exps)
+    x = codes.new_empty(p.shape, dtype=p.dtype)
+    rows, width = codes.shape
+    _check(load().bs_unpack8(codes.data_ptr(), p.exps.data_ptr(), x.data_ptr(), _DTYPES[p.dtype], rows, width, _raw_stream(dev)), "bs_unpack8")
     return x
 
 
