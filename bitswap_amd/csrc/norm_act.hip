@@ -250,11 +250,12 @@ __global__ __launch_bounds__(1024) void k_norm(const NormArgs a) {
         ss.groups<1>(nullptr);
 #pragma unroll
         for (int i = 0; i < V; ++i) rs[i] = i < left ? 1.0f / sqrtf(ss.out[g[i]] * inv + a.eps) : 0.0f;
-        if (a.stats && tid < ss.gs) {
-            float* const o = a.stats + (img * a.G + slab * a.gs + tid) * 2;
-            o[0] = mean_sh[tid] * inv;
-            o[1] = 1.0f / sqrtf(ss.out[tid] * inv + a.eps);
-        }
+        if (a.stats)                                                 // (16-bit groups of one channel: up to 121 of them for 64 threads)
+            for (int j = tid; j < ss.gs; j += ss.nthr) {
+                float* const o = a.stats + (img * a.G + slab * a.gs + j) * 2;
+                o[0] = mean_sh[j] * inv;
+                o[1] = 1.0f / sqrtf(ss.out[j] * inv + a.eps);
+            }
     }
     if (!live) return;
     char* const yp = a.y + (img * a.pixels * a.C + c0 + k) * ES;

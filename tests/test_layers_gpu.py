@@ -814,3 +814,27 @@ def test_group_norm_in_the_largest_workgroups(hip, n, pixels, c, groups, dtype, 
     dx = [hip.group_norm_act_grad(x[i:], hip.group_norm_act(x[i:], groups, gamma, beta, act=1, want_stats=True)[1], groups, g[i:], gamma, beta, act=1)[0]
           for i in (0, n - 1)]
     assert torch.equal(dx[0][-1:], dx[1])
+
+
+# ---- the ends of the range: many groups, no rows, far and not finite arguments -----------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,pixels,c,groups", [(2, 1, 128, 128), (3, 4, 65, 65), (2, 16, 256, 256), (1, 28, 65, 65), (2, 40, 65, 65), (1, 9, 1000, 1000),
+                                               (1, 3, 250, 125), (2, 2000, 66, 66)])
+def test_group_norm_stats_of_many_small_groups(hip, n, pixels, c, groups, dtype):
+    """One channel a group (an instance norm): a workgroup then has more groups than threads, and each has its statistics written.
+    The call itself, into memory that holds NaN."""
+    x = randn((n, pixels, c), dtype, 1, 2.0) + 0.5
+    y, stats = torch.empty_like(x), torch.full((n, groups, 2), math.nan, device="cuda")
+    L, code = hip.load(), hip._DTYPES[dtype]
+    need = L.bs_group_norm_workspace(code, n, pixels, c, groups, 0)
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+    rc = L.bs_group_norm_act(x.data_ptr(), pixels * c, c, None, None, 0, 1e-5, 0, code, n, pixels, c, groups, y.data_ptr(), stats.data_ptr(),
+                             ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    assert rc == hip.OK
+    mean, rstd, h, u = norm64(x, groups, None, None, 1e-5)
+    em, er, eu = norm_bounds(x, mean, rstd, h, u, None, groups)
+    close(stats[:, :, 0], mean, em + E * mean.abs(), "mean")
+    close(stats[:, :, 1], rstd, er + E * rstd, "rstd")
+    close(y, u, eu + U[dtype] * (u.abs() + eu) + TINY[dtype], "y")
+    for saved8 in (False, True):
+        check_norm_grad(hip, x, groups, randn((c,), torch.float32, 2), randn((c,), torch.float32, 3), 2, randn((n, pixels, c), dtype, 4, 0.1), saved8)
