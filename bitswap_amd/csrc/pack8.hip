@@ -195,8 +195,8 @@ int bs_act_grad(const void* g_sum, int64_t ldgs, const void* g_act, int64_t ldga
     hipStream_t st = rows_stream(stream);
     if (rows > 0 && ((!g_sum && !g_act) || (g_sum && ldgs < N) || (g_act && ldga < N) ||
                      (g_act && act != BS_ACT_NONE && (!s || lds < N)))) return BS_EINVAL;
+    if (rows == 0 && !db_out) return BS_OK;                  // (an empty ds has no address)
     if ((!ds_out && !db_out) || (ds_out && ldds < N)) return BS_EINVAL;
-    if (rows == 0 && !db_out) return BS_OK;
     int64_t part, parts;
     split_rows(rows, N, &part, &parts);
     if (db_out && parts > 1 && (!workspace || workspace_bytes < parts * N * 4)) return BS_EINVAL;

@@ -163,3 +163,14 @@ def test_rows_wider_than_the_kernels_offsets_are_refused(L):
     assert L.bs_group_norm_workspace(0, 1, 8, wide, 1, 0) < 0 and L.bs_group_norm_workspace(0, 1 << 40, 8, 8, 1, 1) < 0
     assert L.bs_pack8(p, 1 << 30, p, p, 0, 1 << 40, 1 << 30, None) == E and L.bs_unpack8(p, p, p, 0, 1 << 40, 1 << 30, None) == E
     del keep
+
+
+def test_act_grad_without_rows_needs_no_output(L):
+    """An empty ds has no address: without rows and without db there is nothing to write, and nothing to refuse."""
+    from bitswap_amd import hip
+    keep, p = buf()
+    assert L.bs_act_grad(p, 8, None, 8, None, None, 8, 0, 0, 0, 8, None, 8, None, None, 0, None) == hip.OK
+    assert L.bs_act_grad(None, 8, None, 8, None, None, 8, 1, 0, 0, 8, None, 8, None, None, 0, None) == hip.OK
+    assert L.bs_act_grad(p, 8, None, 8, None, None, 8, 0, 0, 4, 8, None, 8, None, None, 0, None) == hip.EINVAL      # rows, but nothing asked
+    assert L.bs_act_grad(p, 8, None, 8, None, None, 8, 0, 3, 0, 8, None, 8, None, None, 0, None) == hip.EINVAL
+    del keep

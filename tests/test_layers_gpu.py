@@ -838,3 +838,33 @@ def test_group_norm_stats_of_many_small_groups(hip, n, pixels, c, groups, dtype)
     close(y, u, eu + U[dtype] * (u.abs() + eu) + TINY[dtype], "y")
     for saved8 in (False, True):
         check_norm_grad(hip, x, groups, randn((c,), torch.float32, 2), randn((c,), torch.float32, 3), 2, randn((n, pixels, c), dtype, 4, 0.1), saved8)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_no_rows_whatever_is_asked(hip, dtype):
+    """A call without rows is one, whichever gradients are asked for; parameters' gradients are zero."""
+    from itertools import product
+    w = randn((6, 5), dtype, 1)
+    x, s, g = (torch.empty((0, c), dtype=dtype, device="cuda") for c in (5, 6, 6))
+    for act, both, saved8, *ask in product((0, 1), (False, True), (False, True), *[(False, True)] * 4):
+        xs, ss = (hip.pack8(x), hip.pack8(s)) if saved8 else (x, s)
+        dx, dw, db, dr = hip.linear_act_grad(xs, w, ss, act=act, g_sum=g if both else None, g_act=g, want_x=ask[0], want_w=ask[1], want_bias=ask[2],
+                                             want_res=ask[3])
+        assert [v is not None for v in (dx, dw, db, dr)] == ask
+        assert (dx is None or dx.shape == (0, 5)) and (dr is None or dr.shape == (0, 6))
+        assert (dw is None or torch.equal(dw, torch.zeros_like(w))) and (db is None or torch.equal(db, torch.zeros(6, device="cuda")))
+
+
+@pytest.mark.parametrize("save8", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_layers_without_rows(hip, dtype, save8):
+    from bitswap_amd import layers
+    w, x = randn((6, 5), dtype, 1).requires_grad_(), randn((3, 5), dtype, 2)[:0].requires_grad_()
+    y = layers.linear_act(x, w, act="silu", save8=save8)
+    dx, dw = torch.autograd.grad(y, [x, w], torch.empty_like(y))
+    assert y.shape == (0, 6) and dx.shape == (0, 5) and torch.equal(dw, torch.zeros_like(w))
+    layer = make_layer(60, 44, "elu", dtype, save8)
+    x = randn((2, 4, 4, 60), dtype, 2)[:0].requires_grad_()
+    y = layer(x)
+    got = torch.autograd.grad(y, [x] + list(layer.parameters()), torch.empty_like(y))
+    assert y.shape == got[0].shape == (0, 4, 4, 60) and not any(v.any() for v in got[1:])
