@@ -1113,11 +1113,14 @@ int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream
         x = pad_job(ES, a.x, a.ldx, a.rows, a.K, (char*)workspace + lay_bytes(DT, a.K, a.N));
         a.xd = x.out; a.ldxd = a.Kx;
     }
-    if (l.blocks + x.blocks > 0x7fffffff) return BS_EINVAL;
-    if (l.blocks + x.blocks > 0)
-        hipLaunchKernelGGL((k_prepare<DT, EPI == E_PLAIN>), dim3((unsigned)(l.blocks + x.blocks)), dim3(256), 0, st, l, x);
+    if (too_many(l.blocks + x.blocks, 256)) return BS_EINVAL;
+    auto prepare = [&] {
+        if (l.blocks + x.blocks > 0)
+            hipLaunchKernelGGL((k_prepare<DT, EPI == E_PLAIN>), dim3((unsigned)(l.blocks + x.blocks)), dim3(256), 0, st, l, x);
+    };
 #define ROWS(BQ, BP, WQ, WP, BK, NS, PS) do { a.tp = (a.N + BP - 1) / BP; a.tiles = tiles_of(a.rows, a.N, BQ, BP); \
-        const int64_t blocks = (a.tiles + 7) / 8 * 8; if (blocks > 0x7fffffff) return BS_EINVAL; \
+        const int64_t blocks = (a.tiles + 7) / 8 * 8; if (too_many(blocks, (BQ / WQ) * (BP / WP) * 64)) return BS_EINVAL; \
+        prepare(); \
         hipLaunchKernelGGL((k_rows_dma<DT, EPI, BQ, BP, WQ, WP, BK, NS, PS>), dim3((unsigned)blocks), dim3((BQ / WQ) * (BP / WP) * 64), 0, st, a); } while (0)
     if constexpr (DT == BS_DT_F32) {
         if (a.N > 64 && enough(a.rows, a.N, 128, 128) && (a.K >= DEEP_K || fewer_rounds(a.rows, a.N))) ROWS(128, 128, 32, 128, 16, 3, 2);
@@ -1170,7 +1173,7 @@ OverBytes over_bytes(int dtype, int64_t rows, int K, int N, bool codes, bool x_w
 template <int DT>
 int launch_over(OverArgs a, const float* steps, int64_t ld, hipStream_t st) {
 #define OVER(P8, BQ, WQ, BK_, NS) do { a.tp = (a.K + 127) / 128; a.tiles = tiles_of(a.N, a.K, BQ, 128) * a.parts; \
-        const int64_t blocks = (a.tiles + 7) / 8 * 8; if (blocks > 0x7fffffff) return BS_EINVAL; \
+        const int64_t blocks = (a.tiles + 7) / 8 * 8; \
         hipLaunchKernelGGL((k_over_dma<DT, P8, BQ, 128, WQ, 64, BK_, NS>), dim3((unsigned)blocks), dim3(256), 0, st, a, steps, ld); } while (0)
     if (a.exps) {
         if constexpr (DT == BS_DT_F32) {
@@ -1246,7 +1249,6 @@ int bs_linear_grad_w(const void* ds, int64_t ldds, int zeros, const void* x, con
     if (rows > 0 && (!ds || !x || ldds < N || ldx < K)) return BS_EINVAL;
     hipStream_t st = rows_stream(stream);
     const int64_t n = (int64_t)K * N;
-    if ((n + 63) / 64 > 0x7fffffff) return BS_EINVAL;
     const int es = esize(dtype), xe = x_exps ? 1 : es;
     const bool x_whole = whole_rows(x, ldx, K, xe, 0), ds_whole = whole_rows(ds, ldds, N, es, zeros);
     const OverBytes b = over_bytes(dtype, rows, K, N, x_exps != nullptr, x_whole, ds_whole);
@@ -1274,7 +1276,7 @@ int bs_linear_grad_w(const void* ds, int64_t ldds, int zeros, const void* x, con
             a.dd = dj.out; a.lddd = (N + 16 / es - 1) / (16 / es) * (16 / es);
         }
         const int64_t first = sj.blocks + xj.blocks + dj.blocks;
-        if (first > 0x7fffffff) return BS_EINVAL;
+        if (too_many(first, 256) || too_many(tiles_of(N, K, over_bq(dtype, rows, K, N), 128) * parts + 7, 256)) return BS_EINVAL;
         if (first > 0) {
 #define PREPARE(DT) do { if (x_exps) hipLaunchKernelGGL((k_prepare_over<DT, true>), dim3((unsigned)first), dim3(256), 0, st, sj, xj, dj); \
                          else hipLaunchKernelGGL((k_prepare_over<DT, false>), dim3((unsigned)first), dim3(256), 0, st, sj, xj, dj); } while (0)
@@ -1290,10 +1292,15 @@ int bs_linear_grad_w(const void* ds, int64_t ldds, int zeros, const void* x, con
         parts = 0;                                            // the sum of no parts
     }
     const float* const from = (const float*)(ws + b.steps + b.x + b.ds);
-    const dim3 blocks((unsigned)((n + 63) / 64));
-    if (dtype == BS_DT_F32) hipLaunchKernelGGL(k_add_parts<BS_DT_F32>, blocks, dim3(256), 0, st, from, (int)parts, n, (char*)dw);
-    else if (dtype == BS_DT_BF16) hipLaunchKernelGGL(k_add_parts<BS_DT_BF16>, blocks, dim3(256), 0, st, from, (int)parts, n, (char*)dw);
-    else hipLaunchKernelGGL(k_add_parts<BS_DT_F16>, blocks, dim3(256), 0, st, from, (int)parts, n, (char*)dw);
+    constexpr int64_t once = (int64_t)1 << 29;               // values of a launch (only a sum of no parts has more)
+    for (int64_t at = 0; at < n; at += once) {
+        const int64_t count = n - at < once ? n - at : once;
+        const dim3 blocks((unsigned)((count + 63) / 64));
+        char* const to = (char*)dw + at * es;
+        if (dtype == BS_DT_F32) hipLaunchKernelGGL(k_add_parts<BS_DT_F32>, blocks, dim3(256), 0, st, from, (int)parts, count, to);
+        else if (dtype == BS_DT_BF16) hipLaunchKernelGGL(k_add_parts<BS_DT_BF16>, blocks, dim3(256), 0, st, from, (int)parts, count, to);
+        else hipLaunchKernelGGL(k_add_parts<BS_DT_F16>, blocks, dim3(256), 0, st, from, (int)parts, count, to);
+    }
     return rows_rc();
 }
 

@@ -659,7 +659,7 @@ int bs_group_norm_act(const void* x, int64_t ldn, int64_t ldp, const void* gamma
     fill(&a, p);
     hipStream_t st = rows_stream(stream);
     const int64_t blocks = p.fits ? (n * p.slabs + 7) / 8 * 8 : n * p.runs;
-    if (blocks > 0x7fffffff || n * groups > 0x7fffffff) return BS_EINVAL;
+    if (p.fits ? too_many(blocks, p.threads) : too_many(blocks, 256) || too_many(n * groups, 256)) return BS_EINVAL;
     if (p.fits) {
 #define GO(DT) do { if (p.lanes) hipLaunchKernelGGL((k_norm<DT, true>), dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a); \
                     else hipLaunchKernelGGL((k_norm<DT, false>), dim3((unsigned)blocks), dim3(p.threads), p.lds, st, a); } while (0)
@@ -707,7 +707,7 @@ int bs_group_norm_act_grad(const void* g, int64_t ldgn, int64_t ldgp, const void
     a.y = (char*)dx; a.stats = (float*)stats; a.parts = (float*)workspace;
     fill(&a, p);
     const int64_t blocks = p.fits ? (n * p.slabs + 7) / 8 * 8 : n * p.runs;
-    if (blocks > 0x7fffffff || n * groups > 0x7fffffff) return BS_EINVAL;
+    if (p.fits ? too_many(blocks, p.threads) : too_many(blocks, 256) || too_many(n * groups, 256)) return BS_EINVAL;
     if (p.fits) {
         if (!dgamma && !dbeta) a.parts = nullptr;
         // Builds by the registers that a number of threads leaves, in us at (images, pixels, channels, groups), bf16.  Exchanges: 128,

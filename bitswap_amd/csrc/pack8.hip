@@ -154,7 +154,7 @@ int bs_pack8(const void* x, int64_t ldx, int8_t* codes, int8_t* exps, int dtype,
     const int nb = (channels + P8_BLOCK - 1) / P8_BLOCK;
     if (rows > MAX_ROWS / nb) return BS_EINVAL;
     const int64_t threads = rows * nb * (dtype == BS_DT_F32 ? 8 : 4), blocks = (threads + 255) / 256;
-    if (blocks > 0x7fffffff) return BS_EINVAL;
+    if (too_many(blocks, 256)) return BS_EINVAL;
     hipStream_t st = rows_stream(stream);
 #define PACK(DT) hipLaunchKernelGGL(k_pack8<DT>, dim3((unsigned)blocks), dim3(256), 0, st, (const char*)x, ldx, codes, exps, rows, channels, nb)
     if (dtype == BS_DT_F32) PACK(BS_DT_F32);
@@ -171,7 +171,7 @@ int bs_unpack8(const int8_t* codes, const int8_t* exps, void* x, int dtype, int6
     const int nb = (channels + P8_BLOCK - 1) / P8_BLOCK, V = dtype == BS_DT_F32 ? 4 : 8, cpr = (channels + V - 1) / V;
     if (rows > MAX_ROWS / cpr) return BS_EINVAL;
     const int64_t blocks = (rows * cpr + 255) / 256;
-    if (blocks > 0x7fffffff) return BS_EINVAL;
+    if (too_many(blocks, 256)) return BS_EINVAL;
     hipStream_t st = rows_stream(stream);
 #define UNPACK(DT) hipLaunchKernelGGL(k_unpack8<DT>, dim3((unsigned)blocks), dim3(256), 0, st, codes, exps, (char*)x, rows, channels, nb, cpr)
     if (dtype == BS_DT_F32) UNPACK(BS_DT_F32);

@@ -288,6 +288,8 @@ static __global__ __launch_bounds__(1024) void k_sum_columns(const float* __rest
 inline bool bad_type(int dt) { return dt != BS_DT_F32 && dt != BS_DT_BF16 && dt != BS_DT_F16; }
 constexpr int64_t MAX_ROWS = (int64_t)1 << 40;
 inline hipStream_t rows_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
+// a launch has fewer than 2^32 threads along an axis: a call that would need more is refused before its first launch
+inline bool too_many(int64_t blocks, int threads) { return blocks > (int64_t)0xffffffff / threads; }
 inline int rows_rc() { return hipGetLastError() == hipSuccess ? BS_OK : BS_ELAUNCH; }
 
 }  // namespace

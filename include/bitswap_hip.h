@@ -387,7 +387,8 @@ int bs_wino_out_f32(const float* M, const float* bias, const float* res, float* 
  *   bs_unpack8 -- x = code 2^e, exact in every dtype that held x; -128 gives NaN.
  *
  * All of them: BS_EINVAL for null operands, negative sizes, strides below the row length, unknown types or activations, a
- * workspace that is too small; rows == 0 or n == 0 is a call without rows (gradients of parameters are then zero).
+ * workspace that is too small, sizes that would take a launch of 2^32 threads or more (operands of tens of gigabytes; nothing has
+ * been launched then); rows == 0 or n == 0 is a call without rows (gradients of parameters are then zero).
  */
 #define BS_DT_F32 0
 #define BS_DT_BF16 1

@@ -174,3 +174,24 @@ def test_act_grad_without_rows_needs_no_output(L):
     assert L.bs_act_grad(p, 8, None, 8, None, None, 8, 0, 0, 4, 8, None, 8, None, None, 0, None) == hip.EINVAL      # rows, but nothing asked
     assert L.bs_act_grad(p, 8, None, 8, None, None, 8, 0, 3, 0, 8, None, 8, None, None, 0, None) == hip.EINVAL
     del keep
+
+
+def test_calls_of_more_threads_than_a_launch_has_are_refused(L):
+    """2^32 threads along an axis or more: refused on the host, before a first launch writes anything."""
+    from bitswap_amd import hip
+    keep, p = buf()
+    E, room = hip.EINVAL, 1 << 60
+    assert L.bs_pack8(p, 64, p, p, 0, 1 << 30, 64, None) == E and L.bs_pack8(p, 64, p, p, 1, 1 << 30, 64, None) == E
+    assert L.bs_unpack8(p, p, p, 0, 1 << 30, 64, None) == E and L.bs_unpack8(p, p, p, 2, 1 << 30, 64, None) == E
+    for dt in (0, 1, 2):
+        assert L.bs_linear_act(p, 8, p, 8, None, 0, None, 0, p, None, 0, dt, 1 << 34, 8, 64, p, room, None) == E           # tiles
+        assert L.bs_linear_act(p, 4097, p, 4097, None, 0, None, 0, p, None, 0, dt, 1 << 25, 4097, 8, p, room, None) == E   # rows to be copied
+        assert L.bs_linear_grad_x(p, 64, 0, p, 8, p, dt, 1 << 36, 8, 64, p, room, None) == E
+        assert L.bs_linear_grad_w(p, 8, 0, p, None, 4097, p, dt, 1 << 25, 4097, 8, p, room, None) == E                     # rows to be copied
+        assert L.bs_linear_grad_w(p, 1 << 20, 0, p, None, 1 << 20, p, dt, 1, 1 << 20, 1 << 20, p, room, None) == E         # tiles
+        assert L.bs_group_norm_act(p, 8, 8, None, None, 0, 1e-5, 0, dt, 1 << 27, 1, 8, 2, p, None, None, 0, None) == E     # images that fit
+        assert L.bs_group_norm_act(p, 64000, 8, None, None, 0, 1e-5, 0, dt, 1 << 20, 8000, 8, 2, p, None, p, room, None) == E      # runs
+        assert L.bs_group_norm_act(p, 64 * 3000, 64, None, None, 0, 1e-5, 0, dt, 1 << 19, 3000, 64, 64, p, None, p, room, None) == E        # groups
+        assert L.bs_group_norm_act_grad(p, 8, 8, p, None, 8, 8, p, None, None, 0, 0, dt, 1 << 27, 1, 8, 2, p, None, None, p, room, None) == E
+        assert L.bs_group_norm_act_grad(p, 64000, 8, p, None, 64000, 8, p, None, None, 0, 0, dt, 1 << 20, 8000, 8, 2, p, None, None, p, room, None) == E
+    del keep
