@@ -868,3 +868,33 @@ def test_layers_without_rows(hip, dtype, save8):
     y = layer(x)
     got = torch.autograd.grad(y, [x] + list(layer.parameters()), torch.empty_like(y))
     assert y.shape == got[0].shape == (0, 4, 4, 60) and not any(v.any() for v in got[1:])
+
+
+@pytest.mark.parametrize("act", range(4))
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_activations_and_slopes_at_the_ends_of_the_range(hip, dtype, act):
+    """Where a value is not finite the definition's s / (1 + e^-s), s Phi(s) in IEEE arithmetic say what comes out: SiLU and GELU of
+    -inf are -inf 0 = NaN, as their slopes at either infinity are.  Finite arguments, to the type's largest: values and slopes
+    by their bounds -- e^s is off by 2^-24 |s| relative and at most 2^-150 from |s| = 104 on, so |s| counts up to 104."""
+    inf, big = math.inf, torch.finfo(dtype).max
+    ends = torch.tensor([inf, -inf, math.nan], device="cuda").to(dtype)
+    one = torch.ones(1, 1, device="cuda", dtype=dtype)
+    y = hip.linear_act(ends.view(-1, 1), one, act=act)[1].view(-1).float()
+    want = {0: [inf, -inf, math.nan], 1: [inf, -1.0, math.nan], 2: [inf, math.nan, math.nan], 3: [inf, math.nan, math.nan]}[act]
+    assert torch.equal(y.nan_to_num(12345.0, inf, -inf), torch.tensor(want, device="cuda").nan_to_num(12345.0, inf, -inf))
+    slope = hip.linear_act_grad(None, one, ends.view(-1, 1), act=act, g_act=torch.ones_like(ends).view(-1, 1), want_x=False, want_w=False,
+                                want_bias=False, want_res=True)[3].view(-1).float()
+    if act in (0, 1):
+        assert slope[:2].tolist() == ([1.0, 1.0] if act == 0 else [1.0, 0.0])
+    else:
+        assert torch.isnan(slope).all()
+    s = torch.tensor([0.0, -0.0, 1e-30, -1e-30, 1e-6, -1e-6, 0.5, -0.5, 12.0, -12.0, 50.0, -50.0, 88.0, -88.0, 89.0, -89.0, 104.0, -104.0, 1e4, -1e4, big, -big],
+                     device="cuda").to(dtype)
+    g = torch.ones_like(s)
+    ds = hip.linear_act_grad(None, one, s.view(-1, 1), act=act, g_act=g.view(-1, 1), want_x=False, want_w=False, want_bias=False, want_res=True)[3].view(-1)
+    want = slope64(s.double(), act)
+    off = 16 * E * (1 + s.double().abs().clamp(max=104)) * (act != 0)
+    close(ds, want, off + U[dtype] * (want.abs() + off) + TINY[dtype], "slope")
+    y = hip.linear_act(s.view(-1, 1), one, act=act)[1].view(-1)
+    want = act64(s.double(), act)
+    close(y, want, off + U[dtype] * (want.abs() + off) + TINY[dtype], "value")
