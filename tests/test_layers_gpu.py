@@ -898,3 +898,48 @@ def test_activations_and_slopes_at_the_ends_of_the_range(hip, dtype, act):
     y = hip.linear_act(s.view(-1, 1), one, act=act)[1].view(-1)
     want = act64(s.double(), act)
     close(y, want, off + U[dtype] * (want.abs() + off) + TINY[dtype], "value")
+
+
+@pytest.mark.parametrize("saved8", [False, True])
+@pytest.mark.parametrize("c,groups", [(254, 2), (255, 17)])
+def test_group_norm_at_the_presets_odd_widths(hip, c, groups, saved8):
+    x, g = randn((3, 256, c), torch.float32, 1), randn((3, 256, c), torch.float32, 4, 0.1)
+    gamma, beta = randn((c,), torch.float32, 2), randn((c,), torch.float32, 3)
+    check_norm_grad(hip, x, groups, gamma, beta, 1, g, saved8)
+    y, stats, _ = hip.group_norm_act(x, groups, gamma, beta, act=1, want_stats=True)
+    mean, rstd, h, u = norm64(x, groups, gamma, beta, 1e-5)
+    em, er, eu = norm_bounds(x, mean, rstd, h, u, gamma, groups)
+    close(stats[:, :, 0], mean, em + E * mean.abs(), "mean")
+    close(stats[:, :, 1], rstd, er + E * rstd, "rstd")
+    want = act64(u, 1)
+    slack = 1.13 * eu + 16 * E * (u.abs() + 1)
+    close(y, want, slack + E * (want.abs() + slack), "y")
+    assert torch.equal(hip.group_norm_act(x[1:2], groups, gamma, beta, act=1)[0], y[1:2])
+
+
+@pytest.mark.parametrize("dataset,nz", [("cifar", 4), ("mnist", 8)])
+def test_preset_with_pointwise_layers_does_not_depend_on_the_batch(hip, dataset, nz):
+    """A preset's width (254, run at 256 channels by the convolutions, and 61: no whole 16-byte rows): the padding comes off and
+    nothing of it is left, and every chain's (mu, scale) is the same by itself as beside others."""
+    from bitswap_amd.model import preset
+    torch.manual_seed(11)
+    m = preset(dataset, nz, npoint=1)
+    with torch.no_grad():
+        for k, p in m.named_parameters():
+            if k.endswith((".w2", ".beta")):
+                p.add_(0.1 * torch.randn(p.shape))
+    m = m.cuda().eval().fold().fuse()
+    m.compress(True)
+    z = randn((3, m.zdim_flat), torch.float32, 8)
+    width = m.point_gen[1][0].gamma.numel()
+    h = randn((2, width, 16, 16), torch.float32, 9)
+    with torch.no_grad():
+        want = m.point_gen[1](h.permute(0, 2, 3, 1).contiguous()).permute(0, 3, 1, 2)
+        padded = torch.cat([h, h.new_zeros((2, m._cp - width, 16, 16))], 1) if m._cp > width else h
+        assert torch.equal(m._point_fused("point_gen", 1, padded, False), want)
+        for f in (m.generate(0), m.generate(1), m.infer(1)):
+            whole = f(given=z)
+            assert all(torch.isfinite(u).all() for u in whole)
+            for b in range(3):
+                one = f(given=z[b:b + 1])
+                assert all(torch.equal(u[b:b + 1] if u.shape[0] == 3 else u, v) for u, v in zip(whole, one)), b
