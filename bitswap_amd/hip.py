@@ -56,7 +56,15 @@ def load():
             "bitswap_amd has no CPU fallback for the entropy-coding path.")
     L = C.CDLL(path)
     p, i64, i32 = C.c_void_p, C.c_int64, C.c_int
-    L.bs_abi_version.restype = i32
+    # (the version first, then the names: an older library lacks the newer entry points, which would end in an AttributeError below)
+    version = L.bs_abi_version() if hasattr(L, "bs_abi_version") else None
+    if version != ABI_VERSION:
+        raise BitswapHipError(f"{path} has ABI version {version}, this binding needs {ABI_VERSION}: "
+                              "rebuild with `python -m bitswap_amd.build`")
+    missing = [n for n in SYMBOLS if not hasattr(L, n)]
+    if missing:
+        raise BitswapHipError(f"{path} lacks {', '.join(missing[:4])}{' ...' if len(missing) > 4 else ''}: it was built from older sources; "
+                              "rebuild with `python -m bitswap_amd.build`")
     L.bs_cdf_spec.restype = i32
     L.bs_strerror.restype = C.c_char_p
     L.bs_strerror.argtypes = [i32]
@@ -100,9 +108,6 @@ def load():
     for n in SYMBOLS:
         if n != "bs_strerror":
             getattr(L, n).restype = i64 if n.endswith("_workspace") else i32
-    if L.bs_abi_version() != ABI_VERSION:
-        raise BitswapHipError(f"{path} has ABI version {L.bs_abi_version()}, this binding needs {ABI_VERSION}: "
-                              "rebuild with `python -m bitswap_amd.build`")
     _lib = L
     return L
 

@@ -44,7 +44,9 @@ extern "C" {
  * 6: explicit cdf_spec argument (after bin_step) of bs_logistic_tables / _fc, bs_rans_pop_pivot, bs_layer_pop64 / _push64;
  *    CDF spec 3
  * 7: CDF spec 4 accepted wherever a cdf_spec is taken; BS_POP_PIVOT_MAX_D (the pivot pop's documented D limit is what its LDS
- *    allows); bs_wino_gemm_bf16x3 launches its wave-specialised shape by default (same products, same bits) */
+ *    allows); bs_wino_gemm_bf16x3 launches its wave-specialised shape by default (same products, same bits)
+ * A version changes when what was there changes.  Entry points that are only added (the channels-last layer operators below) leave
+ * it as it is: a caller that needs them looks their names up. */
 #define BS_ABI_VERSION 7
 /* highest version of the deterministic logistic-CDF specification this library implements;
  * a stream written with one CDF spec can only be decoded with the same one.

@@ -195,3 +195,18 @@ def test_calls_of_more_threads_than_a_launch_has_are_refused(L):
         assert L.bs_group_norm_act_grad(p, 8, 8, p, None, 8, 8, p, None, None, 0, 0, dt, 1 << 27, 1, 8, 2, p, None, None, p, room, None) == E
         assert L.bs_group_norm_act_grad(p, 64000, 8, p, None, 64000, 8, p, None, None, 0, 0, dt, 1 << 20, 8000, 8, 2, p, None, None, p, room, None) == E
     del keep
+
+
+@pytest.mark.parametrize("version,says", [(6, "ABI version 6"), (None, "ABI version None"), (7, "lacks bs_")])
+def test_a_library_of_older_sources_says_so(tmp_path, monkeypatch, version, says):
+    """Of another version, or of this one but without the newer entry points: what to do, not an AttributeError."""
+    import subprocess
+    from bitswap_amd import hip
+    src, lib = tmp_path / "old.c", tmp_path / "libold.so"
+    src.write_text(f"int bs_abi_version(void) {{ return {version}; }}" if version else "int bs_nothing(void) { return 0; }")
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(lib), str(src)], check=True)
+    monkeypatch.setattr(hip, "_lib", None)
+    monkeypatch.setattr(hip, "lib_path", lambda: str(lib))
+    with pytest.raises(hip.BitswapHipError, match=says) as e:
+        hip.load()
+    assert "rebuild" in str(e.value)
