@@ -23,6 +23,11 @@ ACTS = {"none": hip.ACT_NONE, "elu": hip.ACT_ELU, "silu": hip.ACT_SILU, "gelu": 
 _PLAIN = {hip.ACT_NONE: lambda s: s, hip.ACT_ELU: F.elu, hip.ACT_SILU: F.silu, hip.ACT_GELU: F.gelu}
 
 
+def _wide(dtype):
+    """The type that 16-bit values are computed in."""
+    return torch.float32 if dtype in (torch.bfloat16, torch.float16) else dtype
+
+
 def _code(act):
     if act in ACTS:
         return ACTS[act]
@@ -80,9 +85,16 @@ def linear_act(x, w, bias=None, res=None, act="elu", want_sum=False, save8=False
     """act(x w^T + bias (+ res)), or (sum, act(sum)) with want_sum.  x [..., K], w [N, K], bias [N], res [..., N]."""
     act = _code(act)
     if not x.is_cuda:
-        s = F.linear(x, w, None if bias is None else bias.to(x.dtype))
-        s = s if res is None else s + res
-        y = _PLAIN[act](s)
+        if w.dim() != 2 or w.dtype != x.dtype or x.shape[-1:] != w.shape[1:]:
+            raise hip.BitswapHipError(f"linear_act: x [..., K] and w [N, K] of one type, got {tuple(x.shape)} {x.dtype} and {tuple(w.shape)} {w.dtype}")
+        if bias is not None and (bias.shape != w.shape[:1] or bias.dtype not in (torch.float32, x.dtype)):
+            raise hip.BitswapHipError(f"linear_act: bias must be [{w.shape[0]}] of float32 or {x.dtype}, got {tuple(bias.shape)} {bias.dtype}")
+        if res is not None and (res.shape != (*x.shape[:-1], w.shape[0]) or res.dtype != x.dtype):
+            raise hip.BitswapHipError(f"linear_act: res must be {(*x.shape[:-1], w.shape[0])} of {x.dtype}, got {tuple(res.shape)} {res.dtype}")
+        wide = _wide(x.dtype)
+        s = F.linear(x.to(wide), w.to(wide), None if bias is None else bias.to(wide))
+        s = s if res is None else s + res.to(wide)
+        s, y = s.to(x.dtype), _PLAIN[act](s).to(x.dtype)                # the activation sees s before its rounding
     elif torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias, res)):
         if act == hip.ACT_NONE:
             s = y = _LinearAct.apply(x, w, bias, res, act, save8)[0]

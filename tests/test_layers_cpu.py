@@ -210,3 +210,32 @@ def test_a_library_of_older_sources_says_so(tmp_path, monkeypatch, version, says
     with pytest.raises(hip.BitswapHipError, match=says) as e:
         hip.load()
     assert "rebuild" in str(e.value)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["none", "elu", "silu", "gelu"])
+def test_linear_act_on_the_cpu_rounds_16_bits_once(act, dtype):
+    """As the kernels do: float32 sums, residual and activation before the one rounding of an output.  Half a step of the type beside
+    the float32 sum of 40 terms, and an activation that is at most 1.13 steep."""
+    from bitswap_amd import layers
+    g = torch.Generator().manual_seed(3)
+    x, w, b, r = (torch.randn(sh, generator=g).to(dtype) for sh in ((50, 40), (30, 40), (30,), (50, 30)))
+    s, y = layers.linear_act(x, w, b, r, act=act, want_sum=True)
+    s64 = x.double() @ w.double().t() + b.double() + r.double()
+    mag = x.double().abs() @ w.double().abs().t() + b.double().abs() + r.double().abs()
+    y64 = {"none": lambda v: v, "elu": torch.nn.functional.elu, "silu": torch.nn.functional.silu, "gelu": torch.nn.functional.gelu}[act](s64)
+    half, e = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype], 1.13 * 48 * 2.0 ** -24 * mag
+    assert s.dtype == y.dtype == dtype
+    assert ((s.double() - s64).abs() <= half * (s64.abs() + e) + e).all()
+    assert ((y.double() - y64).abs() <= half * (y64.abs() + e) + e + 8 * 2.0 ** -24).all()
+    assert torch.equal(layers.linear_act(x, w, b, r, act=act), y)
+
+
+def test_linear_act_on_the_cpu_refuses_what_the_kernels_do():
+    from bitswap_amd import hip, layers
+    x, w = torch.zeros(4, 6), torch.zeros(5, 6)
+    for bad in (dict(res=torch.zeros(1, 5)), dict(res=torch.zeros(5)), dict(res=torch.zeros(4, 1)), dict(res=torch.zeros(4, 5, dtype=torch.float64)),
+                dict(bias=torch.zeros(1)), dict(bias=torch.zeros(5, dtype=torch.float64)), dict(w=torch.zeros(5, 7)), dict(w=w.half()), dict(w=w[0])):
+        with pytest.raises(hip.BitswapHipError):
+            layers.linear_act(**{"x": x, "w": w, **bad})
+    assert layers.linear_act(x.bfloat16(), w.bfloat16(), bias=torch.zeros(5)).dtype == torch.bfloat16
