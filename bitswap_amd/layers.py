@@ -12,6 +12,8 @@ First derivatives only.  A gradient of a parameter comes in the parameter's type
 its gradients with torch.autograd.grad inside the capture: `.backward()` accumulates into leaves through nodes that live as long
 as any graph of the same leaves, on the stream that made them.
 """
+import math
+
 import torch
 import torch.nn.functional as F
 from torch import nn
@@ -133,13 +135,17 @@ def group_norm_act(x, groups, gamma=None, beta=None, eps=1e-5, act="elu", save8=
     """act(group norm of x) on channels-last x [n, ..., C], statistics over the pixels and C / groups channels of a group."""
     act = _code(act)
     if not x.is_cuda:
+        if x.dim() < 2 or x.shape[-1] < 1:
+            raise hip.BitswapHipError(f"group_norm_act: expected [n, ..., C], got {tuple(x.shape)}")
         n, c = x.shape[0], x.shape[-1]
+        pixels = math.prod(x.shape[1:-1])                  # (said, not -1: without images or pixels that is ambiguous)
         if groups < 1 or c % groups:
-            raise ValueError(f"{groups} groups do not divide {c} channels")
-        v = x.reshape(n, -1, groups, c // groups)
-        v = v.float() if v.dtype in (torch.bfloat16, torch.float16) else v
+            raise hip.BitswapHipError(f"group_norm_act: {groups} groups do not divide {c} channels")
+        if not eps >= 0:
+            raise hip.BitswapHipError(f"group_norm_act: eps {eps}")
+        v = x.reshape(n, pixels, groups, c // groups).to(_wide(x.dtype))
         d = v - v.mean((1, 3), keepdim=True)
-        u = (d / torch.sqrt(d.square().mean((1, 3), keepdim=True) + eps)).reshape(n, -1, c)
+        u = (d / torch.sqrt(d.square().mean((1, 3), keepdim=True) + eps)).reshape(n, pixels, c)
         u = u if gamma is None else u * gamma
         u = u if beta is None else u + beta
         return _PLAIN[act](u).to(x.dtype).view(x.shape)

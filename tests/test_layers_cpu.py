@@ -239,3 +239,18 @@ def test_linear_act_on_the_cpu_refuses_what_the_kernels_do():
         with pytest.raises(hip.BitswapHipError):
             layers.linear_act(**{"x": x, "w": w, **bad})
     assert layers.linear_act(x.bfloat16(), w.bfloat16(), bias=torch.zeros(5)).dtype == torch.bfloat16
+
+
+def test_group_norm_on_the_cpu_without_images_or_pixels():
+    """As on a HIP device: an empty result, and no gradient of the parameters; the same refusals."""
+    from bitswap_amd import hip, layers
+    layer = layers.PointwiseResNetLayer(6, groups=3)
+    for shape in ((0, 4, 4, 6), (2, 0, 4, 6), (0, 6)):
+        x = torch.zeros(shape, requires_grad=True)
+        y = layer(x)
+        got = torch.autograd.grad(y, [x] + list(layer.parameters()), torch.zeros(shape))
+        assert y.shape == got[0].shape == torch.Size(shape) and not any(v.any() for v in got[1:])
+    x = torch.zeros(2, 4, 6)
+    for bad in (dict(groups=4), dict(groups=0), dict(groups=2, eps=-1.0), dict(groups=2, eps=float("nan")), dict(groups=2, x=x[0, 0])):
+        with pytest.raises(hip.BitswapHipError):
+            layers.group_norm_act(**{"x": x, **bad})
