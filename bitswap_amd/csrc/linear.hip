@@ -1088,7 +1088,7 @@ int launch_rows(RowsArgs a, int zeros, void* workspace, int64_t bytes, hipStream
     const bool big = DT != BS_DT_F32 && a.K >= DEEP_K && fills(a.rows, a.N);
     const bool as_is = DT != BS_DT_F32 && !a.wt && a.K % 64 == 0 && a.ldw % 8 == 0 && ((uintptr_t)a.w & 15) == 0 && a.ldw < (1 << 21);
     const int64_t need = rows_bytes(DT, a.rows, a.K, a.N, whole);
-    if (need > 0 && (!workspace || bytes < need)) return BS_EINVAL;
+    if (bad_workspace(workspace, bytes, need)) return BS_EINVAL;
     if (a.K > MAX_WIDTH || a.N > MAX_WIDTH) return BS_EINVAL;          // 31-bit offsets into a tile's rows, and the grids below
     if (small) {
         a.tp = (a.N + 31) / 32;
@@ -1254,7 +1254,7 @@ int bs_linear_grad_w(const void* ds, int64_t ldds, int zeros, const void* x, con
     const OverBytes b = over_bytes(dtype, rows, K, N, x_exps != nullptr, x_whole, ds_whole);
     int64_t part, parts;
     split_rows(dtype, rows, K, N, &part, &parts);
-    if (rows > 0 && b.all() > 0 && (!workspace || workspace_bytes < b.all())) return BS_EINVAL;
+    if (rows > 0 && bad_workspace(workspace, workspace_bytes, b.all())) return BS_EINVAL;
     char* const ws = (char*)workspace;                       // steps of the codes | copy of x | copy of ds | parts
     const bool joined = parts > 1;
     if (rows > 0) {

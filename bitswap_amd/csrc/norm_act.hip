@@ -651,7 +651,7 @@ int bs_group_norm_act(const void* x, int64_t ldn, int64_t ldp, const void* gamma
     if ((gamma || beta) && affine_dtype != BS_DT_F32 && affine_dtype != dtype) return BS_EINVAL;
     const Plan p = plan(dtype, n, pixels, channels, groups, 0);
     const int64_t need = bs_group_norm_workspace(dtype, n, pixels, channels, groups, 0);
-    if (need > 0 && (!workspace || workspace_bytes < need)) return BS_EINVAL;
+    if (bad_workspace(workspace, workspace_bytes, need)) return BS_EINVAL;
     NormArgs a = {};
     a.x = (const char*)x; a.ldn = ldn; a.ldp = ldp; a.gamma = (const char*)gamma; a.beta = (const char*)beta;
     a.aff_f32 = affine_dtype == BS_DT_F32; a.act = act; a.eps = eps; a.n = n; a.pixels = pixels;
@@ -698,7 +698,7 @@ int bs_group_norm_act_grad(const void* g, int64_t ldgn, int64_t ldgp, const void
     if ((gamma || beta) && affine_dtype != BS_DT_F32 && affine_dtype != dtype) return BS_EINVAL;
     const Plan p = plan(dtype, n, pixels, channels, groups, 1);
     const int64_t need = bs_group_norm_workspace(dtype, n, pixels, channels, groups, 1);
-    if (!workspace || workspace_bytes < need) return BS_EINVAL;
+    if (bad_workspace(workspace, workspace_bytes, need)) return BS_EINVAL;
     NormArgs a = {};
     a.g = (const char*)g; a.ldgn = ldgn; a.ldgp = ldgp;
     a.x = (const char*)x; a.exps = x_exps; a.ldn = ldn; a.ldp = ldp; a.nb = (channels + P8_BLOCK - 1) / P8_BLOCK;

@@ -199,7 +199,7 @@ int bs_act_grad(const void* g_sum, int64_t ldgs, const void* g_act, int64_t ldga
     if ((!ds_out && !db_out) || (ds_out && ldds < N)) return BS_EINVAL;
     int64_t part, parts;
     split_rows(rows, N, &part, &parts);
-    if (db_out && parts > 1 && (!workspace || workspace_bytes < parts * N * 4)) return BS_EINVAL;
+    if (db_out && parts > 1 && bad_workspace(workspace, workspace_bytes, parts * N * 4)) return BS_EINVAL;
     ActGradArgs a = {};
     a.g_sum = (const char*)g_sum; a.g_act = (const char*)g_act; a.s = (const char*)s; a.exps = s_exps;
     a.ldgs = ldgs; a.ldga = ldga; a.lds = lds; a.rows = rows; a.part = part;

@@ -290,6 +290,8 @@ constexpr int64_t MAX_ROWS = (int64_t)1 << 40;
 inline hipStream_t rows_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 // a launch has fewer than 2^32 threads along an axis: a call that would need more is refused before its first launch
 inline bool too_many(int64_t blocks, int threads) { return blocks > (int64_t)0xffffffff / threads; }
+// a workspace that holds what a call needs; the kernels and their DMA move 16 aligned bytes of it at a time
+inline bool bad_workspace(const void* p, int64_t bytes, int64_t need) { return need > 0 && (!p || ((uintptr_t)p & 15) != 0 || bytes < need); }
 inline int rows_rc() { return hipGetLastError() == hipSuccess ? BS_OK : BS_ELAUNCH; }
 
 }  // namespace

@@ -361,7 +361,7 @@ int bs_wino_out_f32(const float* M, const float* bias, const float* res, float* 
  *   bits do not depend on `rows`.  K, N <= 2^20, here and in the gradients.
  *
  * Workspaces: the *_workspace functions give the bytes a call needs (0: none) for w laid out for the kernel, copies of rows that are
- *   not whole, partial sums.  whole: the operand's address, row stride and row are multiples of 16 bytes and the stride is under 4
+ *   not whole, partial sums; their address is a multiple of 16.  Outputs and workspaces overlap no input.  whole: the operand's address, row stride and row are multiples of 16 bytes and the stride is under 4
  *   MiB; rows that are not are copied first.  zeros (of ds): the rows end in zeros up to the next multiple of 16 bytes, which lies
  *   within their stride, as bs_act_grad writes them -- such rows count as whole.
  *
@@ -389,7 +389,7 @@ int bs_wino_out_f32(const float* M, const float* bias, const float* res, float* 
  *   bs_unpack8 -- x = code 2^e, exact in every dtype that held x; -128 gives NaN.
  *
  * All of them: BS_EINVAL for null operands, negative sizes, strides below the row length, unknown types or activations, a
- * workspace that is too small, sizes that would take a launch of 2^32 threads or more (operands of tens of gigabytes; nothing has
+ * workspace that is too small or not aligned, sizes that would take a launch of 2^32 threads or more (operands of tens of gigabytes; nothing has
  * been launched then); rows == 0 or n == 0 is a call without rows (gradients of parameters are then zero).
  */
 #define BS_DT_F32 0

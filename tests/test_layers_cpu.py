@@ -254,3 +254,20 @@ def test_group_norm_on_the_cpu_without_images_or_pixels():
     for bad in (dict(groups=4), dict(groups=0), dict(groups=2, eps=-1.0), dict(groups=2, eps=float("nan")), dict(groups=2, x=x[0, 0])):
         with pytest.raises(hip.BitswapHipError):
             layers.group_norm_act(**{"x": x, **bad})
+
+
+def test_workspaces_that_are_not_aligned_are_refused(L):
+    """The kernels move 16 aligned bytes of a workspace at a time."""
+    from bitswap_amd import hip
+    keep = (ctypes.c_char * 128)()
+    at = (ctypes.addressof(keep) + 15) & ~15
+    p, E, room = ctypes.c_void_p(at), hip.EINVAL, 1 << 40
+    for off in (1, 4, 8):
+        ws = ctypes.c_void_p(at + off)
+        for dt in (0, 1, 2):
+            assert L.bs_linear_act(p, 8, p, 8, None, 0, None, 0, p, None, 0, dt, 100000, 8, 8, ws, room, None) == E
+            assert L.bs_linear_grad_x(p, 8, 0, p, 8, p, dt, 100000, 8, 8, ws, room, None) == E
+            assert L.bs_linear_grad_w(p, 8, 0, p, None, 8, p, dt, 100000, 8, 8, ws, room, None) == E
+            assert L.bs_act_grad(p, 8, None, 8, None, None, 8, 0, dt, 100000, 8, None, 8, p, ws, room, None) == E
+            assert L.bs_group_norm_act(p, 64000, 8, None, None, 0, 1e-5, 0, dt, 2, 8000, 8, 2, p, None, ws, room, None) == E
+            assert L.bs_group_norm_act_grad(p, 64, 8, p, None, 64, 8, p, None, None, 0, 0, dt, 2, 8, 8, 2, p, None, None, ws, room, None) == E
