@@ -9,8 +9,9 @@
 // where it is long (a library product reaches 1420 TFLOP/s in bfloat16 at 16384 x 2048 x 2048; float32 costs six such products), and
 // below some hundred rows the latency of one load, a chain of matrix instructions and one store.
 //
-// float32 operands are split into three bfloat16 limbs (their sum is the float exactly) and multiplied as the six limb products of
-// total order <= 2; what is left out is of relative size 2^-24.  Limb products of an infinity or of a value that rounds to one are
+// float32 operands are split into three bfloat16 limbs (their sum is the float exactly from 2^-110 on; of a smaller one the bits below
+// 2^-133 are lost, which no bfloat16 has) and multiplied as the six limb products of total order <= 2; what is left out is of relative
+// size 2^-24.  Limb products of an infinity or of a value that rounds to one are
 // NaN, so a sum that does not come out finite is added up again in float32.
 //
 // The output channel is the row index of the matrix instruction: a lane then holds, for one row q = lane % 32 of activations, the

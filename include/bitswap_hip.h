@@ -356,7 +356,8 @@ int bs_wino_out_f32(const float* M, const float* bias, const float* res, float* 
  *
  * bs_linear_act -- s = x w^T + bias (+ res), a = act(s); x [rows, K], w [N, K], bias [N] (nullable), res [rows, N] (nullable);
  *   sum_out = s, act_out = a, contiguous [rows, N] (each nullable, at least one).  act sees s before its rounding.  float32
- *   operands are split into three bfloat16 limbs and multiplied as six limb products (as bs_wino_gemm_bf16x3); a sum that does
+ *   operands are split into three bfloat16 limbs and multiplied as six limb products (as bs_wino_gemm_bf16x3), here and in the
+ *   gradients: operands below 2^-110 keep their bits down to 2^-133 only; a sum that does
  *   not come out finite is added up again in float32, so infinities and NaN arrive as they do in float32 arithmetic.  A row's
  *   bits do not depend on `rows`.  K, N <= 2^20, here and in the gradients.
  *

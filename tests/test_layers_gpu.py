@@ -943,3 +943,23 @@ def test_preset_with_pointwise_layers_does_not_depend_on_the_batch(hip, dataset,
             for b in range(3):
                 one = f(given=z[b:b + 1])
                 assert all(torch.equal(u[b:b + 1] if u.shape[0] == 3 else u, v) for u, v in zip(whole, one)), b
+
+
+@pytest.mark.parametrize("rows", [64, 9000])
+@pytest.mark.parametrize("sx,sw", [(1e-33, 1e20), (1e-36, 1e30), (1e-36, 1.0), (1e-38, 1e37), (1e30, 1e-36), (3e-39, 1e36)])
+def test_linear_act_of_tiny_float32_operands(hip, rows, sx, sw):
+    """A bfloat16 limb has no bits below 2^-133, so an operand below 2^-110 loses those of its 24 that would lie there: at most 2^-134 of
+    every operand, times the other one, beside the usual bound.  (k = 48 terms, and 48 of dx; dw has `rows` of them.)"""
+    n, k = 40, 48
+    x, w, g = randn((rows, k), torch.float32, 1, sx), randn((n, k), torch.float32, 2, sw), randn((rows, n), torch.float32, 3, sx)
+    y = hip.linear_act(x, w, act=0)[1]
+    dx, dw, _, _ = hip.linear_act_grad(x, w, g_act=g, act=0)
+    for got, a, b, terms in ((y, x, w.t(), k), (dx, g, w, n), (dw, g.t(), x, rows)):
+        a, b = a.double().contiguous(), b.double().contiguous()
+        lost = 2.0 ** -134 * (a.abs().sum(1, keepdim=True) + b.abs().sum(0, keepdim=True))
+        want = a @ b
+        # (dw of 1e30 times 1e30: every term is beyond the type, so a float32 sum is infinite from its first term on, with that one's sign,
+        # and parts of either sign add up to NaN)
+        over = want.abs() > torch.finfo(torch.float32).max
+        assert not torch.isfinite(got[over]).any()
+        close(got[~over], want[~over], ((terms + 8) * E * (a.abs() @ b.abs()) + lost + TINY[torch.float32])[~over])
