@@ -201,8 +201,9 @@ __device__ __forceinline__ void turn_and_finish(const RowsArgs& a, const f32x16&
 //
 // Measured: bfloat16 16384 x 2048 x 2048 with GELU, both outputs 134 us (1025 TFLOP/s; the library's product alone 97 us, what is more
 // is the epilogue, which nothing covers with one workgroup a compute unit: 256 x 128 tiles, two of them, 156 us); float32
-// 102400 x 256 x 256 with residual and both outputs 118 us (3.5 TB/s of 419 MB; 55 us of matrix instructions, 86 of traffic, one
-// partly behind the other); bfloat16 25600 x 256 x 256 11.8 us.  Kept after trying the other way: the compiler places the limb splits
+// 102400 x 256 x 256 with residual and both outputs 120 us where two sets of tensors alternate (3.5 TB/s of 419 MB; 55 us of matrix
+// instructions, 86 of traffic, one partly behind the other), 100 to 114 over and over on one set, as the comparisons below are timed;
+// bfloat16 25600 x 256 x 256 11.8 us.  Kept after trying the other way: the compiler places the limb splits
 // (places given to them: 105 us against 100 for 102400 x 256 x 256); a third block of reads ahead, six buffers or steps twice as
 // deep change nothing or cost; 16-bit 128x128 tiles over eight wavefronts of 32 rows, not four of 64 (102400 x 256 x 256 43 and 49 us);
 // 64x64 over four of 32x32, not two of 32x64 (4096 x 256 x 256 5.6 and 6.7 us); float32

@@ -124,8 +124,9 @@ __device__ __forceinline__ void store_vec(char* p, int n, const float* f) {
 
 // store_vec for an output that its launch does not read again, rows of `width` channels: past the L2 (nontemporal), where the inputs
 // that are read again stay.  Not for 16-bit rows that are no multiple of 64 bytes: lines written in two pieces cost more than is won
-// (25600x256 -> 264 bf16: 21.5 us kept, 23.5 us past; -> 288: 20.8 and 18.4; float32 102400x256 -> 256 131 and 110, -> 257 still 22.7
-// and 21.2).
+// (25600x256 -> 264 bf16: 21.5 us kept, 23.5 us past; -> 288: 20.8 and 18.4; float32 102400x256 -> 256 131 and 110).  float32 rows that are
+// no such multiple go both ways: 102400x256 -> 257 178 and 164, 8192x256 -> 257 24.7 and 23.0, but 25600x256 -> 252 39 and 43,
+// 102400x256 -> 100 71 and 82.  All of it a launch over and over by itself; what reads the outputs next is not in it.
 template <int DT>
 __device__ __forceinline__ void store_out(char* p, int n, const float* f, int width) {
     typedef uint32_t u32x4_e __attribute__((ext_vector_type(4), aligned(2)));

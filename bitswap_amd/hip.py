@@ -1026,7 +1026,8 @@ def linear_act(x, w, bias=None, res=None, act=ACT_ELU, want_sum=False, want_act=
 def linear_act_grad(x, w, s=None, act=ACT_NONE, g_sum=None, g_act=None, want_x=True, want_w=True, want_bias=True, want_res=False):
     """Gradients of linear_act -> (dx | None, dw | None, db float32 [N] | None, dres | None) for the gradients g_sum of its sum and
     g_act of its activation (either may be None, not both): ds = g_sum + g_act act'(s), dx = ds w, dw = ds^T x, db = sum of ds over
-    the rows, dres = ds (the incoming gradient itself where nothing changes it).  x and s are the saved input and sum -- whole, or
+    the rows, dres = ds (the incoming gradient itself where nothing changes it).  In 16 bits dx and dw are products of ds rounded to
+    the type, as dres returns it; db is not.  x and s are the saved input and sum -- whole, or
     as Packed8, whose codes the kernels read as they are; s is only needed for g_act with an activation, x only for dw."""
     if g_sum is None and g_act is None:
         raise BitswapHipError("linear_act_grad: no gradient")

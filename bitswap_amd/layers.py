@@ -6,7 +6,8 @@
 
 On a HIP device they run the kernels of csrc/linear.hip, norm_act.hip and pack8.hip; on CPU tensors the same formulas in plain
 torch, as the rest of the Model does there.  save8=True keeps the activations that the backward pass needs in 8 bits
-(hip.Packed8: 1.03 bytes a value); the forward results do not change, the gradients are those at the saved values.
+(hip.Packed8: 1.03 bytes a value); the forward results do not change, the gradients are those at the saved values.  On CPU tensors
+save8 changes nothing: activations are kept whole there.
 
 First derivatives only.  A gradient of a parameter comes in the parameter's type.  To capture a training step into a graph take
 its gradients with torch.autograd.grad inside the capture: `.backward()` accumulates into leaves through nodes that live as long

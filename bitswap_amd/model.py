@@ -219,7 +219,7 @@ class Model(nn.Module):
                  save8=False):
         """Beyond the reference's arguments: nn_batch (above); npoint pointwise residual layers (layers.PointwiseResNetLayer,
         group norm + 1x1 convolutions on channels-last activations) close each of the 2 nz conv stacks in front of its heads --
-        0, the reference's architecture, by default; save8 keeps their activations in 8 bits for the backward pass."""
+        0, the reference's architecture, by default; save8 keeps their activations in 8 bits for the backward pass (HIP devices)."""
         super().__init__()
         self.compressing = False
         self.xs, self.nz, self.zchannels, self.nprocessing = tuple(xs), nz, zchannels, nprocessing

@@ -352,7 +352,8 @@ int bs_wino_out_f32(const float* M, const float* bias, const float* res, float* 
  * pixels of channels-last latents, or any [rows, channels] -- and its gradients.  dtype: BS_DT_F32 / BF16 / F16, the type of x, w,
  * res, s, gradients and outputs; bias, gamma and beta may be float32 beside a 16-bit dtype (their own dtype argument).  Row
  * strides (ld*) are in elements, channels of a row are contiguous, addresses need the alignment of an element only.  Sums and
- * statistics are float32; every output is rounded once, to nearest even.
+ * statistics are float32; outputs are rounded once, to nearest even.  dx and dw take the ds they are given, of dtype: in 16 bits, where
+ * bs_act_grad made it, that is one rounding (of ds) before theirs.
  *
  * bs_linear_act -- s = x w^T + bias (+ res), a = act(s); x [rows, K], w [N, K], bias [N] (nullable), res [rows, N] (nullable);
  *   sum_out = s, act_out = a, contiguous [rows, N] (each nullable, at least one).  act sees s before its rounding.  float32
