@@ -144,6 +144,10 @@ def group_norm_act(x, groups, gamma=None, beta=None, eps=1e-5, act="elu", save8=
             raise hip.BitswapHipError(f"group_norm_act: {groups} groups do not divide {c} channels")
         if not eps >= 0:
             raise hip.BitswapHipError(f"group_norm_act: eps {eps}")
+        given = [t for t in (gamma, beta) if t is not None]
+        if any(t.shape != (c,) or t.dtype not in (torch.float32, x.dtype) or t.dtype != given[0].dtype for t in given):
+            raise hip.BitswapHipError(f"group_norm_act: gamma and beta must be [{c}] of one type, float32 or {x.dtype}, got "
+                                      f"{[(tuple(t.shape), t.dtype) for t in given]}")
         v = x.reshape(n, pixels, groups, c // groups).to(_wide(x.dtype))
         d = v - v.mean((1, 3), keepdim=True)
         u = (d / torch.sqrt(d.square().mean((1, 3), keepdim=True) + eps)).reshape(n, pixels, c)

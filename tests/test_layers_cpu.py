@@ -271,3 +271,12 @@ def test_workspaces_that_are_not_aligned_are_refused(L):
             assert L.bs_act_grad(p, 8, None, 8, None, None, 8, 0, dt, 100000, 8, None, 8, p, ws, room, None) == E
             assert L.bs_group_norm_act(p, 64000, 8, None, None, 0, 1e-5, 0, dt, 2, 8000, 8, 2, p, None, ws, room, None) == E
             assert L.bs_group_norm_act_grad(p, 64, 8, p, None, 64, 8, p, None, None, 0, 0, dt, 2, 8, 8, 2, p, None, None, ws, room, None) == E
+
+
+def test_group_norm_on_the_cpu_refuses_parameters_as_the_kernels_do():
+    from bitswap_amd import hip, layers
+    x, one, half = torch.randn(2, 4, 6).bfloat16(), torch.ones(6), torch.ones(6, dtype=torch.bfloat16)
+    for gamma, beta in ((torch.ones(1), None), (None, torch.zeros(2, 3)), (one.double(), None), (one, half), (None, one.half())):
+        with pytest.raises(hip.BitswapHipError):
+            layers.group_norm_act(x, 2, gamma, beta)
+    assert torch.equal(layers.group_norm_act(x, 2, one, one), layers.group_norm_act(x, 2, half, half))
